@@ -14,6 +14,7 @@
 
 #include "common.h"
 #include "gguf.h"
+#include "host_util.h"
 #include "kernels.h"
 #include "noalloc.h"
 #include "tc_gemm.h"
@@ -39,20 +40,6 @@ void clear_error() {
     (void)cudaGetLastError();
 }
 
-#define CUDA_TRY(expr)                                                                              \
-    do {                                                                                            \
-        cudaError_t e_ = (expr);                                                                    \
-        if (e_ != cudaSuccess)                                                                      \
-            return set_error(STT_E_CUDA, "%s failed: %s (%s:%d)", #expr, cudaGetErrorString(e_),    \
-                             __FILE__, __LINE__);                                                   \
-    } while (0)
-
-#define TRY(expr)                  \
-    do {                           \
-        int rc_ = (expr);          \
-        if (rc_ != STT_OK) return rc_; \
-    } while (0)
-
 // Allocation-failure injection for tests (stt_debug_fail_allocation): a countdown over the library's
 // device and pinned-host allocations; the one that brings it to zero fails as if memory had run out.
 std::atomic<int64_t> g_fail_after{-1};
@@ -77,53 +64,6 @@ cudaError_t host_alloc(void** p, size_t bytes) {
     }
     return cudaHostAlloc(p, bytes, cudaHostAllocDefault);
 }
-
-// An allocation: out of memory is STT_E_OOM, any other failure STT_E_CUDA.
-#define ALLOC_TRY(expr)                                                                             \
-    do {                                                                                            \
-        cudaError_t e_ = (expr);                                                                    \
-        if (e_ != cudaSuccess) {                                                                    \
-            (void)cudaGetLastError();                                                               \
-            return set_error(e_ == cudaErrorMemoryAllocation ? STT_E_OOM : STT_E_CUDA,              \
-                             "%s failed: %s (%s:%d)", #expr, cudaGetErrorString(e_), __FILE__,      \
-                             __LINE__);                                                             \
-        }                                                                                           \
-    } while (0)
-
-// Restores the calling thread's current device on scope exit.
-struct DeviceScope {
-    int prev = 0;
-    bool ok = false;
-    explicit DeviceScope(int dev) {
-        if (cudaGetDevice(&prev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) ok = true;
-    }
-    ~DeviceScope() {
-        if (ok) cudaSetDevice(prev);
-    }
-};
-
-// Device buffer that grows on demand.
-struct DevBuf {
-    void* p = nullptr;
-    size_t cap = 0;
-    void release() {
-        if (p) cudaFree(p);
-        p = nullptr;
-        cap = 0;
-    }
-    int ensure(size_t bytes) {
-        if (bytes <= cap) return STT_OK;
-        if (p) cudaFree(p);
-        p = nullptr;
-        cap = 0;
-        ALLOC_TRY(dev_alloc(&p, bytes));
-        cap = bytes;
-        return STT_OK;
-    }
-    ~DevBuf() {
-        if (p) cudaFree(p);
-    }
-};
 
 // Pinned host buffer that grows on demand.
 struct HostBuf {

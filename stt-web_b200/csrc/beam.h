@@ -1,0 +1,52 @@
+// Beam search on the device: selection over beams and vocabulary, and the reordering of the beams'
+// states (beam.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kv8.h"
+
+namespace stt {
+
+constexpr int kMaxBeams = 32;
+constexpr int kBeamThreads = 256;
+constexpr int kBeamPerThread = 16;                            // logits of a thread
+constexpr int kBeamChunk = kBeamThreads * kBeamPerThread;     // logits of a CTA
+
+struct BeamArgs {
+    const void* logits;   // [batch * beams][vocab], rows row_stride elements apart
+    int64_t row_stride;
+    int32_t batch, beams, vocab, chunks;
+    const float* scores;  // [batch][beams]
+    const uint8_t* done;  // [batch][beams] or NULL
+    int32_t eos;          // -1: none
+    float* next_scores;
+    int32_t *parents, *tokens;
+    uint8_t* next_done;   // or NULL
+    // workspace, indexed by row * chunks + chunk
+    float* part_max;
+    double* part_sum;
+    uint64_t* part_keys;  // [kMaxBeams of the selector] best keys of the chunk, descending
+    int32_t key_stride;
+    uint32_t* tickets;    // [batch]
+    int32_t* err;
+};
+
+struct ReorderArgs {
+    uint8_t* states;
+    int64_t row_stride;    // bytes; segment s of a row starts at (s / inner) * outer_stride + (s % inner) * segment_stride
+    int64_t segment_stride, outer_stride;
+    int32_t segments, inner;
+    int32_t first_segment; // of the launch
+    int64_t units, unit_bytes;
+    int32_t groups, beams;
+    const int32_t* parents;
+    const int32_t* held;   // what each row holds, or NULL: `units` units
+    int32_t per_unit;      // of which `per_unit` make one unit
+};
+
+cudaError_t launch_beam_select(const BeamArgs& a, int dtype, cudaStream_t st);
+cudaError_t launch_reorder(const ReorderArgs& a, cudaStream_t st);
+
+}  // namespace stt

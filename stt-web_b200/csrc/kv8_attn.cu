@@ -1,0 +1,441 @@
+// Attention over the 8-bit K/V cache.
+//
+// For query row r (a token and a query head of the K/V head h) at position P:
+//   out = sum_p softmax_p(scale * q . k_p) v_p   over   max(start, P + 1 - window, ring) <= p <= P,
+// zeros where no position is left.  In base 2: s_p = log2(e) * scale * q . k_p, and with V's block
+// exponents folded into the weights
+//   m = max s_p,  l = sum 2^(s_p - m),   M = max(s_p + e_v(p)),  O = sum 2^(s_p + e_v(p) - M) * code_p,
+//   out = O / l * 2^(M - m).
+// One pass over the codes keeps (m, l, M, O) per row and rescales them when a maximum grows.
+//
+// What bounds it: a decode step reads 2 * dim bytes per position and head and does 4 * dim flops per
+// query row with them, so HBM bounds it as long as turning codes into operands costs little.  Hence
+//  - the codes go through mma.sync.m16n8k16 f16 with f32 accumulation.  A code is exact in f16: the
+//    bytes (code + 128) under the high byte 0x64 are the f16 value 1024 + 128 + code, one subtraction
+//    away, 2.5 instructions for 4 codes.  tcgen05 would want the converted tile in shared or tensor
+//    memory first, one more trip for an operand that is used by a handful of rows;
+//  - 8 query rows fill the 16 MMA rows: rows 0-7 hold the leading f16 part of q (or of the weights),
+//    rows 8-15 the rest (x = hi + lo, 22 bits), so scores and outputs keep f32 quality and a lane
+//    finds both parts of its row in one accumulator quad;
+//  - the accumulator layout of the scores is the A-operand layout of the second product, and any
+//    order of dimensions serves as long as both operands agree, so nothing is shuffled: a lane's
+//    operand for K is 16 consecutive codes of one key, for V 16 consecutive codes of its 4 keys;
+//  - every warp streams its own blocks of 16 keys through a private ring in shared memory
+//    (cp.async, 16 bytes per lane), without block-wide barriers, and the 4 warps are merged at the end.
+#include <cfloat>
+#include <algorithm>
+
+#include "kv8.cuh"
+
+namespace stt {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kStages = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kWeightShift = 14;  // weights are scaled by 2^14, so that f16 keeps 2^-28 and up normal
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Bytes `sel` of biased codes (code + 128) as a pair of f16 codes.
+template <int SEL>
+__device__ __forceinline__ uint32_t codes_to_f16(uint32_t biased) {
+    uint32_t r = __byte_perm(biased, 0x64646464u, SEL);
+    const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r), __float2half2_rn(1152.0f));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// x = hi + lo in f16, for two values.
+__device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    *hi = *reinterpret_cast<const uint32_t*>(&h);
+    *lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// Byte offset of 16-byte piece `c` of key row `r` in a staged block of K or V.  The permutations
+// make the reads below conflict-free: a quarter warp reads K rows {2i, 2i+1} x 4 pieces, and V rows
+// {0, 2, 4, 6} (or the others of its residue) x 2 pieces (dim 128) or 4 half pieces (dim 64).
+template <int D>
+__device__ __forceinline__ int k_piece(int r, int c) {
+    return D == 128 ? r * 128 + ((c ^ (4 * (r & 1))) << 4) : r * 64 + (c << 4);
+}
+template <int D>
+__device__ __forceinline__ int v_piece(int r, int c) {
+    if (D == 128) return r * 128 + ((c ^ (2 * ((r >> 1) & 3))) << 4);
+    return (r >> 1) * 128 + ((((r & 1) * 4 + c) ^ (2 * ((r >> 1) & 3))) << 4);
+}
+
+// One row's softmax state in base 2.
+struct RowState {
+    float m, l, M;
+};
+
+template <int DT>
+__device__ __forceinline__ void load16(const void* base, int64_t at, float (&x)[16]) {
+    const typename Elem<DT>::T* p = static_cast<const typename Elem<DT>::T*>(base) + at;
+    float a[8], b[8];
+    load_elems<DT, 8>(p, a);
+    load_elems<DT, 8>(p + 8, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = a[i], x[8 + i] = b[i];
+}
+__device__ __forceinline__ void load16(const void* base, int dtype, int64_t at, float (&x)[16]) {
+    if (dtype == DT_F32) load16<DT_F32>(base, at, x);
+    else if (dtype == DT_BF16) load16<DT_BF16>(base, at, x);
+    else load16<DT_F16>(base, at, x);
+}
+
+// Positions [lo, hi] that the query at position P sees.
+struct Sight {
+    int start, window, ring;
+    __device__ __forceinline__ int lo(int P) const {
+        int a = max(start, ring);
+        return window > 0 && P + 1 - window > a ? P + 1 - window : a;
+    }
+};
+
+// Merges the softmax states of `n` parts and returns the row's output piece: O / l * 2^(M - m).
+// State and piece of part j come from the two functions; an empty part has l = 0.
+template <class State, class Piece>
+__device__ __forceinline__ RowState merge_parts(int n, State state, Piece piece, float4* out) {
+    RowState r{-FLT_MAX, 0.0f, -FLT_MAX};
+    for (int j = 0; j < n; ++j) {
+        const RowState s = state(j);
+        if (s.l != 0.0f) r.m = fmaxf(r.m, s.m), r.M = fmaxf(r.M, s.M);
+    }
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int j = 0; j < n; ++j) {
+        const RowState s = state(j);
+        if (s.l == 0.0f) continue;
+        r.l = fmaf(s.l, exp2f(s.m - r.m), r.l);
+        const float f = exp2f(s.M - r.M);
+        const float4 p = piece(j);
+        o.x = fmaf(p.x, f, o.x), o.y = fmaf(p.y, f, o.y), o.z = fmaf(p.z, f, o.z), o.w = fmaf(p.w, f, o.w);
+    }
+    *out = o;
+    return r;
+}
+__device__ __forceinline__ float4 row_output(const RowState& r, float4 o) {
+    if (r.l == 0.0f) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float f = exp2f(r.M - r.m - (float)kWeightShift) / r.l;
+    return make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+}
+
+// CTA ((batch row * row_groups + row group) * heads + head) * max_splits + split.
+template <int D>
+__global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Batch b, Kv8Attention a, int row_groups,
+                                                                int max_splits) {
+    constexpr int KS = D / 16;          // k steps of the first product
+    constexpr int NT = D / 8;           // n tiles of the second
+    constexpr int HALF = 16 * D;        // bytes of a staged block of K (and of V)
+    constexpr int CH = D / 16;          // 16-byte pieces of a row
+    constexpr int VB = D / 8;           // bytes of V that a lane takes of a key
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ RowState sm_state[kWarps][kKv8Rows];
+    __shared__ uint32_t last;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x % max_splits, item = blockIdx.x / max_splits;
+    const int h = item % c.heads, rg = item / c.heads % row_groups, i = item / c.heads / row_groups;
+    Kv8Row row;
+    if (!kv8_row(c, b, i, &row)) return;
+    // the group's rows: row r is token r / group, query head h * group + r % group
+    const int r0 = rg * kKv8Rows;
+    const int rows = min(kKv8Rows, row.count * a.group - r0);
+    if (rows <= 0) return;
+    const int t0 = r0 / a.group, t1 = (r0 + rows - 1) / a.group;
+    Sight sight;
+    sight.start = a.start ? max(0, __ldg(a.start + i)) : 0;
+    sight.window = a.window;
+    sight.ring = (row.pos + row.count + kKv8Block - 1) / kKv8Block * kKv8Block - c.cap;
+    const int first = sight.lo(row.pos + t0), end = row.pos + t1;  // positions that some row sees
+    const int kb0 = first / kKv8Block;
+    const int nb = first <= end ? end / kKv8Block - kb0 + 1 : 0;
+    // a split takes at least one block per warp, so short contexts use fewer splits than were launched
+    const int splits = max(1, min(max_splits, nb / kWarps));
+    if (split >= splits) return;
+    const int sb0 = kb0 + (int)((int64_t)nb * split / splits), sb1 = kb0 + (int)((int64_t)nb * (split + 1) / splits);
+    const int64_t head = (int64_t)row.seq * c.heads + h;
+    const int8_t* kbase = c.kc + head * c.cap * D;
+    const int8_t* vbase = c.vc + head * c.cap * D;
+    const int cap_blocks = c.cap / kKv8Block;
+    const int8_t* kexp = c.ke + head * cap_blocks;
+    const int8_t* vexp = c.ve + head * cap_blocks;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kStages * 2 * HALF);
+    const int mine = max(0, (sb1 - sb0 - warp + kWarps - 1) / kWarps);  // blocks sb0 + warp + 4 * j
+
+    auto fetch = [&](int j) {
+        if (j < mine) {
+            const int blk = (sb0 + warp + kWarps * j) % cap_blocks;
+            const int8_t* ks = kbase + (int64_t)blk * HALF;
+            const int8_t* vs = vbase + (int64_t)blk * HALF;
+            const uint32_t dst = ring + (j % kStages) * (2 * HALF);
+#pragma unroll
+            for (int u = 0; u < HALF / 512; ++u) {
+                const int p = lane + 32 * u, r = p / CH, ch = p % CH;
+                cp_async16(dst + k_piece<D>(r, ch), ks + p * 16);
+                cp_async16(dst + HALF + v_piece<D>(r, ch), vs + p * 16);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int j = 0; j < kStages - 1; ++j) fetch(j);
+    // lane j: exponents of this warp's blocks j of the current 32, K's in the high half
+    auto fetch_exps = [&](int j) {
+        if (j >= mine) return 0;
+        const int blk = (sb0 + warp + kWarps * j) % cap_blocks;
+        return ((int)kexp[blk] << 16) | (vexp[blk] & 0xFF);
+    };
+    int exps = fetch_exps(lane);
+
+    // q of row g as hi and lo parts: k step s = 4 * (half) + w holds dimensions 64 * half + 16 * t + 4 * w + 0..3
+    const bool live = g < rows;
+    const int tok = live ? (r0 + g) / a.group : t0;
+    const int P = row.pos + tok;
+    const int see_lo = live ? sight.lo(P) : 0x7FFFFFFF, see_hi = live ? P : -1;
+    uint32_t qa[KS][4];
+    float q_step;  // scores = accumulator * q_step * 2^e_k
+    {
+        float x[D / 64][16];
+        float amax = 0.0f;
+#pragma unroll
+        for (int hf = 0; hf < D / 64; ++hf) {
+            if (live) {
+                const int qh = h * a.group + (r0 + g) % a.group;
+                load16(a.q, a.q_dtype, i * a.qs.seq + (int64_t)tok * a.qs.token + qh * a.qs.head + 64 * hf + 16 * t, x[hf]);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                x[hf][e] = live ? x[hf][e] * (a.scale * kLog2e) : 0.0f;
+                amax = fmaxf(amax, fabsf(x[hf][e]));
+            }
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
+        // the row scaled to a maximum in [2^13, 2^14): the parts of its small elements stay normal in f16
+        const int ex = amax > 0.0f ? (__float_as_int(amax) >> 23) - 127 - 13 : 0;
+        const float up = pow2i(-ex);
+        q_step = pow2i(ex);
+#pragma unroll
+        for (int hf = 0; hf < D / 64; ++hf)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t* A = qa[4 * hf + w];
+                split2(x[hf][4 * w] * up, x[hf][4 * w + 1] * up, &A[0], &A[1]);
+                split2(x[hf][4 * w + 2] * up, x[hf][4 * w + 3] * up, &A[2], &A[3]);
+            }
+    }
+
+    float o[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    RowState st{-FLT_MAX, 0.0f, -FLT_MAX};
+    // inside every row's sight: no masking needed
+    const int all_lo = sight.lo(row.pos + t1), all_hi = row.pos + t0;
+
+    for (int j = 0; j < mine; ++j) {
+        if (j > 0 && j % 32 == 0) exps = fetch_exps(j + lane);
+        const int ee = __shfl_sync(0xFFFFFFFFu, exps, j % 32);
+        const float ks = q_step * pow2i(ee >> 16);
+        const float ev = (float)(int8_t)(ee & 0xFF);
+        cp_async_wait<kStages - 2>();
+        __syncwarp();
+        const uint8_t* kst = smem + warp * (kStages * 2 * HALF) + (j % kStages) * (2 * HALF);
+        const uint8_t* vst = kst + HALF;
+        float s[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+            for (int hf = 0; hf < D / 64; ++hf) {
+                const uint4 kq = *reinterpret_cast<const uint4*>(kst + k_piece<D>(8 * n + g, 4 * hf + t));
+                const uint32_t w[4] = {kq.x, kq.y, kq.z, kq.w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t x = w[u] ^ 0x80808080u;
+                    mma16816(s[n], qa[4 * hf + u], codes_to_f16<0x4140>(x), codes_to_f16<0x4342>(x));
+                }
+            }
+        }
+        // scores of row g at keys 2t, 2t + 1 of each n tile
+        const int p0 = (sb0 + warp + kWarps * j) * kKv8Block;
+        float v[4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            v[2 * n] = (s[n][0] + s[n][2]) * ks;
+            v[2 * n + 1] = (s[n][1] + s[n][3]) * ks;
+        }
+        if (p0 < all_lo || p0 + kKv8Block - 1 > all_hi || rows < kKv8Rows) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int p = p0 + 8 * (e >> 1) + 2 * t + (e & 1);
+                if (p < see_lo || p > see_hi) v[e] = -INFINITY;
+            }
+        }
+        float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+        // (mx = -inf leaves the maxima alone: they start at -FLT_MAX, never at -inf)
+        const float m = fmaxf(st.m, mx), M = fmaxf(st.M, mx + ev);
+        if (__any_sync(0xFFFFFFFFu, m != st.m || M != st.M)) {
+            st.l *= exp2f(st.m - m);
+            const float f = exp2f(st.M - M);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n][0] *= f, o[n][1] *= f, o[n][2] *= f, o[n][3] *= f;
+            st.m = m;
+            st.M = M;
+        }
+        uint32_t pa[4];
+        {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                st.l += exp2f(v[e] - m);
+                w[e] = exp2f(v[e] + (ev + (float)kWeightShift - M));
+            }
+            split2(w[0], w[1], &pa[0], &pa[1]);
+            split2(w[2], w[3], &pa[2], &pa[3]);
+        }
+        // V: keys 2t, 2t + 1, 2t + 8, 2t + 9; n tile n holds dimensions VB * g + n
+#pragma unroll
+        for (int u = 0; u < VB / 4; u += 2) {
+            uint2 r[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = 2 * t + (e & 1) + 8 * (e >> 1);
+                const int byte = VB * g + 4 * u;
+                r[e] = *reinterpret_cast<const uint2*>(vst + v_piece<D>(key, byte >> 4) + (byte & 15));
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const uint32_t A = (w ? r[0].y : r[0].x) ^ 0x80808080u, B = (w ? r[1].y : r[1].x) ^ 0x80808080u;
+                const uint32_t C = (w ? r[2].y : r[2].x) ^ 0x80808080u, E = (w ? r[3].y : r[3].x) ^ 0x80808080u;
+                const uint32_t ab0 = __byte_perm(A, B, 0x5140), ab1 = __byte_perm(A, B, 0x7362);
+                const uint32_t ce0 = __byte_perm(C, E, 0x5140), ce1 = __byte_perm(C, E, 0x7362);
+                const int n = 4 * (u + w);
+                mma16816(o[n], pa, codes_to_f16<0x4140>(ab0), codes_to_f16<0x4140>(ce0));
+                mma16816(o[n + 1], pa, codes_to_f16<0x4342>(ab0), codes_to_f16<0x4342>(ce0));
+                mma16816(o[n + 2], pa, codes_to_f16<0x4140>(ab1), codes_to_f16<0x4140>(ce1));
+                mma16816(o[n + 3], pa, codes_to_f16<0x4342>(ab1), codes_to_f16<0x4342>(ce1));
+            }
+        }
+        __syncwarp();
+        fetch(j + kStages - 1);
+    }
+    // l of the row: the 4 lanes hold different keys
+    st.l += __shfl_xor_sync(0xFFFFFFFFu, st.l, 1);
+    st.l += __shfl_xor_sync(0xFFFFFFFFu, st.l, 2);
+    cp_async_wait<0>();
+    __syncthreads();
+    // warp states to shared memory.  A lane holds dimensions 2 * VB * t + 0 .. 2 * VB - 1 of its row;
+    // the 16-byte pieces are permuted so that the lanes of a quarter warp hit different banks.
+    constexpr int PL = D / 16;  // pieces per lane
+    float4* so = reinterpret_cast<float4*>(smem);
+    auto so_at = [&](int w, int r, int piece) {
+        const int lt = piece / PL, k = piece % PL;
+        return (w * kKv8Rows + r) * (D / 4) + lt * PL + (k ^ ((lt + 4 * (r & 1)) & (PL - 1)));
+    };
+    if (live) {
+#pragma unroll
+        for (int k = 0; k < PL; ++k) {
+            const int col = 4 * k / VB, n = 4 * k % VB;
+            so[so_at(warp, g, PL * t + k)] =
+                make_float4(o[n][col] + o[n][col + 2], o[n + 1][col] + o[n + 1][col + 2],
+                            o[n + 2][col] + o[n + 2][col + 2], o[n + 3][col] + o[n + 3][col + 2]);
+        }
+        if (t == 0) sm_state[warp][g] = st;
+    }
+    __syncthreads();
+    const int pieces = rows * (D / 4);
+    auto write_out = [&](int r, int piece, float4 v) {
+        const int token = (r0 + r) / a.group, qh = h * a.group + (r0 + r) % a.group;
+        store4(a.out, a.out_dtype, i * a.os.seq + (int64_t)token * a.os.token + qh * a.os.head + 4 * piece, v);
+    };
+    constexpr int STRIDE = kKv8Rows * (D + 4);
+    float* part = a.part + (int64_t)blockIdx.x * STRIDE;
+    for (int p = threadIdx.x; p < pieces; p += kWarps * 32) {
+        const int r = p / (D / 4), piece = p % (D / 4);
+        float4 v;
+        const RowState rs = merge_parts(
+            kWarps, [&](int w) { return sm_state[w][r]; }, [&](int w) { return so[so_at(w, r, piece)]; }, &v);
+        if (splits == 1) {
+            write_out(r, piece, row_output(rs, v));
+        } else {
+            *reinterpret_cast<float4*>(part + r * (D + 4) + 4 + 4 * piece) = v;
+            if (piece == 0) *reinterpret_cast<float4*>(part + r * (D + 4)) = make_float4(rs.m, rs.l, rs.M, 0.0f);
+        }
+    }
+    if (splits == 1) return;
+    // the last of the item's splits merges them in split order, so the result does not depend on which
+    // one that is, and leaves the ticket at zero for the next call
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(a.tickets + item, 1u) == (uint32_t)(splits - 1);
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    const float* parts = a.part + (int64_t)item * max_splits * STRIDE;
+    for (int p = threadIdx.x; p < pieces; p += kWarps * 32) {
+        const int r = p / (D / 4), piece = p % (D / 4);
+        float4 v;
+        const RowState rs = merge_parts(
+            splits,
+            [&](int w) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(parts + (int64_t)w * STRIDE + r * (D + 4)));
+                return RowState{x.x, x.y, x.z};
+            },
+            [&](int w) { return __ldcg(reinterpret_cast<const float4*>(parts + (int64_t)w * STRIDE + r * (D + 4) + 4 + 4 * piece)); },
+            &v);
+        write_out(r, piece, row_output(rs, v));
+    }
+    if (threadIdx.x == 0) a.tickets[item] = 0u;
+}
+
+template <int D>
+constexpr size_t attend_smem() {
+    return (size_t)kWarps * kStages * 2 * 16 * D;
+}
+
+template <int D>
+cudaError_t attend_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st) {
+    const int row_groups = (b.tokens * a.group + kKv8Rows - 1) / kKv8Rows;
+    const int64_t items = (int64_t)b.n * c.heads * row_groups;
+    // fill the SMs' 3 CTAs twice over where there are few items; never more CTAs than partial slots,
+    // nor more splits than a full context has blocks for
+    const int context = a.window > 0 ? std::min<int64_t>((int64_t)a.window + b.tokens, c.cap) : c.cap;
+    const int64_t want = std::min<int64_t>((6 * a.num_sms + items - 1) / items, context / kKv8Block / kWarps + 1);
+    const int splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, kKv8MaxPartials / items));
+    attend_kernel<D><<<(unsigned)(items * splits), kWarps * 32, attend_smem<D>(), st>>>(c, b, a, row_groups, splits);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t kv8_partial_bytes(int dim) { return (size_t)kKv8MaxPartials * kKv8Rows * (dim + 4) * sizeof(float); }
+
+cudaError_t kv8_configure() {
+    cudaError_t e = cudaFuncSetAttribute(attend_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attend_smem<128>());
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(attend_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attend_smem<64>());
+}
+
+cudaError_t launch_kv8_attention(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st) {
+    return c.dim == 128 ? attend_t<128>(c, b, a, st) : attend_t<64>(c, b, a, st);
+}
+
+}  // namespace stt

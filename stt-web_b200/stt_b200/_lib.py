@@ -79,6 +79,21 @@ class stt_stream_state(C.Structure):
     ]
 
 
+class stt_kv8_cache_info(C.Structure):
+    _fields_ = [
+        ("device", C.c_int32),
+        ("n_seqs", C.c_int32),
+        ("n_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("capacity", C.c_int32),
+        ("block_tokens", C.c_int32),
+        ("d_k_codes", C.c_void_p),
+        ("d_v_codes", C.c_void_p),
+        ("d_k_exponents", C.c_void_p),
+        ("d_v_exponents", C.c_void_p),
+    ]
+
+
 P = C.c_void_p
 U8P = C.POINTER(C.c_uint8)
 U32P = C.POINTER(C.c_uint32)
@@ -116,6 +131,24 @@ SIGNATURES = {
     "stt_q4_tensor_dequant": (C.c_int, [P, F32P]),
     "stt_q4_tensor_status": (C.c_int, [P]),
     "stt_q4_matmul_device_noalloc": (C.c_int, [P, P, C.c_int, C.c_int, C.c_int, P, P]),
+    "stt_kv8_cache_bytes": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
+    "stt_kv8_cache_create": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, P, C.POINTER(P)]),
+    "stt_kv8_cache_destroy": (C.c_int, [P]),
+    "stt_kv8_cache_get_info": (C.c_int, [P, C.POINTER(stt_kv8_cache_info)]),
+    "stt_kv8_cache_status": (C.c_int, [P]),
+    "stt_kv8_append_device": (C.c_int, [P, P, C.c_int, P, P, C.c_int, P, P, C.c_int, C.c_int64, C.c_int64, C.c_int64, P]),
+    "stt_kv8_read_device": (C.c_int, [P, P, C.c_int, P, P, C.c_int, P, P, C.c_int, C.c_int64, C.c_int64, C.c_int64, P]),
+    "stt_kv8_attention_device": (C.c_int, [P, P, C.c_int, P, P, C.c_int, C.c_int, P, C.c_int, C.c_int64, C.c_int64,
+                                           C.c_int64, P, C.c_int, C.c_float, P, C.c_int, C.c_int64, C.c_int64, C.c_int64,
+                                           P]),
+    "stt_kv8_reorder_device": (C.c_int, [P, P, C.c_int, C.c_int, P, P]),
+    "stt_beam_create": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(P)]),
+    "stt_beam_destroy": (C.c_int, [P]),
+    "stt_beam_status": (C.c_int, [P]),
+    "stt_beam_select_device": (C.c_int, [P, P, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, P, P, C.c_int, P, P, P, P,
+                                         P]),
+    "stt_beam_reorder_device": (C.c_int, [C.c_int, P, C.c_int64, C.c_int, C.c_int64, C.c_int64, C.c_int64, P, C.c_int,
+                                          C.c_int, P, P]),
     "stt_spm_decoder_create": (C.c_int, [U8P, C.c_size_t, C.POINTER(P)]),
     "stt_spm_decoder_destroy": (C.c_int, [P]),
     "stt_spm_vocab_len": (C.c_int, [P, C.POINTER(C.c_int64)]),
@@ -155,8 +188,9 @@ def lib() -> C.CDLL:
 class SttError(RuntimeError):
     """An STT_E_* status returned by the library."""
 
-    def __init__(self, code: int, where: str):
-        msg = lib().stt_last_error().decode("utf-8", "replace")
+    def __init__(self, code: int, where: str, msg: str | None = None):
+        if msg is None:
+            msg = lib().stt_last_error().decode("utf-8", "replace")
         super().__init__(f"{where}: status {code}: {msg}")
         self.code = code
 

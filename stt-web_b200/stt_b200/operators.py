@@ -1,0 +1,232 @@
+"""Decode operators that stand beside the model, over device tensors: the 8-bit K/V cache with its
+attention, and beam search's selection and reordering.
+
+Tensors are CUDA tensors of any library whose objects have torch's ``data_ptr()``, ``shape``,
+``stride()`` and ``dtype`` (torch itself is not imported).  Calls are queued on ``stream`` (the integer
+handle of a CUDA stream, 0 = the legacy default stream) and do not wait for the device; the tensors must
+stay alive until it has run them.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Optional
+
+from ._lib import STT_E_INVALID_ARG, SttError, check, lib, stt_kv8_cache_info
+
+_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+
+
+def _refuse(where: str, why: str):
+    raise SttError(STT_E_INVALID_ARG, where, why)
+
+
+def _dtype(t, where: str) -> int:
+    code = _DTYPES.get(str(t.dtype))
+    if code is None:
+        _refuse(where, f"dtype {t.dtype} unknown: f32, bf16 and f16 are")
+    return code
+
+
+def _on(t, device: int, where: str):
+    if t.device.type != "cuda" or t.device.index != device:
+        _refuse(where, f"a tensor is on {t.device}, the operator on cuda:{device}")
+
+
+def _whole(t, n: int, device: int, where: str, what: str, dtype: str = "torch.int32") -> int:
+    """Address of a contiguous device array of n entries."""
+    if str(t.dtype) != dtype or t.numel() != n or not t.is_contiguous():
+        _refuse(where, f"{what} must be {n} contiguous {dtype[6:]} values")
+    _on(t, device, where)
+    return t.data_ptr()
+
+
+class Kv8Cache:
+    """K and V of ``n_seqs`` sequences as signed bytes with a power-of-two scale for each block of 16
+    tokens and head (stt_kv8_* of include/stt_b200.h).  ``memory``: a device tensor of ``bytes()``
+    bytes that holds the cache, or None for memory of the library's own.  Calls on one cache must not
+    overlap in time."""
+
+    def __init__(self, n_seqs: int, n_kv_heads: int, head_dim: int, capacity: int, device: int = 0, memory=None):
+        self._h = None
+        need = self.bytes(n_seqs, n_kv_heads, head_dim, capacity)
+        where = "stt_kv8_cache_create"
+        if memory is not None:
+            _on(memory, device, where)
+            if not memory.is_contiguous() or memory.numel() * memory.element_size() < need:
+                _refuse(where, f"the memory must be contiguous and hold {need} bytes")
+        h = C.c_void_p()
+        check(lib().stt_kv8_cache_create(device, n_seqs, n_kv_heads, head_dim, capacity,
+                                         memory.data_ptr() if memory is not None else None, C.byref(h)), where)
+        self._h = h
+        self.memory = memory
+        self.n_seqs, self.n_kv_heads, self.head_dim, self.capacity, self.device = n_seqs, n_kv_heads, head_dim, capacity, device
+
+    @staticmethod
+    def bytes(n_seqs: int, n_kv_heads: int, head_dim: int, capacity: int) -> int:
+        out = C.c_size_t()
+        check(lib().stt_kv8_cache_bytes(n_seqs, n_kv_heads, head_dim, capacity, C.byref(out)), "stt_kv8_cache_bytes")
+        return out.value
+
+    def close(self) -> None:
+        if self._h:
+            lib().stt_kv8_cache_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def info(self) -> stt_kv8_cache_info:
+        o = stt_kv8_cache_info()
+        check(lib().stt_kv8_cache_get_info(self._h, C.byref(o)), "stt_kv8_cache_get_info")
+        return o
+
+    def status(self) -> None:
+        """Waits for the device; raises SttError for what the calls since the last check reported."""
+        check(lib().stt_kv8_cache_status(self._h), "stt_kv8_cache_status")
+
+    def _rows(self, t, where: str, heads: Optional[int] = None):
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 4 or shape[3] != self.head_dim or stride[3] != 1 or (heads is not None and shape[2] != heads):
+            _refuse(where, f"tensors are [n, tokens, {heads or 'heads'}, {self.head_dim}] with the last dimension contiguous, got "
+                           f"{tuple(shape)} with strides {tuple(stride)}")
+        _on(t, self.device, where)
+        return shape[0], shape[1], shape[2], stride
+
+    def _batch(self, n: int, pos, count, seqs, where: str):
+        d = self.device
+        return (None if seqs is None else _whole(seqs, n, d, where, "seqs"), _whole(pos, n, d, where, "pos"),
+                None if count is None else _whole(count, n, d, where, "count"))
+
+    def append(self, k, v, pos, count=None, seqs=None, stream: int = 0) -> None:
+        """Writes k and v [n, tokens, n_kv_heads, head_dim]: row i's count[i] tokens (None: all) at the
+        positions pos[i] on of sequence seqs[i] (None: i)."""
+        where = "stt_kv8_append_device"
+        n, t, _, s = self._rows(k, where, self.n_kv_heads)
+        if v.shape != k.shape or v.stride() != s or v.dtype != k.dtype:
+            _refuse(where, "k and v must have one shape, one dtype and the same strides")
+        _on(v, self.device, where)
+        a, p, c = self._batch(n, pos, count, seqs, where)
+        check(lib().stt_kv8_append_device(self._h, a, n, p, c, t, k.data_ptr(), v.data_ptr(), _dtype(k, where), s[0], s[1],
+                                          s[2], stream), where)
+
+    def read(self, k, v, pos, count=None, seqs=None, stream: int = 0) -> None:
+        """Reads the values of a range of tokens into k and v [n, tokens, n_kv_heads, head_dim]."""
+        where = "stt_kv8_read_device"
+        n, t, _, s = self._rows(k, where, self.n_kv_heads)
+        if v.shape != k.shape or v.stride() != s or v.dtype != k.dtype:
+            _refuse(where, "k and v must have one shape, one dtype and the same strides")
+        _on(v, self.device, where)
+        a, p, c = self._batch(n, pos, count, seqs, where)
+        check(lib().stt_kv8_read_device(self._h, a, n, p, c, t, k.data_ptr(), v.data_ptr(), _dtype(k, where), s[0], s[1],
+                                        s[2], stream), where)
+
+    def attention(self, q, out, pos, count=None, seqs=None, start=None, window: int = 0, scale: Optional[float] = None,
+                  stream: int = 0) -> None:
+        """Causal attention of q [n, tokens, heads, head_dim], whose K and V an append with the same
+        pos, count and seqs has written, into ``out`` of the same shape (any of the dtypes).
+        scale None: 1 / sqrt(head_dim)."""
+        where = "stt_kv8_attention_device"
+        n, t, heads, qs = self._rows(q, where)
+        m, u, oh, os = self._rows(out, where)
+        if (n, t, heads) != (m, u, oh):
+            _refuse(where, f"q is {tuple(q.shape)}, out {tuple(out.shape)}")
+        a, p, c = self._batch(n, pos, count, seqs, where)
+        check(lib().stt_kv8_attention_device(
+            self._h, a, n, p, c, t, heads, q.data_ptr(), _dtype(q, where), qs[0], qs[1], qs[2],
+            None if start is None else _whole(start, n, self.device, where, "start"), window,
+            1.0 / math.sqrt(self.head_dim) if scale is None else scale, out.data_ptr(), _dtype(out, where), os[0], os[1],
+            os[2], stream), where)
+
+    def reorder(self, parents, held=None, stream: int = 0) -> None:
+        """Sequence g * beams + b becomes what sequence g * beams + parents[g, b] was, in place;
+        ``held`` [groups, beams]: positions that each sequence's new contents have (None: the whole ring)."""
+        where = "stt_kv8_reorder_device"
+        if len(parents.shape) != 2:
+            _refuse(where, "parents must be [groups, beams]")
+        g, b = parents.shape
+        d = self.device
+        check(lib().stt_kv8_reorder_device(self._h, _whole(parents, g * b, d, where, "parents"), g, b,
+                                           None if held is None else _whole(held, g * b, d, where, "held"), stream), where)
+
+
+class BeamSelector:
+    """Beam search's selection (stt_beam_select_device), with workspace for up to ``max_batch``
+    utterances, ``max_beams`` (at most 32) beams and ``max_vocab`` tokens.  Calls on one selector must
+    not overlap in time."""
+
+    def __init__(self, max_batch: int, max_beams: int, max_vocab: int, device: int = 0):
+        self._h = None
+        h = C.c_void_p()
+        check(lib().stt_beam_create(device, max_batch, max_beams, max_vocab, C.byref(h)), "stt_beam_create")
+        self._h = h
+        self.device = device
+
+    def close(self) -> None:
+        if self._h:
+            lib().stt_beam_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def status(self) -> None:
+        """Waits for the device; raises SttError if a beam had a NaN or +inf logit or score."""
+        check(lib().stt_beam_status(self._h), "stt_beam_status")
+
+    def select(self, logits, scores, next_scores, parents, tokens, done=None, next_done=None, eos: int = -1,
+               stream: int = 0) -> None:
+        """logits [batch * beams, vocab] (rows may be strided), scores f32 [batch, beams]; writes the
+        best ``beams`` continuations of each utterance, best first: next_scores (f32), parents and
+        tokens (int32), next_done (uint8, may be None).  done (uint8): beams that ended, whose only
+        continuation is ``eos``."""
+        where = "stt_beam_select_device"
+        if len(logits.shape) != 2 or len(scores.shape) != 2:
+            _refuse(where, "logits must be [batch * beams, vocab] and scores [batch, beams]")
+        rows, vocab = logits.shape
+        batch, beams = scores.shape
+        stride = logits.stride()
+        if rows != batch * beams or (stride[1] != 1 and vocab > 1):
+            _refuse(where, f"logits {tuple(logits.shape)} with strides {tuple(stride)} for {batch} x {beams} beams")
+        d = self.device
+        _on(logits, d, where)
+        check(lib().stt_beam_select_device(
+            self._h, logits.data_ptr(), _dtype(logits, where), stride[0] if rows > 1 else vocab, batch, beams, vocab,
+            _whole(scores, rows, d, where, "scores", "torch.float32"),
+            None if done is None else _whole(done, rows, d, where, "done", "torch.uint8"), eos,
+            _whole(next_scores, rows, d, where, "next_scores", "torch.float32"),
+            _whole(parents, rows, d, where, "parents"), _whole(tokens, rows, d, where, "tokens"),
+            None if next_done is None else _whole(next_done, rows, d, where, "next_done", "torch.uint8"), stream), where)
+
+
+def beam_reorder(states, parents, held=None, stream: int = 0) -> None:
+    """Row g * beams + b of ``states`` [groups * beams, segments, units, ...] becomes what row
+    g * beams + parents[g, b] was, in place.  ``held`` [groups, beams]: the first units of each segment
+    that count (None: all); the rest stays.  Everything behind the first two dimensions is contiguous."""
+    where = "stt_beam_reorder_device"
+    shape, stride = states.shape, states.stride()
+    if len(parents.shape) != 2 or len(shape) < 3:
+        _refuse(where, "states must be [groups * beams, segments, units, ...] and parents [groups, beams]")
+    groups, beams = parents.shape
+    inner = 1
+    for size, step in zip(reversed(shape[2:]), reversed(stride[2:])):
+        if size > 1 and step != inner:
+            _refuse(where, f"states of strides {tuple(stride)} are not contiguous behind the segments")
+        inner *= size
+    if shape[0] != groups * beams or 0 in shape:
+        _refuse(where, f"states {tuple(shape)} for {groups} x {beams} beams")
+    size = states.element_size()
+    if states.device.type != "cuda":
+        _refuse(where, f"the states are on {states.device}")
+    d = states.device.index
+    check(lib().stt_beam_reorder_device(d, states.data_ptr(), stride[0] * size, shape[1], stride[1] * size, shape[2],
+                                        inner // shape[2] * size, _whole(parents, groups * beams, d, where, "parents"),
+                                        groups, beams, None if held is None else _whole(held, groups * beams, d, where, "held"),
+                                        stream), where)
