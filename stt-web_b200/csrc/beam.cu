@@ -1,20 +1,22 @@
 // Beam search's selection over beams and vocabulary, and the reordering of the beams' states.
 //
 // Selection.  With x_b the logits of beam b and s_b its score so far, the `beams` best of
-//   s_b + (x_bv - max x_b - log sum_w exp(x_bw - max x_b)),   ties to the lowest b * vocab + v.
-// The logits are read once.  A CTA takes a chunk of a row into registers and leaves its maximum, its
-// sum of exponentials and its `beams` best logits (no more of one row can be among the best of all);
-// the last CTA of an utterance adds up the rows' sums and picks among the chunks' bests.  The order
-// of two beams' candidates can hang on the last digits, so sums are joined and candidates compared in
-// 64 bits; the exponentials themselves are f32 (their rounding errors, 2^-24 each, average out).
+//   s_b + (x_bv - log sum_w exp(x_bw)),   ties to the lowest b * vocab + v.
+// The logits are read once.  A CTA takes a chunk of a row, tile by tile through registers, and leaves a
+// reference value, its sum of exponentials over it, and its `beams` best logits (no more of one row can
+// be among the best of all); the last CTA of an utterance joins the rows' sums and picks among the
+// chunks' bests.  The order of two beams' candidates can hang on the last digits, so sums are joined and
+// candidates compared in 64 bits; the exponentials themselves are f32, 16 of a thread added at a time
+// (their rounding errors, 2^-24 each, average out: 1e-8 of the sum at 8000 logits).
 //
-// The `beams` best of a chunk without sorting it: each warp sorts its 32 lanes' maxima, the beams-th of
-// them is a lower bound of the chunk's beams-th best, the largest bound of the 8 warps leaves little
-// more than the `beams` best themselves, and those few are ranked by counting.
-#include "beam.h"
-
+// The best of a tile of 8192 logits: the k-th largest of its 32 half warps' maxima bounds the k-th best
+// logit from below, and little more than the k best reach it; those few go to a list in shared memory,
+// with the list's and the tiles' bounds carried from tile to tile, and are ranked by counting.  A tile
+// costs a maximum, an exponential and a comparison per logit.  Where more reach the bound than the list
+// takes (ties, masked rows), the warps sort them 32 at a time by a bitonic network instead.
 #include <algorithm>
 
+#include "beam.h"
 #include "kv8.cuh"
 
 namespace stt {
@@ -22,6 +24,7 @@ namespace stt {
 namespace {
 
 constexpr int kWarps = kBeamThreads / 32;
+static_assert(kWarps == 16, "the tile's bound is taken from 32 half warps");
 
 // Order-preserving 32 bits of an f32 (no NaN; -0 counts as +0).
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -65,106 +68,235 @@ __device__ __forceinline__ float to_f32(typename Elem<DT>::T x) {
     else if constexpr (DT == DT_BF16) return __bfloat162float(x);
     else return __half2float(x);
 }
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// Maximum that a NaN wins.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// A warp's best keys: lane l holds the l-th best.
+struct Best {
+    uint64_t top = 0;
+    // Takes the 32 best of the two sets; `o` sorted as `top` is.
+    __device__ __forceinline__ void merge_sorted(uint64_t o, int lane) {
+        o = __shfl_sync(0xFFFFFFFFu, o, 31 - lane);
+        top = o > top ? o : top;  // the 32 best of the 64, as a bitonic sequence
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            const uint64_t p = __shfl_xor_sync(0xFFFFFFFFu, top, d);
+            if ((p > top) == ((lane & d) == 0)) top = p;
+        }
+    }
+    // Adds up to 32 keys (0: none), one per lane.
+    __device__ __forceinline__ void merge(uint64_t k, int lane) {
+        merge_sorted(warp_sort(k, lane, [](uint64_t p, uint64_t q) { return p > q; },
+                               [](uint64_t p, int d) { return __shfl_xor_sync(0xFFFFFFFFu, p, d); }), lane);
+    }
+};
+
+constexpr int kList = 512;     // keys of the list: one per thread
+constexpr int kCounted = 96;   // up to this many are ranked by counting (4 instructions a pair); more by sorting
+static_assert(kList == kBeamThreads, "a thread loads one key of the list");
 
 template <int DT>
-__global__ void __launch_bounds__(kBeamThreads) select_kernel(BeamArgs a) {
+__global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
     using T = typename Elem<DT>::T;
     constexpr int VEC = 16 / (int)sizeof(T);            // elements of a 16-byte load
     constexpr int LOADS = kBeamPerThread / VEC;
-    __shared__ uint64_t list[kBeamChunk];
-    __shared__ uint64_t bound[kWarps];
-    __shared__ float wmax[kWarps];
+    constexpr int kRoom = 1024;                         // candidates of an utterance that are ranked at once
+    __shared__ union {
+        struct {
+            uint64_t list[kList], pending[kWarps][64], top[kWarps][32];
+        } s;
+        Cand cands[kRoom];
+    } sm;
+    __shared__ float wref[kWarps], half_max[2][2 * kWarps];
     __shared__ double wsum[kWarps];
     __shared__ uint32_t many, last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int chunk = blockIdx.x % a.chunks, r = blockIdx.x / a.chunks;
     const int g = r / a.beams, k = a.beams;
     const int64_t part = (int64_t)r * a.chunks + chunk;
-    const bool ended = a.done && a.done[r];
     if (tid == 0) many = 0;
-    if (!ended) {
-        // The chunk is cut at 16-byte boundaries of memory, whatever the row's own alignment: vector j
-        // of thread t covers elements from -lead + (chunk * CTA + j * 256 + t) * VEC on.
+    if (!(a.done && a.done[r])) {
+        // Tiles are cut at 16-byte boundaries of memory, whatever the row's own alignment: vector j of
+        // thread t of a tile covers elements -lead + (tile * CTA + j * 512 + t) * VEC on.
         const T* row = static_cast<const T*>(a.logits) + r * a.row_stride;
         const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-        float x[kBeamPerThread];
-        int base[LOADS];
+        const int inside = lead ? VEC - lead : 0;
+        const bool any_whole = inside + VEC <= a.vocab;
+        float ref = -INFINITY;    // the sum's reference: within 60 of the largest so far
+        double sum = 0.0;
+        float bound = -INFINITY;  // the chunk has at least k logits that reach it
+        int listed = 0;           // keys of the list
+        uint64_t* const list = sm.s.list;
+        // The list's k best, descending, from the sorted 32 best of every warp: a tree of merges.
+        auto join_warps = [&](Best best) {
+            sm.s.top[warp][lane] = best.top;
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-            base[j] = (chunk * (kBeamChunk / VEC) + j * kBeamThreads + tid) * VEC - lead;
-            if (base[j] >= 0 && base[j] + VEC <= a.vocab) {
-                float y[VEC];
-                if constexpr (DT == DT_F32) load_elems<DT, 4>(row + base[j], y);
-                else load_elems<DT, 8>(row + base[j], y);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) x[j * VEC + e] = y[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int v = base[j] + e;
-                    x[j * VEC + e] = v >= 0 && v < a.vocab ? to_f32<DT>(row[v]) : -INFINITY;
+            for (int s = kWarps / 2; s > 0; s >>= 1) {
+                __syncthreads();
+                if (warp < s) {
+                    best.merge_sorted(sm.s.top[warp + s][lane], lane);
+                    sm.s.top[warp][lane] = best.top;
                 }
             }
-        }
-        uint64_t best = 0;
-        float mx = -INFINITY;
-        bool bad = false;
+            __syncthreads();
+            listed = 0;
+            for (int j = 0; j < k; ++j) listed += sm.s.top[0][j] != 0;
+            if (tid < k) list[tid] = sm.s.top[0][tid];
+            if (listed == k) bound = fmaxf(bound, from_ordered((uint32_t)(sm.s.top[0][k - 1] >> 32)));
+            if (tid == 0) many = listed;
+            __syncthreads();
+        };
+        const int tile0 = chunk * a.tiles_per_chunk;
+        const int tile1 = min(tile0 + a.tiles_per_chunk, (a.vocab + lead + kBeamChunk - 1) / kBeamChunk);
+        for (int tile = tile0; tile < tile1; ++tile) {
+            float x[kBeamPerThread];
+            const int base = tile * kBeamChunk + tid * VEC - lead;  // of vector 0; vector j is j * 512 * VEC on
+            auto index = [&](int e) { return base + e / VEC * (kBeamThreads * VEC) + e % VEC; };
+            // Vectors that lie inside the row are loaded whole, all of them before the first is used (the
+            // others read vector `inside` instead); the row's ragged ends element by element.
+            bool whole[LOADS];
 #pragma unroll
-        for (int e = 0; e < kBeamPerThread; ++e) {
-            const int v = base[e / VEC] + e % VEC;
-            bad |= !(x[e] < INFINITY);  // NaN or +inf
-            mx = fmaxf(mx, x[e]);
-            if (v >= 0 && v < a.vocab) {
-                const uint64_t key = make_key(x[e], (uint32_t)v);
-                best = key > best ? key : best;
+            for (int j = 0; j < LOADS; ++j) {
+                const int v0 = base + j * kBeamThreads * VEC;
+                whole[j] = v0 >= 0 && v0 + VEC <= a.vocab;
+                float y[VEC];
+                if (any_whole) load_elems<DT, VEC>(row + (whole[j] ? v0 : inside), y);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[j * VEC + e] = whole[j] ? y[e] : -INFINITY;
+            }
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
+                const int v0 = base + j * kBeamThreads * VEC;
+                if (!whole[j] && v0 + VEC > 0 && v0 < a.vocab) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (v0 + e >= 0 && v0 + e < a.vocab) x[j * VEC + e] = to_f32<DT>(row[v0 + e]);
+                }
+            }
+            float lane_max = x[0];
+#pragma unroll
+            for (int e = 1; e < kBeamPerThread; ++e) lane_max = max_nan(lane_max, x[e]);
+            float mx = lane_max;
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+            if ((lane & 15) == 0) half_max[tile & 1][2 * warp + (lane >> 4)] = mx;
+            mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+            // the warp's sum; NaN and +inf carry into it and mark the row
+            if (!(mx < INFINITY)) {
+                ref = INFINITY;
+            } else if (mx > -INFINITY && ref < INFINITY) {
+                if (mx > ref + 60.0f || ref == -INFINITY) {
+                    if (sum != 0.0) sum *= exp((double)ref - (double)mx);
+                    ref = mx;
+                }
+                // e^(x - ref) as 2^((x - ref) log2 e): the argument is off by 2^-23 of its size, the power
+                // by 2^-22; the difference first, since ref may be the type's lowest value
+                float s = 0.0f;
+#pragma unroll
+                for (int e = 0; e < kBeamPerThread; ++e) s += exp2_approx((x[e] - ref) * kLog2e);
+                sum += s;
+            }
+            if (tile + 1 == tile1) {
+                double total = sum;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+                if (lane == 0) wref[warp] = ref, wsum[warp] = total;
+            }
+            __syncthreads();
+            // k groups or more of neighbouring half warps: the least of their maxima
+            uint32_t hm = ordered(half_max[tile & 1][lane]);
+            for (int o = 1; 32 / (2 * o) >= k; o <<= 1) hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, o));
+            float least = from_ordered(__reduce_min_sync(0xFFFFFFFFu, hm));
+            if (least == -INFINITY) {
+                // a short or masked row leaves groups empty: the k-th of the half warps
+                const uint32_t sorted = warp_sort(
+                    ordered(half_max[tile & 1][lane]), lane, [](uint32_t p, uint32_t q) { return p > q; },
+                    [](uint32_t p, int d) { return __shfl_xor_sync(0xFFFFFFFFu, p, d); });
+                least = from_ordered(__shfl_sync(0xFFFFFFFFu, sorted, k - 1));
+            }
+            bound = fmaxf(bound, least);
+            if (lane_max >= bound) {
+#pragma unroll
+                for (int e = 0; e < kBeamPerThread; ++e) {
+                    const int v = index(e);
+                    if (x[e] >= bound && v >= 0 && v < a.vocab) {
+                        const uint32_t at = atomicAdd(&many, 1u);
+                        if (at < kList) list[at] = make_key(x[e], (uint32_t)v);
+                    }
+                }
+            }
+            __syncthreads();
+            const int now = (int)many;
+            if (now <= kList && (tile + 1 == tile1 ? now <= kCounted : now <= kList / 2)) {
+                listed = now;
+            } else if (now <= kList) {
+                Best best;
+                best.merge(tid < now ? list[tid] : 0, lane);
+                join_warps(best);
+            } else {
+                // too many for the list: what it held before this tile, and the tile's again, by ballots
+                Best best;
+                best.merge(tid < listed ? list[tid] : 0, lane);
+                uint64_t* pending = sm.s.pending[warp];
+                uint64_t kth = 0;  // the warp's k-th best
+                int pend = 0;
+                auto flush = [&]() {
+                    __syncwarp();
+                    best.merge(lane < pend ? pending[lane] : 0, lane);
+                    const uint64_t rest = lane + 32 < pend ? pending[lane + 32] : 0;
+                    __syncwarp();
+                    pending[lane] = rest;
+                    pend = max(0, pend - 32);
+                    kth = __shfl_sync(0xFFFFFFFFu, best.top, k - 1);
+                };
+#pragma unroll
+                for (int e = 0; e < kBeamPerThread; ++e) {
+                    const int v = index(e);
+                    uint64_t key = 0;
+                    if (x[e] >= bound && v >= 0 && v < a.vocab) key = make_key(x[e], (uint32_t)v);
+                    const uint32_t vote = __ballot_sync(0xFFFFFFFFu, key > kth);
+                    if (vote == 0) continue;
+                    if (key > kth) pending[pend + __popc(vote & ((1u << lane) - 1u))] = key;
+                    pend += __popc(vote);
+                    if (pend >= 32) flush();
+                }
+                while (pend > 0) flush();
+                join_warps(best);
             }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-        float sum = 0.0f;
-        if (mx > -INFINITY) {
-#pragma unroll
-            for (int e = 0; e < kBeamPerThread; ++e) sum += expf(x[e] - mx);
+        if (tile1 <= tile0) {  // the row ends before this chunk
+            if (lane == 0) wref[warp] = -INFINITY, wsum[warp] = 0.0;
+            __syncthreads();
         }
-        double total = sum;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
-        const uint64_t sorted = warp_sort(
-            best, lane, [](uint64_t p, uint64_t q) { return p > q; },
-            [](uint64_t p, int d) { return __shfl_xor_sync(0xFFFFFFFFu, p, d); });
-        const uint64_t mine = __shfl_sync(0xFFFFFFFFu, sorted, k - 1);
-        if (__any_sync(0xFFFFFFFFu, bad)) mx = INFINITY;  // marks the row
-        if (lane == 0) wmax[warp] = mx, wsum[warp] = total, bound[warp] = mine;
-        __syncthreads();
-        uint64_t T0 = 1;  // every element's key is above 0, the key of no element
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) T0 = bound[w] > T0 ? bound[w] : T0;
-#pragma unroll
-        for (int e = 0; e < kBeamPerThread; ++e) {
-            const int v = base[e / VEC] + e % VEC;
-            if (v < 0 || v >= a.vocab) continue;
-            const uint64_t key = make_key(x[e], (uint32_t)v);
-            if (key >= T0) list[atomicAdd(&many, 1u)] = key;
-        }
-        __syncthreads();
-        const int n = (int)many;
+        // the k best of the list: a key's rank is the number of larger ones
         uint64_t* out = a.part_keys + part * a.key_stride;
-        for (int q = tid; q < n; q += kBeamThreads) {
-            const uint64_t key = list[q];
+        if (tid < listed) {
+            const uint64_t key = list[tid];
             int rank = 0;
-            for (int j = 0; j < n; ++j) rank += list[j] > key;
+            for (int j = 0; j < listed; ++j) rank += list[j] > key;
             if (rank < k) out[rank] = key;
+        } else if (tid < k) {
+            out[tid] = 0;  // a chunk of fewer elements
         }
-        for (int q = n + tid; q < k; q += kBeamThreads) out[q] = 0;  // a chunk of fewer elements
-        if (tid == 0) {
-            float m = wmax[0];
-            for (int w = 1; w < kWarps; ++w) m = fmaxf(m, wmax[w]);
-            double s = 0.0;
-            if (m > -INFINITY && m < INFINITY)
-                for (int w = 0; w < kWarps; ++w)
-                    if (wmax[w] > -INFINITY) s += wsum[w] * exp((double)wmax[w] - (double)m);
-            a.part_max[part] = m;
-            a.part_sum[part] = s;
+        if (warp == kWarps - 1) {
+            const float m = lane < kWarps ? wref[lane] : -INFINITY;
+            float top = m;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            double s = m > -INFINITY && top < INFINITY ? wsum[lane] * exp((double)m - (double)top) : 0.0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+            if (lane == 0) a.part_max[part] = top, a.part_sum[part] = s;
         }
     }
     __threadfence();
@@ -251,22 +383,21 @@ __global__ void __launch_bounds__(kBeamThreads) select_kernel(BeamArgs a) {
         const Cand c = candidate(l, 0);
         if (better(c, best)) best = c;
     }
-    const Cand sorted = warp_sort(best, lane, better, shuffle);
-    if (lane == k - 1) limit[warp] = sorted;
+    if (warp * 32 < lists) best = warp_sort(best, lane, better, shuffle);
+    if (lane == k - 1) limit[warp] = best;
     __syncthreads();
     Cand L = limit[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w)
         if (better(limit[w], L)) L = limit[w];
-    Cand* cands = reinterpret_cast<Cand*>(list);
-    constexpr int kRoom = (int)(sizeof(list) / sizeof(Cand));
-    for (int l = tid; l < lists; l += kBeamThreads)
-        for (int j = 0; j < k; ++j) {
-            const Cand c = candidate(l, j);
-            if (c.at == 0x7FFFFFFF || better(L, c)) break;
-            const uint32_t at = atomicAdd(&many, 1u);
-            if (at < kRoom) cands[at] = c;
-        }
+    Cand* cands = sm.cands;
+#pragma unroll 4
+    for (int q = tid; q < lists * k; q += kBeamThreads) {
+        const Cand c = candidate(q / k, q % k);
+        if (c.at == 0x7FFFFFFF || better(L, c)) continue;
+        const uint32_t at = atomicAdd(&many, 1u);
+        if (at < kRoom) cands[at] = c;
+    }
     __syncthreads();
     const int n = (int)many;
     if (n <= kRoom) {

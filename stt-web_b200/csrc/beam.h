@@ -10,14 +10,16 @@
 namespace stt {
 
 constexpr int kMaxBeams = 32;
-constexpr int kBeamThreads = 256;
+constexpr int kBeamThreads = 512;
 constexpr int kBeamPerThread = 16;                            // logits of a thread
-constexpr int kBeamChunk = kBeamThreads * kBeamPerThread;     // logits of a CTA
+constexpr int kBeamChunk = kBeamThreads * kBeamPerThread;     // logits of a CTA's tile
+constexpr int kBeamMaxChunks = 16;                            // CTAs of a row
 
 struct BeamArgs {
     const void* logits;   // [batch * beams][vocab], rows row_stride elements apart
     int64_t row_stride;
-    int32_t batch, beams, vocab, chunks;
+    int32_t batch, beams, vocab;
+    int32_t chunks, tiles_per_chunk;  // CTAs of a row, tiles of a CTA
     const float* scores;  // [batch][beams]
     const uint8_t* done;  // [batch][beams] or NULL
     int32_t eos;          // -1: none

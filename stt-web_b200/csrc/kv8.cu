@@ -27,6 +27,16 @@ __device__ __forceinline__ void store_codes(int8_t* p, uint32_t w) {
     else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w;
 }
 
+// rint(x * f) of N values, as bytes: f is a power of two and |x * f| <= 127.5.
+template <int N>
+__device__ __forceinline__ uint32_t pack_codes(const float (&x)[N], float f) {
+    uint32_t u[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) u[j] = __float_as_uint(__fmaf_rn(x[j], f, 12582912.0f));
+    if constexpr (N == 4) return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+    else return __byte_perm(u[0], u[1], 0x0040);
+}
+
 // Raises the error word where a sequence comes twice in one append: its two rows would write the
 // same blocks.  One warp per batch row looks at the rows before it.
 __device__ __forceinline__ void check_repeated(const Kv8Dev& c, const Kv8Batch& b, int i, int seq, int lane) {
@@ -38,25 +48,27 @@ __device__ __forceinline__ void check_repeated(const Kv8Dev& c, const Kv8Batch& 
 
 // One warp per (block, K or V, head) of a batch row: every new token of the block is loaded once
 // (32 lanes x dim / 32 elements, all rows in flight together), the maximum goes through shuffles,
-// and a token's codes leave as one row of `dim` bytes.  Heads are the innermost index, so that
-// neighbouring warps read neighbouring pieces of a token.
-template <int D, int DT>
-__global__ void __launch_bounds__(kThreads) append_kernel(Kv8Dev c, Kv8Batch b, const typename Elem<DT>::T* __restrict__ k,
-                                                          const typename Elem<DT>::T* __restrict__ v, Kv8Strides s, int nb) {
+// and a token's codes leave as one row of `dim` bytes.  A CTA's warps take neighbouring heads, so that
+// they read neighbouring pieces of a token.  MAX is the most new tokens of a block: 1 for calls of one
+// token, whose warps then need a third of the registers.
+//
+// The maximum is taken over the bit patterns of |x| (they order like the values; anything from
+// 0x7F800000 on is not finite and sends the warp through the checked conversion below), and a code is
+// the low byte of x * 2^-e + 1.5 * 2^23, whose unit is 1: the addition rounds to nearest, ties to even.
+template <int D, int DT, int MAX>
+__global__ void __launch_bounds__(kThreads, MAX == 1 ? 6 : 2) append_kernel(Kv8Dev c, Kv8Batch b, const typename Elem<DT>::T* __restrict__ k,
+                                                          const typename Elem<DT>::T* __restrict__ v, Kv8Strides s, int nb,
+                                                          int ctas_per_block) {
     constexpr int N = D / 32;
     const int lane = threadIdx.x & 31;
-    int64_t task = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    const int h = (int)(task % c.heads);
-    task /= c.heads;
-    const int kv = (int)(task & 1);
-    task >>= 1;
-    const int blk = (int)(task % nb);
-    task /= nb;
-    if (task >= b.n) return;
-    const int i = (int)task;
+    const int rest = blockIdx.x / ctas_per_block;
+    const int task = (blockIdx.x - rest * ctas_per_block) * (kThreads / 32) + (threadIdx.x >> 5);
+    if (task >= 2 * c.heads) return;
+    const int kv = task >= c.heads, h = task - kv * c.heads;
+    const int i = rest / nb, blk = rest - i * nb;
     Kv8Row r;
     if (!kv8_row(c, b, i, &r)) return;
-    if (h == 0 && kv == 0 && blk == 0) check_repeated(c, b, i, r.seq, lane);
+    if (task == 0 && blk == 0) check_repeated(c, b, i, r.seq, lane);
     if (r.count > 0 && (r.pos + r.count - 1) / kKv8Block - r.pos / kKv8Block >= c.cap / kKv8Block) {
         if (lane == 0) atomicCAS(c.err, 0, -1);  // the call's tokens would overwrite one another in the ring
         return;
@@ -70,79 +82,108 @@ __global__ void __launch_bounds__(kThreads) append_kernel(Kv8Dev c, Kv8Batch b, 
     int8_t* exps = (kv ? c.ve : c.ke) + head * (c.cap / kKv8Block) + slot / kKv8Block;
     const typename Elem<DT>::T* src = (kv ? v : k) + i * s.seq + (int64_t)(lo - r.pos) * s.token + h * s.head + lane * N;
     const int old = lo - p0, many = hi - lo;
+    float x[MAX][N];
+    // (a block with fewer tokens loads its last one again: no branch keeps the loads apart)
+#pragma unroll
+    for (int t = 0; t < MAX; ++t) load_elems<DT, N>(src + min(t, many - 1) * s.token, x[t]);
     const int was = old ? *exps : kKv8MinExp;
-    float x[kKv8Block][N];
+    uint32_t amax = 0;
 #pragma unroll
-    for (int t = 0; t < kKv8Block; ++t)
-        if (t < many) load_elems<DT, N>(src + t * s.token, x[t]);
-    float amax = 0.0f;
-    bool finite = true;
+    for (int t = 0; t < MAX; ++t)
 #pragma unroll
-    for (int t = 0; t < kKv8Block; ++t)
-        if (t < many) {
+        for (int j = 0; j < N; ++j) amax = max(amax, __float_as_uint(x[t][j]) & 0x7FFFFFFFu);
+    amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+    int e;
+    float f;
+    if (amax >= 0x7F800000u) {
+        // infinities or NaN: the exponent of the finite values; infinities become +-127 steps, NaN 0
+        if (lane == 0) atomicCAS(c.err, 0, -5);  // STT_E_DEVICE_FLAG
+        amax = 0;
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const float a = fabsf(x[t][e]);
-                if (a < __int_as_float(0x7F800000)) amax = fmaxf(amax, a);
-                else finite = false;
+        for (int t = 0; t < MAX; ++t)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const uint32_t u = __float_as_uint(x[t][j]) & 0x7FFFFFFFu;
+                if (u < 0x7F800000u) amax = max(amax, u);
             }
-        }
+        amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+        e = max(was, kv8_exponent(__uint_as_float(amax)));
+        const float inv = pow2i(-e);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-    if (!__all_sync(0xFFFFFFFFu, finite) && lane == 0) atomicCAS(c.err, 0, -5);  // STT_E_DEVICE_FLAG
-    const int e = max(was, kv8_exponent(amax));
-    const float inv = pow2i(-e);
+        for (int t = 0; t < MAX; ++t)
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[t][j] = x[t][j] != x[t][j] ? 0.0f : fminf(fmaxf(x[t][j] * inv, -127.0f), 127.0f);
+        f = 1.0f;
+    } else {
+        e = max(was, kv8_exponent(__uint_as_float(amax)));
+        f = pow2i(-e);
+    }
     if (old && e > was) {
         const float shift = pow2i(was - e);
+#pragma unroll 4
         for (int t = 0; t < old; ++t) {
-            int8_t* row = codes + t * D;
-            const uint32_t q = load_codes<N>(row);
-            uint32_t w = 0;
+            const uint32_t q = load_codes<N>(codes + t * D);
+            float y[N];
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                w |= (uint32_t)(__float2int_rn((float)(int8_t)(q >> (8 * j)) * shift) & 0xFF) << (8 * j);
-            store_codes<N>(row, w);
+            for (int j = 0; j < N; ++j) y[j] = (float)(int8_t)(q >> (8 * j));
+            store_codes<N>(codes + t * D, pack_codes<N>(y, shift));
         }
     }
 #pragma unroll
-    for (int t = 0; t < kKv8Block; ++t)
-        if (t < many) {
-            uint32_t w = 0;
-#pragma unroll
-            for (int j = 0; j < N; ++j) w |= (uint32_t)(kv8_code(x[t][j], inv) & 0xFF) << (8 * j);
-            store_codes<N>(codes + (old + t) * D, w);
-        }
+    for (int t = 0; t < MAX; ++t)
+        if (t < many) store_codes<N>(codes + (old + t) * D, pack_codes<N>(x[t], f));
     if (lane == 0 && (e != was || !old)) *exps = (int8_t)e;
 }
 
-// Values of a range of tokens.  A thread turns 8 codes into 8 values.
+constexpr int kReadTokens = 16;  // of a CTA
+
+// Values of a range of tokens.  A thread keeps its place in a token (as many codes as fill 16 bytes of
+// values, in K and in V) and walks over the tokens, several in flight.  A code becomes a value in two
+// instructions: the byte code + 128 under 0x4B0000 is the f32 value 2^23 + 128 + code, and
+// (2^23 + 128 + code) * step - (2^23 + 128) * step is exact in one fused multiply-add.
 template <int D, int DT>
 __global__ void __launch_bounds__(kThreads) read_kernel(Kv8Dev c, Kv8Batch b, void* __restrict__ k, void* __restrict__ v,
-                                                        Kv8Strides s) {
-    int64_t item = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    const int piece = (int)(item % (D / 8));
-    item /= D / 8;
-    const int h = (int)(item % c.heads);
-    item /= c.heads;
-    const int t = (int)(item % b.tokens);
-    item /= b.tokens;
-    if (item >= b.n) return;
-    const int i = (int)item;
+                                                        Kv8Strides s, int token_ctas, int head_ctas) {
+    constexpr int N = 16 / (int)sizeof(typename Elem<DT>::T);
+    const int part = blockIdx.x / head_ctas, item = (blockIdx.x - part * head_ctas) * kThreads + threadIdx.x;
+    const int i = part / token_ctas, t0 = (part - i * token_ctas) * kReadTokens;
+    const int piece = item % (D / N), h = item / (D / N);
     Kv8Row r;
-    if (!kv8_row(c, b, i, &r) || t >= r.count) return;
-    const int slot = (r.pos + t) % c.cap;
+    if (!kv8_row(c, b, i, &r) || h >= c.heads) return;
+    const int t1 = min(t0 + kReadTokens, r.count);
     const int64_t head = (int64_t)r.seq * c.heads + h;
-    const int64_t at = i * s.seq + t * s.token + h * s.head + piece * 8;
-    const int64_t ce = head * (c.cap / kKv8Block) + slot / kKv8Block, cc = (head * c.cap + slot) * D + piece * 8;
+    const int8_t *kc = c.kc + head * c.cap * D + piece * N, *vc = c.vc + head * c.cap * D + piece * N;
+    const int8_t *ke = c.ke + head * (c.cap / kKv8Block), *ve = c.ve + head * (c.cap / kKv8Block);
+    const int64_t at0 = i * s.seq + h * s.head + piece * N;
+    int slot = t0 < t1 ? (r.pos + t0) % c.cap : 0;
+#pragma unroll 4
+    for (int t = t0; t < t1; ++t) {
+        uint32_t q[2][N / 4];
+        float step[2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const float step = pow2i((half ? c.ve : c.ke)[ce]);
-        const char4* q = reinterpret_cast<const char4*>((half ? c.vc : c.kc) + cc);
-        void* out = half ? v : k;
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const char4 w = q[j];
-            store4<DT>(out, at + 4 * j, make_float4(w.x * step, w.y * step, w.z * step, w.w * step));
+            for (int j = 0; j < N / 4; ++j)
+                q[half][j] = __ldg(reinterpret_cast<const uint32_t*>((half ? vc : kc) + (int64_t)slot * D) + j);
+            step[half] = pow2i(__ldg((half ? ve : ke) + slot / kKv8Block));
+        }
+        if (++slot == c.cap) slot = 0;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const float bias = -8388736.0f * step[half];
+            float y[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                y[j] = fmaf(__uint_as_float(__byte_perm(q[half][j / 4] ^ 0x80808080u, 0x4B000000u, 0x7650 | (j % 4))), step[half], bias);
+            void* out = half ? v : k;
+            const int64_t at = at0 + t * s.token;
+            if constexpr (DT == DT_F32) {
+                *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = make_float4(y[0], y[1], y[2], y[3]);
+            } else {
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) =
+                    make_uint4(pack2(y[0], y[1], Elem<DT>()), pack2(y[2], y[3], Elem<DT>()), pack2(y[4], y[5], Elem<DT>()),
+                               pack2(y[6], y[7], Elem<DT>()));
+            }
         }
     }
 }
@@ -151,17 +192,21 @@ template <int D, int DT>
 cudaError_t append_t(const Kv8Dev& c, const Kv8Batch& b, const void* k, const void* v, const Kv8Strides& s,
                      cudaStream_t st) {
     using T = typename Elem<DT>::T;
+    const T *kt = static_cast<const T*>(k), *vt = static_cast<const T*>(v);
     const int nb = (b.tokens + 2 * kKv8Block - 2) / kKv8Block;  // blocks that `tokens` tokens can touch
-    const int64_t tasks = (int64_t)b.n * nb * 2 * c.heads;
-    const int64_t ctas = (tasks + kThreads / 32 - 1) / (kThreads / 32);
-    append_kernel<D, DT><<<(unsigned)ctas, kThreads, 0, st>>>(c, b, static_cast<const T*>(k), static_cast<const T*>(v), s, nb);
+    const int per_block = (2 * c.heads + kThreads / 32 - 1) / (kThreads / 32);
+    const unsigned grid = (unsigned)((int64_t)b.n * nb * per_block);
+    if (b.tokens == 1) append_kernel<D, DT, 1><<<grid, kThreads, 0, st>>>(c, b, kt, vt, s, nb, per_block);
+    else append_kernel<D, DT, kKv8Block><<<grid, kThreads, 0, st>>>(c, b, kt, vt, s, nb, per_block);
     return cudaGetLastError();
 }
 
 template <int D, int DT>
 cudaError_t read_t(const Kv8Dev& c, const Kv8Batch& b, void* k, void* v, const Kv8Strides& s, cudaStream_t st) {
-    const int64_t items = (int64_t)b.n * b.tokens * c.heads * (D / 8);
-    read_kernel<D, DT><<<(unsigned)((items + kThreads - 1) / kThreads), kThreads, 0, st>>>(c, b, k, v, s);
+    const int token_ctas = (b.tokens + kReadTokens - 1) / kReadTokens;
+    const int head_ctas = (c.heads * (D * (int)sizeof(typename Elem<DT>::T) / 16) + kThreads - 1) / kThreads;
+    read_kernel<D, DT><<<(unsigned)((int64_t)b.n * token_ctas * head_ctas), kThreads, 0, st>>>(c, b, k, v, s, token_ctas,
+                                                                                              head_ctas);
     return cudaGetLastError();
 }
 

@@ -19,13 +19,6 @@ __device__ __forceinline__ int kv8_exponent(float amax) {
     return max(kKv8MinExp, e);
 }
 
-// Code of x in a block of exponent e: to nearest, ties to even.  Infinities take the largest code of
-// their sign and NaN takes 0 (the caller raises the error word for both).
-__device__ __forceinline__ int kv8_code(float x, float inv) {
-    const int q = __float2int_rn(x * inv);
-    return x != x ? 0 : max(-127, min(127, q));
-}
-
 // Row i of the batch.  false (and the error word raised) where its entries are out of range.
 struct Kv8Row {
     int seq, pos, count;

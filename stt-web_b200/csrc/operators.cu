@@ -22,7 +22,7 @@ struct stt_kv8_cache {
 };
 
 struct stt_beam {
-    int device = 0;
+    int device = 0, num_sms = 0;
     int max_batch = 0, max_beams = 0, max_vocab = 0;
     void* scratch = nullptr;
     int32_t* err = nullptr;
@@ -33,7 +33,9 @@ namespace {
 
 int elem_bytes(int dtype) { return dtype == DT_F32 ? 4 : 2; }
 
-int beam_chunks(int vocab) { return (vocab + 7 + kBeamChunk - 1) / kBeamChunk; }  // a row may start 7 elements into its first vector
+// Tiles of a row, which may start 7 elements into its first vector, and the most CTAs that share them.
+int beam_tiles(int vocab) { return (vocab + 7 + kBeamChunk - 1) / kBeamChunk; }
+int beam_max_chunks(int vocab) { return std::min(kBeamMaxChunks, beam_tiles(vocab)); }
 
 // n_seqs * heads * capacity * dim and the sizes derived from it; false if the arguments do not make a cache.
 bool kv8_sizes(int n_seqs, int heads, int dim, int cap, size_t* codes, size_t* exps) {
@@ -167,7 +169,7 @@ extern "C" int stt_kv8_append_device(stt_kv8_cache* h, const int32_t* d_seqs, in
     const Kv8Strides s{seq_stride, token_stride, head_stride};
     TRY(check_rows("K", d_k, dtype, s));
     TRY(check_rows("V", d_v, dtype, s));
-    if ((int64_t)n * h->c.heads * (n_tokens / kKv8Block + 2) * 2 > INT_MAX)
+    if ((int64_t)n * (n_tokens / kKv8Block + 2) > INT_MAX / (h->c.heads + 8))
         return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", n, n_tokens);
     DeviceScope ds(h->device);
     if (!ds.ok) return set_error(STT_E_CUDA, "cudaSetDevice(%d) failed", h->device);
@@ -186,7 +188,7 @@ extern "C" int stt_kv8_read_device(const stt_kv8_cache* h, const int32_t* d_seqs
     const Kv8Strides s{seq_stride, token_stride, head_stride};
     TRY(check_rows("K", d_k, dtype, s));
     TRY(check_rows("V", d_v, dtype, s));
-    if ((int64_t)n * h->c.heads > INT_MAX / n_tokens)
+    if ((int64_t)n * (n_tokens / 16 + 1) > INT_MAX / (h->c.heads / 8 + 1))
         return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", n, n_tokens);
     DeviceScope ds(h->device);
     if (!ds.ok) return set_error(STT_E_CUDA, "cudaSetDevice(%d) failed", h->device);
@@ -274,7 +276,7 @@ extern "C" int stt_beam_create(int device, int max_batch, int max_beams, int max
     if (max_batch <= 0 || max_beams <= 0 || max_beams > kMaxBeams || max_vocab <= 0)
         return set_error(STT_E_INVALID_ARG, "no selection of %d utterances, %d beams (1..%d), %d tokens", max_batch, max_beams,
                          kMaxBeams, max_vocab);
-    if ((int64_t)max_beams * max_vocab > INT_MAX - kBeamChunk || (int64_t)max_batch * max_beams * beam_chunks(max_vocab) > INT_MAX)
+    if ((int64_t)max_beams * max_vocab > INT_MAX - kBeamChunk || (int64_t)max_batch * max_beams * beam_max_chunks(max_vocab) > INT_MAX)
         return set_error(STT_E_INVALID_ARG, "%d utterances of %d beams over %d tokens are too many", max_batch, max_beams, max_vocab);
     DeviceScope ds(device);
     if (!ds.ok) {
@@ -290,10 +292,11 @@ extern "C" int stt_beam_create(int device, int max_batch, int max_beams, int max
             if (h) stt_beam_destroy(h);
         }
     } release{h};
+    CUDA_TRY(cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, device));
     h->max_batch = max_batch;
     h->max_beams = max_beams;
     h->max_vocab = max_vocab;
-    const size_t parts = (size_t)max_batch * max_beams * beam_chunks(max_vocab);
+    const size_t parts = (size_t)max_batch * max_beams * beam_max_chunks(max_vocab);
     size_t off = 256;
     auto take = [&](size_t bytes) {
         const size_t o = off;
@@ -363,7 +366,11 @@ extern "C" int stt_beam_select_device(stt_beam* h, const void* d_logits, int dty
     a.batch = batch;
     a.beams = beams;
     a.vocab = vocab;
-    a.chunks = beam_chunks(vocab);
+    // about four CTAs per SM; a CTA takes whole tiles
+    const int tiles = beam_tiles(vocab), rows = batch * beams;
+    const int want = std::min(beam_max_chunks(vocab), (4 * h->num_sms + rows - 1) / rows);
+    a.tiles_per_chunk = (tiles + want - 1) / want;
+    a.chunks = (tiles + a.tiles_per_chunk - 1) / a.tiles_per_chunk;
     a.scores = d_scores;
     a.done = d_done;
     a.eos = eos;

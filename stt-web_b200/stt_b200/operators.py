@@ -2,7 +2,7 @@
 attention, and beam search's selection and reordering.
 
 Tensors are CUDA tensors of any library whose objects have torch's ``data_ptr()``, ``shape``,
-``stride()`` and ``dtype`` (torch itself is not imported).  Calls are queued on ``stream`` (the integer
+``stride()``, ``dtype`` and ``get_device()`` (torch itself is not imported).  Calls are queued on ``stream`` (the integer
 handle of a CUDA stream, 0 = the legacy default stream) and do not wait for the device; the tensors must
 stay alive until it has run them.
 """
@@ -14,7 +14,16 @@ from typing import Optional
 
 from ._lib import STT_E_INVALID_ARG, SttError, check, lib, stt_kv8_cache_info
 
-_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+_NAMES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2, "torch.int32": 3, "torch.uint8": 4}
+_F32, _I32, _U8 = 0, 3, 4
+_codes = {}  # the same by dtype object: these checks are a good part of a small call's time
+
+
+def _code(dtype) -> int:
+    code = _codes.get(dtype)
+    if code is None:
+        code = _codes[dtype] = _NAMES.get(str(dtype), -1)
+    return code
 
 
 def _refuse(where: str, why: str):
@@ -22,22 +31,23 @@ def _refuse(where: str, why: str):
 
 
 def _dtype(t, where: str) -> int:
-    code = _DTYPES.get(str(t.dtype))
-    if code is None:
+    code = _code(t.dtype)
+    if not 0 <= code <= 2:
         _refuse(where, f"dtype {t.dtype} unknown: f32, bf16 and f16 are")
     return code
 
 
 def _on(t, device: int, where: str):
-    if t.device.type != "cuda" or t.device.index != device:
+    if t.get_device() != device:  # -1 off the GPUs
         _refuse(where, f"a tensor is on {t.device}, the operator on cuda:{device}")
 
 
-def _whole(t, n: int, device: int, where: str, what: str, dtype: str = "torch.int32") -> int:
+def _whole(t, n: int, device: int, where: str, what: str, code: int = _I32) -> int:
     """Address of a contiguous device array of n entries."""
-    if str(t.dtype) != dtype or t.numel() != n or not t.is_contiguous():
-        _refuse(where, f"{what} must be {n} contiguous {dtype[6:]} values")
-    _on(t, device, where)
+    if _code(t.dtype) != code or t.numel() != n or not t.is_contiguous():
+        _refuse(where, f"{what} must be {n} contiguous {('f32', '', '', 'int32', 'uint8')[code]} values")
+    if t.get_device() != device:
+        _on(t, device, where)
     return t.data_ptr()
 
 
@@ -199,11 +209,11 @@ class BeamSelector:
         _on(logits, d, where)
         check(lib().stt_beam_select_device(
             self._h, logits.data_ptr(), _dtype(logits, where), stride[0] if rows > 1 else vocab, batch, beams, vocab,
-            _whole(scores, rows, d, where, "scores", "torch.float32"),
-            None if done is None else _whole(done, rows, d, where, "done", "torch.uint8"), eos,
-            _whole(next_scores, rows, d, where, "next_scores", "torch.float32"),
+            _whole(scores, rows, d, where, "scores", _F32),
+            None if done is None else _whole(done, rows, d, where, "done", _U8), eos,
+            _whole(next_scores, rows, d, where, "next_scores", _F32),
             _whole(parents, rows, d, where, "parents"), _whole(tokens, rows, d, where, "tokens"),
-            None if next_done is None else _whole(next_done, rows, d, where, "next_done", "torch.uint8"), stream), where)
+            None if next_done is None else _whole(next_done, rows, d, where, "next_done", _U8), stream), where)
 
 
 def beam_reorder(states, parents, held=None, stream: int = 0) -> None:
@@ -223,9 +233,9 @@ def beam_reorder(states, parents, held=None, stream: int = 0) -> None:
     if shape[0] != groups * beams or 0 in shape:
         _refuse(where, f"states {tuple(shape)} for {groups} x {beams} beams")
     size = states.element_size()
-    if states.device.type != "cuda":
+    d = states.get_device()
+    if d < 0:
         _refuse(where, f"the states are on {states.device}")
-    d = states.device.index
     check(lib().stt_beam_reorder_device(d, states.data_ptr(), stride[0] * size, shape[1], stride[1] * size, shape[2],
                                         inner // shape[2] * size, _whole(parents, groups * beams, d, where, "parents"),
                                         groups, beams, None if held is None else _whole(held, groups * beams, d, where, "held"),

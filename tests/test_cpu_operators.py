@@ -80,6 +80,7 @@ class FakeTensor:
         self._dense = list(self._stride) == dense
 
     def stride(self): return self._stride
+    def get_device(self): return -1 if self.device.index is None else self.device.index
     def numel(self): return int(np.prod(self.shape))
     def element_size(self): return 4 if "32" in self.dtype else 2
     def is_contiguous(self): return self._dense
