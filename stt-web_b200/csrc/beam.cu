@@ -53,6 +53,14 @@ __device__ __forceinline__ Key warp_sort(Key k, int lane, Greater greater, Shuff
     return k;
 }
 
+// How many of the n indexes the warp finds ahead: a comparison per lane, a ballot per 32.
+template <class Ahead>
+__device__ __forceinline__ int warp_rank(int n, int lane, Ahead ahead) {
+    int rank = 0;
+    for (int j0 = 0; j0 < n; j0 += 32) rank += __popc(__ballot_sync(0xFFFFFFFFu, j0 + lane < n && ahead(j0 + lane)));
+    return rank;
+}
+
 // A candidate of the whole utterance.
 struct Cand {
     double total;
@@ -105,6 +113,66 @@ constexpr int kList = 512;     // keys of the list: one per thread
 constexpr int kCounted = 96;   // up to this many are ranked by counting (4 instructions a pair); more by sorting
 static_assert(kList == kBeamThreads, "a thread loads one key of the list");
 
+struct Lists {
+    uint64_t list[kList], pending[kWarps][64], top[kWarps][32];
+};
+struct Sorted {
+    int listed;
+    float bound;
+};
+// Leaves the k best, descending, of the list's first `from` keys and (row != NULL) of the row's logits
+// from index v0 on, one tile, that reach the bound.  Rarely needed and long: kept out of the tile loop's
+// code, whose instruction fetches it would stretch (it did: 900 cycles a tile).
+template <int DT>
+__device__ __noinline__ Sorted sort_list(Lists& s, uint32_t* many, int from, const typename Elem<DT>::T* row, int v0, int vocab,
+                                         float bound, int k) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    Best best;
+    best.merge(tid < from ? s.list[tid] : 0, lane);
+    if (row) {
+        uint64_t* pending = s.pending[warp];
+        uint64_t kth = 0;  // the warp's k-th best
+        int pend = 0;
+        for (int i = 0; i < kBeamPerThread || pend > 0; ++i) {
+            if (i < kBeamPerThread) {
+                const int v = v0 + (warp * kBeamPerThread + i) * 32 + lane;
+                uint64_t key = 0;
+                if (v >= 0 && v < vocab) {
+                    const float x = to_f32<DT>(row[v]);
+                    if (x >= bound) key = make_key(x, (uint32_t)v);
+                }
+                const uint32_t vote = __ballot_sync(0xFFFFFFFFu, key > kth);
+                if (key > kth) pending[pend + __popc(vote & ((1u << lane) - 1u))] = key;
+                pend += __popc(vote);
+                if (pend < 32) continue;
+            }
+            __syncwarp();
+            best.merge(lane < pend ? pending[lane] : 0, lane);
+            const uint64_t rest = lane + 32 < pend ? pending[lane + 32] : 0;
+            __syncwarp();
+            pending[lane] = rest;
+            pend = max(0, pend - 32);
+            kth = __shfl_sync(0xFFFFFFFFu, best.top, k - 1);
+        }
+    }
+    s.top[warp][lane] = best.top;
+    for (int d = kWarps / 2; d > 0; d >>= 1) {  // a tree of merges
+        __syncthreads();
+        if (warp < d) {
+            best.merge_sorted(s.top[warp + d][lane], lane);
+            s.top[warp][lane] = best.top;
+        }
+    }
+    __syncthreads();
+    Sorted r{0, bound};
+    for (int j = 0; j < k; ++j) r.listed += s.top[0][j] != 0;
+    if (tid < k) s.list[tid] = s.top[0][tid];
+    if (r.listed == k) r.bound = fmaxf(bound, from_ordered((uint32_t)(s.top[0][k - 1] >> 32)));
+    if (tid == 0) *many = r.listed;
+    __syncthreads();
+    return r;
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
     using T = typename Elem<DT>::T;
@@ -112,9 +180,7 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
     constexpr int LOADS = kBeamPerThread / VEC;
     constexpr int kRoom = 1024;                         // candidates of an utterance that are ranked at once
     __shared__ union {
-        struct {
-            uint64_t list[kList], pending[kWarps][64], top[kWarps][32];
-        } s;
+        Lists s;
         Cand cands[kRoom];
     } sm;
     __shared__ float wref[kWarps], half_max[2][2 * kWarps];
@@ -137,52 +203,51 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
         float bound = -INFINITY;  // the chunk has at least k logits that reach it
         int listed = 0;           // keys of the list
         uint64_t* const list = sm.s.list;
-        // The list's k best, descending, from the sorted 32 best of every warp: a tree of merges.
-        auto join_warps = [&](Best best) {
-            sm.s.top[warp][lane] = best.top;
-#pragma unroll
-            for (int s = kWarps / 2; s > 0; s >>= 1) {
-                __syncthreads();
-                if (warp < s) {
-                    best.merge_sorted(sm.s.top[warp + s][lane], lane);
-                    sm.s.top[warp][lane] = best.top;
-                }
-            }
-            __syncthreads();
-            listed = 0;
-            for (int j = 0; j < k; ++j) listed += sm.s.top[0][j] != 0;
-            if (tid < k) list[tid] = sm.s.top[0][tid];
-            if (listed == k) bound = fmaxf(bound, from_ordered((uint32_t)(sm.s.top[0][k - 1] >> 32)));
-            if (tid == 0) many = listed;
-            __syncthreads();
-        };
         const int tile0 = chunk * a.tiles_per_chunk;
         const int tile1 = min(tile0 + a.tiles_per_chunk, (a.vocab + lead + kBeamChunk - 1) / kBeamChunk);
-        for (int tile = tile0; tile < tile1; ++tile) {
-            float x[kBeamPerThread];
-            const int base = tile * kBeamChunk + tid * VEC - lead;  // of vector 0; vector j is j * 512 * VEC on
-            auto index = [&](int e) { return base + e / VEC * (kBeamThreads * VEC) + e % VEC; };
-            // Vectors that lie inside the row are loaded whole, all of them before the first is used (the
-            // others read vector `inside` instead); the row's ragged ends element by element.
-            bool whole[LOADS];
+        // Vectors that lie inside the row are loaded whole and without a branch (the others read vector
+        // `inside` instead); the row's ragged ends are put in element by element.
+        auto first = [&](int tile) { return tile * kBeamChunk + tid * VEC - lead; };  // vector j is j * 512 * VEC on
+        auto whole = [&](int v0) { return v0 >= 0 && v0 + VEC <= a.vocab; };
+        auto issue = [&](int tile, uint4 (&raw)[LOADS]) {
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) {
-                const int v0 = base + j * kBeamThreads * VEC;
-                whole[j] = v0 >= 0 && v0 + VEC <= a.vocab;
-                float y[VEC];
-                if (any_whole) load_elems<DT, VEC>(row + (whole[j] ? v0 : inside), y);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) x[j * VEC + e] = whole[j] ? y[e] : -INFINITY;
+                const int v0 = first(tile) + j * kBeamThreads * VEC;
+                if (any_whole) raw[j] = __ldg(reinterpret_cast<const uint4*>(row + (whole(v0) ? v0 : inside)));
             }
+        };
+        auto unpack = [&](int tile, const uint4 (&raw)[LOADS], float (&x)[kBeamPerThread]) {
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) {
-                const int v0 = base + j * kBeamThreads * VEC;
-                if (!whole[j] && v0 + VEC > 0 && v0 < a.vocab) {
+                const int v0 = first(tile) + j * kBeamThreads * VEC;
+                const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+                const bool all = whole(v0);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    float y;
+                    if constexpr (DT == DT_F32) {
+                        y = __uint_as_float(w[e]);
+                    } else {
+                        const float2 f = unpack2(w[e / 2], Elem<DT>());
+                        y = e % 2 ? f.y : f.x;
+                    }
+                    x[j * VEC + e] = y;
+                }
+                if (!all) {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e)
-                        if (v0 + e >= 0 && v0 + e < a.vocab) x[j * VEC + e] = to_f32<DT>(row[v0 + e]);
+                        x[j * VEC + e] = v0 + e >= 0 && v0 + e < a.vocab ? to_f32<DT>(row[v0 + e]) : -INFINITY;
                 }
             }
+        };
+        uint4 raw[LOADS] = {};
+        if (tile0 < tile1) issue(tile0, raw);
+        for (int tile = tile0; tile < tile1; ++tile) {
+            float x[kBeamPerThread];
+            const int base = first(tile);
+            auto index = [&](int e) { return base + e / VEC * (kBeamThreads * VEC) + e % VEC; };
+            unpack(tile, raw, x);
+            if (tile + 1 < tile1) issue(tile + 1, raw);  // on their way while this tile is worked on
             float lane_max = x[0];
 #pragma unroll
             for (int e = 1; e < kBeamPerThread; ++e) lane_max = max_nan(lane_max, x[e]);
@@ -215,10 +280,13 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
             __syncthreads();
             // k groups or more of neighbouring half warps: the least of their maxima
             uint32_t hm = ordered(half_max[tile & 1][lane]);
-            for (int o = 1; 32 / (2 * o) >= k; o <<= 1) hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, o));
+            for (int o = 1, groups = 16; groups >= k && groups > 0; o <<= 1, groups >>= 1)
+                hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, o));
             float least = from_ordered(__reduce_min_sync(0xFFFFFFFFu, hm));
-            if (least == -INFINITY) {
-                // a short or masked row leaves groups empty: the k-th of the half warps
+            if (k > 8 || least == -INFINITY) {
+                // more groups than half of the half warps, or groups that a short or masked row leaves
+                // empty: the k-th largest of the half warps is worth the sort (at 16 beams 23 logits reach
+                // it, 54 the least of 16)
                 const uint32_t sorted = warp_sort(
                     ordered(half_max[tile & 1][lane]), lane, [](uint32_t p, uint32_t q) { return p > q; },
                     [](uint32_t p, int d) { return __shfl_xor_sync(0xFFFFFFFFu, p, d); });
@@ -226,52 +294,36 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
             }
             bound = fmaxf(bound, least);
             if (lane_max >= bound) {
+                uint32_t reach = 0;
 #pragma unroll
-                for (int e = 0; e < kBeamPerThread; ++e) {
-                    const int v = index(e);
-                    if (x[e] >= bound && v >= 0 && v < a.vocab) {
-                        const uint32_t at = atomicAdd(&many, 1u);
-                        if (at < kList) list[at] = make_key(x[e], (uint32_t)v);
-                    }
+                for (int e = 0; e < kBeamPerThread; ++e) reach |= (uint32_t)(x[e] >= bound) << e;
+                if (bound == -INFINITY) {  // the places outside the row count as -inf: not candidates
+#pragma unroll
+                    for (int e = 0; e < kBeamPerThread; ++e)
+                        if (index(e) < 0 || index(e) >= a.vocab) reach &= ~(1u << e);
+                }
+                const uint32_t mine = __popc(reach);
+                uint32_t at = mine ? atomicAdd(&many, mine) : 0;
+                if (mine == 1) {  // as a rule
+                    if (at < kList) list[at] = make_key(lane_max, (uint32_t)index(__ffs(reach) - 1));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kBeamPerThread; ++e)
+                        if (reach >> e & 1u) {
+                            if (at < kList) list[at] = make_key(x[e], (uint32_t)index(e));
+                            ++at;
+                        }
                 }
             }
             __syncthreads();
             const int now = (int)many;
-            if (now <= kList && (tile + 1 == tile1 ? now <= kCounted : now <= kList / 2)) {
+            if (now <= (tile + 1 == tile1 ? kCounted : kList / 2)) {
                 listed = now;
-            } else if (now <= kList) {
-                Best best;
-                best.merge(tid < now ? list[tid] : 0, lane);
-                join_warps(best);
             } else {
-                // too many for the list: what it held before this tile, and the tile's again, by ballots
-                Best best;
-                best.merge(tid < listed ? list[tid] : 0, lane);
-                uint64_t* pending = sm.s.pending[warp];
-                uint64_t kth = 0;  // the warp's k-th best
-                int pend = 0;
-                auto flush = [&]() {
-                    __syncwarp();
-                    best.merge(lane < pend ? pending[lane] : 0, lane);
-                    const uint64_t rest = lane + 32 < pend ? pending[lane + 32] : 0;
-                    __syncwarp();
-                    pending[lane] = rest;
-                    pend = max(0, pend - 32);
-                    kth = __shfl_sync(0xFFFFFFFFu, best.top, k - 1);
-                };
-#pragma unroll
-                for (int e = 0; e < kBeamPerThread; ++e) {
-                    const int v = index(e);
-                    uint64_t key = 0;
-                    if (x[e] >= bound && v >= 0 && v < a.vocab) key = make_key(x[e], (uint32_t)v);
-                    const uint32_t vote = __ballot_sync(0xFFFFFFFFu, key > kth);
-                    if (vote == 0) continue;
-                    if (key > kth) pending[pend + __popc(vote & ((1u << lane) - 1u))] = key;
-                    pend += __popc(vote);
-                    if (pend >= 32) flush();
-                }
-                while (pend > 0) flush();
-                join_warps(best);
+                const Sorted s = sort_list<DT>(sm.s, &many, now <= kList ? now : listed, now <= kList ? nullptr : row,
+                                               tile * kBeamChunk - lead, a.vocab, bound, k);
+                listed = s.listed;
+                bound = s.bound;
             }
         }
         if (tile1 <= tile0) {  // the row ends before this chunk
@@ -280,14 +332,12 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
         }
         // the k best of the list: a key's rank is the number of larger ones
         uint64_t* out = a.part_keys + part * a.key_stride;
-        if (tid < listed) {
-            const uint64_t key = list[tid];
-            int rank = 0;
-            for (int j = 0; j < listed; ++j) rank += list[j] > key;
-            if (rank < k) out[rank] = key;
-        } else if (tid < k) {
-            out[tid] = 0;  // a chunk of fewer elements
+        for (int q = warp; q < listed; q += kWarps) {
+            const uint64_t key = list[q];
+            const int rank = warp_rank(listed, lane, [&](int j) { return list[j] > key; });
+            if (lane == 0 && rank < k) out[rank] = key;
         }
+        if (tid >= listed && tid < k) out[tid] = 0;  // a chunk of fewer elements
         if (warp == kWarps - 1) {
             const float m = lane < kWarps ? wref[lane] : -INFINITY;
             float top = m;
@@ -299,43 +349,40 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
             if (lane == 0) a.part_max[part] = top, a.part_sum[part] = s;
         }
     }
-    __threadfence();
     __syncthreads();
-    if (tid == 0) last = atomicAdd(a.tickets + g, 1u) == (uint32_t)(a.beams * a.chunks - 1);
+    if (tid == 0) last = ticket(a.tickets + g) == (uint32_t)(a.beams * a.chunks - 1);
     __syncthreads();
     if (!last) return;
-    __threadfence();
 
     // ---- the utterance: log sums of its beams, then the best of the chunks' bests
     __shared__ double lse[kMaxBeams], score[kMaxBeams];
     __shared__ float rmax[kMaxBeams];
     __shared__ uint8_t state[kMaxBeams], over[kMaxBeams];  // state 0 live, 1 ended, 2 all candidates at -inf
     const int64_t row0 = (int64_t)g * k;
+    static_assert(kBeamMaxChunks <= 32, "a lane joins one chunk");
     for (int b = warp; b < k; b += kWarps) {
-        const int64_t p0 = (row0 + b) * a.chunks;
-        const bool end_b = a.done && a.done[row0 + b];
+        const int64_t p = (row0 + b) * a.chunks + lane;
+        const bool end_b = a.done && a.done[row0 + b], here = !end_b && lane < a.chunks;
         const float s = a.scores[row0 + b];
-        float m = -INFINITY;
-        if (!end_b)
-            for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, __ldcg(a.part_max + p0 + c));
+        const float mc = here ? __ldcg(a.part_max + p) : -INFINITY;
+        double sum = here ? __ldcg(a.part_sum + p) : 0.0;
+        float m = mc;
+        if (a.chunks > 1) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        double sum = 0.0;
-        if (!end_b && m > -INFINITY && m < INFINITY)
-            for (int c = lane; c < a.chunks; c += 32) {
-                const float mc = __ldcg(a.part_max + p0 + c);
-                if (mc > -INFINITY) sum += __ldcg(a.part_sum + p0 + c) * exp((double)mc - (double)m);
-            }
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            sum = mc > -INFINITY && m < INFINITY ? sum * exp((double)mc - (double)m) : 0.0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        }
         if (lane == 0) {
             const bool bad = !(s < INFINITY) || (!end_b && m == INFINITY);
             if (bad) atomicCAS(a.err, 0, -5);  // STT_E_DEVICE_FLAG
-            state[b] = bad || s == -INFINITY || (!end_b && m == -INFINITY) ? 2 : end_b ? 1 : 0;
+            const int st = bad || s == -INFINITY || (!end_b && m == -INFINITY) ? 2 : end_b ? 1 : 0;
+            state[b] = (uint8_t)st;
             over[b] = end_b;
             score[b] = s;
             rmax[b] = m;
-            lse[b] = log(sum);
+            if (st == 0) lse[b] = log(sum);
         }
     }
     if (tid == 0) many = 0;
@@ -373,25 +420,23 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
         a.tokens[o] = token;
         if (a.next_done) a.next_done[o] = over[b] || token == a.eos;
     };
-    auto shuffle = [](const Cand& c, int d) {
-        return Cand{__shfl_xor_sync(0xFFFFFFFFu, c.total, d), __shfl_xor_sync(0xFFFFFFFFu, c.at, d)};
-    };
-    // the bound as above, from the lists' first candidates
-    __shared__ Cand limit[kWarps];
-    Cand best = kNone;
-    for (int l = tid; l < lists; l += kBeamThreads) {
-        const Cand c = candidate(l, 0);
-        if (better(c, best)) best = c;
-    }
-    if (warp * 32 < lists) best = warp_sort(best, lane, better, shuffle);
-    if (lane == k - 1) limit[warp] = best;
-    __syncthreads();
-    Cand L = limit[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w)
-        if (better(limit[w], L)) L = limit[w];
+    // Where there are many, only candidates that reach the k-th best of the lists' first ones count.
+    Cand L = kNone;
     Cand* cands = sm.cands;
-#pragma unroll 4
+    __shared__ Cand limit[kWarps];
+    if (lists >= k && lists * k > kCounted) {
+        for (int l = tid; l < lists; l += kBeamThreads) cands[l] = candidate(l, 0);
+        // (fewer than k of them may be candidates: then everything counts)
+        if (tid == 0) limit[0] = kNone;
+        __syncthreads();
+        for (int l = warp; l < lists; l += kWarps) {
+            const Cand c = cands[l];
+            if (c.at != 0x7FFFFFFF && warp_rank(lists, lane, [&](int j) { return better(cands[j], c); }) == k - 1 && lane == 0) limit[0] = c;
+        }
+        __syncthreads();
+        L = limit[0];
+        __syncthreads();
+    }
     for (int q = tid; q < lists * k; q += kBeamThreads) {
         const Cand c = candidate(q / k, q % k);
         if (c.at == 0x7FFFFFFF || better(L, c)) continue;
@@ -401,17 +446,16 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
     __syncthreads();
     const int n = (int)many;
     if (n <= kRoom) {
-        for (int q = tid; q < n; q += kBeamThreads) {
+        for (int q = warp; q < n; q += kWarps) {
             const Cand c = cands[q];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += better(cands[j], c);
-            if (rank < k) write(rank, c);
+            const int rank = warp_rank(n, lane, [&](int j) { return better(cands[j], c); });
+            if (lane == 0 && rank < k) write(rank, c);
         }
     } else {
         // more than the list holds (a bound that a few poor lists pulled down): merged best by best
         Cand prev{INFINITY, -1};
         for (int rank = 0; rank < k; ++rank) {
-            best = kNone;
+            Cand best = kNone;
             for (int l = tid; l < lists; l += kBeamThreads)
                 for (int j = 0; j < k; ++j) {
                     const Cand c = candidate(l, j);
@@ -423,7 +467,7 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
                 }
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) {
-                const Cand o = shuffle(best, d);
+                const Cand o{__shfl_xor_sync(0xFFFFFFFFu, best.total, d), __shfl_xor_sync(0xFFFFFFFFu, best.at, d)};
                 if (better(o, best)) best = o;
             }
             __syncthreads();

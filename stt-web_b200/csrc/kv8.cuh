@@ -19,6 +19,14 @@ __device__ __forceinline__ int kv8_exponent(float amax) {
     return max(kKv8MinExp, e);
 }
 
+// Takes a ticket after the CTA's writes: called by one thread behind a barrier, it releases what the
+// CTA wrote and, for the thread that comes last, acquires what the others did.
+__device__ __forceinline__ uint32_t ticket(uint32_t* counter) {
+    uint32_t before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    return before;
+}
+
 // Row i of the batch.  false (and the error word raised) where its entries are out of range.
 struct Kv8Row {
     int seq, pos, count;

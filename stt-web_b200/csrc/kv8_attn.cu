@@ -383,12 +383,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
     if (splits == 1) return;
     // the last of the item's splits merges them in split order, so the result does not depend on which
     // one that is, and leaves the ticket at zero for the next call
-    __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(a.tickets + item, 1u) == (uint32_t)(splits - 1);
+    if (threadIdx.x == 0) last = ticket(a.tickets + item) == (uint32_t)(splits - 1);
     __syncthreads();
     if (!last) return;
-    __threadfence();
     const float* parts = a.part + (int64_t)item * max_splits * STRIDE;
     for (int p = threadIdx.x; p < pieces; p += kWarps * 32) {
         const int r = p / (D / 4), piece = p % (D / 4);

@@ -366,7 +366,7 @@ extern "C" int stt_beam_select_device(stt_beam* h, const void* d_logits, int dty
     a.batch = batch;
     a.beams = beams;
     a.vocab = vocab;
-    // about four CTAs per SM; a CTA takes whole tiles
+    // about four CTAs per SM, twice what is resident (rows that ended leave gaps); a CTA takes whole tiles
     const int tiles = beam_tiles(vocab), rows = batch * beams;
     const int want = std::min(beam_max_chunks(vocab), (4 * h->num_sms + rows - 1) / rows);
     a.tiles_per_chunk = (tiles + want - 1) / want;
