@@ -25,7 +25,7 @@
 #include <cfloat>
 #include <algorithm>
 
-#include "kv8.cuh"
+#include "kv8_attn.cuh"
 
 namespace stt {
 
@@ -33,7 +33,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kStages = 4;
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWeightShift = 14;  // weights are scaled by 2^14, so that f16 keeps 2^-28 and up normal
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -48,14 +47,6 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// Bytes `sel` of biased codes (code + 128) as a pair of f16 codes.
-template <int SEL>
-__device__ __forceinline__ uint32_t codes_to_f16(uint32_t biased) {
-    uint32_t r = __byte_perm(biased, 0x64646464u, SEL);
-    const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r), __float2half2_rn(1152.0f));
-    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // x = hi + lo in f16, for two values.
@@ -99,15 +90,6 @@ __device__ __forceinline__ void load16(const void* base, int dtype, int64_t at, 
     else if (dtype == DT_BF16) load16<DT_BF16>(base, at, x);
     else load16<DT_F16>(base, at, x);
 }
-
-// Positions [lo, hi] that the query at position P sees.
-struct Sight {
-    int start, window, ring;
-    __device__ __forceinline__ int lo(int P) const {
-        int a = max(start, ring);
-        return window > 0 && P + 1 - window > a ? P + 1 - window : a;
-    }
-};
 
 // Merges the softmax states of `n` parts and returns the row's output piece: O / l * 2^(M - m).
 // State and piece of part j come from the two functions; an empty part has l = 0.
@@ -429,10 +411,12 @@ size_t kv8_partial_bytes(int dim) { return (size_t)kKv8MaxPartials * kKv8Rows * 
 cudaError_t kv8_configure() {
     cudaError_t e = cudaFuncSetAttribute(attend_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attend_smem<128>());
     if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(attend_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attend_smem<64>());
+    e = cudaFuncSetAttribute(attend_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attend_smem<64>());
+    return e != cudaSuccess ? e : kv8_configure_prompt();
 }
 
 cudaError_t launch_kv8_attention(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st) {
+    if (a.q_dtype != DT_F32 && a.out_dtype != DT_F32 && (int64_t)b.tokens * a.group >= 64) return launch_kv8_prompt(c, b, a, st);
     return c.dim == 128 ? attend_t<128>(c, b, a, st) : attend_t<64>(c, b, a, st);
 }
 

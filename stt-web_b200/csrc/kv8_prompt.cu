@@ -1,0 +1,472 @@
+// Attention over the 8-bit K/V cache for chunks of many query rows, on the 5th-generation tensor cores.
+//
+// The formula is kv8_attn.cu's.  A CTA takes up to 256 query rows of a K/V head (rows are tokens x the
+// head's group of query heads) as two tiles of 128, and walks over the keys 128 at a time:
+//   S = Q K^T   (tcgen05, f16 x f16 -> f32 in TMEM),  weights in registers,  O += P V  (P from TMEM).
+// What bounds it: per tile of 128 x 128 scores and 128 dimensions the two products take 1024 cycles of
+// the tensor cores, the 16384 exponentials 1024 cycles of the 16-per-cycle special function units; the
+// codes of K and V are turned into f16 once for both tiles.  Hence
+//  - roles per warp: 4 + 4 warps of softmax (a thread owns a row: no shuffles), 4 that turn codes into
+//    f16 operands, one that issues products, one that copies codes (bulk copies), with mbarriers
+//    between them: while one tile is in its softmax the other is on the tensor cores;
+//  - K's and V's codes go to shared memory as whole numbers, exact in f16; the blocks' exponents enter
+//    in the softmax, where they are free: a score is the accumulator times (row step * 2^e_k), the
+//    argument of the exponential takes + e_v, and so the weight is 2^(s + e_v - M) with the running
+//    maximum M of s + e_v: any spread of exponents is held.  The sum of the softmax takes the
+//    weight times 2^(E - e_v), one fused multiply-add in the place of the addition;
+//  - q is exact in f16 once its row is scaled by a power of two; weights are rounded to f16, scaled by
+//    2^6 (2^-12 of each, the outputs being 16-bit themselves);
+//  - M moves only when a score exceeds it by 8 (weights then reach 2^14, inside f16), so that O, which
+//    lives in TMEM, is rescaled a few times per row instead of at every tile.
+// Both operands of a product lie in core matrices of 8 rows x 16 bytes: a key's 8 dimensions are one
+// row of K's K-major matrix and of V's MN-major one, so both are written alike.
+// Every wait is bounded: one that gives up sets the CTA's abort word, all roles leave, the copies and
+// products in flight are waited for, and the cache's error word records it.
+#include <cfloat>
+#include <algorithm>
+
+#include "kv8_attn.cuh"
+#include "tcgen05.cuh"
+
+namespace stt {
+
+namespace {
+
+constexpr int kTile = 128;                // rows of a query tile and keys of a step
+constexpr int kStepBlocks = kTile / kKv8Block;
+constexpr int kSoftmaxWarps = 8, kDequantWarps = 4;
+constexpr int kMmaWarp = kSoftmaxWarps + kDequantWarps, kCopyWarp = kMmaWarp + 1;
+constexpr int kThreads = 32 * (kCopyWarp + 1);
+constexpr uint32_t kTmemCols = 512;       // S of both tiles, O of both tiles
+constexpr uint32_t kOCol = 256;
+constexpr int kExpSlots = 4;              // steps whose exponents are kept
+constexpr float kWeightShift = 6.0f;
+constexpr float kLazy = 8.0f;             // how far a score may exceed M
+
+template <int D>
+struct PromptSmem {
+    uint8_t q[2][kTile * D * 2];          // f16, core matrices of 8 rows x 16 bytes, D / 8 of them per 8 rows
+    uint8_t k[2][kTile * D * 2], v[2][kTile * D * 2];
+    uint8_t k_raw[kTile * D], v_raw[kTile * D];
+    float k_step[kExpSlots][kStepBlocks], v_exp[kExpSlots][kStepBlocks];
+    uint64_t q_full[2], s_full[2], p_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], e_full[kExpSlots];
+    uint64_t kr_full, kr_empty, vr_full, vr_empty, done;
+    uint32_t tmem;
+    int abort;
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 128 rows of codes to f16 in core matrices; thread r (of 128) takes row r, its 16-code pieces in an
+// order of its own, so that the 8 threads of a quarter warp read and write different banks.
+template <int D>
+__device__ __forceinline__ void dequant_rows(const uint8_t* raw, uint8_t* dst, int r) {
+    constexpr int CH = D / 16;
+    uint8_t* out = dst + (r >> 3) * (D / 8) * 128 + (r & 7) * 16;
+#pragma unroll
+    for (int s = 0; s < CH; ++s) {
+        const int c = (s + r) % CH;
+        const uint4 w = *reinterpret_cast<const uint4*>(raw + r * D + c * 16);
+        const uint32_t x[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+            *reinterpret_cast<uint4*>(out + (2 * c + half) * 128) =
+                make_uint4(codes_to_f16<0x4140>(x[2 * half]), codes_to_f16<0x4342>(x[2 * half]),
+                           codes_to_f16<0x4140>(x[2 * half + 1]), codes_to_f16<0x4342>(x[2 * half + 1]));
+    }
+}
+
+// 32 raw scores from TMEM, those outside [lo, hi] (column numbers) at -inf.
+__device__ __forceinline__ void load_scores(uint32_t taddr, bool masked, int lo, int hi, float (&x)[32]) {
+    tmem_ld32(taddr, x);
+    if (masked) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+            if (e < lo || e > hi) x[e] = -INFINITY;
+    }
+}
+
+// CTA (row block from the last to the first, batch row, head).
+template <int D, int DT>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch b, Kv8Attention a, int row_blocks) {
+    extern __shared__ __align__(128) uint8_t prompt_smem[];
+    PromptSmem<D>& sm = *reinterpret_cast<PromptSmem<D>*>(prompt_smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.x % c.heads, i = blockIdx.x / c.heads % b.n;
+    const int rb = row_blocks - 1 - blockIdx.x / c.heads / b.n;  // the later rows see more keys: they start first
+    Kv8Row row;
+    if (!kv8_row(c, b, i, &row)) return;
+    const int r0 = rb * 2 * kTile;
+    const int rows = min(2 * kTile, row.count * a.group - r0);
+    if (rows <= 0) return;
+    const int tiles = rows > kTile ? 2 : 1;
+    const int t0 = r0 / a.group, t1 = (r0 + rows - 1) / a.group;
+    Sight sight;
+    sight.start = a.start ? max(0, __ldg(a.start + i)) : 0;
+    sight.window = a.window;
+    sight.ring = (row.pos + row.count + kKv8Block - 1) / kKv8Block * kKv8Block - c.cap;
+    const int first = sight.lo(row.pos + t0), end = row.pos + t1;
+    const int kb0 = first / kKv8Block;
+    const int nb = first <= end ? end / kKv8Block - kb0 + 1 : 0;
+    const int steps = (nb + kStepBlocks - 1) / kStepBlocks;
+    const int64_t head = (int64_t)row.seq * c.heads + h;
+    const int cap_blocks = c.cap / kKv8Block;
+    volatile int* abort = &sm.abort;
+
+    if (threadIdx.x == 0) {
+        for (int j = 0; j < 2; ++j) {
+            mbar_init(&sm.q_full[j], 4);
+            mbar_init(&sm.s_full[j], 1);
+            mbar_init(&sm.p_full[j], 4);
+            mbar_init(&sm.k_full[j], kDequantWarps);
+            mbar_init(&sm.k_empty[j], 1);
+            mbar_init(&sm.v_full[j], kDequantWarps);
+            mbar_init(&sm.v_empty[j], 1);
+        }
+        for (int j = 0; j < kExpSlots; ++j) mbar_init(&sm.e_full[j], 1);
+        mbar_init(&sm.kr_full, 1);
+        mbar_init(&sm.kr_empty, kDequantWarps);
+        mbar_init(&sm.vr_full, 1);
+        mbar_init(&sm.vr_empty, kDequantWarps);
+        mbar_init(&sm.done, 1);
+        sm.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
+                     "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = sm.tmem;
+
+    if (warp == kCopyWarp) {
+        // codes of step j: at most two runs of blocks, where the ring wraps
+        int issued_k = 0, issued_v = 0;
+        const int8_t* kc = c.kc + head * c.cap * D;
+        const int8_t* vc = c.vc + head * c.cap * D;
+        for (int j = 0; j < steps; ++j) {
+            const int many = min(kStepBlocks, nb - j * kStepBlocks);
+            const int b0 = (kb0 + j * kStepBlocks) % cap_blocks;
+            const int run = min(many, cap_blocks - b0);
+            constexpr uint32_t BB = kKv8Block * D;
+            auto copy = [&](uint8_t* dst, const int8_t* src, uint64_t* full) {
+                if (elect_one()) {
+                    mbar_expect_tx(full, many * BB);
+                    bulk_g2s(dst, src + (int64_t)b0 * BB, run * BB, full);
+                    // (a ring shorter than a step: the rest starts over at its first block)
+                    if (run < many) bulk_g2s(dst + run * BB, src, (many - run) * BB, full);
+                }
+                __syncwarp();
+            };
+            if (j > 0 && !__all_sync(0xFFFFFFFFu, mbar_wait(&sm.kr_empty, (j - 1) & 1, abort, 64))) break;
+            copy(sm.k_raw, kc, &sm.kr_full);
+            issued_k = j + 1;
+            if (j > 0 && !__all_sync(0xFFFFFFFFu, mbar_wait(&sm.vr_empty, (j - 1) & 1, abort, 64))) break;
+            copy(sm.v_raw, vc, &sm.vr_full);
+            issued_v = j + 1;
+        }
+        // the last copies have landed before the CTA can exit
+        if (issued_k > 0) mbar_drain(&sm.kr_full, (issued_k - 1) & 1);
+        if (issued_v > 0) mbar_drain(&sm.vr_full, (issued_v - 1) & 1);
+    } else if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
+        const int r = threadIdx.x - kSoftmaxWarps * 32;
+        const int8_t* ke = c.ke + head * cap_blocks;
+        const int8_t* ve = c.ve + head * cap_blocks;
+        for (int j = 0; j < steps; ++j) {
+            const int st = j & 1;
+            if (warp == kSoftmaxWarps) {
+                // the slot is free: K of step j - 1 was only taken after the softmax of step j - 3 or later
+                if (lane < kStepBlocks) {
+                    const int blk = j * kStepBlocks + lane;
+                    const int at = (kb0 + blk) % cap_blocks;
+                    sm.k_step[j % kExpSlots][lane] = blk < nb ? pow2i(ke[at]) : 1.0f;
+                    sm.v_exp[j % kExpSlots][lane] = blk < nb ? (float)ve[at] : 0.0f;
+                }
+            }
+            bool ok = mbar_wait(&sm.kr_full, j & 1, abort);
+            if (ok && j >= 2) ok = mbar_wait(&sm.k_empty[st], ((j >> 1) - 1) & 1, abort);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            dequant_rows<D>(sm.k_raw, sm.k[st], r);
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.k_full[st]);
+                mbar_arrive(&sm.kr_empty);
+                if (warp == kSoftmaxWarps) mbar_arrive(&sm.e_full[j % kExpSlots]);
+            }
+            ok = mbar_wait(&sm.vr_full, j & 1, abort);
+            if (ok && j >= 2) ok = mbar_wait(&sm.v_empty[st], ((j >> 1) - 1) & 1, abort);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            dequant_rows<D>(sm.v_raw, sm.v[st], r);
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.v_full[st]);
+                mbar_arrive(&sm.vr_empty);
+            }
+        }
+    } else if (warp == kMmaWarp) {
+        constexpr uint32_t GROUP = D * 16;  // bytes of 8 rows: D / 8 core matrices
+        const uint32_t qk_desc = instr_desc_f16(kTile, kTile);
+        const uint32_t pv_desc = instr_desc_f16(kTile, D) | (1u << 16);  // V is MN-major
+        auto qk = [&](int q, int st) {
+            const uint32_t qa = smem_u32(sm.q[q]), ka = smem_u32(sm.k[st]);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+                mma_f16_ss(tmem + q * kTile, smem_desc(qa + k * 256, 128, GROUP), smem_desc(ka + k * 256, 128, GROUP), qk_desc,
+                           k > 0);
+            mma_commit(&sm.s_full[q]);
+        };
+        auto pv = [&](int q, int st, bool add) {
+            const uint32_t va = smem_u32(sm.v[st]);
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+                mma_f16_ts(tmem + kOCol + q * kTile, tmem + q * kTile + k * 8, smem_desc(va + k * 2 * GROUP, GROUP, 128), pv_desc,
+                           add || k > 0);
+        };
+        bool ok = steps > 0;
+        for (int q = 0; ok && q < tiles; ++q) ok = mbar_wait(&sm.q_full[q], 0, abort);
+        if (ok) ok = mbar_wait(&sm.k_full[0], 0, abort);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (ok) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (elect_one()) {
+                for (int q = 0; q < tiles; ++q) qk(q, 0);
+                mma_commit(&sm.k_empty[0]);
+            }
+            __syncwarp();
+        }
+        for (int j = 0; ok && j < steps; ++j) {
+            const int st = j & 1, nx = (j + 1) & 1;
+            const bool more = j + 1 < steps;
+            ok = mbar_wait(&sm.v_full[st], (j >> 1) & 1, abort);
+            if (ok && more) ok = mbar_wait(&sm.k_full[nx], ((j + 1) >> 1) & 1, abort);
+            for (int q = 0; ok && q < tiles; ++q) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.p_full[q], j & 1, abort));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (elect_one()) {
+                    pv(q, st, j > 0);
+                    if (more) qk(q, nx);
+                }
+                __syncwarp();
+            }
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            if (elect_one()) {
+                mma_commit(&sm.v_empty[st]);
+                if (more) mma_commit(&sm.k_empty[nx]);
+            }
+            __syncwarp();
+        }
+        if (elect_one()) mma_commit(&sm.done);  // also on abort: arrives once the products issued so far are done
+        __syncwarp();
+    } else if (warp / 4 < tiles) {
+        const int q = warp / 4, quarter = warp & 3, r = q * kTile + quarter * 32 + lane;
+        const bool live = r < rows;
+        const int tok = live ? (r0 + r) / a.group : t0, qh = h * a.group + (r0 + r) % a.group;
+        const int P = row.pos + tok;
+        const int see_lo = live ? sight.lo(P) : 0x7FFFFFFF, see_hi = live ? P : -1;
+        float q_step;
+        {
+            // the row of q: scaled to a maximum in [2^13, 2^14), which is exact, and with scale's sign
+            const typename Elem<DT>::T* src =
+                static_cast<const typename Elem<DT>::T*>(a.q) + i * a.qs.seq + (int64_t)tok * a.qs.token + qh * a.qs.head;
+            uint4 raw[D / 8];
+#pragma unroll
+            for (int e = 0; e < D / 8; ++e) raw[e] = live ? __ldg(reinterpret_cast<const uint4*>(src) + e) : make_uint4(0, 0, 0, 0);
+            float amax = 0.0f;
+#pragma unroll
+            for (int e = 0; e < D / 8; ++e) {
+                const uint32_t w[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float2 f = unpack2(w[u], Elem<DT>());
+                    amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
+            }
+            const int ex = amax > 0.0f ? (__float_as_int(amax) >> 23) - 127 - 13 : 0;
+            const float up = a.scale == 0.0f ? 0.0f : copysignf(pow2i(-ex), a.scale);
+            q_step = pow2i(ex) * (a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e);
+            uint8_t* dst = sm.q[q] + ((quarter * 32 + lane) >> 3) * (D / 8) * 128 + (lane & 7) * 16;
+#pragma unroll
+            for (int e = 0; e < D / 8; ++e) {
+                const uint32_t w[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
+                uint32_t o[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float2 f = unpack2(w[u], Elem<DT>());
+                    o[u] = pack_f16(f.x * up, f.y * up);
+                }
+                *reinterpret_cast<uint4*>(dst + e * 128) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.q_full[q]);
+        }
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t s_col = lane_base + q * kTile, o_col = lane_base + kOCol + q * kTile;
+        // the tile's rows see all of [all_lo, all_hi]
+        const int tt0 = (r0 + q * kTile) / a.group, tt1 = (r0 + min(rows, (q + 1) * kTile) - 1) / a.group;
+        const int all_lo = sight.lo(row.pos + tt1), all_hi = row.pos + tt0;
+        // the softmax's sum is held over 2^E; any E near the exponents of V serves
+        const float E = steps > 0 ? fminf(fmaxf((float)c.ve[head * cap_blocks + kb0 % cap_blocks], -60.0f), 60.0f) : 0.0f;
+        float M = -FLT_MAX, l = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < steps; ++j) {
+            ok = mbar_wait(&sm.s_full[q], j & 1, abort) && mbar_wait(&sm.e_full[j % kExpSlots], (j / kExpSlots) & 1, abort);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float* k_step = sm.k_step[j % kExpSlots];
+            const float* v_exp = sm.v_exp[j % kExpSlots];
+            const int p0 = (kb0 + j * kStepBlocks) * kKv8Block;
+            const bool masked = p0 < all_lo || p0 + kTile - 1 > all_hi;
+            const int lo = see_lo - p0, hi = see_hi - p0;  // (no overflow: see_lo <= 2^31 - 1, p0 >= 0)
+            float mx = -INFINITY;
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+                float x[32];
+                load_scores(s_col + 32 * ch, masked, lo - 32 * ch, hi - 32 * ch, x);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float bm = x[16 * u];
+#pragma unroll
+                    for (int e = 1; e < 16; ++e) bm = fmaxf(bm, x[16 * u + e]);
+                    const float step = fmaxf(q_step * k_step[2 * ch + u], 1e-37f);
+                    mx = fmaxf(mx, fmaf(bm, step, v_exp[2 * ch + u]));
+                }
+            }
+            const bool grow = mx > M + kLazy;
+            if (__any_sync(0xFFFFFFFFu, grow)) {
+                const float f = grow ? exp2f(M - mx) : 1.0f;
+                if (grow) M = mx;
+                l *= f;
+                if (j > 0) {
+#pragma unroll
+                    for (int ch = 0; ch < D / 32; ++ch) {
+                        float o[32];
+                        tmem_ld32(o_col + 32 * ch, o);
+                        uint32_t w[2][16];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) w[e >> 4][e & 15] = __float_as_uint(o[e] * f);
+                        tmem_st(o_col + 32 * ch, w[0]);
+                        tmem_st(o_col + 32 * ch + 16, w[1]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+                float x[32];
+                load_scores(s_col + 32 * ch, masked, lo - 32 * ch, hi - 32 * ch, x);
+                uint32_t w[16];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float step = fmaxf(q_step * k_step[2 * ch + u], 1e-37f);
+                    const float ev = v_exp[2 * ch + u];
+                    const float add = ev + (kWeightShift - M);
+                    const float to_sum = pow2i((int)(E - ev));
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float w0 = exp2_approx(fmaf(x[16 * u + e], step, add));
+                        const float w1 = exp2_approx(fmaf(x[16 * u + e + 1], step, add));
+                        l = fmaf(w0, to_sum, l);
+                        l = fmaf(w1, to_sum, l);
+                        w[8 * u + e / 2] = pack_f16(w0, w1);
+                    }
+                }
+                tmem_st(s_col + 16 * ch, w);  // over scores that this thread has read
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.p_full[q]);
+        }
+        mbar_drain(&sm.done, 0);
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (__all_sync(0xFFFFFFFFu, ok && *abort == 0)) {
+            const float f = l == 0.0f ? 0.0f : pow2i((int)E) / l;
+            uint16_t* dst = static_cast<uint16_t*>(a.out) + i * a.os.seq + (int64_t)tok * a.os.token + qh * a.os.head;
+            const bool bf = a.out_dtype == DT_BF16;
+#pragma unroll
+            for (int ch = 0; ch < D / 32; ++ch) {
+                float o[32];
+                if (steps > 0) {
+                    tmem_ld32(o_col + 32 * ch, o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                }
+                if (live) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const float x = l == 0.0f ? 0.0f : o[e + 2 * u] * f, y = l == 0.0f ? 0.0f : o[e + 2 * u + 1] * f;
+                            w[u] = bf ? pack2(x, y, Elem<DT_BF16>()) : pack2(x, y, Elem<DT_F16>());
+                        }
+                        *reinterpret_cast<uint4*>(dst + 32 * ch + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort) atomicCAS(c.err, 0, -5);  // STT_E_DEVICE_FLAG
+    if (warp == kMmaWarp)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+// at least 120 KB, so that one CTA holds an SM and all of its tensor memory
+template <int D>
+constexpr size_t prompt_smem_bytes() {
+    return sizeof(PromptSmem<D>) > 120 * 1024 ? sizeof(PromptSmem<D>) : 120 * 1024;
+}
+static_assert(prompt_smem_bytes<128>() <= 227 * 1024, "the stages fit one SM's shared memory");
+
+template <int D, int DT>
+cudaError_t prompt_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st) {
+    const int row_blocks = (b.tokens * a.group + 2 * kTile - 1) / (2 * kTile);
+    prompt_kernel<D, DT><<<(unsigned)((int64_t)b.n * c.heads * row_blocks), kThreads, prompt_smem_bytes<D>(), st>>>(c, b, a,
+                                                                                                                 row_blocks);
+    return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t configure_t() {
+    cudaError_t e = cudaFuncSetAttribute(prompt_kernel<D, DT_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)prompt_smem_bytes<D>());
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(prompt_kernel<D, DT_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)prompt_smem_bytes<D>());
+}
+
+}  // namespace
+
+cudaError_t kv8_configure_prompt() {
+    const cudaError_t e = configure_t<128>();
+    return e != cudaSuccess ? e : configure_t<64>();
+}
+
+cudaError_t launch_kv8_prompt(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st) {
+    if (c.dim == 128) return a.q_dtype == DT_BF16 ? prompt_t<128, DT_BF16>(c, b, a, st) : prompt_t<128, DT_F16>(c, b, a, st);
+    return a.q_dtype == DT_BF16 ? prompt_t<64, DT_BF16>(c, b, a, st) : prompt_t<64, DT_F16>(c, b, a, st);
+}
+
+}  // namespace stt

@@ -54,6 +54,7 @@
 
 #include "kernels.h"
 #include "tc_layout.cuh"
+#include "tcgen05.cuh"
 
 namespace stt {
 
@@ -70,7 +71,6 @@ constexpr int kBWarp = 2 + kDqWarps;
 constexpr int kThreads = 32 * (kBWarp + 1);
 constexpr uint32_t kRNib = kTM * 128;  // raw nibble bytes per stage
 constexpr uint32_t kRSc = kTM * 16;    // raw scale bytes per stage
-constexpr uint32_t kSpin = 1u << 22;
 constexpr uint32_t kNap = 64;  // ns between polls of a wait off the critical path
 constexpr float kWUnscale = 1.0f / 1024.0f;
 
@@ -91,73 +91,6 @@ struct TcCfg {
     static constexpr int kStep = kWide ? 1 : kNarrow ? 3 : 2;  // chunks per MMA round
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-// Shared-memory matrix descriptor: K-major, no swizzle; start address, leading byte offset (the
-// next core matrix along K) and stride byte offset (the next 8-row group), in 16-byte units.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    uint64_t d = 0;
-    d |= (uint64_t)((addr >> 4) & 0x3FFFu);
-    d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
-    d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
-    d |= (uint64_t)1 << 46;  // descriptor version of the 5th-generation tensor cores
-    // base offset 0, leading-byte-offset mode 0, layout type 0 (no swizzle)
-    return d;
-}
-
-// Instruction descriptor of kind::f16: f32 accumulator, f16 A and B, both K-major, M x N.
-__host__ __device__ constexpr uint32_t instr_desc_f16(int M, int N) {
-    return (1u << 4)                     // D format: f32
-           | (0u << 7) | (0u << 10)      // A, B format: f16
-           | (0u << 15) | (0u << 16)     // A, B K-major
-           | ((uint32_t)(N >> 3) << 17)  // N / 8
-           | ((uint32_t)(M >> 4) << 24); // M / 16
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t* m, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(m)), "r"(count) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint64_t* m, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(m)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Bounded wait for the phase of parity `parity`; gives up when the CTA's abort word is set or
-// after kSpin polls (then sets it).  Waits off the critical path back off by `nap` ns between
-// polls, so that they leave the barrier unit to the MMA-issuing warp.
-__device__ __forceinline__ bool mbar_wait(uint64_t* m, uint32_t parity, volatile int* abort, uint32_t nap = 0) {
-    for (uint32_t i = 0; i < kSpin; ++i) {
-        if (mbar_try(m, parity)) return true;
-        if ((i & 63u) == 63u && *abort) return false;
-        if (nap) __nanosleep(nap);
-    }
-    *abort = 1;
-    return false;
-}
-// Bounded wait that ignores the abort word (draining copies and MMAs before exit).
-__device__ __forceinline__ void mbar_drain(uint64_t* m, uint32_t parity) {
-    for (uint32_t i = 0; i < kSpin; ++i)
-        if (mbar_try(m, parity)) return;
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* m) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(m)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* m, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(m)), "r"(bytes) : "memory");
-}
-// Bulk copy global -> this CTA's shared memory, completing `bytes` on the mbarrier (no multicast).
-__device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* m) {
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-        "l"(src), "r"(bytes), "r"(smem_u32(m))
-        : "memory");
-}
 // 2-D TMA tile load (x = innermost coordinate in elements), completing on the mbarrier (no multicast).
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* m) {
     asm volatile(
@@ -167,17 +100,6 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
         : "memory");
 }
 
-// D (+)= A * B, f16 operands, f32 accumulator in TMEM, with A read from tensor memory (row i of A
-// in TMEM lane i, two f16 per 32-bit column) and B from shared memory through its descriptor.
-__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                           uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(acc)
-        : "memory");
-}
 // Named barrier of `count` threads; bar_any also returns whether any of them passed cond.
 __device__ __forceinline__ void bar_sync_n(int id, int count) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
@@ -199,22 +121,6 @@ __device__ __forceinline__ float gated(float g, float v) {
     return __fmul_rn(__fmul_rn(g, __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-g)))), v);
 }
 
-// True in exactly one lane of the (converged) warp.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t pred;
-    asm volatile(
-        "{\n\t.reg .pred P;\n\t"
-        "elect.sync _|P, 0xFFFFFFFF;\n\t"
-        "selp.u32 %0, 1, 0, P;\n\t}"
-        : "=r"(pred));
-    return pred != 0;
-}
-// Arrives on the mbarrier once every MMA issued so far by this thread has completed.
-__device__ __forceinline__ void mma_commit(uint64_t* m) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(m))
-                 : "memory");
-}
-
 // 16 consecutive f32 columns of this thread's TMEM lane, scaled back by 2^-10.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
     uint32_t r[16];
@@ -227,16 +133,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __fmul_rn(__uint_as_float(r[i]), kWUnscale);  // exact: a power of two
-}
-
-// 16 consecutive 32-bit columns of this thread's TMEM lane (warp-collective).
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-        : "memory");
 }
 
 template <int NT>

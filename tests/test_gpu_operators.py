@@ -7,7 +7,10 @@ log2(e) (2^-24 twice), so it is off by at most (16 + 3) * 2^-23 * S; with exp2's
 two f16 parts (2^-22) a weight is off by 19 * 2^-23 * S + 4 * 2^-23, numerator and denominator together
 by twice that, plus the accumulation of the keys (at most 2^-23 per 16 keys of a warp's share, 64 such
 steps at the lengths used here) and of the merges (under 64 * 2^-24): in all
-(2 * (19 * S + 4) + 128) * 2^-23 of the largest |v|.  The output's rounding adds eps / 2 of its value."""
+(2 * (19 * S + 4) + 128) * 2^-23 of the largest |v|.  The output's rounding adds eps / 2 of its value.
+Where queries and output have 16 bits and a K/V head has 64 query rows or more, the weights of the
+numerator may be f16: 2^-12 of each (and 2^-31 of the largest below f16's normal range, at most 2^12
+keys), so at most 2^-12 + 2^-19 of the largest |v|."""
 import numpy as np
 import pytest
 
@@ -211,6 +214,8 @@ def check_attention(p, q, out, before, pos, count, seqs, scale, window=0, start=
         total = pos[i] + count[i]
         big = np.abs(p.v.values(s, range(max(0, total - p.shape[2]), max(1, total)))).max()
         tol = (2 * (19 * S + 4) + 128) * 2.0 ** -23 * big
+        if eps and q.dtype != torch.float32 and q.shape[1] * q.shape[2] // p.shape[1] >= 64:
+            tol += (2.0 ** -12 + 2.0 ** -19) * big
         assert (np.abs(got[i, :count[i]] - exp) <= tol + eps * np.abs(exp) + 2.0 ** -24 * (eps > 0)).all(), \
             (i, np.abs(got[i, :count[i]] - exp).max(), tol)
         assert torch.equal(out[i, count[i]:], before[i, count[i]:])
@@ -234,6 +239,18 @@ ATTENTION = [
     (2, 2, 128, 130, [0, 33, 100], 256, 0, [0, 7, 0], "bf16", "bf16"),
     (1, 16, 64, 100, [0, 33, 1000], 256, 77, [0, 7, 0], "f16", "f32"),
     (1, 1, 128, 200, [0, 57], 272, 0, None, "f32", "f32"),
+    # many rows of 16 bits: tiles of 128 rows and steps of 128 keys
+    (1, 1, 128, 64, [0], 64, 0, None, "bf16", "bf16"),
+    (1, 1, 64, 64, [0], 64, 0, None, "f16", "f16"),
+    (2, 1, 128, 128, [0, 1, 900], 1040, 0, None, "f16", "f16"),
+    (1, 1, 128, 300, [0, 57, 700], 1024, 0, None, "bf16", "f16"),
+    (1, 4, 64, 150, [0, 15, 333], 512, 0, None, "f16", "bf16"),
+    (2, 5, 128, 77, [3, 600, 1000], 160, 0, None, "f16", "f16"),     # rings that wrapped inside a step
+    (1, 3, 64, 40, [3, 600, 1000], 80, 0, None, "f16", "f16"),       # a ring shorter than a step
+    (1, 2, 128, 260, [0, 200, 1000], 1280, 100, None, "f16", "f16"),
+    (1, 2, 64, 260, [0, 200, 1000], 1280, 1, None, "f16", "f16"),
+    (2, 1, 128, 140, [0, 200, 500], 640, 0, [0, 330, 100], "bf16", "bf16"),
+    (1, 1, 64, 129, [0, 10], 160, 0, [200, 100], "f16", "f16"),      # no row sees anything; some rows do not
 ]
 
 
@@ -276,6 +293,12 @@ def test_attention_of_codes_in_masked_slots_and_uneven_exponents():
         out = torch.zeros(2, 1, 1, 64, device="cuda")
         p.cache.attention(q, out, i32(pos), scale=0.125)
         check_attention(p, q, out, out, pos, [1, 1], [0, 1], 0.125)
+    q = rand((2, 1, 64, 64), "f16", 10)
+    for pos in ([5, 15], [20, 32], [32, 63]):
+        for scale in (0.125, -0.25, 0.0):
+            out = torch.zeros(2, 1, 64, 64, dtype=torch.float16, device="cuda")
+            p.cache.attention(q, out, i32(pos), scale=scale)
+            check_attention(p, q, out, out, pos, [1, 1], [0, 1], scale)
 
 
 def test_attention_with_large_and_small_queries_and_nan():
@@ -286,6 +309,13 @@ def test_attention_with_large_and_small_queries_and_nan():
         out = torch.zeros(1, 1, 8, 128, device="cuda")
         p.cache.attention(q, out, i32([50]), scale=1.0)
         check_attention(p, q, out, out, [50], [1], [0], 1.0)
+    q = rand((1, 80, 3, 128), "bf16", 11)
+    q[0, 5, 1, 5], q[0, 79, 2, 7] = float("nan"), float("inf")
+    out = torch.zeros(1, 80, 3, 128, dtype=torch.bfloat16, device="cuda")
+    p = Pair(1, 1, 128, 128)
+    p.cache.attention(q, out, i32([40]))
+    assert torch.isnan(out[0, 5, 1]).all() and torch.isnan(out[0, 79, 2]).all()
+    assert int(torch.isnan(out).sum()) == 2 * 128
     q = rand((1, 2, 8, 128), "f32", 11)
     q[0, 0, 3, 5] = float("nan")
     out = torch.zeros(1, 2, 8, 128, device="cuda")
