@@ -2,11 +2,11 @@
 //
 // For query row r (a token and a query head of the K/V head h) at position P:
 //   out = sum_p softmax_p(scale * q . k_p) v_p   over   max(start, P + 1 - window, ring) <= p <= P,
-// zeros where no position is left.  In base 2: s_p = log2(e) * scale * q . k_p, and with V's block
-// exponents folded into the weights
-//   m = max s_p,  l = sum 2^(s_p - m),   M = max(s_p + e_v(p)),  O = sum 2^(s_p + e_v(p) - M) * code_p,
-//   out = O / l * 2^(M - m).
-// One pass over the codes keeps (m, l, M, O) per row and rescales them when a maximum grows.
+// zeros where no position is left.  In base 2, s_p = log2(e) * scale * q . k_p, and V's block exponents
+// are folded into the weights:
+//   w_p = 2^(s_p + e_v(p) - M),   O = sum w_p * code_p,   l = sum w_p * 2^-e_v(p),   out = O / l,
+// with M the running maximum of s_p + e_v(p).  One pass over the codes keeps (M, l, O) per row.  M moves
+// only when it falls more than 8 behind, so that O is rescaled a few times per row.
 //
 // What bounds it: a decode step reads 2 * dim bytes per position and head and does 4 * dim flops per
 // query row with them, so HBM bounds it as long as turning codes into operands costs little.  Hence
@@ -33,7 +33,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kStages = 4;
-constexpr int kWeightShift = 14;  // weights are scaled by 2^14, so that f16 keeps 2^-28 and up normal
+constexpr float kWeightShift = 7.0f;  // weights are scaled by 2^7: at most 2^15 in f16, normal down to 2^-21
+constexpr float kLazy = 8.0f;         // how far s + e_v may exceed M
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -73,7 +74,7 @@ __device__ __forceinline__ int v_piece(int r, int c) {
 
 // One row's softmax state in base 2.
 struct RowState {
-    float m, l, M;
+    float M, l;
 };
 
 template <int DT>
@@ -91,21 +92,21 @@ __device__ __forceinline__ void load16(const void* base, int dtype, int64_t at, 
     else load16<DT_F16>(base, at, x);
 }
 
-// Merges the softmax states of `n` parts and returns the row's output piece: O / l * 2^(M - m).
+// Merges the softmax states of `n` parts and returns the row's output piece O / l times 2^-M.
 // State and piece of part j come from the two functions; an empty part has l = 0.
 template <class State, class Piece>
 __device__ __forceinline__ RowState merge_parts(int n, State state, Piece piece, float4* out) {
-    RowState r{-FLT_MAX, 0.0f, -FLT_MAX};
+    RowState r{-FLT_MAX, 0.0f};
     for (int j = 0; j < n; ++j) {
         const RowState s = state(j);
-        if (s.l != 0.0f) r.m = fmaxf(r.m, s.m), r.M = fmaxf(r.M, s.M);
+        if (s.l != 0.0f) r.M = fmaxf(r.M, s.M);
     }
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int j = 0; j < n; ++j) {
         const RowState s = state(j);
         if (s.l == 0.0f) continue;
-        r.l = fmaf(s.l, exp2f(s.m - r.m), r.l);
         const float f = exp2f(s.M - r.M);
+        r.l = fmaf(s.l, f, r.l);
         const float4 p = piece(j);
         o.x = fmaf(p.x, f, o.x), o.y = fmaf(p.y, f, o.y), o.z = fmaf(p.z, f, o.z), o.w = fmaf(p.w, f, o.w);
     }
@@ -114,7 +115,7 @@ __device__ __forceinline__ RowState merge_parts(int n, State state, Piece piece,
 }
 __device__ __forceinline__ float4 row_output(const RowState& r, float4 o) {
     if (r.l == 0.0f) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const float f = exp2f(r.M - r.m - (float)kWeightShift) / r.l;
+    const float f = 1.0f / r.l;
     return make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
 }
 
@@ -127,6 +128,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
     constexpr int HALF = 16 * D;        // bytes of a staged block of K (and of V)
     constexpr int CH = D / 16;          // 16-byte pieces of a row
     constexpr int VB = D / 8;           // bytes of V that a lane takes of a key
+    constexpr int VW = VB / 4;          // in words
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ RowState sm_state[kWarps][kKv8Rows];
     __shared__ uint32_t last;
@@ -160,30 +162,46 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kStages * 2 * HALF);
     const int mine = max(0, (sb1 - sb0 - warp + kWarps - 1) / kWarps);  // blocks sb0 + warp + 4 * j
 
+    // Blocks are taken in turn from the ring; a lane copies the same 16-byte pieces of each.
+    const int8_t* ksrc = kbase + lane * 16;
+    const int8_t* vsrc = vbase + lane * 16;
+    uint32_t kdst[HALF / 512], vdst[HALF / 512];
+#pragma unroll
+    for (int u = 0; u < HALF / 512; ++u) {
+        const int p = lane + 32 * u, r = p / CH, ch = p % CH;
+        kdst[u] = ring + k_piece<D>(r, ch);
+        vdst[u] = ring + HALF + v_piece<D>(r, ch);
+    }
+    int next = (sb0 + warp) % cap_blocks;           // ring block of the next fetch
+    const int stride = kWarps % cap_blocks;
+    uint32_t stage = 0;                             // its place in the ring, in bytes
     auto fetch = [&](int j) {
         if (j < mine) {
-            const int blk = (sb0 + warp + kWarps * j) % cap_blocks;
-            const int8_t* ks = kbase + (int64_t)blk * HALF;
-            const int8_t* vs = vbase + (int64_t)blk * HALF;
-            const uint32_t dst = ring + (j % kStages) * (2 * HALF);
+            const int64_t at = (int64_t)next * HALF;
 #pragma unroll
             for (int u = 0; u < HALF / 512; ++u) {
-                const int p = lane + 32 * u, r = p / CH, ch = p % CH;
-                cp_async16(dst + k_piece<D>(r, ch), ks + p * 16);
-                cp_async16(dst + HALF + v_piece<D>(r, ch), vs + p * 16);
+                cp_async16(kdst[u] + stage, ksrc + at + 512 * u);
+                cp_async16(vdst[u] + stage, vsrc + at + 512 * u);
             }
+            next += stride;
+            if (next >= cap_blocks) next -= cap_blocks;
+            stage = stage == (kStages - 1) * 2 * HALF ? 0 : stage + 2 * HALF;
         }
         cp_async_commit();
     };
 #pragma unroll
     for (int j = 0; j < kStages - 1; ++j) fetch(j);
-    // lane j: exponents of this warp's blocks j of the current 32, K's in the high half
+    // lane j: 2^e_k, e_v and 2^-e_v of this warp's block j of the current 32
+    float blk_k = 1.0f, blk_e = 0.0f, blk_l = 1.0f;
     auto fetch_exps = [&](int j) {
-        if (j >= mine) return 0;
+        if (j >= mine) return;
         const int blk = (sb0 + warp + kWarps * j) % cap_blocks;
-        return ((int)kexp[blk] << 16) | (vexp[blk] & 0xFF);
+        const int ev = vexp[blk];
+        blk_k = pow2i(kexp[blk]);
+        blk_e = (float)ev;
+        blk_l = pow2i(-ev);
     };
-    int exps = fetch_exps(lane);
+    fetch_exps(lane);
 
     // q of row g as hi and lo parts: k step s = 4 * (half) + w holds dimensions 64 * half + 16 * t + 4 * w + 0..3
     const bool live = g < rows;
@@ -226,19 +244,21 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
     float o[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-    RowState st{-FLT_MAX, 0.0f, -FLT_MAX};
+    RowState st{-FLT_MAX, 0.0f};
     // inside every row's sight: no masking needed
     const int all_lo = sight.lo(row.pos + t1), all_hi = row.pos + t0;
 
+    uint32_t read = 0;  // place of block j in the ring, in bytes
     for (int j = 0; j < mine; ++j) {
-        if (j > 0 && j % 32 == 0) exps = fetch_exps(j + lane);
-        const int ee = __shfl_sync(0xFFFFFFFFu, exps, j % 32);
-        const float ks = q_step * pow2i(ee >> 16);
-        const float ev = (float)(int8_t)(ee & 0xFF);
+        if (j > 0 && j % 32 == 0) fetch_exps(j + lane);
+        const float ks = q_step * __shfl_sync(0xFFFFFFFFu, blk_k, j % 32);
+        const float ev = __shfl_sync(0xFFFFFFFFu, blk_e, j % 32);
+        const float to_sum = __shfl_sync(0xFFFFFFFFu, blk_l, j % 32);
         cp_async_wait<kStages - 2>();
         __syncwarp();
-        const uint8_t* kst = smem + warp * (kStages * 2 * HALF) + (j % kStages) * (2 * HALF);
+        const uint8_t* kst = smem + warp * (kStages * 2 * HALF) + read;
         const uint8_t* vst = kst + HALF;
+        read = read == (kStages - 1) * 2 * HALF ? 0 : read + 2 * HALF;
         float s[2][4];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -262,7 +282,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
             v[2 * n] = (s[n][0] + s[n][2]) * ks;
             v[2 * n + 1] = (s[n][1] + s[n][3]) * ks;
         }
-        if (p0 < all_lo || p0 + kKv8Block - 1 > all_hi || rows < kKv8Rows) {
+        if (p0 < all_lo || p0 + kKv8Block - 1 > all_hi) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int p = p0 + 8 * (e >> 1) + 2 * t + (e & 1);
@@ -271,42 +291,45 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
         }
         float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
-        // (mx = -inf leaves the maxima alone: they start at -FLT_MAX, never at -inf)
-        const float m = fmaxf(st.m, mx), M = fmaxf(st.M, mx + ev);
-        if (__any_sync(0xFFFFFFFFu, m != st.m || M != st.M)) {
-            st.l *= exp2f(st.m - m);
-            const float f = exp2f(st.M - M);
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2)) + ev;
+        // (mx = -inf leaves M alone: it starts at -FLT_MAX, never at -inf)
+        const bool grow = mx > st.M + kLazy;
+        if (__any_sync(0xFFFFFFFFu, grow)) {
+            const float f = grow ? exp2f(st.M - mx) : 1.0f;
+            if (grow) st.M = mx;
+            st.l *= f;
 #pragma unroll
             for (int n = 0; n < NT; ++n) o[n][0] *= f, o[n][1] *= f, o[n][2] *= f, o[n][3] *= f;
-            st.m = m;
-            st.M = M;
         }
         uint32_t pa[4];
         {
-            float w[4];
+            const float add = ev + (kWeightShift - st.M);
+            float w[4], sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                st.l += exp2f(v[e] - m);
-                w[e] = exp2f(v[e] + (ev + (float)kWeightShift - M));
+                w[e] = exp2_approx(v[e] + add);
+                sum += w[e];
             }
+            st.l = fmaf(sum, to_sum, st.l);
             split2(w[0], w[1], &pa[0], &pa[1]);
             split2(w[2], w[3], &pa[2], &pa[3]);
         }
         // V: keys 2t, 2t + 1, 2t + 8, 2t + 9; n tile n holds dimensions VB * g + n
 #pragma unroll
-        for (int u = 0; u < VB / 4; u += 2) {
-            uint2 r[4];
+        for (int u = 0; u < VB / 4; u += VW) {
+            uint32_t r[4][VW];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int key = 2 * t + (e & 1) + 8 * (e >> 1);
                 const int byte = VB * g + 4 * u;
-                r[e] = *reinterpret_cast<const uint2*>(vst + v_piece<D>(key, byte >> 4) + (byte & 15));
+                const uint8_t* src = vst + v_piece<D>(key, byte >> 4) + (byte & 15);
+                if constexpr (VW == 4) *reinterpret_cast<uint4*>(r[e]) = *reinterpret_cast<const uint4*>(src);
+                else *reinterpret_cast<uint2*>(r[e]) = *reinterpret_cast<const uint2*>(src);
             }
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const uint32_t A = (w ? r[0].y : r[0].x) ^ 0x80808080u, B = (w ? r[1].y : r[1].x) ^ 0x80808080u;
-                const uint32_t C = (w ? r[2].y : r[2].x) ^ 0x80808080u, E = (w ? r[3].y : r[3].x) ^ 0x80808080u;
+            for (int w = 0; w < VW; ++w) {
+                const uint32_t A = r[0][w] ^ 0x80808080u, B = r[1][w] ^ 0x80808080u;
+                const uint32_t C = r[2][w] ^ 0x80808080u, E = r[3][w] ^ 0x80808080u;
                 const uint32_t ab0 = __byte_perm(A, B, 0x5140), ab1 = __byte_perm(A, B, 0x7362);
                 const uint32_t ce0 = __byte_perm(C, E, 0x5140), ce1 = __byte_perm(C, E, 0x7362);
                 const int n = 4 * (u + w);
@@ -359,7 +382,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
             write_out(r, piece, row_output(rs, v));
         } else {
             *reinterpret_cast<float4*>(part + r * (D + 4) + 4 + 4 * piece) = v;
-            if (piece == 0) *reinterpret_cast<float4*>(part + r * (D + 4)) = make_float4(rs.m, rs.l, rs.M, 0.0f);
+            if (piece == 0) *reinterpret_cast<float4*>(part + r * (D + 4)) = make_float4(rs.M, rs.l, 0.0f, 0.0f);
         }
     }
     if (splits == 1) return;
@@ -377,7 +400,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
             splits,
             [&](int w) {
                 const float4 x = __ldcg(reinterpret_cast<const float4*>(parts + (int64_t)w * STRIDE + r * (D + 4)));
-                return RowState{x.x, x.y, x.z};
+                return RowState{x.x, x.y};
             },
             [&](int w) { return __ldcg(reinterpret_cast<const float4*>(parts + (int64_t)w * STRIDE + r * (D + 4) + 4 + 4 * piece)); },
             &v);

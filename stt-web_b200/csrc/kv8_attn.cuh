@@ -7,6 +7,11 @@ namespace stt {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 // Bytes `sel` of biased codes (code + 128) as a pair of f16 codes.
 template <int SEL>
 __device__ __forceinline__ uint32_t codes_to_f16(uint32_t biased) {
