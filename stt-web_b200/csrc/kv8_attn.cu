@@ -14,11 +14,13 @@
 //    bytes (code + 128) under the high byte 0x64 are the f16 value 1024 + 128 + code, one subtraction
 //    away, 2.5 instructions for 4 codes.  tcgen05 would want the converted tile in shared or tensor
 //    memory first, one more trip for an operand that is used by a handful of rows;
-//  - 8 query rows fill the 16 MMA rows: rows 0-7 hold the leading f16 part of q (or of the weights),
-//    rows 8-15 the rest (x = hi + lo, 22 bits), so scores and outputs keep f32 quality and a lane
-//    finds both parts of its row in one accumulator quad;
-//  - the accumulator layout of the scores is the A-operand layout of the second product, and any
-//    order of dimensions serves as long as both operands agree, so nothing is shuffled: a lane's
+//  - q and the weights are split into two f16 parts (x = hi + lo, 22 bits), so scores and outputs keep
+//    f32 quality.  Up to 8 query rows: the parts are rows 0-7 and 8-15 of the A operand, the codes the B
+//    operand, and the scores' accumulator is the layout of the second product's A operand.  Up to 4 rows
+//    (a single token of up to 4 query heads per K/V head): the other way round, the codes are the 16
+//    rows of A and the parts are columns 0-3 and 4-7 of B, which takes half the products and half the
+//    accumulators (so 4 CTAs fit an SM instead of 3), for one transposition of the weights per block;
+//  - any order of dimensions serves as long as both operands agree, so no code is shuffled: a lane's
 //    operand for K is 16 consecutive codes of one key, for V 16 consecutive codes of its 4 keys;
 //  - every warp streams its own blocks of 16 keys through a private ring in shared memory
 //    (cp.async, 16 bytes per lane), without block-wide barriers, and the 4 warps are merged at the end.
@@ -32,7 +34,11 @@ namespace stt {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStages = 4;
+// Query rows of a CTA, stages of a warp's ring, CTAs per SM.
+template <bool NARROW>
+struct Shape {
+    static constexpr int kRows = NARROW ? 4 : 8, kStages = NARROW ? 3 : 4, kCtas = NARROW ? 4 : 3;
+};
 constexpr float kWeightShift = 7.0f;  // weights are scaled by 2^7: at most 2^15 in f16, normal down to 2^-21
 constexpr float kLazy = 8.0f;         // how far s + e_v may exceed M
 
@@ -48,6 +54,13 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Transposes the 8 x 8 matrix of 16-bit elements that the warp holds two to a lane, row g columns 2t, 2t + 1.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 
 // x = hi + lo in f16, for two values.
@@ -120,17 +133,18 @@ __device__ __forceinline__ float4 row_output(const RowState& r, float4 o) {
 }
 
 // CTA ((batch row * row_groups + row group) * heads + head) * max_splits + split.
-template <int D>
-__global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Batch b, Kv8Attention a, int row_groups,
+template <int D, bool NARROW>
+__global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kernel(Kv8Dev c, Kv8Batch b, Kv8Attention a, int row_groups,
                                                                 int max_splits) {
     constexpr int KS = D / 16;          // k steps of the first product
-    constexpr int NT = D / 8;           // n tiles of the second
+    constexpr int NT = NARROW ? D / 16 : D / 8;  // tiles of 16 (8) dimensions of the second
+    constexpr int ROWS = Shape<NARROW>::kRows, kStages = Shape<NARROW>::kStages;
     constexpr int HALF = 16 * D;        // bytes of a staged block of K (and of V)
     constexpr int CH = D / 16;          // 16-byte pieces of a row
     constexpr int VB = D / 8;           // bytes of V that a lane takes of a key
     constexpr int VW = VB / 4;          // in words
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ RowState sm_state[kWarps][kKv8Rows];
+    __shared__ RowState sm_state[kWarps][ROWS];
     __shared__ uint32_t last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int split = blockIdx.x % max_splits, item = blockIdx.x / max_splits;
@@ -138,8 +152,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
     Kv8Row row;
     if (!kv8_row(c, b, i, &row)) return;
     // the group's rows: row r is token r / group, query head h * group + r % group
-    const int r0 = rg * kKv8Rows;
-    const int rows = min(kKv8Rows, row.count * a.group - r0);
+    const int r0 = rg * ROWS;
+    const int rows = min(ROWS, row.count * a.group - r0);
     if (rows <= 0) return;
     const int t0 = r0 / a.group, t1 = (r0 + rows - 1) / a.group;
     Sight sight;
@@ -203,12 +217,11 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
     };
     fetch_exps(lane);
 
-    // q of row g as hi and lo parts: k step s = 4 * (half) + w holds dimensions 64 * half + 16 * t + 4 * w + 0..3
-    const bool live = g < rows;
-    const int tok = live ? (r0 + g) / a.group : t0;
-    const int P = row.pos + tok;
-    const int see_lo = live ? sight.lo(P) : 0x7FFFFFFF, see_hi = live ? P : -1;
-    uint32_t qa[KS][4];
+    // q of row qr as hi and lo parts: k step s = 4 * (half) + w holds dimensions 64 * half + 16 * t + 4 * w + 0..3
+    const int qr = NARROW ? g & 3 : g;
+    const bool live = qr < rows;
+    const int tok = live ? (r0 + qr) / a.group : t0;
+    uint32_t qa[KS][NARROW ? 2 : 4];
     float q_step;  // scores = accumulator * q_step * 2^e_k
     {
         float x[D / 64][16];
@@ -216,7 +229,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
 #pragma unroll
         for (int hf = 0; hf < D / 64; ++hf) {
             if (live) {
-                const int qh = h * a.group + (r0 + g) % a.group;
+                const int qh = h * a.group + (r0 + qr) % a.group;
                 load16(a.q, a.q_dtype, i * a.qs.seq + (int64_t)tok * a.qs.token + qh * a.qs.head + 64 * hf + 16 * t, x[hf]);
             }
 #pragma unroll
@@ -236,22 +249,43 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 uint32_t* A = qa[4 * hf + w];
-                split2(x[hf][4 * w] * up, x[hf][4 * w + 1] * up, &A[0], &A[1]);
-                split2(x[hf][4 * w + 2] * up, x[hf][4 * w + 3] * up, &A[2], &A[3]);
+                uint32_t hi[2], lo[2];
+                split2(x[hf][4 * w] * up, x[hf][4 * w + 1] * up, &hi[0], &lo[0]);
+                split2(x[hf][4 * w + 2] * up, x[hf][4 * w + 3] * up, &hi[1], &lo[1]);
+                if constexpr (NARROW) {
+                    A[0] = g < 4 ? hi[0] : lo[0], A[1] = g < 4 ? hi[1] : lo[1];
+                } else {
+                    A[0] = hi[0], A[1] = lo[0], A[2] = hi[1], A[3] = lo[1];
+                }
             }
+    }
+    // the rows whose scores this lane sees: row g at keys 2t, 2t + 1, 2t + 8, 2t + 9, or (narrow) rows
+    // sr and sr + 1 at keys g and g + 8
+    constexpr int LR = NARROW ? 2 : 1;
+    const int sr = NARROW ? 2 * (t & 1) : g;
+    int see_lo[LR], see_hi[LR];
+    float step[LR];
+#pragma unroll
+    for (int e = 0; e < LR; ++e) {
+        const int P = row.pos + (r0 + sr + e) / a.group;
+        see_lo[e] = sr + e < rows ? sight.lo(P) : 0x7FFFFFFF;
+        see_hi[e] = sr + e < rows ? P : -1;
+        step[e] = NARROW ? __shfl_sync(0xFFFFFFFFu, q_step, 4 * (sr + e)) : q_step;
     }
 
     float o[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-    RowState st{-FLT_MAX, 0.0f};
+    RowState st[LR];
+#pragma unroll
+    for (int e = 0; e < LR; ++e) st[e] = RowState{-FLT_MAX, 0.0f};
     // inside every row's sight: no masking needed
     const int all_lo = sight.lo(row.pos + t1), all_hi = row.pos + t0;
 
     uint32_t read = 0;  // place of block j in the ring, in bytes
     for (int j = 0; j < mine; ++j) {
         if (j > 0 && j % 32 == 0) fetch_exps(j + lane);
-        const float ks = q_step * __shfl_sync(0xFFFFFFFFu, blk_k, j % 32);
+        const float k_step = __shfl_sync(0xFFFFFFFFu, blk_k, j % 32);
         const float ev = __shfl_sync(0xFFFFFFFFu, blk_e, j % 32);
         const float to_sum = __shfl_sync(0xFFFFFFFFu, blk_l, j % 32);
         cp_async_wait<kStages - 2>();
@@ -259,69 +293,108 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
         const uint8_t* kst = smem + warp * (kStages * 2 * HALF) + read;
         const uint8_t* vst = kst + HALF;
         read = read == (kStages - 1) * 2 * HALF ? 0 : read + 2 * HALF;
-        float s[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+        const int p0 = (sb0 + warp + kWarps * j) * kKv8Block;
+        // scores: v[e] of key e's and row e's of this lane
+        float v[4];
+        auto key_of = [&](int e) { return NARROW ? g + 8 * (e >> 1) : 2 * t + (e & 1) + 8 * (e >> 1); };
+        auto row_of = [](int e) { return NARROW ? e & 1 : 0; };
+        if constexpr (NARROW) {
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int hf = 0; hf < D / 64; ++hf) {
-                const uint4 kq = *reinterpret_cast<const uint4*>(kst + k_piece<D>(8 * n + g, 4 * hf + t));
-                const uint32_t w[4] = {kq.x, kq.y, kq.z, kq.w};
+                const uint4 k0 = *reinterpret_cast<const uint4*>(kst + k_piece<D>(g, 4 * hf + t));
+                const uint4 k1 = *reinterpret_cast<const uint4*>(kst + k_piece<D>(8 + g, 4 * hf + t));
+                const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const uint32_t x = w[u] ^ 0x80808080u;
-                    mma16816(s[n], qa[4 * hf + u], codes_to_f16<0x4140>(x), codes_to_f16<0x4342>(x));
+                    const uint32_t x = w0[u] ^ 0x80808080u, y = w1[u] ^ 0x80808080u;
+                    const uint32_t A[4] = {codes_to_f16<0x4140>(x), codes_to_f16<0x4140>(y), codes_to_f16<0x4342>(x),
+                                           codes_to_f16<0x4342>(y)};
+                    mma16816(s, A, qa[4 * hf + u][0], qa[4 * hf + u][1]);
                 }
             }
-        }
-        // scores of row g at keys 2t, 2t + 1 of each n tile
-        const int p0 = (sb0 + warp + kWarps * j) * kKv8Block;
-        float v[4];
+            // columns 2t, 2t + 1 are one part of rows sr, sr + 1; lane t ^ 2 holds the other
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            v[2 * n] = (s[n][0] + s[n][2]) * ks;
-            v[2 * n + 1] = (s[n][1] + s[n][3]) * ks;
+            for (int e = 0; e < 4; ++e) v[e] = (s[e] + __shfl_xor_sync(0xFFFFFFFFu, s[e], 2)) * (step[e & 1] * k_step);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int hf = 0; hf < D / 64; ++hf) {
+                    const uint4 kq = *reinterpret_cast<const uint4*>(kst + k_piece<D>(8 * n + g, 4 * hf + t));
+                    const uint32_t w[4] = {kq.x, kq.y, kq.z, kq.w};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t x = w[u] ^ 0x80808080u;
+                        mma16816(s, qa[4 * hf + u], codes_to_f16<0x4140>(x), codes_to_f16<0x4342>(x));
+                    }
+                }
+                v[2 * n] = (s[0] + s[2]) * (step[0] * k_step);
+                v[2 * n + 1] = (s[1] + s[3]) * (step[0] * k_step);
+            }
         }
         if (p0 < all_lo || p0 + kKv8Block - 1 > all_hi) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int p = p0 + 8 * (e >> 1) + 2 * t + (e & 1);
-                if (p < see_lo || p > see_hi) v[e] = -INFINITY;
+                const int p = p0 + key_of(e);
+                if (p < see_lo[row_of(e)] || p > see_hi[row_of(e)]) v[e] = -INFINITY;
             }
         }
-        float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2)) + ev;
-        // (mx = -inf leaves M alone: it starts at -FLT_MAX, never at -inf)
-        const bool grow = mx > st.M + kLazy;
+        bool grow = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) grow |= v[e] + ev > st[row_of(e)].M + kLazy;
         if (__any_sync(0xFFFFFFFFu, grow)) {
-            const float f = grow ? exp2f(st.M - mx) : 1.0f;
-            if (grow) st.M = mx;
-            st.l *= f;
+            // (a row of -inf leaves M alone: it starts at -FLT_MAX, never at -inf)
+            float f[LR];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) o[n][0] *= f, o[n][1] *= f, o[n][2] *= f, o[n][3] *= f;
-        }
-        uint32_t pa[4];
-        {
-            const float add = ev + (kWeightShift - st.M);
-            float w[4], sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                w[e] = exp2_approx(v[e] + add);
-                sum += w[e];
+            for (int e = 0; e < LR; ++e) {
+                float mx = NARROW ? fmaxf(v[e], v[2 + e]) : fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+                if constexpr (NARROW) {
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16)) + ev;
+                } else {
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2)) + ev;
+                }
+                f[e] = mx > st[e].M + kLazy ? exp2f(st[e].M - mx) : 1.0f;
+                if (mx > st[e].M + kLazy) st[e].M = mx;
+                st[e].l *= f[e];
             }
-            st.l = fmaf(sum, to_sum, st.l);
-            split2(w[0], w[1], &pa[0], &pa[1]);
-            split2(w[2], w[3], &pa[2], &pa[3]);
-        }
-        // V: keys 2t, 2t + 1, 2t + 8, 2t + 9; n tile n holds dimensions VB * g + n
 #pragma unroll
-        for (int u = 0; u < VB / 4; u += VW) {
+            for (int n = 0; n < NT; ++n) o[n][0] *= f[0], o[n][1] *= f[LR - 1], o[n][2] *= f[0], o[n][3] *= f[LR - 1];
+        }
+        uint32_t pa[NARROW ? 2 : 4];
+        {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = exp2_approx(v[e] + (ev + (kWeightShift - st[row_of(e)].M)));
+            if constexpr (NARROW) {
+                st[0].l = fmaf(w[0] + w[2], to_sum, st[0].l);
+                st[LR - 1].l = fmaf(w[1] + w[3], to_sum, st[LR - 1].l);
+            } else {
+                st[0].l = fmaf((w[0] + w[1]) + (w[2] + w[3]), to_sum, st[0].l);
+            }
+            uint32_t hi[2], lo[2];
+            split2(w[0], w[1], &hi[0], &lo[0]);
+            split2(w[2], w[3], &hi[1], &lo[1]);
+            if constexpr (NARROW) {
+                // lanes t < 2 hand on the leading parts, the others the rest: columns 0-3 and 4-7 of B
+                pa[0] = transpose8x8(t < 2 ? hi[0] : lo[0]);
+                pa[1] = transpose8x8(t < 2 ? hi[1] : lo[1]);
+            } else {
+                pa[0] = hi[0], pa[1] = lo[0], pa[2] = hi[1], pa[3] = lo[1];
+            }
+        }
+        // V: keys 2t, 2t + 1, 2t + 8, 2t + 9 of dimensions VB * g + 0 .. VB - 1: n tile n takes dimension n
+        // of each lane, or (narrow) the 16 rows of tile n dimensions 2n and 2n + 1 of each
+        {
             uint32_t r[4][VW];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int key = 2 * t + (e & 1) + 8 * (e >> 1);
-                const int byte = VB * g + 4 * u;
+                const int byte = VB * g;
                 const uint8_t* src = vst + v_piece<D>(key, byte >> 4) + (byte & 15);
                 if constexpr (VW == 4) *reinterpret_cast<uint4*>(r[e]) = *reinterpret_cast<const uint4*>(src);
                 else *reinterpret_cast<uint2*>(r[e]) = *reinterpret_cast<const uint2*>(src);
@@ -332,30 +405,58 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
                 const uint32_t C = r[2][w] ^ 0x80808080u, E = r[3][w] ^ 0x80808080u;
                 const uint32_t ab0 = __byte_perm(A, B, 0x5140), ab1 = __byte_perm(A, B, 0x7362);
                 const uint32_t ce0 = __byte_perm(C, E, 0x5140), ce1 = __byte_perm(C, E, 0x7362);
-                const int n = 4 * (u + w);
-                mma16816(o[n], pa, codes_to_f16<0x4140>(ab0), codes_to_f16<0x4140>(ce0));
-                mma16816(o[n + 1], pa, codes_to_f16<0x4342>(ab0), codes_to_f16<0x4342>(ce0));
-                mma16816(o[n + 2], pa, codes_to_f16<0x4140>(ab1), codes_to_f16<0x4140>(ce1));
-                mma16816(o[n + 3], pa, codes_to_f16<0x4342>(ab1), codes_to_f16<0x4342>(ce1));
+                const uint32_t x0 = codes_to_f16<0x4140>(ab0), x1 = codes_to_f16<0x4342>(ab0), x2 = codes_to_f16<0x4140>(ab1),
+                               x3 = codes_to_f16<0x4342>(ab1), y0 = codes_to_f16<0x4140>(ce0), y1 = codes_to_f16<0x4342>(ce0),
+                               y2 = codes_to_f16<0x4140>(ce1), y3 = codes_to_f16<0x4342>(ce1);
+                if constexpr (NARROW) {
+                    const uint32_t A0[4] = {x0, x1, y0, y1}, A1[4] = {x2, x3, y2, y3};
+                    mma16816(o[2 * w], A0, pa[0], pa[1]);
+                    mma16816(o[2 * w + 1], A1, pa[0], pa[1]);
+                } else {
+                    mma16816(o[4 * w], pa, x0, y0);
+                    mma16816(o[4 * w + 1], pa, x1, y1);
+                    mma16816(o[4 * w + 2], pa, x2, y2);
+                    mma16816(o[4 * w + 3], pa, x3, y3);
+                }
             }
         }
         __syncwarp();
         fetch(j + kStages - 1);
     }
-    // l of the row: the 4 lanes hold different keys
-    st.l += __shfl_xor_sync(0xFFFFFFFFu, st.l, 1);
-    st.l += __shfl_xor_sync(0xFFFFFFFFu, st.l, 2);
+    // the row's l: its lanes hold different keys
+#pragma unroll
+    for (int e = 0; e < LR; ++e)
+#pragma unroll
+        for (int d = NARROW ? 4 : 1; d <= (NARROW ? 16 : 2); d <<= 1) st[e].l += __shfl_xor_sync(0xFFFFFFFFu, st[e].l, d);
     cp_async_wait<0>();
     __syncthreads();
-    // warp states to shared memory.  A lane holds dimensions 2 * VB * t + 0 .. 2 * VB - 1 of its row;
-    // the 16-byte pieces are permuted so that the lanes of a quarter warp hit different banks.
-    constexpr int PL = D / 16;  // pieces per lane
+    // warp states to shared memory, the 16-byte pieces of a row permuted so that the lanes of a quarter
+    // warp hit different banks
     float4* so = reinterpret_cast<float4*>(smem);
+    constexpr int PL = NARROW ? VW : D / 16;  // pieces of a lane
     auto so_at = [&](int w, int r, int piece) {
         const int lt = piece / PL, k = piece % PL;
-        return (w * kKv8Rows + r) * (D / 4) + lt * PL + (k ^ ((lt + 4 * (r & 1)) & (PL - 1)));
+        const int turn = NARROW ? r : lt + 4 * (r & 1);
+        return (w * ROWS + r) * (D / 4) + lt * PL + (k ^ (turn & (PL - 1)));
     };
-    if (live) {
+    if constexpr (NARROW) {
+        // the two parts' sums; lanes t and t ^ 2 both have them, and write one row each: dimensions
+        // VB * g + 0 .. VB - 1
+        const int second = t >> 1, r = sr + second;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] += __shfl_xor_sync(0xFFFFFFFFu, o[n][e], 2);
+        if (r < rows) {
+#pragma unroll
+            for (int k = 0; k < PL; ++k)
+                so[so_at(warp, r, PL * g + k)] =
+                    second ? make_float4(o[2 * k][1], o[2 * k][3], o[2 * k + 1][1], o[2 * k + 1][3])
+                           : make_float4(o[2 * k][0], o[2 * k][2], o[2 * k + 1][0], o[2 * k + 1][2]);
+            if (g == 0) sm_state[warp][r] = st[second ? LR - 1 : 0];
+        }
+    } else if (live) {
+        // dimensions 2 * VB * t + 0 .. 2 * VB - 1
 #pragma unroll
         for (int k = 0; k < PL; ++k) {
             const int col = 4 * k / VB, n = 4 * k % VB;
@@ -363,7 +464,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
                 make_float4(o[n][col] + o[n][col + 2], o[n + 1][col] + o[n + 1][col + 2],
                             o[n + 2][col] + o[n + 2][col + 2], o[n + 3][col] + o[n + 3][col + 2]);
         }
-        if (t == 0) sm_state[warp][g] = st;
+        if (t == 0) sm_state[warp][g] = st[0];
     }
     __syncthreads();
     const int pieces = rows * (D / 4);
@@ -371,7 +472,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
         const int token = (r0 + r) / a.group, qh = h * a.group + (r0 + r) % a.group;
         store4(a.out, a.out_dtype, i * a.os.seq + (int64_t)token * a.os.token + qh * a.os.head + 4 * piece, v);
     };
-    constexpr int STRIDE = kKv8Rows * (D + 4);
+    constexpr int STRIDE = ROWS * (D + 4);
     float* part = a.part + (int64_t)blockIdx.x * STRIDE;
     for (int p = threadIdx.x; p < pieces; p += kWarps * 32) {
         const int r = p / (D / 4), piece = p % (D / 4);
@@ -409,22 +510,30 @@ __global__ void __launch_bounds__(kWarps * 32, 3) attend_kernel(Kv8Dev c, Kv8Bat
     if (threadIdx.x == 0) a.tickets[item] = 0u;
 }
 
-template <int D>
+template <int D, bool NARROW>
 constexpr size_t attend_smem() {
-    return (size_t)kWarps * kStages * 2 * 16 * D;
+    return (size_t)kWarps * Shape<NARROW>::kStages * 2 * 16 * D;
 }
 
-template <int D>
+template <int D, bool NARROW>
 cudaError_t attend_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st) {
-    const int row_groups = (b.tokens * a.group + kKv8Rows - 1) / kKv8Rows;
+    using S = Shape<NARROW>;
+    const int row_groups = (b.tokens * a.group + S::kRows - 1) / S::kRows;
     const int64_t items = (int64_t)b.n * c.heads * row_groups;
-    // fill the SMs' 3 CTAs twice over where there are few items; never more CTAs than partial slots,
-    // nor more splits than a full context has blocks for
+    // Where there are few items: as many splits as fill the SMs twice over without a CTA too many, no
+    // more than partial slots, nor than a full context has blocks for.
     const int context = a.window > 0 ? std::min<int64_t>((int64_t)a.window + b.tokens, c.cap) : c.cap;
-    const int64_t want = std::min<int64_t>((6 * a.num_sms + items - 1) / items, context / kKv8Block / kWarps + 1);
+    const int64_t want = std::min<int64_t>(2 * S::kCtas * a.num_sms / items, context / kKv8Block / kWarps + 1);
     const int splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, kKv8MaxPartials / items));
-    attend_kernel<D><<<(unsigned)(items * splits), kWarps * 32, attend_smem<D>(), st>>>(c, b, a, row_groups, splits);
+    attend_kernel<D, NARROW><<<(unsigned)(items * splits), kWarps * 32, attend_smem<D, NARROW>(), st>>>(c, b, a, row_groups,
+                                                                                                     splits);
     return cudaGetLastError();
+}
+
+template <int D, bool NARROW>
+cudaError_t configure_t() {
+    return cudaFuncSetAttribute(attend_kernel<D, NARROW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)attend_smem<D, NARROW>());
 }
 
 }  // namespace
@@ -432,15 +541,17 @@ cudaError_t attend_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, 
 size_t kv8_partial_bytes(int dim) { return (size_t)kKv8MaxPartials * kKv8Rows * (dim + 4) * sizeof(float); }
 
 cudaError_t kv8_configure() {
-    cudaError_t e = cudaFuncSetAttribute(attend_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attend_smem<128>());
-    if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(attend_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attend_smem<64>());
-    return e != cudaSuccess ? e : kv8_configure_prompt();
+    for (const cudaError_t e : {configure_t<128, true>(), configure_t<128, false>(), configure_t<64, true>(),
+                                configure_t<64, false>(), kv8_configure_prompt()})
+        if (e != cudaSuccess) return e;
+    return cudaSuccess;
 }
 
 cudaError_t launch_kv8_attention(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st) {
-    if (a.q_dtype != DT_F32 && a.out_dtype != DT_F32 && (int64_t)b.tokens * a.group >= 64) return launch_kv8_prompt(c, b, a, st);
-    return c.dim == 128 ? attend_t<128>(c, b, a, st) : attend_t<64>(c, b, a, st);
+    const int64_t rows = (int64_t)b.tokens * a.group;  // of a K/V head
+    if (a.q_dtype != DT_F32 && a.out_dtype != DT_F32 && rows >= 64) return launch_kv8_prompt(c, b, a, st);
+    if (rows <= Shape<true>::kRows) return c.dim == 128 ? attend_t<128, true>(c, b, a, st) : attend_t<64, true>(c, b, a, st);
+    return c.dim == 128 ? attend_t<128, false>(c, b, a, st) : attend_t<64, false>(c, b, a, st);
 }
 
 }  // namespace stt
