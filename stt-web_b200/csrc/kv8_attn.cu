@@ -34,6 +34,7 @@ namespace stt {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kMaxSplits = 256;
 // Query rows of a CTA, stages of a warp's ring, CTAs per SM.
 template <bool NARROW>
 struct Shape {
@@ -493,26 +494,68 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kern
     if (threadIdx.x == 0) last = ticket(a.tickets + item) == (uint32_t)(splits - 1);
     __syncthreads();
     if (!last) return;
+    // each row's factors first, then the pieces, with the splits shared among as many threads as a piece
+    // can have: every load is independent of the others
     const float* parts = a.part + (int64_t)item * max_splits * STRIDE;
-    for (int p = threadIdx.x; p < pieces; p += kWarps * 32) {
+    float2* factor = reinterpret_cast<float2*>(smem);                                      // [rows][splits] (M, l), then 2^(M - max)
+    float4* sums = reinterpret_cast<float4*>(smem + kMaxSplits * ROWS * sizeof(float2));   // [threads]
+    for (int p = threadIdx.x; p < rows * splits; p += kWarps * 32)
+        factor[p] = __ldcg(reinterpret_cast<const float2*>(parts + (int64_t)(p % splits) * STRIDE + p / splits * (D + 4)));
+    __syncthreads();
+    for (int r = warp; r < rows; r += kWarps) {
+        float M = -FLT_MAX, l = 0.0f;
+        for (int j = lane; j < splits; j += 32) {
+            const float2 x = factor[r * splits + j];
+            if (x.y != 0.0f) M = fmaxf(M, x.x);
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
+        for (int j = lane; j < splits; j += 32) {
+            const float2 x = factor[r * splits + j];
+            const float f = x.y != 0.0f ? exp2f(x.x - M) : 0.0f;
+            l = fmaf(x.y, f, l);
+            factor[r * splits + j].x = f;
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, d);
+        if (lane == 0) sm_state[0][r] = RowState{M, l};
+    }
+    __syncthreads();
+    constexpr int PIECES = ROWS * (D / 4);
+    constexpr int SHARE = PIECES >= kWarps * 32 ? 1 : kWarps * 32 / PIECES;  // threads of a piece
+    for (int p0 = 0; p0 < pieces; p0 += kWarps * 32 / SHARE) {
+        const int p = p0 + threadIdx.x / SHARE, part_of = threadIdx.x % SHARE;
         const int r = p / (D / 4), piece = p % (D / 4);
-        float4 v;
-        const RowState rs = merge_parts(
-            splits,
-            [&](int w) {
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(parts + (int64_t)w * STRIDE + r * (D + 4)));
-                return RowState{x.x, x.y};
-            },
-            [&](int w) { return __ldcg(reinterpret_cast<const float4*>(parts + (int64_t)w * STRIDE + r * (D + 4) + 4 + 4 * piece)); },
-            &v);
-        write_out(r, piece, row_output(rs, v));
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (p < pieces) {
+            const float* src = parts + r * (D + 4) + 4 + 4 * piece;
+#pragma unroll 8
+            for (int j = part_of; j < splits; j += SHARE) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)j * STRIDE));
+                const float f = factor[r * splits + j].x;
+                v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
+            }
+        }
+        if constexpr (SHARE > 1) {
+            sums[threadIdx.x] = v;
+            __syncthreads();
+            if (part_of == 0)
+                for (int e = 1; e < SHARE; ++e) {
+                    const float4 x = sums[threadIdx.x + e];
+                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                }
+            __syncthreads();
+        }
+        if (p < pieces && part_of == 0) write_out(r, piece, row_output(sm_state[0][r], v));
     }
     if (threadIdx.x == 0) a.tickets[item] = 0u;
 }
 
 template <int D, bool NARROW>
 constexpr size_t attend_smem() {
-    return (size_t)kWarps * Shape<NARROW>::kStages * 2 * 16 * D;
+    // the warps' rings; at the end of a split context the factors and shared sums of its merge
+    return std::max((size_t)kWarps * Shape<NARROW>::kStages * 2 * 16 * D,
+                    kMaxSplits * Shape<NARROW>::kRows * sizeof(float2) + kWarps * 32 * sizeof(float4));
 }
 
 template <int D, bool NARROW>
@@ -524,7 +567,7 @@ cudaError_t attend_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, 
     // more than partial slots, nor than a full context has blocks for.
     const int context = a.window > 0 ? std::min<int64_t>((int64_t)a.window + b.tokens, c.cap) : c.cap;
     const int64_t want = std::min<int64_t>(2 * S::kCtas * a.num_sms / items, context / kKv8Block / kWarps + 1);
-    const int splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, kKv8MaxPartials / items));
+    const int splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, kMaxSplits, kKv8MaxPartials / items}));
     attend_kernel<D, NARROW><<<(unsigned)(items * splits), kWarps * 32, attend_smem<D, NARROW>(), st>>>(c, b, a, row_groups,
                                                                                                      splits);
     return cudaGetLastError();
