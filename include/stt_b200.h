@@ -66,6 +66,9 @@ void stt_config_default(stt_config* cfg);
 /* Storage type of the KV ring on the device. */
 #define STT_KV_BF16 0   /* default: bf16 K and V (half the bytes of the reference's f32)    */
 #define STT_KV_F32 1    /* f32 K and V, the reference's own precision (model.rs:185-192)    */
+#define STT_KV_INT8 2   /* signed bytes with a power-of-two scale per 16 positions and head:
+                           half the bytes of bf16 (the 8-bit cache below; one stream alone then
+                           takes the batched kernels)                                       */
 
 typedef struct stt_model stt_model;      /* loaded weights on one device                    */
 typedef struct stt_streams stt_streams;  /* N independent streams: KV rings + step state    */
@@ -104,7 +107,7 @@ int stt_model_get_info(const stt_model* model, stt_model_info* out);
  * Streams — replaces SttModel::create_cache (model.rs:728-738) plus one SttStream::new
  * (stream.rs:53-64) per stream.  Each stream owns a ring of sliding_window + 1 K/V slots per
  * layer (model.rs:130-153) and the stream-loop state of stream.rs:20-41.
- * kv_dtype is STT_KV_BF16 or STT_KV_F32.
+ * kv_dtype is STT_KV_BF16, STT_KV_F32 or STT_KV_INT8.
  * ------------------------------------------------------------------------------------- */
 int stt_streams_create(stt_model* model, int n_streams, int kv_dtype, stt_streams** out);
 int stt_streams_destroy(stt_streams* streams);
@@ -198,6 +201,26 @@ int stt_stream_reset_async(stt_streams* streams, int stream_id, int keep_buffers
 #define STT_PRODUCTS_F16X3 0
 #define STT_PRODUCTS_F16X2 1
 int stt_streams_set_product_precision(stt_streams* streams, int precision);
+
+/* Beam search over stream sets (no counterpart in the reference, which decodes greedily).  Each of
+ * `groups` utterances holds `beams` (1..32) streams of the set, ids[g * beams + b], all distinct.
+ *
+ * stt_streams_reorder: stream ids[g * beams + b] becomes what stream ids[g * beams + parents[g * beams + b]]
+ * was, K/V ring and stream-loop state, in place.  Host arrays, 0 <= parents < beams.
+ *
+ * stt_streams_beam_frame: one frame of every utterance.  Each beam consumes the utterance's audio
+ * (groups * num_codebooks ids) and its own last text token, as stt_forward does; the selector (one of the
+ * model's device, made for at least groups, beams and vocab_size) picks the `beams` best continuations by
+ * score + log_softmax(logits), and the streams are reordered so that stream ids[g * beams + b] carries the
+ * b-th best, with the chosen token as its last text token and its frame count advanced.  scores
+ * (groups * beams floats, in and out), parents_out and tokens_out are host arrays, best first.  Begin an
+ * utterance with reset streams and scores 0, -inf, -inf, ...: its beams start alike.  Tokens of frames
+ * inside the text delay (frame_count of stt_stream_get_state below text_delay) count for the scores but
+ * are not part of the transcript. */
+int stt_streams_reorder(stt_streams* streams, const int32_t* ids, int groups, int beams, const int32_t* parents);
+typedef struct stt_beam stt_beam;
+int stt_streams_beam_frame(stt_streams* streams, stt_beam* beam, const int32_t* ids, int groups, int beams,
+                           const uint32_t* audio_tokens, float* scores, int32_t* parents_out, int32_t* tokens_out);
 
 /* Replaces SttStream::set_last_text_token (stream.rs:190-192). */
 int stt_stream_set_last_text_token(stt_streams* streams, int stream_id, uint32_t token);
@@ -337,8 +360,7 @@ int stt_kv8_reorder_device(stt_kv8_cache* cache, const int32_t* d_parents, int g
 /* ---------------------------------------------------------------------------------------
  * Beam search.  No counterpart in the reference, which decodes greedily (stream.rs:104).
  * ------------------------------------------------------------------------------------- */
-typedef struct stt_beam stt_beam;
-/* A selector with workspace for up to max_batch utterances, max_beams (1..32) beams and max_vocab
+/* A selector (stt_beam) with workspace for up to max_batch utterances, max_beams (1..32) beams and max_vocab
  * tokens.  Calls on one selector share the workspace: they must not overlap in time. */
 int stt_beam_create(int device, int max_batch, int max_beams, int max_vocab, stt_beam** out);
 int stt_beam_destroy(stt_beam* beam);

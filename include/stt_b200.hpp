@@ -55,7 +55,7 @@ struct SttConfig : stt_config {
     SttConfig() : stt_config() { stt_config_default(this); }
 };
 
-enum class KvDtype : int { Bf16 = STT_KV_BF16, F32 = STT_KV_F32 };
+enum class KvDtype : int { Bf16 = STT_KV_BF16, F32 = STT_KV_F32, Int8 = STT_KV_INT8 };
 
 namespace detail {
 struct ModelDel { void operator()(stt_model* m) const { stt_model_destroy(m); } };

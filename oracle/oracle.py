@@ -15,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "liboracle.so")
 
 KV_BF16 = 1
+KV_INT8 = 4
 GEMM_BF16 = 2
 
 

@@ -371,6 +371,7 @@ struct orc_stream {
     uint32_t flags;
     int32_t max_len;
     float *k, *v; /* [L][H][max_len][HD] */
+    int *ek, *ev; /* [L][H]: exponents of the blocks being filled (ORC_KV_INT8) */
     int32_t offset, len, write_pos;
     int32_t frame_count;
     uint32_t last_text_token;
@@ -525,6 +526,8 @@ orc_stream* orc_stream_new(const orc_model* m, uint32_t flags) {
     const size_t kv = (size_t)m->cfg.num_layers * m->H * s->max_len * m->HD;
     s->k = (float*)calloc(kv, sizeof(float));
     s->v = (float*)calloc(kv, sizeof(float));
+    s->ek = (int*)calloc((size_t)m->cfg.num_layers * m->H, sizeof(int));
+    s->ev = (int*)calloc((size_t)m->cfg.num_layers * m->H, sizeof(int));
     orc_stream_reset(s);
     return s;
 }
@@ -533,6 +536,8 @@ void orc_stream_free(orc_stream* s) {
     if (!s) return;
     free(s->k);
     free(s->v);
+    free(s->ek);
+    free(s->ev);
     free(s);
 }
 
@@ -602,6 +607,34 @@ static void rope_rotate(const orc_model* m, float* x, int32_t pos) {
 
 static float silu(float x) { return x * (1.0f / (1.0f + expf(-x))); }
 
+/* Smallest e >= -100 with amax <= 127 * 2^e. */
+static int int8_exponent(float amax) {
+    int e;
+    if (amax == 0.0f) return -100;
+    const float m = frexpf(amax, &e); /* amax = m * 2^e, 0.5 <= m < 1 */
+    e = m * 128.0f <= 127.0f ? e - 7 : e - 6;
+    return e < -100 ? -100 : e;
+}
+
+/* Position `pos` of one head of an 8-bit ring: x becomes whole multiples of 2^e, |.| <= 127, in slot
+ * pos % ML of `ring`; *exp is the exponent of the block of 16 positions that pos lies in, and the
+ * block's earlier positions are rounded again where it grows. */
+static void int8_store(float* ring, int32_t ML, int32_t HD, int32_t pos, int* exp, const float* x) {
+    float amax = 0.0f;
+    for (int d = 0; d < HD; ++d) amax = fabsf(x[d]) > amax ? fabsf(x[d]) : amax;
+    int e = int8_exponent(amax);
+    const int32_t first = pos / 16 * 16;
+    if (pos > first && *exp > e) e = *exp;
+    if (pos > first && e > *exp)
+        for (int32_t p = first; p < pos; ++p)
+            for (int d = 0; d < HD; ++d) {
+                float* v = ring + (size_t)(p % ML) * HD + d;
+                *v = ldexpf(rintf(ldexpf(*v, -e)), e);
+            }
+    *exp = e;
+    for (int d = 0; d < HD; ++d) ring[(size_t)(pos % ML) * HD + d] = ldexpf(rintf(ldexpf(x[d], -e)), e);
+}
+
 /* Attention of head h of one stream at layer l (model.rs:426-474): RoPE on q and k at the
  * stream's position, the K/V ring write at write_pos (KVCache::update, model.rs:176-222), then
  * softmax(q . k^T * scale) . v over the len + 1 valid slots (masks are no-ops at q_len == 1,
@@ -614,7 +647,11 @@ static void head_attention(orc_stream* s, int l, int h, float* qkv, float* out, 
     rope_rotate(m, k, s->offset);
     float* kd = s->k + (((size_t)l * H + h) * ML + s->write_pos) * HD;
     float* vd = s->v + (((size_t)l * H + h) * ML + s->write_pos) * HD;
-    for (int d = 0; d < HD; ++d) {
+    if (s->flags & ORC_KV_INT8) {
+        const size_t lh = (size_t)l * H + h;
+        int8_store(s->k + lh * ML * HD, ML, HD, s->offset, &s->ek[lh], k);
+        int8_store(s->v + lh * ML * HD, ML, HD, s->offset, &s->ev[lh], v);
+    } else for (int d = 0; d < HD; ++d) {
         kd[d] = (s->flags & ORC_KV_BF16) ? round_bf16(k[d]) : k[d];
         vd[d] = (s->flags & ORC_KV_BF16) ? round_bf16(v[d]) : v[d];
     }

@@ -22,6 +22,10 @@ extern "C" {
 #define ORC_GEMM_BF16 2u  /* each Q4 matmul rounds its input to bf16 and its weight          */
                           /* (nibble-8)*scale to bf16 before the f32 dot product             */
 
+#define ORC_KV_INT8 4u    /* K and V held as signed bytes with one power-of-two scale for each  */
+                          /* 16 positions and head; a block whose scale grows while it fills   */
+                          /* rounds its earlier positions again                                */
+
 typedef struct orc_config {
     int32_t num_layers, num_heads, num_codebooks, text_delay, max_seq_len, sliding_window;
     double rope_theta;

@@ -12,10 +12,12 @@
 #include <thread>
 #include <vector>
 
+#include "beam.h"
 #include "common.h"
 #include "gguf.h"
 #include "host_util.h"
 #include "kernels.h"
+#include "kv8.h"
 #include "noalloc.h"
 #include "tc_gemm.h"
 #include "mega.h"
@@ -626,7 +628,12 @@ struct stt_streams {
     stt_model* m = nullptr;
     int S = 0;
     int kv_f32 = 0;
-    void* d_kv = nullptr;
+    int kv8_cap = 0;             // slots of an 8-bit ring; 0: the rings are bf16 or f32
+    void* d_kv = nullptr;        // 8-bit: codes [layer][K|V][stream][head][slot][128], then exponents [..][slot / 16]
+    int8_t* d_exps = nullptr;
+    float* d_kv8_part = nullptr; // workspace of the 8-bit rings' attention
+    uint32_t* d_kv8_tickets = nullptr;
+    int32_t* d_pos = nullptr;    // each batch row's position in this step
     size_t kv_stream_bytes = 0;
     StreamState* d_state = nullptr;
     std::vector<StreamState> h_state;
@@ -639,8 +646,8 @@ struct stt_streams {
     float* d_tc_part = nullptr; // their K-slice partial sums
     int32_t* d_ids = nullptr;
     StepDesc* d_desc = nullptr;
-    DevBuf in_audio, in_text, out_tokens, out_logits, mega_xa;
-    HostBuf h_stage, h_tokens;
+    DevBuf in_audio, in_text, out_tokens, out_logits, mega_xa, beam_dev;
+    HostBuf h_stage, h_tokens, h_beam;
     void* d_scratch = nullptr;
     cudaStream_t stream = nullptr;
     std::map<int, cudaGraphExec_t> graphs;
@@ -694,7 +701,7 @@ Ctx make_ctx(stt_streams* s, int n) {
     c.attn_scale = m->attn_scale;
     c.pad_id = m->cfg.text_padding_id;
     c.text_delay = m->cfg.text_delay;
-    c.kv = s->d_kv;
+    c.kv = s->kv8_cap ? nullptr : s->d_kv;
     c.kv_f32 = s->kv_f32;
     c.kv_half_stride = (int64_t)m->H * m->ML * m->HD;
     c.kv_layer_stride = 2 * c.kv_half_stride;
@@ -711,12 +718,46 @@ Ctx make_ctx(stt_streams* s, int n) {
     return c;
 }
 
+// Layer l of a set of 8-bit rings.
+Kv8Dev kv8_layer(const stt_streams* s, int l) {
+    const stt_model* m = s->m;
+    const size_t codes = (size_t)s->S * m->H * s->kv8_cap * m->HD, exps = codes / m->HD / kKv8Block;
+    int8_t* c = static_cast<int8_t*>(s->d_kv) + 2 * l * codes;
+    int8_t* e = s->d_exps + 2 * l * exps;
+    return Kv8Dev{c, c + codes, e, e + exps, s->S, m->H, m->HD, s->kv8_cap, &s->d_desc->error};
+}
+
+// The step's attention over 8-bit rings: k and v of the step's buffer into the rings, then q's attention
+// over the last ML positions; for a tensor-core step (x16) its output as the next product's input too.
+int enqueue_kv8_attention(stt_streams* s, const Ctx& c, int layer, __half* x16, cudaStream_t st) {
+    const stt_model* m = s->m;
+    const Kv8Dev kv = kv8_layer(s, layer);
+    const Kv8Batch batch{s->d_ids, s->d_pos, nullptr, c.n, 1};
+    const Kv8Strides rows{3 * m->D, 3 * m->D, m->HD};
+    CUDA_TRY(launch_kv8_append(kv, batch, s->d_qkv + m->D, s->d_qkv + 2 * m->D, DT_F32, rows, st));
+    Kv8Attention a{};
+    a.q = s->d_qkv;
+    a.out = s->d_attn;
+    a.qs = rows;
+    a.os = Kv8Strides{m->D, m->D, m->HD};
+    a.group = 1;
+    a.window = m->ML;
+    a.scale = m->attn_scale;
+    a.part = s->d_kv8_part;
+    a.tickets = s->d_kv8_tickets;
+    a.num_sms = m->num_sms;
+    CUDA_TRY(launch_kv8_attention(kv, batch, a, st));
+    if (x16) CUDA_TRY(launch_tc_prep(s->d_attn, nullptr, m->D, c.n, x16, st));
+    return STT_OK;
+}
+
 // Enqueues one decode step for batch size n on stream st.
 int enqueue_step(stt_streams* s, int n, cudaStream_t st) {
     stt_model* m = s->m;
     const Ctx c = make_ctx(s, n);
     const int grid = 2 * m->num_sms;
     CUDA_TRY(launch_embed(c, st));
+    if (s->kv8_cap) CUDA_TRY(launch_positions(c, s->d_pos, st));
     // batches of kTcMinBatch streams or more: layer products on the tensor cores, each product's
     // epilogue writing the next one's f16 input tiles
     if (n >= kTcMinBatch && m->tc_ok && std::getenv("STT_DISABLE_TC") == nullptr) {
@@ -737,7 +778,8 @@ int enqueue_step(stt_streams* s, int n, cudaStream_t st) {
             GemvArgs a{};
             a.W = L.qkv; a.out = s->d_qkv; a.ldo = 3 * m->D; a.layer = l; a.n_units = 3 * m->D / 2;
             CUDA_TRY(launch_tc_epilogue(c, a, EPI_QKV, n, part, slices, st));
-            CUDA_TRY(launch_attention(ca, l, st));
+            if (s->kv8_cap) TRY(enqueue_kv8_attention(s, c, l, s->d_x16, st));
+            else CUDA_TRY(launch_attention(ca, l, st));
             CUDA_TRY(launch_tc_product(m->tc_w[4 * l + 1], s->d_x16, n, part, err, m->num_sms, &slices, st, x_lo));
             CUDA_TRY(launch_tc_resid_norm(s->d_x, part, slices, n, m->D, L.norm2, s->d_x16, st));
             if (gate_fused) {  // the gate in linear_in's epilogue, its output in the second input buffer
@@ -765,7 +807,8 @@ int enqueue_step(stt_streams* s, int n, cudaStream_t st) {
         a.W = L.qkv; a.in = s->d_x; a.norm = L.norm1; a.out = s->d_qkv; a.ldo = 3 * m->D; a.layer = l;
         a.n_units = 3 * m->D / 2; a.maps = &gm[4 * l + 0];
         CUDA_TRY(launch_gemv(c, a, EPI_QKV, n, st));
-        CUDA_TRY(launch_attention(c, l, st));
+        if (s->kv8_cap) TRY(enqueue_kv8_attention(s, c, l, nullptr, st));
+        else CUDA_TRY(launch_attention(c, l, st));
         a = GemvArgs{};
         a.W = L.out; a.in = s->d_attn; a.out = s->d_x; a.ldo = m->D; a.n_units = m->D / 2; a.maps = &gm[4 * l + 1];
         CUDA_TRY(launch_gemv(c, a, EPI_RESID, n, st));
@@ -873,7 +916,8 @@ int run_steps(stt_streams* s, const int32_t* ids, int n, int steps, const uint32
     init.desc = StepDesc{d_audio, d_text, d_tokens, d_logits, 0, mode, 0, 0};
     init.n = n;
     std::memcpy(init.ids, ids, sizeof(int32_t) * n);
-    const bool use_mega = n == 1 && mega_supported(m->L, m->D, m->F, m->HD, m->V, m->num_sms, m->ML, s->kv_f32);
+    // (the persistent kernel reads bf16 and f32 rings)
+    const bool use_mega = n == 1 && !s->kv8_cap && mega_supported(m->L, m->D, m->F, m->HD, m->V, m->num_sms, m->ML, s->kv_f32);
     cudaGraphExec_t exec = nullptr;
     if (!use_mega) TRY(graph_for(s, n, &exec));
     CUDA_TRY(launch_set_desc(s->d_desc, s->d_ids, init, st));
@@ -949,7 +993,8 @@ int run_host(stt_streams* s, const int32_t* ids, int n, int steps, const uint32_
 extern "C" int stt_streams_create(stt_model* m, int n_streams, int kv_dtype, stt_streams** out) {
     clear_error();
     if (!m || !out || n_streams <= 0) return set_error(STT_E_INVALID_ARG, "bad arguments");
-    if (kv_dtype != STT_KV_BF16 && kv_dtype != STT_KV_F32) return set_error(STT_E_INVALID_ARG, "kv_dtype must be 0 or 1");
+    if (kv_dtype != STT_KV_BF16 && kv_dtype != STT_KV_F32 && kv_dtype != STT_KV_INT8)
+        return set_error(STT_E_INVALID_ARG, "kv_dtype must be 0, 1 or 2");
     *out = nullptr;
     DeviceScope ds(m->device);
     auto s = std::make_unique<stt_streams>();
@@ -958,6 +1003,15 @@ extern "C" int stt_streams_create(stt_model* m, int n_streams, int kv_dtype, stt
     s->kv_f32 = kv_dtype == STT_KV_F32;
     const size_t elem = s->kv_f32 ? 4 : 2;
     s->kv_stream_bytes = (size_t)m->L * 2 * m->H * m->ML * m->HD * elem;
+    size_t kv_codes = 0;  // bytes of all streams' codes of 8-bit rings
+    if (kv_dtype == STT_KV_INT8) {
+        if (m->HD != 128) return set_error(STT_E_INVALID_ARG, "8-bit K/V rings need head_dim 128, got %d", m->HD);
+        // the block that a position begins anew must hold nothing that the window still sees
+        s->kv8_cap = (m->ML + 2 * kKv8Block - 2) / kKv8Block * kKv8Block;
+        const size_t slots = (size_t)m->L * 2 * m->H * s->kv8_cap;
+        kv_codes = slots * m->HD * n_streams;
+        s->kv_stream_bytes = slots * m->HD + slots / kKv8Block;
+    }
     int max_np = 0;
     for (int n = 1; n <= n_streams; ++n) max_np = std::max(max_np, n * nsplit_for(m, n));
     const size_t S = (size_t)n_streams;
@@ -987,6 +1041,9 @@ extern "C" int stt_streams_create(stt_model* m, int n_streams, int kv_dtype, stt
     const size_t o_x16 = take(x16_bytes);
     const size_t o_x16b = take(m->tc_gate_ok ? x16_bytes : 0);
     const size_t o_tc_part = take(tc_part_bytes_max);
+    const size_t o_pos = take(S * 4);
+    const size_t o_kv8_tickets = take(s->kv8_cap ? kKv8MaxPartials * sizeof(uint32_t) : 0);
+    const size_t o_kv8_part = take(s->kv8_cap ? kv8_partial_bytes(m->HD) : 0);
     const size_t o_trace_ctas = take((size_t)m->num_sms * kTraceSlots * sizeof(unsigned long long));
     if (dev_alloc(&s->d_scratch, off) != cudaSuccess) {
         cudaGetLastError();
@@ -1024,6 +1081,13 @@ extern "C" int stt_streams_create(stt_model* m, int n_streams, int kv_dtype, stt
     s->d_tc_part = reinterpret_cast<float*>(b + o_tc_part);
     s->mega.trace_ctas = reinterpret_cast<unsigned long long*>(b + o_trace_ctas);
     s->mega.trace_slots = kTraceSlots;
+    s->d_pos = reinterpret_cast<int32_t*>(b + o_pos);
+    s->d_kv8_tickets = reinterpret_cast<uint32_t*>(b + o_kv8_tickets);
+    s->d_kv8_part = reinterpret_cast<float*>(b + o_kv8_part);
+    if (s->kv8_cap) {
+        s->d_exps = static_cast<int8_t*>(s->d_kv) + kv_codes;
+        CUDA_TRY(kv8_configure());
+    }
     CUDA_TRY(cudaMemset(s->d_scratch, 0, off));
     CUDA_TRY(cudaMemset(s->d_kv, 0, s->kv_stream_bytes * S));
     s->h_state.assign(S, fresh_state(m));
@@ -1056,6 +1120,8 @@ extern "C" int stt_streams_destroy(stt_streams* s) {
         s->mega_xa.release();
         s->h_stage.release();
         s->h_tokens.release();
+        s->beam_dev.release();
+        s->h_beam.release();
     }
     delete s;
     return STT_OK;
@@ -1251,6 +1317,20 @@ extern "C" int stt_stream_flush(stt_streams* s, int stream_id, uint32_t* tokens_
     return STT_OK;
 }
 
+namespace {
+int zero_rings(stt_streams* s, int stream_id, cudaStream_t st) {
+    if (!s->kv8_cap) {
+        CUDA_TRY(cudaMemsetAsync(static_cast<uint8_t*>(s->d_kv) + s->kv_stream_bytes * stream_id, 0, s->kv_stream_bytes, st));
+        return STT_OK;
+    }
+    // a stream's codes and exponents lie once in every layer's K and V
+    const size_t codes = (size_t)s->m->H * s->kv8_cap * s->m->HD, exps = codes / s->m->HD / kKv8Block;
+    CUDA_TRY(cudaMemset2DAsync(static_cast<uint8_t*>(s->d_kv) + codes * stream_id, codes * s->S, 0, codes, 2 * s->m->L, st));
+    CUDA_TRY(cudaMemset2DAsync(s->d_exps + exps * stream_id, exps * s->S, 0, exps, 2 * s->m->L, st));
+    return STT_OK;
+}
+}  // namespace
+
 extern "C" int stt_stream_reset(stt_streams* s, int stream_id, int keep_buffers) {
     clear_error();
     if (!s || stream_id < 0 || stream_id >= s->S) return set_error(STT_E_INVALID_ARG, "bad stream id");
@@ -1259,9 +1339,7 @@ extern "C" int stt_stream_reset(stt_streams* s, int stream_id, int keep_buffers)
     s->h_state[stream_id] = fresh_state(s->m);
     CUDA_TRY(cudaMemcpy(s->d_state + stream_id, &s->h_state[stream_id], sizeof(StreamState),
                         cudaMemcpyHostToDevice));
-    if (keep_buffers)
-        CUDA_TRY(cudaMemsetAsync(static_cast<uint8_t*>(s->d_kv) + s->kv_stream_bytes * stream_id, 0,
-                                 s->kv_stream_bytes, s->stream));
+    if (keep_buffers) TRY(zero_rings(s, stream_id, s->stream));
     CUDA_TRY(cudaStreamSynchronize(s->stream));
     return STT_OK;
 }
@@ -1273,9 +1351,7 @@ extern "C" int stt_stream_reset_async(stt_streams* s, int stream_id, int keep_bu
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     const StreamState fresh = fresh_state(s->m);
     CUDA_TRY(launch_set_state(s->d_state + stream_id, fresh, st));
-    if (keep_buffers)
-        CUDA_TRY(cudaMemsetAsync(static_cast<uint8_t*>(s->d_kv) + s->kv_stream_bytes * stream_id, 0,
-                                 s->kv_stream_bytes, st));
+    if (keep_buffers) TRY(zero_rings(s, stream_id, st));
     // the offset mirror is exact; the other host fields are refreshed on the next synchronous call
     s->h_state[stream_id] = fresh;
     s->state_stale = true;
@@ -1323,6 +1399,158 @@ extern "C" int stt_stream_get_state(stt_streams* s, int stream_id, stt_stream_st
     out->last_text_token = st.last_text;
     out->delay_prev[0] = st.prev0;
     out->delay_prev[1] = st.prev1;
+    return STT_OK;
+}
+
+// ------------------------------------------------------------------------------------ beams
+
+namespace {
+
+int check_beams(stt_streams* s, const int32_t* ids, int groups, int beams) {
+    if (groups <= 0 || beams <= 0 || beams > kMaxBeams)
+        return set_error(STT_E_INVALID_ARG, "%d groups of %d beams (1..%d)", groups, beams, kMaxBeams);
+    if (groups > s->S / beams) return set_error(STT_E_INVALID_ARG, "%d groups of %d beams on %d streams", groups, beams, s->S);
+    return check_ids(s, ids, groups * beams);
+}
+
+// Device and pinned arrays of a beam call for n streams.
+struct BeamBufs {
+    int32_t *ids, *parents, *tokens, *held;
+    float* scores;
+};
+int beam_bufs(stt_streams* s, int n, BeamBufs* d, BeamBufs* h) {
+    TRY(s->beam_dev.ensure((size_t)5 * n * 4));
+    TRY(s->h_beam.ensure((size_t)5 * n * 4));
+    for (int i = 0; i < 2; ++i) {
+        int32_t* p = static_cast<int32_t*>(i ? s->h_beam.p : s->beam_dev.p);
+        *(i ? h : d) = BeamBufs{p, p + n, p + 2 * n, p + 3 * n, reinterpret_cast<float*>(p + 4 * n)};
+    }
+    return STT_OK;
+}
+
+// Queues the reordering of the streams' states and rings by d.parents; with tokens, as a beam step's end.
+int queue_reorder(stt_streams* s, int groups, int beams, const BeamBufs& d, bool step) {
+    const stt_model* m = s->m;
+    CUDA_TRY(launch_beam_states(s->d_state, d.ids, groups, beams, d.parents, step ? d.tokens : nullptr, s->kv8_cap != 0, d.held,
+                                s->stream));
+    ReorderArgs a{};
+    a.groups = groups;
+    a.beams = beams;
+    a.rows = d.ids;
+    a.parents = d.parents;
+    a.held = d.held;
+    a.states = static_cast<uint8_t*>(s->d_kv);
+    if (!s->kv8_cap) {
+        // [stream][layer][K|V][head] segments of ML slots
+        a.segments = a.inner = 2 * m->L * m->H;
+        a.units = m->ML;
+        a.unit_bytes = m->HD * (s->kv_f32 ? 4 : 2);
+        a.per_unit = 1;
+        a.segment_stride = a.units * a.unit_bytes;
+        a.row_stride = s->kv_stream_bytes;
+        CUDA_TRY(launch_reorder(a, s->stream));
+        return STT_OK;
+    }
+    // [layer][K|V][stream][head] segments of blocks, the codes and then the exponents
+    a.segments = 2 * m->L * m->H;
+    a.inner = m->H;
+    a.units = s->kv8_cap / kKv8Block;
+    a.per_unit = kKv8Block;
+    for (const bool codes : {true, false}) {
+        if (!codes) a.states = reinterpret_cast<uint8_t*>(s->d_exps);
+        a.unit_bytes = codes ? kKv8Block * m->HD : 1;
+        a.segment_stride = a.units * a.unit_bytes;
+        a.row_stride = a.segment_stride * m->H;
+        a.outer_stride = a.row_stride * s->S;
+        CUDA_TRY(launch_reorder(a, s->stream));
+    }
+    return STT_OK;
+}
+
+// The host keeps the offsets itself: they move with the streams.
+void move_offsets(stt_streams* s, const int32_t* ids, int groups, int beams, const int32_t* parents) {
+    std::vector<int32_t> off(beams);
+    for (int g = 0; g < groups; ++g) {
+        for (int b = 0; b < beams; ++b) off[b] = s->h_state[ids[g * beams + parents[g * beams + b]]].offset;
+        for (int b = 0; b < beams; ++b) s->h_state[ids[g * beams + b]].offset = off[b];
+    }
+    s->state_stale = true;
+}
+
+}  // namespace
+
+extern "C" int stt_streams_reorder(stt_streams* s, const int32_t* ids, int groups, int beams, const int32_t* parents) {
+    clear_error();
+    if (!s || !ids || !parents) return set_error(STT_E_INVALID_ARG, "NULL argument");
+    TRY(check_beams(s, ids, groups, beams));
+    const int n = groups * beams;
+    for (int i = 0; i < n; ++i)
+        if (parents[i] < 0 || parents[i] >= beams)
+            return set_error(STT_E_INVALID_ARG, "parent %d (index %d) outside the %d beams", parents[i], i, beams);
+    DeviceScope ds(s->m->device);
+    if (s->state_stale) CUDA_TRY(cudaDeviceSynchronize());  // frames may be queued on other streams
+    BeamBufs d, h;
+    TRY(beam_bufs(s, n, &d, &h));
+    std::memcpy(h.ids, ids, sizeof(int32_t) * n);
+    std::memcpy(h.parents, parents, sizeof(int32_t) * n);
+    CUDA_TRY(cudaMemcpyAsync(d.ids, h.ids, sizeof(int32_t) * 2 * n, cudaMemcpyHostToDevice, s->stream));
+    TRY(queue_reorder(s, groups, beams, d, false));
+    CUDA_TRY(cudaStreamSynchronize(s->stream));
+    move_offsets(s, ids, groups, beams, parents);
+    return STT_OK;
+}
+
+extern "C" int stt_streams_beam_frame(stt_streams* s, stt_beam* beam, const int32_t* ids, int groups, int beams,
+                                      const uint32_t* audio, float* scores, int32_t* parents_out, int32_t* tokens_out) {
+    clear_error();
+    if (!s || !beam || !ids || !audio || !scores || !parents_out || !tokens_out)
+        return set_error(STT_E_INVALID_ARG, "NULL argument");
+    TRY(check_beams(s, ids, groups, beams));
+    const stt_model* m = s->m;
+    if (beam_device(beam) != m->device)
+        return set_error(STT_E_INVALID_ARG, "the selector is on device %d, the streams on %d", beam_device(beam), m->device);
+    if (!beam_fits(beam, groups, beams, m->V))
+        return set_error(STT_E_INVALID_ARG, "the selector was made for less than %d utterances of %d beams over %d tokens", groups,
+                         beams, m->V);
+    if (m->V > m->TV)
+        return set_error(STT_E_STATE, "a chosen token can be outside the %d text embeddings (%d outputs)", m->TV, m->V);
+    const int n = groups * beams, nc = m->NC;
+    DeviceScope ds(m->device);
+    TRY(check_tokens(m, audio, (size_t)groups * nc, nullptr, 0));
+    TRY(check_positions(s, ids, n, 1));
+    if (s->state_stale) CUDA_TRY(cudaDeviceSynchronize());
+    BeamBufs d, h;
+    TRY(beam_bufs(s, n, &d, &h));
+    TRY(s->in_audio.ensure((size_t)n * nc * 4));
+    TRY(s->out_tokens.ensure((size_t)n * 4));
+    TRY(s->out_logits.ensure((size_t)n * m->V * 4));
+    TRY(s->h_tokens.ensure(std::max((size_t)n * nc * 4, sizeof(StepDesc))));
+    uint32_t* rep = static_cast<uint32_t*>(s->h_tokens.p);  // every beam of an utterance hears the same frame
+    for (int i = 0; i < n; ++i) std::memcpy(rep + (size_t)i * nc, audio + (size_t)(i / beams) * nc, sizeof(uint32_t) * nc);
+    std::memcpy(h.ids, ids, sizeof(int32_t) * n);
+    std::memcpy(h.scores, scores, sizeof(float) * n);
+    CUDA_TRY(cudaMemcpyAsync(s->in_audio.p, rep, (size_t)n * nc * 4, cudaMemcpyHostToDevice, s->stream));
+    CUDA_TRY(cudaMemcpyAsync(d.ids, h.ids, sizeof(int32_t) * n, cudaMemcpyHostToDevice, s->stream));
+    CUDA_TRY(cudaMemcpyAsync(d.scores, h.scores, sizeof(float) * n, cudaMemcpyHostToDevice, s->stream));
+    float* logits = static_cast<float*>(s->out_logits.p);
+    TRY(run_steps(s, ids, n, 1, static_cast<uint32_t*>(s->in_audio.p), nullptr, static_cast<int32_t*>(s->out_tokens.p), logits, 0,
+                  s->stream));
+    TRY(stt_beam_select_device(beam, logits, DT_F32, m->V, groups, beams, m->V, d.scores, nullptr, -1, d.scores, d.parents,
+                               d.tokens, nullptr, s->stream));
+    TRY(queue_reorder(s, groups, beams, d, true));
+    CUDA_TRY(cudaMemcpyAsync(h.parents, d.parents, sizeof(int32_t) * 2 * n, cudaMemcpyDeviceToHost, s->stream));
+    CUDA_TRY(cudaMemcpyAsync(h.scores, d.scores, sizeof(float) * n, cudaMemcpyDeviceToHost, s->stream));
+    TRY(s->h_stage.ensure(sizeof(StepDesc)));
+    StepDesc* desc = static_cast<StepDesc*>(s->h_stage.p);
+    CUDA_TRY(cudaMemcpyAsync(desc, s->d_desc, sizeof(StepDesc), cudaMemcpyDeviceToHost, s->stream));
+    CUDA_TRY(cudaStreamSynchronize(s->stream));
+    move_offsets(s, ids, groups, beams, h.parents);
+    if (desc->error != 0)
+        return set_error(desc->error == STT_E_INVALID_ARG ? STT_E_INVALID_ARG : STT_E_DEVICE_FLAG,
+                         "a kernel raised error %d", desc->error);
+    std::memcpy(parents_out, h.parents, sizeof(int32_t) * n);
+    std::memcpy(tokens_out, h.tokens, sizeof(int32_t) * n);
+    std::memcpy(scores, h.scores, sizeof(float) * n);
     return STT_OK;
 }
 

@@ -491,6 +491,7 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
 template <int B, class V, int U>
 __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a, int64_t per_segment) {
     __shared__ int parent[B];
+    __shared__ int64_t place[B];
     __shared__ int64_t limit[B];
     const int g = blockIdx.z, s = a.first_segment + blockIdx.y;
     const int64_t row0 = (int64_t)g * a.beams;
@@ -504,10 +505,11 @@ __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a, int64_t per
             m = held <= 0 ? 0 : min((held + a.per_unit - 1) / a.per_unit, a.units);
         }
         parent[b] = p;
+        place[b] = (a.rows && b < a.beams ? __ldg(a.rows + row0 + b) : row0 + b) * a.row_stride;
         limit[b] = p == b ? 0 : m * per_unit;
     }
     __syncthreads();
-    uint8_t* base = a.states + row0 * a.row_stride + (s / a.inner) * a.outer_stride + (s % a.inner) * a.segment_stride;
+    uint8_t* base = a.states + (s / a.inner) * a.outer_stride + (s % a.inner) * a.segment_stride;
     const int64_t first = (int64_t)blockIdx.x * 256 * U + threadIdx.x;
     V v[U][B];
 #pragma unroll
@@ -515,14 +517,14 @@ __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a, int64_t per
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t q = first + u * 256;
-            if (q < limit[b]) v[u][b] = *reinterpret_cast<const V*>(base + parent[b] * a.row_stride + q * sizeof(V));
+            if (q < limit[b]) v[u][b] = *reinterpret_cast<const V*>(base + place[parent[b]] + q * sizeof(V));
         }
 #pragma unroll
     for (int b = 0; b < B; ++b)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t q = first + u * 256;
-            if (q < limit[b]) *reinterpret_cast<V*>(base + b * a.row_stride + q * sizeof(V)) = v[u][b];
+            if (q < limit[b]) *reinterpret_cast<V*>(base + place[b] + q * sizeof(V)) = v[u][b];
         }
 }
 
@@ -536,7 +538,8 @@ cudaError_t reorder_t(const ReorderArgs& a, cudaStream_t st) {
             ReorderArgs b = a;
             b.groups = std::min(65535, a.groups - g0);
             b.segments = std::min(65535, a.segments - s0);
-            b.states += (int64_t)g0 * a.beams * a.row_stride;
+            if (b.rows) b.rows += (int64_t)g0 * a.beams;
+            else b.states += (int64_t)g0 * a.beams * a.row_stride;
             b.first_segment = s0;
             b.parents += (int64_t)g0 * a.beams;
             if (b.held) b.held += (int64_t)g0 * a.beams;

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/stt_b200.h"
 #include "kv8.h"
 
 namespace stt {
@@ -43,11 +44,15 @@ struct ReorderArgs {
     int32_t first_segment; // of the launch
     int64_t units, unit_bytes;
     int32_t groups, beams;
+    const int32_t* rows;   // place of each row (row_stride apart), or NULL: its number
     const int32_t* parents;
     const int32_t* held;   // what each row holds, or NULL: `units` units
     int32_t per_unit;      // of which `per_unit` make one unit
 };
 
+// The selector's device, and whether it was made for such a call.
+int beam_device(const stt_beam* beam);
+bool beam_fits(const stt_beam* beam, int batch, int beams, int vocab);
 cudaError_t launch_beam_select(const BeamArgs& a, int dtype, cudaStream_t st);
 cudaError_t launch_reorder(const ReorderArgs& a, cudaStream_t st);
 

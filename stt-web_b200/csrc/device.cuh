@@ -76,7 +76,7 @@ struct Ctx {
     uint32_t pad_id;
     int32_t text_delay;
     // streams
-    void* kv;
+    void* kv;                  // bf16 or f32 rings; NULL for 8-bit ones
     int32_t kv_f32;
     int64_t kv_stream_stride;  // elements
     int64_t kv_layer_stride;   // elements (K and V of one layer)

@@ -27,7 +27,7 @@ __device__ __forceinline__ void unit_rows(const GemvArgs& a, int u, int* ra, int
 
 // The QKV epilogue of output pair (ra, rb = ra + 1) of batch row bm (stream sid, state st, RoPE
 // factors cs): RoPE on q and k, the row's q, k, v to the step's buffer and k, v to the stream's K/V
-// ring.
+// ring (an 8-bit ring takes them from the buffer, all heads' blocks at once).
 __device__ __forceinline__ void qkv_store(const Ctx& c, const GemvArgs& a, int bm, int sid, const StreamState& st,
                                           float2 cs, int ra, int rb, float va, float vb) {
     float* o = a.out + (int64_t)bm * a.ldo;
@@ -39,7 +39,7 @@ __device__ __forceinline__ void qkv_store(const Ctx& c, const GemvArgs& a, int b
     }
     o[ra] = va;
     o[rb] = vb;
-    if (part >= 1) {
+    if (part >= 1 && c.kv) {
         const int64_t off = qkv_kv_offset(c, a.layer, sid, st, ra);
         if (c.kv_f32) {
             float* kv = reinterpret_cast<float*>(c.kv) + off;

@@ -1189,6 +1189,38 @@ cudaError_t launch_attention(const Ctx& c, int layer, cudaStream_t st) {
                 : launch_attention_ch<__nv_bfloat16, 48>(c, layer, grid, st);
 }
 
+static __global__ void positions_kernel(Ctx c, int32_t* pos) {
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < c.n) pos[i] = c.state[c.ids[i]].offset;
+}
+
+cudaError_t launch_positions(const Ctx& c, int32_t* pos, cudaStream_t st) {
+    positions_kernel<<<(c.n + 127) / 128, 128, 0, st>>>(c, pos);
+    return cudaGetLastError();
+}
+
+// One CTA per group: all of its beams' states are read before any is written.
+static __global__ void beam_states_kernel(StreamState* state, const int32_t* ids, int beams, const int32_t* parents,
+                                          const int32_t* tokens, int whole, int32_t* held) {
+    const int r0 = blockIdx.x * beams, b = threadIdx.x;
+    StreamState st{};
+    if (b < beams) st = state[ids[r0 + parents[r0 + b]]];
+    __syncthreads();
+    if (b >= beams) return;
+    held[r0 + b] = whole ? st.offset : st.len;
+    if (tokens) {
+        st.last_text = (uint32_t)tokens[r0 + b];
+        st.frame_count += 1;
+    }
+    state[ids[r0 + b]] = st;
+}
+
+cudaError_t launch_beam_states(StreamState* state, const int32_t* ids, int groups, int beams, const int32_t* parents,
+                               const int32_t* tokens, int whole, int32_t* held, cudaStream_t st) {
+    beam_states_kernel<<<groups, 32, 0, st>>>(state, ids, beams, parents, tokens, whole, held);
+    return cudaGetLastError();
+}
+
 cudaError_t launch_finish(const Ctx& c, cudaStream_t st) {
     finish_kernel<<<c.n, 1024, 0, st>>>(c);
     return cudaGetLastError();

@@ -66,6 +66,13 @@ cudaError_t configure_gemv_mma();
 cudaError_t launch_embed(const Ctx& c, cudaStream_t st);
 cudaError_t launch_attention(const Ctx& c, int layer, cudaStream_t st);
 cudaError_t launch_finish(const Ctx& c, cudaStream_t st);
+// pos[i] = position of batch row i's stream before this step.
+cudaError_t launch_positions(const Ctx& c, int32_t* pos, cudaStream_t st);
+// Stream states of a beam step: stream ids[g * beams + b] takes the state of stream
+// ids[g * beams + parents[g * beams + b]]; with tokens, its last text token becomes tokens[..] and its frame
+// count advances.  held[..] receives what its new K/V ring holds: `whole` ? positions : valid slots.
+cudaError_t launch_beam_states(StreamState* state, const int32_t* ids, int groups, int beams, const int32_t* parents,
+                               const int32_t* tokens, int whole, int32_t* held, cudaStream_t st);
 // Adds the K-slice partial sums part[slices][rows][a.W.n] of a tensor-core product in slice order
 // and applies the epilogue `epi` as launch_gemv does.
 cudaError_t launch_tc_epilogue(const Ctx& c, const GemvArgs& a, int epi, int rows, const float* part, int slices,

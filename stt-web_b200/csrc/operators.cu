@@ -64,6 +64,11 @@ int check_batch(const stt_kv8_cache* h, const int32_t* d_seqs, int n, const int3
 
 }  // namespace
 
+int stt::beam_device(const stt_beam* beam) { return beam->device; }
+bool stt::beam_fits(const stt_beam* h, int batch, int beams, int vocab) {
+    return batch <= h->max_batch && beams <= h->max_beams && vocab <= h->max_vocab;
+}
+
 extern "C" int stt_kv8_cache_bytes(int n_seqs, int n_kv_heads, int head_dim, int capacity, size_t* out) {
     clear_error();
     size_t codes, exps;
@@ -351,7 +356,7 @@ extern "C" int stt_beam_select_device(stt_beam* h, const void* d_logits, int dty
     if (!h || batch < 0 || (batch > 0 && (!d_logits || !d_scores || !d_next_scores || !d_parents || !d_tokens)))
         return set_error(STT_E_INVALID_ARG, "bad arguments");
     if (dtype < DT_F32 || dtype > DT_F16) return set_error(STT_E_INVALID_ARG, "dtype %d unknown", dtype);
-    if (beams < 1 || vocab < 1 || batch > h->max_batch || beams > h->max_beams || vocab > h->max_vocab)
+    if (beams < 1 || vocab < 1 || !beam_fits(h, batch, beams, vocab))
         return set_error(STT_E_INVALID_ARG, "%d utterances, %d beams, %d tokens: the selector was made for %d, %d, %d", batch,
                          beams, vocab, h->max_batch, h->max_beams, h->max_vocab);
     if (row_stride < vocab) return set_error(STT_E_INVALID_ARG, "row stride %lld < vocab %d", (long long)row_stride, vocab);

@@ -21,6 +21,7 @@ STT_E_STATE = -6
 
 STT_KV_BF16 = 0
 STT_KV_F32 = 1
+STT_KV_INT8 = 2
 
 STT_PRODUCTS_F16X3 = 0
 STT_PRODUCTS_F16X2 = 1
@@ -121,6 +122,8 @@ SIGNATURES = {
     "stt_stream_flush": (C.c_int, [P, C.c_int, U32P, C.c_int, I32P]),
     "stt_stream_reset": (C.c_int, [P, C.c_int, C.c_int]),
     "stt_stream_reset_async": (C.c_int, [P, C.c_int, C.c_int, P]),
+    "stt_streams_reorder": (C.c_int, [P, I32P, C.c_int, C.c_int, I32P]),
+    "stt_streams_beam_frame": (C.c_int, [P, P, I32P, C.c_int, C.c_int, U32P, F32P, I32P, I32P]),
     "stt_stream_set_last_text_token": (C.c_int, [P, C.c_int, C.c_uint32]),
     "stt_streams_set_product_precision": (C.c_int, [P, C.c_int]),
     "stt_stream_get_state": (C.c_int, [P, C.c_int, C.POINTER(stt_stream_state)]),

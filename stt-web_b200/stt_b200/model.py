@@ -17,7 +17,8 @@ from typing import List, Optional, Sequence
 
 import numpy as np
 
-from ._lib import (STT_KV_BF16, STT_KV_F32, SttError, check, lib, stt_config, stt_model_info,
+from .operators import BeamSelector
+from ._lib import (STT_KV_BF16, STT_KV_F32, STT_KV_INT8, SttError, check, lib, stt_config, stt_model_info,
                    stt_stream_state)
 
 
@@ -118,7 +119,7 @@ class LayerCaches:
     def __init__(self, model: SttModel, n_streams: int, kv_dtype: str = "bf16"):
         self.model = model
         self.n_streams = n_streams
-        kv = {"bf16": STT_KV_BF16, "f32": STT_KV_F32}[kv_dtype]
+        kv = {"bf16": STT_KV_BF16, "f32": STT_KV_F32, "int8": STT_KV_INT8}[kv_dtype]
         h = C.c_void_p()
         check(lib().stt_streams_create(model._h, n_streams, kv, C.byref(h)), "stt_streams_create")
         self._h = h
@@ -167,6 +168,32 @@ class LayerCaches:
         check(lib().stt_streams_submit_frame(self._h, _ptr(ids, C.c_int32), ids.size, _ptr(a, C.c_uint32),
                                              C.byref(t)), "stt_streams_submit_frame")
         return PendingFrame(self, t.value, ids.size)
+
+    def reorder(self, stream_ids, parents) -> None:
+        """stream_ids and parents [groups, beams]: stream stream_ids[g, b] becomes what stream
+        stream_ids[g, parents[g, b]] was."""
+        ids = np.ascontiguousarray(np.asarray(stream_ids, dtype=np.int32))
+        par = np.ascontiguousarray(np.asarray(parents, dtype=np.int32))
+        if ids.ndim != 2 or par.shape != ids.shape:
+            raise SttError(-1, "stt_streams_reorder", "stream_ids and parents must both be [groups, beams]")
+        check(lib().stt_streams_reorder(self._h, _ptr(ids, C.c_int32), ids.shape[0], ids.shape[1], _ptr(par, C.c_int32)),
+              "stt_streams_reorder")
+
+    def beam_frame(self, beam: "BeamSelector", stream_ids, audio, scores):
+        """One frame of beam search: stream_ids [groups, beams], audio [groups, num_codebooks], scores
+        [groups, beams].  Returns (scores, parents, tokens), each [groups, beams], best first; the
+        streams then carry the beams in that order."""
+        ids = np.ascontiguousarray(np.asarray(stream_ids, dtype=np.int32))
+        sc = np.array(scores, dtype=np.float32, order="C")
+        a = _u32(audio)
+        if ids.ndim != 2 or sc.shape != ids.shape or a.size != ids.shape[0] * self.model.info.num_codebooks:
+            raise SttError(-1, "stt_streams_beam_frame",
+                           "stream_ids and scores must be [groups, beams], audio [groups, num_codebooks]")
+        par, tok = np.empty_like(ids), np.empty_like(ids)
+        check(lib().stt_streams_beam_frame(self._h, beam._h, _ptr(ids, C.c_int32), ids.shape[0], ids.shape[1],
+                                           _ptr(a, C.c_uint32), _ptr(sc, C.c_float), _ptr(par, C.c_int32),
+                                           _ptr(tok, C.c_int32)), "stt_streams_beam_frame")
+        return sc, par, tok
 
     def state(self, stream_id: int) -> dict:
         st = stt_stream_state()

@@ -154,3 +154,24 @@ def test_reference_selection():
     assert np.allclose(s, [[math.log(0.5), math.log(0.8) - 1]])
     s, p, t, d = R.select(np.zeros((1, 2, 4)), np.array([[0.0, 0.0]]), np.array([[0, 1]]), 2)
     assert p.tolist() == [[1, 0]] and t.tolist() == [[2, 0]] and d.tolist() == [[True, False]]
+
+
+def test_oracle_int8_rings_are_close_to_f32_ones(tiny_ref_gguf):
+    """The oracle's 8-bit rings round K and V by at most a step of 1/64 of a block's largest value: its
+    logits stay near, and are not, the f32 rings' (the GPU tests compare with them exactly that way)."""
+    from oracle import oracle as O
+    om = O.OracleModel(tiny_ref_gguf, num_layers=2, num_heads=2, num_codebooks=4, text_start_token=1000, sliding_window=20)
+    a, b = om.stream(0), om.stream(O.KV_INT8)
+    rng = np.random.default_rng(0)
+    far = 0.0
+    for _ in range(40):
+        audio, text = rng.integers(0, 300, 4), int(rng.integers(0, 1000))
+        x, y = a.forward(audio, text)[0], b.forward(audio, text)[0]
+        far = max(far, float(np.abs(x - y).max() / np.abs(x).max()))
+    assert 1e-6 < far < 1 / 16
+
+
+def test_beam_calls_without_a_set_are_refused():
+    L = lib()
+    refused(L.stt_streams_reorder(None, None, 1, 1, None), "NULL")
+    refused(L.stt_streams_beam_frame(None, None, None, 1, 1, None, None, None, None), "NULL")
