@@ -286,12 +286,12 @@ int stt_q4_tensor_dequant(const stt_q4_tensor* w, float* out_host);
  * lives in slot p % capacity.  A cache is thus a ring of the last positions: once position
  * 16 b + capacity is written, the 16 positions from 16 b on are gone.
  *
- * Batches.  A call takes n rows.  Row i concerns sequence d_seqs[i] (d_seqs == NULL: sequence i) and
- * its d_count[i] positions (d_count == NULL: n_tokens; at most n_tokens) from d_pos[i] on: device
- * arrays, so that a captured graph can be replayed for other positions.  Tensors are
- * [n][n_tokens][heads][head_dim] of `dtype` (0 f32, 1 bf16, 2 f16) with strides in elements, head_dim
- * contiguous; they start at, and their strides are, multiples of 16 bytes.  What lies behind a row's
- * count is neither read nor written.
+ * Batches (stt_kv8_batch).  A call takes n rows.  Row i concerns sequence d_seqs[i] (d_seqs == NULL:
+ * sequence i) and its d_count[i] positions (d_count == NULL: n_tokens; at most n_tokens) from d_pos[i]
+ * on: device arrays, so that a captured graph can be replayed for other positions.  Tensors
+ * (stt_kv8_tensor) are [n][n_tokens][heads][head_dim] on the device, dtype 0 f32, 1 bf16, 2 f16, with
+ * strides in elements, head_dim contiguous; they start at, and their strides are, multiples of 16
+ * bytes.  What lies behind a row's count is neither read nor written.
  *
  * Calls are queued on cuda_stream (NULL = legacy default stream) without synchronisation and
  * allocate nothing.  Calls on one cache share its workspace: they must not overlap in time, nor may
@@ -308,6 +308,16 @@ typedef struct stt_kv8_cache_info {
     int8_t *d_k_codes, *d_v_codes, *d_k_exponents, *d_v_exponents;
 } stt_kv8_cache_info;
 
+typedef struct stt_kv8_batch {
+    const int32_t *d_seqs, *d_pos, *d_count;
+    int32_t n, n_tokens;
+} stt_kv8_batch;
+typedef struct stt_kv8_tensor {
+    void* d_data;  /* only read where the call takes a const tensor */
+    int64_t seq_stride, token_stride, head_stride;
+    int32_t dtype, reserved;
+} stt_kv8_tensor;
+
 /* head_dim 64 or 128, capacity a multiple of 16. */
 int stt_kv8_cache_bytes(int n_seqs, int n_kv_heads, int head_dim, int capacity, size_t* out);
 /* d_memory: device memory of stt_kv8_cache_bytes, 16-byte aligned, that outlives the cache and is used
@@ -323,32 +333,28 @@ int stt_kv8_cache_get_info(const stt_kv8_cache* cache, stt_kv8_cache_info* out);
  * that was appended. */
 int stt_kv8_cache_status(stt_kv8_cache* cache);
 
-/* Writes positions d_pos[i] .. d_pos[i] + d_count[i] - 1 of K and V.  The new tokens of a block take
- * the smallest exponent e >= -100 with max|x| <= 127 * 2^e over them and head_dim, or the block's own
- * where that is larger and the block holds earlier positions; those move along when the exponent
- * grows.  Codes are rounded to nearest, ties to even.  Token by token or many at once, a value ends up
- * within one step 2^e of what was appended (half a step where its block's exponent did not grow
- * afterwards).  K and V share the strides.  Sequences of one call are distinct. */
-int stt_kv8_append_device(stt_kv8_cache* cache, const int32_t* d_seqs, int n, const int32_t* d_pos,
-                          const int32_t* d_count, int n_tokens, const void* d_k, const void* d_v, int dtype,
-                          int64_t seq_stride, int64_t token_stride, int64_t head_stride, void* cuda_stream);
+/* Writes positions d_pos[i] .. d_pos[i] + d_count[i] - 1 of K and V (one dtype).  The new tokens of a
+ * block take the smallest exponent e >= -100 with max|x| <= 127 * 2^e over them and head_dim, or the
+ * block's own where that is larger and the block holds earlier positions; those move along when the
+ * exponent grows.  Codes are rounded to nearest, ties to even.  Token by token or many at once, a value
+ * ends up within one step 2^e of what was appended (half a step where its block's exponent did not grow
+ * afterwards).  Sequences of one call are distinct. */
+int stt_kv8_append_device(stt_kv8_cache* cache, const stt_kv8_batch* batch, const stt_kv8_tensor* k,
+                          const stt_kv8_tensor* v, void* cuda_stream);
 /* The way back: the values of positions d_pos[i] .. d_pos[i] + d_count[i] - 1 (which the ring must
- * still hold), exact in every dtype unless an exponent leaves f16's range. */
-int stt_kv8_read_device(const stt_kv8_cache* cache, const int32_t* d_seqs, int n, const int32_t* d_pos,
-                        const int32_t* d_count, int n_tokens, void* d_k, void* d_v, int dtype, int64_t seq_stride,
-                        int64_t token_stride, int64_t head_stride, void* cuda_stream);
+ * still hold) into k and v (one dtype), exact in every dtype unless an exponent leaves f16's range. */
+int stt_kv8_read_device(const stt_kv8_cache* cache, const stt_kv8_batch* batch, const stt_kv8_tensor* k,
+                        const stt_kv8_tensor* v, void* cuda_stream);
 /* Causal attention of the positions that an append with the same batch has just written: the query of
  * row i, token t, at P = d_pos[i] + t, sees the positions p <= P that are at least
  *   d_start[i] (NULL: 0), P + 1 - window (window 0: no such bound), and the oldest that the ring holds
  *   once d_pos[i] + d_count[i] - 1 is written;
- * out = softmax(scale * q . k) v over them, 0 where there is none.  n_heads is a multiple of
- * n_kv_heads; query head j reads K/V head j / (n_heads / n_kv_heads).  Sums and the softmax are f32,
- * the output is rounded once.  A sequence may come in several rows. */
-int stt_kv8_attention_device(stt_kv8_cache* cache, const int32_t* d_seqs, int n, const int32_t* d_pos,
-                             const int32_t* d_count, int n_tokens, int n_heads, const void* d_q, int q_dtype,
-                             int64_t q_seq_stride, int64_t q_token_stride, int64_t q_head_stride,
-                             const int32_t* d_start, int window, float scale, void* d_out, int out_dtype,
-                             int64_t out_seq_stride, int64_t out_token_stride, int64_t out_head_stride,
+ * out = softmax(scale * q . k) v over them, 0 where there is none.  n_heads (of q and out) is a multiple
+ * of n_kv_heads; query head j reads K/V head j / (n_heads / n_kv_heads).  Sums and the softmax are f32,
+ * the output is rounded once (where q and out both have 16 bits, the weights may be rounded to f16
+ * first).  q and out are of any dtype each.  A sequence may come in several rows. */
+int stt_kv8_attention_device(stt_kv8_cache* cache, const stt_kv8_batch* batch, const stt_kv8_tensor* q, int n_heads,
+                             const int32_t* d_start, int window, float scale, const stt_kv8_tensor* out,
                              void* cuda_stream);
 /* Beam search's reordering of the first groups * beams sequences: sequence g * beams + b becomes what
  * sequence g * beams + d_parents[g * beams + b] was (0 <= parent < beams; another value leaves it as it
@@ -368,26 +374,40 @@ int stt_beam_destroy(stt_beam* beam);
  * scores of the calls since the last check; such a beam's candidates counted as -inf. */
 int stt_beam_status(stt_beam* beam);
 /* The `beams` best continuations of each utterance, best first.  Row g * beams + b of the logits (dtype
- * 0, 1 or 2, rows row_stride elements apart) and of the other arrays is beam b of utterance g; the
- * candidates are
+ * 0 f32, 1 bf16, 2 f16, rows row_stride elements apart) and of the other device arrays is beam b of
+ * utterance g; the candidates are
  *   d_scores[b] + log_softmax(logits[b])[token]   for every beam and token,
- * computed and compared in 64 bits, equal ones by the lowest b * vocab + token.  A beam with d_done != 0
- * (d_done may be NULL) has ended: its only finite candidate is the token `eos` at its unchanged score.
- * d_parents and d_tokens receive the beam and token of each chosen candidate, d_next_scores its score,
- * d_next_done (may be NULL) whether its parent had ended or the token is `eos` (-1: no token ends a
- * beam).  -inf scores and logits are ordinary values that rank last.  d_next_scores and d_next_done may
- * be the arrays that d_scores and d_done are.  Queued on cuda_stream, no synchronisation, no allocation. */
-int stt_beam_select_device(stt_beam* beam, const void* d_logits, int dtype, int64_t row_stride, int batch, int beams,
-                           int vocab, const float* d_scores, const uint8_t* d_done, int eos, float* d_next_scores,
-                           int32_t* d_parents, int32_t* d_tokens, uint8_t* d_next_done, void* cuda_stream);
+ * computed and compared in 64 bits (the exponentials in 32), equal ones by the lowest b * vocab + token.
+ * A beam with d_done != 0 (d_done may be NULL) has ended: its only finite candidate is the token `eos` at
+ * its unchanged score.  d_parents and d_tokens receive the beam and token of each chosen candidate,
+ * d_next_scores its score, d_next_done (may be NULL) whether its parent had ended or the token is `eos`
+ * (-1: no token ends a beam).  -inf scores and logits are ordinary values that rank last.  d_next_scores
+ * and d_next_done may be the arrays that d_scores and d_done are.  Queued on cuda_stream, no
+ * synchronisation, no allocation. */
+typedef struct stt_beam_step {
+    const void* d_logits;
+    int64_t row_stride;
+    int32_t dtype, batch, beams, vocab;
+    const float* d_scores;
+    const uint8_t* d_done;
+    float* d_next_scores;
+    int32_t *d_parents, *d_tokens;
+    uint8_t* d_next_done;
+    int32_t eos, reserved;
+} stt_beam_step;
+int stt_beam_select_device(stt_beam* beam, const stt_beam_step* step, void* cuda_stream);
 /* Reorders the states of groups * beams rows in place: row g * beams + b becomes what row
  * g * beams + d_parents[g * beams + b] was (a parent outside 0 .. beams - 1 leaves it as it is).  A row's
  * state is `segments` pieces of units * unit_bytes bytes, segment_stride bytes apart; rows are
  * row_stride bytes apart.  Of each segment of row r the first d_held[r] units are moved (NULL: all), the
  * rest stays.  Works on any device memory of `device`, needs no workspace. */
-int stt_beam_reorder_device(int device, void* d_states, int64_t row_stride, int segments, int64_t segment_stride,
-                            int64_t units, int64_t unit_bytes, const int32_t* d_parents, int groups, int beams,
-                            const int32_t* d_held, void* cuda_stream);
+typedef struct stt_beam_states {
+    void* d_states;
+    int64_t row_stride, segment_stride, units, unit_bytes;
+    const int32_t *d_parents, *d_held;
+    int32_t segments, groups, beams, reserved;
+} stt_beam_states;
+int stt_beam_reorder_device(int device, const stt_beam_states* states, void* cuda_stream);
 
 /* ---------------------------------------------------------------------------------------
  * SentencePiece detokeniser: the step after the decode path.  Replaces SpmDecoder

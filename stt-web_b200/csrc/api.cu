@@ -734,7 +734,7 @@ int enqueue_kv8_attention(stt_streams* s, const Ctx& c, int layer, __half* x16, 
     const Kv8Dev kv = kv8_layer(s, layer);
     const Kv8Batch batch{s->d_ids, s->d_pos, nullptr, c.n, 1};
     const Kv8Strides rows{3 * m->D, 3 * m->D, m->HD};
-    CUDA_TRY(launch_kv8_append(kv, batch, s->d_qkv + m->D, s->d_qkv + 2 * m->D, DT_F32, rows, st));
+    CUDA_TRY(launch_kv8_append(kv, batch, s->d_qkv + m->D, s->d_qkv + 2 * m->D, DT_F32, rows, rows, st));
     Kv8Attention a{};
     a.q = s->d_qkv;
     a.out = s->d_attn;
@@ -1535,8 +1535,8 @@ extern "C" int stt_streams_beam_frame(stt_streams* s, stt_beam* beam, const int3
     float* logits = static_cast<float*>(s->out_logits.p);
     TRY(run_steps(s, ids, n, 1, static_cast<uint32_t*>(s->in_audio.p), nullptr, static_cast<int32_t*>(s->out_tokens.p), logits, 0,
                   s->stream));
-    TRY(stt_beam_select_device(beam, logits, DT_F32, m->V, groups, beams, m->V, d.scores, nullptr, -1, d.scores, d.parents,
-                               d.tokens, nullptr, s->stream));
+    const stt_beam_step step{logits, m->V, DT_F32, groups, beams, m->V, d.scores, nullptr, d.scores, d.parents, d.tokens, nullptr, -1, 0};
+    TRY(stt_beam_select_device(beam, &step, s->stream));
     TRY(queue_reorder(s, groups, beams, d, true));
     CUDA_TRY(cudaMemcpyAsync(h.parents, d.parents, sizeof(int32_t) * 2 * n, cudaMemcpyDeviceToHost, s->stream));
     CUDA_TRY(cudaMemcpyAsync(h.scores, d.scores, sizeof(float) * n, cudaMemcpyDeviceToHost, s->stream));

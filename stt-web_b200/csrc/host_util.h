@@ -38,15 +38,22 @@ cudaError_t host_alloc(void** p, size_t bytes);
         }                                                                                           \
     } while (0)
 
-// Restores the calling thread's current device on scope exit.
+// Makes `dev` the calling thread's current device and restores the one before on scope exit.
 struct DeviceScope {
     int prev = 0;
-    bool ok = false;
+    bool ok = false, moved = false;
     explicit DeviceScope(int dev) {
-        if (cudaGetDevice(&prev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) ok = true;
+        if (cudaGetDevice(&prev) != cudaSuccess) return;
+        // (a thread that has made no call yet has device 0 as current, without a context: set it)
+        thread_local bool set = false;
+        if (prev == dev && set) {
+            ok = true;
+            return;
+        }
+        ok = set = moved = cudaSetDevice(dev) == cudaSuccess;
     }
     ~DeviceScope() {
-        if (ok) cudaSetDevice(prev);
+        if (moved && cudaSetDevice(prev) != cudaSuccess) (void)cudaGetLastError();
     }
 };
 

@@ -57,8 +57,8 @@ __device__ __forceinline__ void check_repeated(const Kv8Dev& c, const Kv8Batch& 
 // the low byte of x * 2^-e + 1.5 * 2^23, whose unit is 1: the addition rounds to nearest, ties to even.
 template <int D, int DT, int MAX>
 __global__ void __launch_bounds__(kThreads, MAX == 1 ? 6 : 2) append_kernel(Kv8Dev c, Kv8Batch b, const typename Elem<DT>::T* __restrict__ k,
-                                                          const typename Elem<DT>::T* __restrict__ v, Kv8Strides s, int nb,
-                                                          int ctas_per_block) {
+                                                          const typename Elem<DT>::T* __restrict__ v, Kv8Strides ks, Kv8Strides vs,
+                                                          int nb, int ctas_per_block) {
     constexpr int N = D / 32;
     const int lane = threadIdx.x & 31;
     const int rest = blockIdx.x / ctas_per_block;
@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(kThreads, MAX == 1 ? 6 : 2) append_kernel(Kv8D
     const int64_t head = (int64_t)r.seq * c.heads + h;
     int8_t* codes = (kv ? c.vc : c.kc) + (head * c.cap + slot) * D + lane * N;
     int8_t* exps = (kv ? c.ve : c.ke) + head * (c.cap / kKv8Block) + slot / kKv8Block;
+    const Kv8Strides s = kv ? vs : ks;
     const typename Elem<DT>::T* src = (kv ? v : k) + i * s.seq + (int64_t)(lo - r.pos) * s.token + h * s.head + lane * N;
     const int old = lo - p0, many = hi - lo;
     float x[MAX][N];
@@ -143,7 +144,7 @@ constexpr int kReadTokens = 16;  // of a CTA
 // (2^23 + 128 + code) * step - (2^23 + 128) * step is exact in one fused multiply-add.
 template <int D, int DT>
 __global__ void __launch_bounds__(kThreads) read_kernel(Kv8Dev c, Kv8Batch b, void* __restrict__ k, void* __restrict__ v,
-                                                        Kv8Strides s, int token_ctas, int head_ctas) {
+                                                        Kv8Strides ks, Kv8Strides vs, int token_ctas, int head_ctas) {
     constexpr int N = 16 / (int)sizeof(typename Elem<DT>::T);
     const int part = blockIdx.x / head_ctas, item = (blockIdx.x - part * head_ctas) * kThreads + threadIdx.x;
     const int i = part / token_ctas, t0 = (part - i * token_ctas) * kReadTokens;
@@ -154,7 +155,6 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Kv8Dev c, Kv8Batch b, vo
     const int64_t head = (int64_t)r.seq * c.heads + h;
     const int8_t *kc = c.kc + head * c.cap * D + piece * N, *vc = c.vc + head * c.cap * D + piece * N;
     const int8_t *ke = c.ke + head * (c.cap / kKv8Block), *ve = c.ve + head * (c.cap / kKv8Block);
-    const int64_t at0 = i * s.seq + h * s.head + piece * N;
     int slot = t0 < t1 ? (r.pos + t0) % c.cap : 0;
 #pragma unroll 4
     for (int t = t0; t < t1; ++t) {
@@ -176,7 +176,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Kv8Dev c, Kv8Batch b, vo
             for (int j = 0; j < N; ++j)
                 y[j] = fmaf(__uint_as_float(__byte_perm(q[half][j / 4] ^ 0x80808080u, 0x4B000000u, 0x7650 | (j % 4))), step[half], bias);
             void* out = half ? v : k;
-            const int64_t at = at0 + t * s.token;
+            const Kv8Strides& s = half ? vs : ks;
+            const int64_t at = i * s.seq + t * s.token + h * s.head + piece * N;
             if constexpr (DT == DT_F32) {
                 *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = make_float4(y[0], y[1], y[2], y[3]);
             } else {
@@ -189,23 +190,24 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Kv8Dev c, Kv8Batch b, vo
 }
 
 template <int D, int DT>
-cudaError_t append_t(const Kv8Dev& c, const Kv8Batch& b, const void* k, const void* v, const Kv8Strides& s,
-                     cudaStream_t st) {
+cudaError_t append_t(const Kv8Dev& c, const Kv8Batch& b, const void* k, const void* v, const Kv8Strides& ks,
+                     const Kv8Strides& vs, cudaStream_t st) {
     using T = typename Elem<DT>::T;
     const T *kt = static_cast<const T*>(k), *vt = static_cast<const T*>(v);
     const int nb = (b.tokens + 2 * kKv8Block - 2) / kKv8Block;  // blocks that `tokens` tokens can touch
     const int per_block = (2 * c.heads + kThreads / 32 - 1) / (kThreads / 32);
     const unsigned grid = (unsigned)((int64_t)b.n * nb * per_block);
-    if (b.tokens == 1) append_kernel<D, DT, 1><<<grid, kThreads, 0, st>>>(c, b, kt, vt, s, nb, per_block);
-    else append_kernel<D, DT, kKv8Block><<<grid, kThreads, 0, st>>>(c, b, kt, vt, s, nb, per_block);
+    if (b.tokens == 1) append_kernel<D, DT, 1><<<grid, kThreads, 0, st>>>(c, b, kt, vt, ks, vs, nb, per_block);
+    else append_kernel<D, DT, kKv8Block><<<grid, kThreads, 0, st>>>(c, b, kt, vt, ks, vs, nb, per_block);
     return cudaGetLastError();
 }
 
 template <int D, int DT>
-cudaError_t read_t(const Kv8Dev& c, const Kv8Batch& b, void* k, void* v, const Kv8Strides& s, cudaStream_t st) {
+cudaError_t read_t(const Kv8Dev& c, const Kv8Batch& b, void* k, void* v, const Kv8Strides& ks, const Kv8Strides& vs,
+                   cudaStream_t st) {
     const int token_ctas = (b.tokens + kReadTokens - 1) / kReadTokens;
     const int head_ctas = (c.heads * (D * (int)sizeof(typename Elem<DT>::T) / 16) + kThreads - 1) / kThreads;
-    read_kernel<D, DT><<<(unsigned)((int64_t)b.n * token_ctas * head_ctas), kThreads, 0, st>>>(c, b, k, v, s, token_ctas,
+    read_kernel<D, DT><<<(unsigned)((int64_t)b.n * token_ctas * head_ctas), kThreads, 0, st>>>(c, b, k, v, ks, vs, token_ctas,
                                                                                               head_ctas);
     return cudaGetLastError();
 }
@@ -213,27 +215,27 @@ cudaError_t read_t(const Kv8Dev& c, const Kv8Batch& b, void* k, void* v, const K
 }  // namespace
 
 cudaError_t launch_kv8_append(const Kv8Dev& c, const Kv8Batch& b, const void* k, const void* v, int dtype,
-                              const Kv8Strides& s, cudaStream_t st) {
+                              const Kv8Strides& ks, const Kv8Strides& vs, cudaStream_t st) {
     if (c.dim == 128) {
-        if (dtype == DT_F32) return append_t<128, DT_F32>(c, b, k, v, s, st);
-        if (dtype == DT_BF16) return append_t<128, DT_BF16>(c, b, k, v, s, st);
-        return append_t<128, DT_F16>(c, b, k, v, s, st);
+        if (dtype == DT_F32) return append_t<128, DT_F32>(c, b, k, v, ks, vs, st);
+        if (dtype == DT_BF16) return append_t<128, DT_BF16>(c, b, k, v, ks, vs, st);
+        return append_t<128, DT_F16>(c, b, k, v, ks, vs, st);
     }
-    if (dtype == DT_F32) return append_t<64, DT_F32>(c, b, k, v, s, st);
-    if (dtype == DT_BF16) return append_t<64, DT_BF16>(c, b, k, v, s, st);
-    return append_t<64, DT_F16>(c, b, k, v, s, st);
+    if (dtype == DT_F32) return append_t<64, DT_F32>(c, b, k, v, ks, vs, st);
+    if (dtype == DT_BF16) return append_t<64, DT_BF16>(c, b, k, v, ks, vs, st);
+    return append_t<64, DT_F16>(c, b, k, v, ks, vs, st);
 }
 
-cudaError_t launch_kv8_read(const Kv8Dev& c, const Kv8Batch& b, void* k, void* v, int dtype, const Kv8Strides& s,
-                            cudaStream_t st) {
+cudaError_t launch_kv8_read(const Kv8Dev& c, const Kv8Batch& b, void* k, void* v, int dtype, const Kv8Strides& ks,
+                            const Kv8Strides& vs, cudaStream_t st) {
     if (c.dim == 128) {
-        if (dtype == DT_F32) return read_t<128, DT_F32>(c, b, k, v, s, st);
-        if (dtype == DT_BF16) return read_t<128, DT_BF16>(c, b, k, v, s, st);
-        return read_t<128, DT_F16>(c, b, k, v, s, st);
+        if (dtype == DT_F32) return read_t<128, DT_F32>(c, b, k, v, ks, vs, st);
+        if (dtype == DT_BF16) return read_t<128, DT_BF16>(c, b, k, v, ks, vs, st);
+        return read_t<128, DT_F16>(c, b, k, v, ks, vs, st);
     }
-    if (dtype == DT_F32) return read_t<64, DT_F32>(c, b, k, v, s, st);
-    if (dtype == DT_BF16) return read_t<64, DT_BF16>(c, b, k, v, s, st);
-    return read_t<64, DT_F16>(c, b, k, v, s, st);
+    if (dtype == DT_F32) return read_t<64, DT_F32>(c, b, k, v, ks, vs, st);
+    if (dtype == DT_BF16) return read_t<64, DT_BF16>(c, b, k, v, ks, vs, st);
+    return read_t<64, DT_F16>(c, b, k, v, ks, vs, st);
 }
 
 }  // namespace stt

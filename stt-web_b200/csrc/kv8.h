@@ -60,9 +60,9 @@ size_t kv8_partial_bytes(int dim);
 
 cudaError_t kv8_configure();
 cudaError_t launch_kv8_append(const Kv8Dev& c, const Kv8Batch& b, const void* k, const void* v, int dtype,
-                              const Kv8Strides& s, cudaStream_t st);
-cudaError_t launch_kv8_read(const Kv8Dev& c, const Kv8Batch& b, void* k, void* v, int dtype, const Kv8Strides& s,
-                            cudaStream_t st);
+                              const Kv8Strides& ks, const Kv8Strides& vs, cudaStream_t st);
+cudaError_t launch_kv8_read(const Kv8Dev& c, const Kv8Batch& b, void* k, void* v, int dtype, const Kv8Strides& ks,
+                            const Kv8Strides& vs, cudaStream_t st);
 // The two kernels of the attention: 8 query rows against a split of the keys (any type), and 256 query
 // rows on the 5th-generation tensor cores (16-bit queries and output).
 cudaError_t launch_kv8_prompt(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st);

@@ -47,18 +47,35 @@ bool kv8_sizes(int n_seqs, int heads, int dim, int cap, size_t* codes, size_t* e
     return true;
 }
 
-int check_rows(const char* what, const void* p, int dtype, const Kv8Strides& s) {
-    const int64_t eb = elem_bytes(dtype);
-    if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || s.seq * eb % 16 != 0 || s.token * eb % 16 != 0 || s.head * eb % 16 != 0)
+Kv8Strides strides(const stt_kv8_tensor& t) { return Kv8Strides{t.seq_stride, t.token_stride, t.head_stride}; }
+
+int check_tensor(const char* what, const stt_kv8_tensor& t) {
+    if (t.dtype < DT_F32 || t.dtype > DT_F16) return set_error(STT_E_INVALID_ARG, "%s: dtype %d unknown", what, t.dtype);
+    if (!t.d_data) return set_error(STT_E_INVALID_ARG, "%s: NULL data", what);
+    const int64_t eb = elem_bytes(t.dtype);
+    if ((reinterpret_cast<uintptr_t>(t.d_data) | (uint64_t)(t.seq_stride * eb) | (uint64_t)(t.token_stride * eb) |
+         (uint64_t)(t.head_stride * eb)) % 16 != 0)
         return set_error(STT_E_INVALID_ARG, "%s must start at, and have strides of, multiples of 16 bytes", what);
     return STT_OK;
 }
 
-int check_batch(const stt_kv8_cache* h, const int32_t* d_seqs, int n, const int32_t* d_pos, int n_tokens, int dtype) {
-    if (!h || n < 0 || n_tokens < 0 || (!d_pos && n > 0 && n_tokens > 0)) return set_error(STT_E_INVALID_ARG, "bad arguments");
-    if (dtype < DT_F32 || dtype > DT_F16) return set_error(STT_E_INVALID_ARG, "dtype %d unknown", dtype);
-    if (!d_seqs && n > h->c.n_seqs)
-        return set_error(STT_E_INVALID_ARG, "%d rows for the %d sequences of the cache", n, h->c.n_seqs);
+// A batch's host-side checks; *some is false for one without rows or tokens, which is nothing to do.
+int check_batch(const stt_kv8_cache* h, const stt_kv8_batch* b, bool* some) {
+    if (!h || !b || b->n < 0 || b->n_tokens < 0) return set_error(STT_E_INVALID_ARG, "bad arguments");
+    *some = b->n > 0 && b->n_tokens > 0;
+    if (*some && !b->d_pos) return set_error(STT_E_INVALID_ARG, "NULL positions");
+    if (!b->d_seqs && b->n > h->c.n_seqs)
+        return set_error(STT_E_INVALID_ARG, "%d rows for the %d sequences of the cache", b->n, h->c.n_seqs);
+    return STT_OK;
+}
+Kv8Batch device_batch(const stt_kv8_batch& b) { return Kv8Batch{b.d_seqs, b.d_pos, b.d_count, b.n, b.n_tokens}; }
+
+// K and V of an append or a read.
+int check_kv(const stt_kv8_tensor* k, const stt_kv8_tensor* v) {
+    if (!k || !v) return set_error(STT_E_INVALID_ARG, "NULL argument");
+    TRY(check_tensor("K", *k));
+    TRY(check_tensor("V", *v));
+    if (k->dtype != v->dtype) return set_error(STT_E_INVALID_ARG, "K has dtype %d, V %d", k->dtype, v->dtype);
     return STT_OK;
 }
 
@@ -162,69 +179,60 @@ extern "C" int stt_kv8_cache_status(stt_kv8_cache* h) {
     return set_error(STT_E_DEVICE_FLAG, "an infinity or NaN was appended to this cache and stored as a finite value");
 }
 
-extern "C" int stt_kv8_append_device(stt_kv8_cache* h, const int32_t* d_seqs, int n, const int32_t* d_pos,
-                                     const int32_t* d_count, int n_tokens, const void* d_k, const void* d_v, int dtype,
-                                     int64_t seq_stride, int64_t token_stride, int64_t head_stride, void* cuda_stream) {
+extern "C" int stt_kv8_append_device(stt_kv8_cache* h, const stt_kv8_batch* b, const stt_kv8_tensor* k,
+                                     const stt_kv8_tensor* v, void* cuda_stream) {
     clear_error();
-    TRY(check_batch(h, d_seqs, n, d_pos, n_tokens, dtype));
-    if (n == 0 || n_tokens == 0) return STT_OK;
-    if (!d_k || !d_v) return set_error(STT_E_INVALID_ARG, "NULL argument");
-    if (n_tokens > h->c.cap)
-        return set_error(STT_E_INVALID_ARG, "%d tokens in one call exceed the capacity %d", n_tokens, h->c.cap);
-    const Kv8Strides s{seq_stride, token_stride, head_stride};
-    TRY(check_rows("K", d_k, dtype, s));
-    TRY(check_rows("V", d_v, dtype, s));
-    if ((int64_t)n * (n_tokens / kKv8Block + 2) > INT_MAX / (h->c.heads + 8))
-        return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", n, n_tokens);
+    bool some;
+    TRY(check_batch(h, b, &some));
+    if (!some) return STT_OK;
+    TRY(check_kv(k, v));
+    if (b->n_tokens > h->c.cap)
+        return set_error(STT_E_INVALID_ARG, "%d tokens in one call exceed the capacity %d", b->n_tokens, h->c.cap);
+    if ((int64_t)b->n * (b->n_tokens / kKv8Block + 2) > INT_MAX / (h->c.heads + 8))
+        return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", b->n, b->n_tokens);
     DeviceScope ds(h->device);
     if (!ds.ok) return set_error(STT_E_CUDA, "cudaSetDevice(%d) failed", h->device);
-    CUDA_TRY(launch_kv8_append(h->c, Kv8Batch{d_seqs, d_pos, d_count, n, n_tokens}, d_k, d_v, dtype, s,
+    CUDA_TRY(launch_kv8_append(h->c, device_batch(*b), k->d_data, v->d_data, k->dtype, strides(*k), strides(*v),
                                static_cast<cudaStream_t>(cuda_stream)));
     return STT_OK;
 }
 
-extern "C" int stt_kv8_read_device(const stt_kv8_cache* h, const int32_t* d_seqs, int n, const int32_t* d_pos,
-                                   const int32_t* d_count, int n_tokens, void* d_k, void* d_v, int dtype,
-                                   int64_t seq_stride, int64_t token_stride, int64_t head_stride, void* cuda_stream) {
+extern "C" int stt_kv8_read_device(const stt_kv8_cache* h, const stt_kv8_batch* b, const stt_kv8_tensor* k,
+                                   const stt_kv8_tensor* v, void* cuda_stream) {
     clear_error();
-    TRY(check_batch(h, d_seqs, n, d_pos, n_tokens, dtype));
-    if (n == 0 || n_tokens == 0) return STT_OK;
-    if (!d_k || !d_v) return set_error(STT_E_INVALID_ARG, "NULL argument");
-    const Kv8Strides s{seq_stride, token_stride, head_stride};
-    TRY(check_rows("K", d_k, dtype, s));
-    TRY(check_rows("V", d_v, dtype, s));
-    if ((int64_t)n * (n_tokens / 16 + 1) > INT_MAX / (h->c.heads / 8 + 1))
-        return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", n, n_tokens);
+    bool some;
+    TRY(check_batch(h, b, &some));
+    if (!some) return STT_OK;
+    TRY(check_kv(k, v));
+    if ((int64_t)b->n * (b->n_tokens / 16 + 1) > INT_MAX / (h->c.heads / 8 + 1))
+        return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", b->n, b->n_tokens);
     DeviceScope ds(h->device);
     if (!ds.ok) return set_error(STT_E_CUDA, "cudaSetDevice(%d) failed", h->device);
-    CUDA_TRY(launch_kv8_read(h->c, Kv8Batch{d_seqs, d_pos, d_count, n, n_tokens}, d_k, d_v, dtype, s,
+    CUDA_TRY(launch_kv8_read(h->c, device_batch(*b), k->d_data, v->d_data, k->dtype, strides(*k), strides(*v),
                              static_cast<cudaStream_t>(cuda_stream)));
     return STT_OK;
 }
 
-extern "C" int stt_kv8_attention_device(stt_kv8_cache* h, const int32_t* d_seqs, int n, const int32_t* d_pos,
-                                        const int32_t* d_count, int n_tokens, int n_heads, const void* d_q, int q_dtype,
-                                        int64_t q_seq_stride, int64_t q_token_stride, int64_t q_head_stride,
-                                        const int32_t* d_start, int window, float scale, void* d_out, int out_dtype,
-                                        int64_t out_seq_stride, int64_t out_token_stride, int64_t out_head_stride,
+extern "C" int stt_kv8_attention_device(stt_kv8_cache* h, const stt_kv8_batch* b, const stt_kv8_tensor* q, int n_heads,
+                                        const int32_t* d_start, int window, float scale, const stt_kv8_tensor* out,
                                         void* cuda_stream) {
     clear_error();
-    TRY(check_batch(h, d_seqs, n, d_pos, n_tokens, q_dtype));
-    if (window < 0 || !std::isfinite(scale)) return set_error(STT_E_INVALID_ARG, "bad arguments");
-    if (out_dtype < DT_F32 || out_dtype > DT_F16) return set_error(STT_E_INVALID_ARG, "dtype %d unknown", out_dtype);
+    bool some;
+    TRY(check_batch(h, b, &some));
+    if (window < 0 || !std::isfinite(scale)) return set_error(STT_E_INVALID_ARG, "window %d, scale %g", window, scale);
     if (n_heads <= 0 || n_heads % h->c.heads != 0)
         return set_error(STT_E_INVALID_ARG, "%d query heads over %d K/V heads", n_heads, h->c.heads);
-    if (n == 0 || n_tokens == 0) return STT_OK;
-    if (!d_q || !d_out) return set_error(STT_E_INVALID_ARG, "NULL argument");
+    if (!some) return STT_OK;
+    if (!q || !out) return set_error(STT_E_INVALID_ARG, "NULL argument");
+    TRY(check_tensor("the queries", *q));
+    TRY(check_tensor("the output", *out));
     Kv8Attention a{};
-    a.q = d_q;
-    a.out = d_out;
-    a.qs = Kv8Strides{q_seq_stride, q_token_stride, q_head_stride};
-    a.os = Kv8Strides{out_seq_stride, out_token_stride, out_head_stride};
-    TRY(check_rows("the queries", d_q, q_dtype, a.qs));
-    TRY(check_rows("the output", d_out, out_dtype, a.os));
-    a.q_dtype = q_dtype;
-    a.out_dtype = out_dtype;
+    a.q = q->d_data;
+    a.out = out->d_data;
+    a.qs = strides(*q);
+    a.os = strides(*out);
+    a.q_dtype = q->dtype;
+    a.out_dtype = out->dtype;
     a.group = n_heads / h->c.heads;
     a.window = window;
     a.start = d_start;
@@ -232,13 +240,12 @@ extern "C" int stt_kv8_attention_device(stt_kv8_cache* h, const int32_t* d_seqs,
     a.part = h->part;
     a.tickets = h->tickets;
     a.num_sms = h->num_sms;
-    const int64_t row_groups = ((int64_t)n_tokens * a.group + kKv8Rows - 1) / kKv8Rows;
-    if ((int64_t)n_tokens * a.group > INT_MAX - kKv8Rows || (int64_t)n * h->c.heads > INT_MAX / row_groups)
-        return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", n, n_tokens);
+    const int64_t rows = (int64_t)b->n_tokens * a.group;
+    if (rows > INT_MAX - 256 || (int64_t)b->n * h->c.heads > INT_MAX / (rows / 8 + 1))
+        return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", b->n, b->n_tokens);
     DeviceScope ds(h->device);
     if (!ds.ok) return set_error(STT_E_CUDA, "cudaSetDevice(%d) failed", h->device);
-    CUDA_TRY(launch_kv8_attention(h->c, Kv8Batch{d_seqs, d_pos, d_count, n, n_tokens}, a,
-                                  static_cast<cudaStream_t>(cuda_stream)));
+    CUDA_TRY(launch_kv8_attention(h->c, device_batch(*b), a, static_cast<cudaStream_t>(cuda_stream)));
     return STT_OK;
 }
 
@@ -348,63 +355,62 @@ extern "C" int stt_beam_status(stt_beam* h) {
     return set_error(STT_E_DEVICE_FLAG, "a beam had a NaN or +inf logit or score: its candidates were taken as -inf");
 }
 
-extern "C" int stt_beam_select_device(stt_beam* h, const void* d_logits, int dtype, int64_t row_stride, int batch,
-                                      int beams, int vocab, const float* d_scores, const uint8_t* d_done, int eos,
-                                      float* d_next_scores, int32_t* d_parents, int32_t* d_tokens, uint8_t* d_next_done,
-                                      void* cuda_stream) {
+extern "C" int stt_beam_select_device(stt_beam* h, const stt_beam_step* s, void* cuda_stream) {
     clear_error();
-    if (!h || batch < 0 || (batch > 0 && (!d_logits || !d_scores || !d_next_scores || !d_parents || !d_tokens)))
-        return set_error(STT_E_INVALID_ARG, "bad arguments");
-    if (dtype < DT_F32 || dtype > DT_F16) return set_error(STT_E_INVALID_ARG, "dtype %d unknown", dtype);
-    if (beams < 1 || vocab < 1 || !beam_fits(h, batch, beams, vocab))
-        return set_error(STT_E_INVALID_ARG, "%d utterances, %d beams, %d tokens: the selector was made for %d, %d, %d", batch,
-                         beams, vocab, h->max_batch, h->max_beams, h->max_vocab);
-    if (row_stride < vocab) return set_error(STT_E_INVALID_ARG, "row stride %lld < vocab %d", (long long)row_stride, vocab);
-    if (eos < -1 || eos >= vocab) return set_error(STT_E_INVALID_ARG, "end token %d outside the %d tokens", eos, vocab);
-    if (d_done && eos < 0) return set_error(STT_E_INVALID_ARG, "beams that ended need an end token");
-    if (reinterpret_cast<uintptr_t>(d_logits) % elem_bytes(dtype) != 0)
+    if (!h || !s || s->batch < 0) return set_error(STT_E_INVALID_ARG, "bad arguments");
+    if (s->batch > 0 && (!s->d_logits || !s->d_scores || !s->d_next_scores || !s->d_parents || !s->d_tokens))
+        return set_error(STT_E_INVALID_ARG, "NULL array");
+    if (s->dtype < DT_F32 || s->dtype > DT_F16) return set_error(STT_E_INVALID_ARG, "dtype %d unknown", s->dtype);
+    if (s->beams < 1 || s->vocab < 1 || !beam_fits(h, s->batch, s->beams, s->vocab))
+        return set_error(STT_E_INVALID_ARG, "%d utterances, %d beams, %d tokens: the selector was made for %d, %d, %d", s->batch,
+                         s->beams, s->vocab, h->max_batch, h->max_beams, h->max_vocab);
+    if (s->row_stride < s->vocab)
+        return set_error(STT_E_INVALID_ARG, "row stride %lld < vocab %d", (long long)s->row_stride, s->vocab);
+    if (s->eos < -1 || s->eos >= s->vocab) return set_error(STT_E_INVALID_ARG, "end token %d outside the %d tokens", s->eos, s->vocab);
+    if (s->d_done && s->eos < 0) return set_error(STT_E_INVALID_ARG, "beams that ended need an end token");
+    if (reinterpret_cast<uintptr_t>(s->d_logits) % elem_bytes(s->dtype) != 0)
         return set_error(STT_E_INVALID_ARG, "the logits must be aligned to their type");
-    if (batch == 0) return STT_OK;
+    if (s->batch == 0) return STT_OK;
     BeamArgs a = h->ws;
-    a.logits = d_logits;
-    a.row_stride = row_stride;
-    a.batch = batch;
-    a.beams = beams;
-    a.vocab = vocab;
+    a.logits = s->d_logits;
+    a.row_stride = s->row_stride;
+    a.batch = s->batch;
+    a.beams = s->beams;
+    a.vocab = s->vocab;
     // about four CTAs per SM, twice what is resident (rows that ended leave gaps); a CTA takes whole tiles
-    const int tiles = beam_tiles(vocab), rows = batch * beams;
-    const int want = std::min(beam_max_chunks(vocab), (4 * h->num_sms + rows - 1) / rows);
+    const int tiles = beam_tiles(s->vocab), rows = s->batch * s->beams;
+    const int want = std::min(beam_max_chunks(s->vocab), (4 * h->num_sms + rows - 1) / rows);
     a.tiles_per_chunk = (tiles + want - 1) / want;
     a.chunks = (tiles + a.tiles_per_chunk - 1) / a.tiles_per_chunk;
-    a.scores = d_scores;
-    a.done = d_done;
-    a.eos = eos;
-    a.next_scores = d_next_scores;
-    a.parents = d_parents;
-    a.tokens = d_tokens;
-    a.next_done = d_next_done;
+    a.scores = s->d_scores;
+    a.done = s->d_done;
+    a.eos = s->eos;
+    a.next_scores = s->d_next_scores;
+    a.parents = s->d_parents;
+    a.tokens = s->d_tokens;
+    a.next_done = s->d_next_done;
     DeviceScope ds(h->device);
     if (!ds.ok) return set_error(STT_E_CUDA, "cudaSetDevice(%d) failed", h->device);
-    CUDA_TRY(launch_beam_select(a, dtype, static_cast<cudaStream_t>(cuda_stream)));
+    CUDA_TRY(launch_beam_select(a, s->dtype, static_cast<cudaStream_t>(cuda_stream)));
     return STT_OK;
 }
 
-extern "C" int stt_beam_reorder_device(int device, void* d_states, int64_t row_stride, int segments,
-                                       int64_t segment_stride, int64_t units, int64_t unit_bytes,
-                                       const int32_t* d_parents, int groups, int beams, const int32_t* d_held,
-                                       void* cuda_stream) {
+extern "C" int stt_beam_reorder_device(int device, const stt_beam_states* s, void* cuda_stream) {
     clear_error();
-    if (!d_states || !d_parents || segments < 0 || units < 0 || unit_bytes <= 0 || groups < 0)
+    if (!s || !s->d_states || !s->d_parents || s->segments < 0 || s->units < 0 || s->unit_bytes <= 0 || s->groups < 0)
         return set_error(STT_E_INVALID_ARG, "bad arguments");
-    if (beams < 1 || beams > kMaxBeams) return set_error(STT_E_INVALID_ARG, "beams %d out of range [1, %d]", beams, kMaxBeams);
-    const __int128 segment = (__int128)units * unit_bytes;
-    if (segment > (__int128)1 << 38) return set_error(STT_E_INVALID_ARG, "segments of %lld x %lld bytes are too large", (long long)units, (long long)unit_bytes);
+    if (s->beams < 1 || s->beams > kMaxBeams)
+        return set_error(STT_E_INVALID_ARG, "beams %d out of range [1, %d]", s->beams, kMaxBeams);
+    const __int128 segment = (__int128)s->units * s->unit_bytes;
+    const int64_t rows = (int64_t)s->groups * s->beams;
+    if (segment > (__int128)1 << 38)
+        return set_error(STT_E_INVALID_ARG, "segments of %lld x %lld bytes are too large", (long long)s->units, (long long)s->unit_bytes);
     // rows and segments must not overlap: a position belongs to one of them
-    if ((segments > 1 && segment_stride < segment) || (groups * (int64_t)beams > 1 && row_stride < 0))
+    if ((s->segments > 1 && s->segment_stride < segment) || (rows > 1 && s->row_stride < 0))
         return set_error(STT_E_INVALID_ARG, "segments overlap");
-    const __int128 row = segments == 0 ? 0 : (__int128)(segments - 1) * segment_stride + segment;
-    const bool interleaved = (int64_t)groups * beams > 1 && row_stride < row;
-    if (interleaved && !(row_stride >= segment && segment_stride >= (__int128)row_stride * ((int64_t)groups * beams - 1) + segment))
+    const __int128 row = s->segments == 0 ? 0 : (__int128)(s->segments - 1) * s->segment_stride + segment;
+    if (rows > 1 && s->row_stride < row &&
+        !(s->row_stride >= segment && s->segment_stride >= (__int128)s->row_stride * (rows - 1) + segment))
         return set_error(STT_E_INVALID_ARG, "rows overlap");
     DeviceScope ds(device);
     if (!ds.ok) {
@@ -412,18 +418,18 @@ extern "C" int stt_beam_reorder_device(int device, void* d_states, int64_t row_s
         return set_error(STT_E_INVALID_ARG, "cannot select device %d", device);
     }
     ReorderArgs a{};
-    a.states = static_cast<uint8_t*>(d_states);
-    a.row_stride = row_stride;
-    a.segment_stride = segment_stride;
-    a.inner = std::max(1, segments);
+    a.states = static_cast<uint8_t*>(s->d_states);
+    a.row_stride = s->row_stride;
+    a.segment_stride = s->segment_stride;
+    a.segments = s->segments;
+    a.inner = std::max(1, s->segments);
+    a.units = s->units;
+    a.unit_bytes = s->unit_bytes;
     a.per_unit = 1;
-    a.units = units;
-    a.unit_bytes = unit_bytes;
-    a.segments = segments;
-    a.groups = groups;
-    a.beams = beams;
-    a.parents = d_parents;
-    a.held = d_held;
+    a.groups = s->groups;
+    a.beams = s->beams;
+    a.parents = s->d_parents;
+    a.held = s->d_held;
     CUDA_TRY(launch_reorder(a, static_cast<cudaStream_t>(cuda_stream)));
     return STT_OK;
 }

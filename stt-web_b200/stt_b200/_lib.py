@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsttb200.so")
@@ -95,6 +96,12 @@ class stt_kv8_cache_info(C.Structure):
     ]
 
 
+# stt_kv8_batch, stt_kv8_tensor, stt_beam_step and stt_beam_states, packed (native alignment)
+KV8_BATCH = struct.Struct("PPPii")
+KV8_TENSOR = struct.Struct("Pqqqii")
+BEAM_STEP = struct.Struct("PqiiiiPPPPPPii")
+BEAM_STATES = struct.Struct("PqqqqPPiiii")
+
 P = C.c_void_p
 U8P = C.POINTER(C.c_uint8)
 U32P = C.POINTER(C.c_uint32)
@@ -139,19 +146,15 @@ SIGNATURES = {
     "stt_kv8_cache_destroy": (C.c_int, [P]),
     "stt_kv8_cache_get_info": (C.c_int, [P, C.POINTER(stt_kv8_cache_info)]),
     "stt_kv8_cache_status": (C.c_int, [P]),
-    "stt_kv8_append_device": (C.c_int, [P, P, C.c_int, P, P, C.c_int, P, P, C.c_int, C.c_int64, C.c_int64, C.c_int64, P]),
-    "stt_kv8_read_device": (C.c_int, [P, P, C.c_int, P, P, C.c_int, P, P, C.c_int, C.c_int64, C.c_int64, C.c_int64, P]),
-    "stt_kv8_attention_device": (C.c_int, [P, P, C.c_int, P, P, C.c_int, C.c_int, P, C.c_int, C.c_int64, C.c_int64,
-                                           C.c_int64, P, C.c_int, C.c_float, P, C.c_int, C.c_int64, C.c_int64, C.c_int64,
-                                           P]),
+    "stt_kv8_append_device": (C.c_int, [P, P, P, P, P]),
+    "stt_kv8_read_device": (C.c_int, [P, P, P, P, P]),
+    "stt_kv8_attention_device": (C.c_int, [P, P, P, C.c_int, P, C.c_int, C.c_float, P, P]),
     "stt_kv8_reorder_device": (C.c_int, [P, P, C.c_int, C.c_int, P, P]),
     "stt_beam_create": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(P)]),
     "stt_beam_destroy": (C.c_int, [P]),
     "stt_beam_status": (C.c_int, [P]),
-    "stt_beam_select_device": (C.c_int, [P, P, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, P, P, C.c_int, P, P, P, P,
-                                         P]),
-    "stt_beam_reorder_device": (C.c_int, [C.c_int, P, C.c_int64, C.c_int, C.c_int64, C.c_int64, C.c_int64, P, C.c_int,
-                                          C.c_int, P, P]),
+    "stt_beam_select_device": (C.c_int, [P, P, P]),
+    "stt_beam_reorder_device": (C.c_int, [C.c_int, P, P]),
     "stt_spm_decoder_create": (C.c_int, [U8P, C.c_size_t, C.POINTER(P)]),
     "stt_spm_decoder_destroy": (C.c_int, [P]),
     "stt_spm_vocab_len": (C.c_int, [P, C.POINTER(C.c_int64)]),

@@ -12,7 +12,8 @@ import ctypes as C
 import math
 from typing import Optional
 
-from ._lib import STT_E_INVALID_ARG, SttError, check, lib, stt_kv8_cache_info
+from ._lib import (BEAM_STATES, BEAM_STEP, KV8_BATCH, KV8_TENSOR, STT_E_INVALID_ARG, SttError, check, lib,
+                   stt_kv8_cache_info)
 
 _NAMES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2, "torch.int32": 3, "torch.uint8": 4}
 _F32, _I32, _U8 = 0, 3, 4
@@ -51,6 +52,11 @@ def _whole(t, n: int, device: int, where: str, what: str, code: int = _I32) -> i
     return t.data_ptr()
 
 
+# places of a call's batch and its two tensors among the packed arguments
+_A = KV8_BATCH.size
+_B = _A + KV8_TENSOR.size
+
+
 class Kv8Cache:
     """K and V of ``n_seqs`` sequences as signed bytes with a power-of-two scale for each block of 16
     tokens and head (stt_kv8_* of include/stt_b200.h).  ``memory``: a device tensor of ``bytes()``
@@ -70,7 +76,14 @@ class Kv8Cache:
                                          memory.data_ptr() if memory is not None else None, C.byref(h)), where)
         self._h = h
         self.memory = memory
+        self._prepare()
         self.n_seqs, self.n_kv_heads, self.head_dim, self.capacity, self.device = n_seqs, n_kv_heads, head_dim, capacity, device
+
+    def _prepare(self) -> None:
+        L = lib()
+        self._append, self._read, self._attention = L.stt_kv8_append_device, L.stt_kv8_read_device, L.stt_kv8_attention_device
+        self._args = C.create_string_buffer(_B + KV8_TENSOR.size)
+        self._at = C.addressof(self._args)
 
     @staticmethod
     def bytes(n_seqs: int, n_kv_heads: int, head_dim: int, capacity: int) -> int:
@@ -99,41 +112,47 @@ class Kv8Cache:
         """Waits for the device; raises SttError for what the calls since the last check reported."""
         check(lib().stt_kv8_cache_status(self._h), "stt_kv8_cache_status")
 
-    def _rows(self, t, where: str, heads: Optional[int] = None):
-        shape, stride = t.shape, t.stride()
-        if len(shape) != 4 or shape[3] != self.head_dim or stride[3] != 1 or (heads is not None and shape[2] != heads):
+    def _tensor(self, t, at: int, where: str, heads: int = 0):
+        """Packs tensor t into place `at` of the call's arguments; returns (n, tokens, heads)."""
+        n, tokens, h, dim = shape = t.shape if len(t.shape) == 4 else (0, 0, 0, -1)
+        seq, token, head, last = t.stride() if dim >= 0 else (0, 0, 0, 0)
+        if dim != self.head_dim or last != 1 or (heads and h != heads):
             _refuse(where, f"tensors are [n, tokens, {heads or 'heads'}, {self.head_dim}] with the last dimension contiguous, got "
-                           f"{tuple(shape)} with strides {tuple(stride)}")
-        _on(t, self.device, where)
-        return shape[0], shape[1], shape[2], stride
+                           f"{tuple(t.shape)} with strides {tuple(t.stride())}")
+        if t.get_device() != self.device:
+            _on(t, self.device, where)
+        KV8_TENSOR.pack_into(self._args, at, t.data_ptr(), seq, token, head, _dtype(t, where), 0)
+        return shape[:3]
 
-    def _batch(self, n: int, pos, count, seqs, where: str):
+    def _batch(self, n: int, tokens: int, pos, count, seqs, where: str):
         d = self.device
-        return (None if seqs is None else _whole(seqs, n, d, where, "seqs"), _whole(pos, n, d, where, "pos"),
-                None if count is None else _whole(count, n, d, where, "count"))
+        KV8_BATCH.pack_into(self._args, 0, 0 if seqs is None else _whole(seqs, n, d, where, "seqs"),
+                            _whole(pos, n, d, where, "pos"), 0 if count is None else _whole(count, n, d, where, "count"), n, tokens)
 
     def append(self, k, v, pos, count=None, seqs=None, stream: int = 0) -> None:
         """Writes k and v [n, tokens, n_kv_heads, head_dim]: row i's count[i] tokens (None: all) at the
         positions pos[i] on of sequence seqs[i] (None: i)."""
         where = "stt_kv8_append_device"
-        n, t, _, s = self._rows(k, where, self.n_kv_heads)
-        if v.shape != k.shape or v.stride() != s or v.dtype != k.dtype:
-            _refuse(where, "k and v must have one shape, one dtype and the same strides")
-        _on(v, self.device, where)
-        a, p, c = self._batch(n, pos, count, seqs, where)
-        check(lib().stt_kv8_append_device(self._h, a, n, p, c, t, k.data_ptr(), v.data_ptr(), _dtype(k, where), s[0], s[1],
-                                          s[2], stream), where)
+        shape = self._tensor(k, _A, where, self.n_kv_heads)
+        if self._tensor(v, _B, where, self.n_kv_heads) != shape:
+            _refuse(where, f"k is {tuple(k.shape)}, v {tuple(v.shape)}")
+        self._batch(shape[0], shape[1], pos, count, seqs, where)
+        at = self._at
+        code = self._append(self._h, at, at + _A, at + _B, stream)
+        if code:
+            check(code, where)
 
     def read(self, k, v, pos, count=None, seqs=None, stream: int = 0) -> None:
         """Reads the values of a range of tokens into k and v [n, tokens, n_kv_heads, head_dim]."""
         where = "stt_kv8_read_device"
-        n, t, _, s = self._rows(k, where, self.n_kv_heads)
-        if v.shape != k.shape or v.stride() != s or v.dtype != k.dtype:
-            _refuse(where, "k and v must have one shape, one dtype and the same strides")
-        _on(v, self.device, where)
-        a, p, c = self._batch(n, pos, count, seqs, where)
-        check(lib().stt_kv8_read_device(self._h, a, n, p, c, t, k.data_ptr(), v.data_ptr(), _dtype(k, where), s[0], s[1],
-                                        s[2], stream), where)
+        shape = self._tensor(k, _A, where, self.n_kv_heads)
+        if self._tensor(v, _B, where, self.n_kv_heads) != shape:
+            _refuse(where, f"k is {tuple(k.shape)}, v {tuple(v.shape)}")
+        self._batch(shape[0], shape[1], pos, count, seqs, where)
+        at = self._at
+        code = self._read(self._h, at, at + _A, at + _B, stream)
+        if code:
+            check(code, where)
 
     def attention(self, q, out, pos, count=None, seqs=None, start=None, window: int = 0, scale: Optional[float] = None,
                   stream: int = 0) -> None:
@@ -141,16 +160,17 @@ class Kv8Cache:
         pos, count and seqs has written, into ``out`` of the same shape (any of the dtypes).
         scale None: 1 / sqrt(head_dim)."""
         where = "stt_kv8_attention_device"
-        n, t, heads, qs = self._rows(q, where)
-        m, u, oh, os = self._rows(out, where)
-        if (n, t, heads) != (m, u, oh):
+        shape = self._tensor(q, _A, where)
+        if self._tensor(out, _B, where) != shape:
             _refuse(where, f"q is {tuple(q.shape)}, out {tuple(out.shape)}")
-        a, p, c = self._batch(n, pos, count, seqs, where)
-        check(lib().stt_kv8_attention_device(
-            self._h, a, n, p, c, t, heads, q.data_ptr(), _dtype(q, where), qs[0], qs[1], qs[2],
-            None if start is None else _whole(start, n, self.device, where, "start"), window,
-            1.0 / math.sqrt(self.head_dim) if scale is None else scale, out.data_ptr(), _dtype(out, where), os[0], os[1],
-            os[2], stream), where)
+        n, tokens, heads = shape
+        self._batch(n, tokens, pos, count, seqs, where)
+        at = self._at
+        code = self._attention(self._h, at, at + _A, heads,
+                               None if start is None else _whole(start, n, self.device, where, "start"), window,
+                               1.0 / math.sqrt(self.head_dim) if scale is None else scale, at + _B, stream)
+        if code:
+            check(code, where)
 
     def reorder(self, parents, held=None, stream: int = 0) -> None:
         """Sequence g * beams + b becomes what sequence g * beams + parents[g, b] was, in place;
@@ -175,6 +195,12 @@ class BeamSelector:
         check(lib().stt_beam_create(device, max_batch, max_beams, max_vocab, C.byref(h)), "stt_beam_create")
         self._h = h
         self.device = device
+        self._prepare()
+
+    def _prepare(self) -> None:
+        self._select = lib().stt_beam_select_device
+        self._args = C.create_string_buffer(BEAM_STEP.size)
+        self._at = C.addressof(self._args)
 
     def close(self) -> None:
         if self._h:
@@ -207,13 +233,15 @@ class BeamSelector:
             _refuse(where, f"logits {tuple(logits.shape)} with strides {tuple(stride)} for {batch} x {beams} beams")
         d = self.device
         _on(logits, d, where)
-        check(lib().stt_beam_select_device(
-            self._h, logits.data_ptr(), _dtype(logits, where), stride[0] if rows > 1 else vocab, batch, beams, vocab,
-            _whole(scores, rows, d, where, "scores", _F32),
-            None if done is None else _whole(done, rows, d, where, "done", _U8), eos,
-            _whole(next_scores, rows, d, where, "next_scores", _F32),
-            _whole(parents, rows, d, where, "parents"), _whole(tokens, rows, d, where, "tokens"),
-            None if next_done is None else _whole(next_done, rows, d, where, "next_done", _U8), stream), where)
+        BEAM_STEP.pack_into(
+            self._args, 0, logits.data_ptr(), stride[0] if rows > 1 else vocab, _dtype(logits, where), batch, beams, vocab,
+            _whole(scores, rows, d, where, "scores", _F32), 0 if done is None else _whole(done, rows, d, where, "done", _U8),
+            _whole(next_scores, rows, d, where, "next_scores", _F32), _whole(parents, rows, d, where, "parents"),
+            _whole(tokens, rows, d, where, "tokens"),
+            0 if next_done is None else _whole(next_done, rows, d, where, "next_done", _U8), eos, 0)
+        code = self._select(self._h, self._at, stream)
+        if code:
+            check(code, where)
 
 
 def beam_reorder(states, parents, held=None, stream: int = 0) -> None:
@@ -236,7 +264,8 @@ def beam_reorder(states, parents, held=None, stream: int = 0) -> None:
     d = states.get_device()
     if d < 0:
         _refuse(where, f"the states are on {states.device}")
-    check(lib().stt_beam_reorder_device(d, states.data_ptr(), stride[0] * size, shape[1], stride[1] * size, shape[2],
-                                        inner // shape[2] * size, _whole(parents, groups * beams, d, where, "parents"),
-                                        groups, beams, None if held is None else _whole(held, groups * beams, d, where, "held"),
-                                        stream), where)
+    n = groups * beams
+    args = BEAM_STATES.pack(states.data_ptr(), stride[0] * size, stride[1] * size, shape[2], inner // shape[2] * size,
+                            _whole(parents, n, d, where, "parents"), 0 if held is None else _whole(held, n, d, where, "held"),
+                            shape[1], groups, beams, 0)
+    check(lib().stt_beam_reorder_device(d, args, stream), where)

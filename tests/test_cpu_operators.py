@@ -8,7 +8,7 @@ import pytest
 
 import operators_ref as R
 from stt_b200 import BeamSelector, Kv8Cache, SttError, beam_reorder
-from stt_b200._lib import STT_E_INVALID_ARG, lib
+from stt_b200._lib import BEAM_STATES, STT_E_INVALID_ARG, lib
 
 
 def refused(rc, text):
@@ -37,14 +37,14 @@ def test_cache_bytes():
 
 def test_calls_without_a_handle_are_refused():
     L = lib()
-    refused(L.stt_kv8_append_device(None, None, 1, None, None, 1, None, None, 0, 0, 0, 0, None), "bad arguments")
-    refused(L.stt_kv8_read_device(None, None, 1, None, None, 1, None, None, 0, 0, 0, 0, None), "bad arguments")
-    refused(L.stt_kv8_attention_device(None, None, 1, None, None, 1, 1, None, 0, 0, 0, 0, None, 0, 1.0, None, 0, 0, 0, 0, None),
-            "bad arguments")
+    refused(L.stt_kv8_append_device(None, None, None, None, None), "bad arguments")
+    refused(L.stt_kv8_read_device(None, None, None, None, None), "bad arguments")
+    refused(L.stt_kv8_attention_device(None, None, None, 1, None, 0, 1.0, None, None), "bad arguments")
     refused(L.stt_kv8_reorder_device(None, None, 1, 1, None, None), "bad arguments")
     refused(L.stt_kv8_cache_status(None), "NULL")
     refused(L.stt_kv8_cache_get_info(None, None), "NULL")
-    refused(L.stt_beam_select_device(None, None, 0, 1, 1, 1, 1, None, None, -1, None, None, None, None, None), "bad arguments")
+    refused(L.stt_beam_select_device(None, None, None), "bad arguments")
+    refused(L.stt_beam_reorder_device(0, None, None), "bad arguments")
     refused(L.stt_beam_status(None), "NULL")
     assert L.stt_kv8_cache_destroy(None) == 0 and L.stt_beam_destroy(None) == 0
 
@@ -56,11 +56,12 @@ def test_selector_sizes_are_checked(args):
 
 
 def test_reorder_layouts_are_checked():
-    L, p = lib(), C.c_void_p(16)
-    call = lambda **k: L.stt_beam_reorder_device(*{**dict(device=0, states=p, row=64, segments=2, segment=32, units=4, unit=8,  # noqa: E731
-                                                          parents=p, groups=1, beams=2, held=None, stream=None), **k}.values())
-    refused(call(states=None), "bad arguments")
-    refused(call(parents=None), "bad arguments")
+    def call(**k):
+        f = dict(states=16, row=64, segment=32, units=4, unit=8, parents=16, held=0, segments=2, groups=1, beams=2, reserved=0)
+        return lib().stt_beam_reorder_device(0, BEAM_STATES.pack(*{**f, **k}.values()), None)
+
+    refused(call(states=0), "bad arguments")
+    refused(call(parents=0), "bad arguments")
     refused(call(unit=0), "bad arguments")
     refused(call(units=-1), "bad arguments")
     refused(call(beams=0), "beams")
@@ -89,6 +90,7 @@ class FakeTensor:
 
 def cache():
     c = Kv8Cache.__new__(Kv8Cache)
+    c._prepare()
     c._h, c.n_seqs, c.n_kv_heads, c.head_dim, c.capacity, c.device = None, 4, 2, 64, 32, 0
     return c
 
@@ -118,6 +120,7 @@ def test_the_binding_checks_tensors_before_it_calls():
     with pytest.raises(SttError):
         c.reorder(FakeTensor([4], "torch.int32"))
     s = BeamSelector.__new__(BeamSelector)
+    s._prepare()
     s._h, s.device = None, 0
     f = lambda d="torch.float32", shape=(2, 3): FakeTensor(shape, d)  # noqa: E731
     good = dict(logits=f(shape=(6, 9)), scores=f(), next_scores=f(), parents=f("torch.int32"), tokens=f("torch.int32"))

@@ -127,6 +127,10 @@ def test_append_and_read_take_strided_tensors():
     p.cache.append(heads_first, heads_first, i32([8, 19, 45]))
     p.append(heads_first, heads_first, [8, 19, 45], [5, 5, 5], [0, 1, 2])
     p.same()
+    # V laid out another way than K
+    p.cache.append(x, heads_first.to(torch.bfloat16), i32([13, 24, 50]))
+    p.append(x, heads_first.to(torch.bfloat16), [13, 24, 50], [5, 5, 5], [0, 1, 2])
+    p.same()
     out = torch.zeros(3, 5, 3, 2, 128, device="cuda")
     p.cache.read(out[:, :, 0], out[:, :, 2], i32([8, 19, 45]))
     for i, first in enumerate([8, 19, 45]):
