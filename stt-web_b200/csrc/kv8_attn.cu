@@ -28,13 +28,16 @@
 #include <algorithm>
 
 #include "kv8_attn.cuh"
+#include "tcgen05.cuh"
 
 namespace stt {
 
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kMaxSplits = 256;
+constexpr int kMaxParts = 64;
+constexpr int kMaxCluster = 8;
+constexpr int kMinBlocks = 4;   // of a warp in a part that is joined through memory
 // Query rows of a CTA, stages of a warp's ring, CTAs per SM.
 template <bool NARROW>
 struct Shape {
@@ -55,6 +58,29 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Cluster barrier, and loads from the same place of CTA `rank`'s shared memory.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_at(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr, int rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_at(addr, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_at(addr, rank))
+                 : "memory");
+    return v;
 }
 
 // Transposes the 8 x 8 matrix of 16-bit elements that the warp holds two to a lane, row g columns 2t, 2t + 1.
@@ -111,11 +137,13 @@ __device__ __forceinline__ void load16(const void* base, int dtype, int64_t at, 
 template <class State, class Piece>
 __device__ __forceinline__ RowState merge_parts(int n, State state, Piece piece, float4* out) {
     RowState r{-FLT_MAX, 0.0f};
+#pragma unroll
     for (int j = 0; j < n; ++j) {
         const RowState s = state(j);
         if (s.l != 0.0f) r.M = fmaxf(r.M, s.M);
     }
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
     for (int j = 0; j < n; ++j) {
         const RowState s = state(j);
         if (s.l == 0.0f) continue;
@@ -133,10 +161,12 @@ __device__ __forceinline__ float4 row_output(const RowState& r, float4 o) {
     return make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
 }
 
-// CTA ((batch row * row_groups + row group) * heads + head) * max_splits + split.
+// CTA (((batch row * row_groups + row group) * heads + head) * max_parts + part) * cluster + rank.  An
+// item's keys are cut into parts x cluster equal runs of blocks; a cluster joins its runs through shared
+// memory, the last cluster of an item its parts through global memory.
 template <int D, bool NARROW>
 __global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kernel(Kv8Dev c, Kv8Batch b, Kv8Attention a, int row_groups,
-                                                                int max_splits) {
+                                                                int max_parts, int cluster) {
     constexpr int KS = D / 16;          // k steps of the first product
     constexpr int NT = NARROW ? D / 16 : D / 8;  // tiles of 16 (8) dimensions of the second
     constexpr int ROWS = Shape<NARROW>::kRows, kStages = Shape<NARROW>::kStages;
@@ -146,9 +176,10 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kern
     constexpr int VW = VB / 4;          // in words
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ RowState sm_state[kWarps][ROWS];
+    __shared__ RowState own_state[ROWS];
     __shared__ uint32_t last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % max_splits, item = blockIdx.x / max_splits;
+    const int rank = blockIdx.x % cluster, part_of = blockIdx.x / cluster % max_parts, item = blockIdx.x / cluster / max_parts;
     const int h = item % c.heads, rg = item / c.heads % row_groups, i = item / c.heads / row_groups;
     Kv8Row row;
     if (!kv8_row(c, b, i, &row)) return;
@@ -164,10 +195,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kern
     const int first = sight.lo(row.pos + t0), end = row.pos + t1;  // positions that some row sees
     const int kb0 = first / kKv8Block;
     const int nb = first <= end ? end / kKv8Block - kb0 + 1 : 0;
-    // a split takes at least one block per warp, so short contexts use fewer splits than were launched
-    const int splits = max(1, min(max_splits, nb / kWarps));
-    if (split >= splits) return;
-    const int sb0 = kb0 + (int)((int64_t)nb * split / splits), sb1 = kb0 + (int)((int64_t)nb * (split + 1) / splits);
+    // a short context uses fewer parts than were launched
+    const int parts = max(1, min(max_parts, nb / (cluster * kWarps * kMinBlocks)));
+    if (part_of >= parts) return;
+    const int runs = parts * cluster, run = part_of * cluster + rank;
+    const int sb0 = kb0 + (int)((int64_t)nb * run / runs), sb1 = kb0 + (int)((int64_t)nb * (run + 1) / runs);
     const int64_t head = (int64_t)row.seq * c.heads + h;
     const int8_t* kbase = c.kc + head * c.cap * D;
     const int8_t* vbase = c.vc + head * c.cap * D;
@@ -473,48 +505,79 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kern
         const int token = (r0 + r) / a.group, qh = h * a.group + (r0 + r) % a.group;
         store4(a.out, a.out_dtype, i * a.os.seq + (int64_t)token * a.os.token + qh * a.os.head + 4 * piece, v);
     };
+    // the CTA's pieces, then the cluster's: each CTA of it joins and passes on a share of them, from all
+    // CTAs' shared memory
+    float4* own = so + kWarps * ROWS * (D / 4);
     constexpr int STRIDE = ROWS * (D + 4);
-    float* part = a.part + (int64_t)blockIdx.x * STRIDE;
-    for (int p = threadIdx.x; p < pieces; p += kWarps * 32) {
+    float* part = a.part + ((int64_t)item * max_parts + part_of) * STRIDE;
+    auto pass_on = [&](int p, const RowState& rs, float4 v) {
         const int r = p / (D / 4), piece = p % (D / 4);
-        float4 v;
-        const RowState rs = merge_parts(
-            kWarps, [&](int w) { return sm_state[w][r]; }, [&](int w) { return so[so_at(w, r, piece)]; }, &v);
-        if (splits == 1) {
+        if (parts == 1) {
             write_out(r, piece, row_output(rs, v));
         } else {
             *reinterpret_cast<float4*>(part + r * (D + 4) + 4 + 4 * piece) = v;
             if (piece == 0) *reinterpret_cast<float4*>(part + r * (D + 4)) = make_float4(rs.M, rs.l, 0.0f, 0.0f);
         }
+    };
+    for (int p = threadIdx.x; p < pieces; p += kWarps * 32) {
+        const int r = p / (D / 4), piece = p % (D / 4);
+        float4 v;
+        const RowState rs = merge_parts(
+            kWarps, [&](int w) { return sm_state[w][r]; }, [&](int w) { return so[so_at(w, r, piece)]; }, &v);
+        if (cluster == 1) {
+            pass_on(p, rs, v);
+        } else {
+            own[p] = v;
+            if (piece == 0) own_state[r] = rs;
+        }
     }
-    if (splits == 1) return;
-    // the last of the item's splits merges them in split order, so the result does not depend on which
+    if (cluster > 1) {
+        cluster_sync();
+        for (int p = threadIdx.x * cluster + rank; p < pieces; p += kWarps * 32 * cluster) {
+            float2 st_of[kMaxCluster];
+            float4 v_of[kMaxCluster];
+#pragma unroll
+            for (int j = 0; j < kMaxCluster; ++j) {
+                const int from = j < cluster ? j : rank;
+                st_of[j] = cluster_load2(smem_u32(&own_state[p / (D / 4)]), from);
+                v_of[j] = cluster_load4(smem_u32(&own[p]), from);
+                if (j >= cluster) st_of[j].y = 0.0f;
+            }
+            float4 v;
+            const RowState rs = merge_parts(
+                kMaxCluster, [&](int j) { return RowState{st_of[j].x, st_of[j].y}; }, [&](int j) { return v_of[j]; }, &v);
+            pass_on(p, rs, v);
+        }
+        cluster_sync();  // no CTA leaves while another reads its shared memory
+    }
+    if (parts == 1) return;
+    // the last of the item's CTAs joins the parts in their order, so the result does not depend on which
     // one that is, and leaves the ticket at zero for the next call
     __syncthreads();
-    if (threadIdx.x == 0) last = ticket(a.tickets + item) == (uint32_t)(splits - 1);
+    if (threadIdx.x == 0) last = ticket(a.tickets + item) == (uint32_t)(parts * cluster - 1);
     __syncthreads();
     if (!last) return;
-    // each row's factors first, then the pieces, with the splits shared among as many threads as a piece
+    // each row's factors first, then the pieces, with the parts shared among as many threads as a piece
     // can have: every load is independent of the others
-    const float* parts = a.part + (int64_t)item * max_splits * STRIDE;
-    float2* factor = reinterpret_cast<float2*>(smem);                                      // [rows][splits] (M, l), then 2^(M - max)
-    float4* sums = reinterpret_cast<float4*>(smem + kMaxSplits * ROWS * sizeof(float2));   // [threads]
-    for (int p = threadIdx.x; p < rows * splits; p += kWarps * 32)
-        factor[p] = __ldcg(reinterpret_cast<const float2*>(parts + (int64_t)(p % splits) * STRIDE + p / splits * (D + 4)));
+    const float* all = a.part + (int64_t)item * max_parts * STRIDE;
+    float2* factor = reinterpret_cast<float2*>(smem);                                      // [rows][parts] (M, l), then 2^(M - max)
+    float4* sums = reinterpret_cast<float4*>(smem + kMaxParts * ROWS * sizeof(float2));   // [threads]
+    for (int p = threadIdx.x; p < rows * parts; p += kWarps * 32)
+        factor[p] = __ldcg(reinterpret_cast<const float2*>(all + (int64_t)(p % parts) * STRIDE + p / parts * (D + 4)));
     __syncthreads();
     for (int r = warp; r < rows; r += kWarps) {
         float M = -FLT_MAX, l = 0.0f;
-        for (int j = lane; j < splits; j += 32) {
-            const float2 x = factor[r * splits + j];
+        for (int j = lane; j < parts; j += 32) {
+            const float2 x = factor[r * parts + j];
             if (x.y != 0.0f) M = fmaxf(M, x.x);
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
-        for (int j = lane; j < splits; j += 32) {
-            const float2 x = factor[r * splits + j];
+        for (int j = lane; j < parts; j += 32) {
+            const float2 x = factor[r * parts + j];
             const float f = x.y != 0.0f ? exp2f(x.x - M) : 0.0f;
             l = fmaf(x.y, f, l);
-            factor[r * splits + j].x = f;
+            factor[r * parts + j].x = f;
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, d);
@@ -524,29 +587,29 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kern
     constexpr int PIECES = ROWS * (D / 4);
     constexpr int SHARE = PIECES >= kWarps * 32 ? 1 : kWarps * 32 / PIECES;  // threads of a piece
     for (int p0 = 0; p0 < pieces; p0 += kWarps * 32 / SHARE) {
-        const int p = p0 + threadIdx.x / SHARE, part_of = threadIdx.x % SHARE;
+        const int p = p0 + threadIdx.x / SHARE, share_of = threadIdx.x % SHARE;
         const int r = p / (D / 4), piece = p % (D / 4);
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (p < pieces) {
-            const float* src = parts + r * (D + 4) + 4 + 4 * piece;
+            const float* src = all + r * (D + 4) + 4 + 4 * piece;
 #pragma unroll 8
-            for (int j = part_of; j < splits; j += SHARE) {
+            for (int j = share_of; j < parts; j += SHARE) {
                 const float4 x = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)j * STRIDE));
-                const float f = factor[r * splits + j].x;
+                const float f = factor[r * parts + j].x;
                 v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
             }
         }
         if constexpr (SHARE > 1) {
             sums[threadIdx.x] = v;
             __syncthreads();
-            if (part_of == 0)
+            if (share_of == 0)
                 for (int e = 1; e < SHARE; ++e) {
                     const float4 x = sums[threadIdx.x + e];
                     v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
                 }
             __syncthreads();
         }
-        if (p < pieces && part_of == 0) write_out(r, piece, row_output(sm_state[0][r], v));
+        if (p < pieces && share_of == 0) write_out(r, piece, row_output(sm_state[0][r], v));
     }
     if (threadIdx.x == 0) a.tickets[item] = 0u;
 }
@@ -555,7 +618,33 @@ template <int D, bool NARROW>
 constexpr size_t attend_smem() {
     // the warps' rings; at the end of a split context the factors and shared sums of its merge
     return std::max((size_t)kWarps * Shape<NARROW>::kStages * 2 * 16 * D,
-                    kMaxSplits * Shape<NARROW>::kRows * sizeof(float2) + kWarps * 32 * sizeof(float4));
+                    kMaxParts * Shape<NARROW>::kRows * sizeof(float2) + kWarps * 32 * sizeof(float4));
+}
+
+// How an item's keys are cut: the runs that a model of the time finds best.  It was fitted to calls of
+// 16 heads over 16 .. 751 positions at 1 .. 64 streams and of 8 heads over 4,000 .. 65,000: a CTA takes
+// 3 us besides its blocks, a block of 16 keys takes a warp 0.6 us on an idle SM and 1.5 us on a full
+// one, joining a cluster takes 1 us and joining parts through memory 3 us and a little for each.
+struct Cut {
+    int parts, cluster;
+};
+Cut cut_items(int64_t items, int64_t blocks, int slots) {
+    Cut best{1, 1};
+    double least = 1e30;
+    for (int cluster = 1; cluster <= kMaxCluster; cluster *= 2)
+        for (int parts = 1; parts <= kMaxParts; parts = parts < 8 ? parts + 1 : parts + parts / 4) {
+            const int64_t runs = (int64_t)parts * cluster;
+            if ((runs > 1 && runs * kWarps > blocks + kWarps) || (parts > 1 && (cluster < kMaxCluster / 2 || items * parts > kKv8MaxPartials ||
+                                                                         runs * kWarps * kMinBlocks > blocks)))
+                break;
+            const double fill = std::min(1.0, (double)(items * runs) / slots);
+            const double waves = (double)((items * runs + slots - 1) / slots);
+            const double block_us = std::max(0.6, 1.5 * fill);
+            const double us = waves * (3.0 + block_us * (double)((blocks + runs * kWarps - 1) / (runs * kWarps))) +
+                              (cluster > 1 ? 1.0 : 0.0) + (parts > 1 ? 3.0 + 0.1 * parts : 0.0);
+            if (us < least) least = us, best = Cut{parts, cluster};
+        }
+    return best;
 }
 
 template <int D, bool NARROW>
@@ -563,20 +652,29 @@ cudaError_t attend_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, 
     using S = Shape<NARROW>;
     const int row_groups = (b.tokens * a.group + S::kRows - 1) / S::kRows;
     const int64_t items = (int64_t)b.n * c.heads * row_groups;
-    // Where there are few items: as many splits as fill the SMs twice over without a CTA too many, no
-    // more than partial slots, nor than a full context has blocks for.
-    const int context = a.window > 0 ? std::min<int64_t>((int64_t)a.window + b.tokens, c.cap) : c.cap;
-    const int64_t want = std::min<int64_t>(2 * S::kCtas * a.num_sms / items, context / kKv8Block / kWarps + 1);
-    const int splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, kMaxSplits, kKv8MaxPartials / items}));
-    attend_kernel<D, NARROW><<<(unsigned)(items * splits), kWarps * 32, attend_smem<D, NARROW>(), st>>>(c, b, a, row_groups,
-                                                                                                     splits);
-    return cudaGetLastError();
+    const int64_t blocks = (a.window > 0 ? std::min<int64_t>((int64_t)a.window + b.tokens, c.cap) : c.cap) / kKv8Block + 1;
+    const Cut cut = cut_items(items, blocks, S::kCtas * a.num_sms);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(items * cut.parts * cut.cluster));
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = attend_smem<D, NARROW>();
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cut.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cut.cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, attend_kernel<D, NARROW>, c, b, a, row_groups, cut.parts, cut.cluster);
 }
 
-template <int D, bool NARROW>
+template <int D>
 cudaError_t configure_t() {
-    return cudaFuncSetAttribute(attend_kernel<D, NARROW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)attend_smem<D, NARROW>());
+    const cudaError_t e = cudaFuncSetAttribute(attend_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)attend_smem<D, true>());
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(attend_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)attend_smem<D, false>());
 }
 
 }  // namespace
@@ -584,8 +682,7 @@ cudaError_t configure_t() {
 size_t kv8_partial_bytes(int dim) { return (size_t)kKv8MaxPartials * kKv8Rows * (dim + 4) * sizeof(float); }
 
 cudaError_t kv8_configure() {
-    for (const cudaError_t e : {configure_t<128, true>(), configure_t<128, false>(), configure_t<64, true>(),
-                                configure_t<64, false>(), kv8_configure_prompt()})
+    for (const cudaError_t e : {configure_t<128>(), configure_t<64>(), kv8_configure_prompt()})
         if (e != cudaSuccess) return e;
     return cudaSuccess;
 }

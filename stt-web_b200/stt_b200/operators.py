@@ -45,10 +45,11 @@ def _on(t, device: int, where: str):
 
 def _whole(t, n: int, device: int, where: str, what: str, code: int = _I32) -> int:
     """Address of a contiguous device array of n entries."""
+    if _codes.get(t.dtype) == code and t.numel() == n and t.is_contiguous() and t.get_device() == device:
+        return t.data_ptr()
     if _code(t.dtype) != code or t.numel() != n or not t.is_contiguous():
         _refuse(where, f"{what} must be {n} contiguous {('f32', '', '', 'int32', 'uint8')[code]} values")
-    if t.get_device() != device:
-        _on(t, device, where)
+    _on(t, device, where)
     return t.data_ptr()
 
 
@@ -114,15 +115,17 @@ class Kv8Cache:
 
     def _tensor(self, t, at: int, where: str, heads: int = 0):
         """Packs tensor t into place `at` of the call's arguments; returns (n, tokens, heads)."""
-        n, tokens, h, dim = shape = t.shape if len(t.shape) == 4 else (0, 0, 0, -1)
-        seq, token, head, last = t.stride() if dim >= 0 else (0, 0, 0, 0)
-        if dim != self.head_dim or last != 1 or (heads and h != heads):
-            _refuse(where, f"tensors are [n, tokens, {heads or 'heads'}, {self.head_dim}] with the last dimension contiguous, got "
-                           f"{tuple(t.shape)} with strides {tuple(t.stride())}")
-        if t.get_device() != self.device:
-            _on(t, self.device, where)
-        KV8_TENSOR.pack_into(self._args, at, t.data_ptr(), seq, token, head, _dtype(t, where), 0)
-        return shape[:3]
+        shape, strides = t.shape, t.stride()
+        if len(shape) == 4 and shape[3] == self.head_dim and strides[3] == 1 and (not heads or shape[2] == heads):
+            code = _codes.get(t.dtype, -1)
+            if not 0 <= code <= 2:
+                code = _dtype(t, where)
+            if t.get_device() != self.device:
+                _on(t, self.device, where)
+            KV8_TENSOR.pack_into(self._args, at, t.data_ptr(), strides[0], strides[1], strides[2], code, 0)
+            return shape[:3]
+        _refuse(where, f"tensors are [n, tokens, {heads or 'heads'}, {self.head_dim}] with the last dimension contiguous, got "
+                       f"{tuple(shape)} with strides {tuple(strides)}")
 
     def _batch(self, n: int, tokens: int, pos, count, seqs, where: str):
         d = self.device

@@ -232,6 +232,8 @@ ATTENTION = [
     (1, 8, 128, 1, [0, 300, 511], 512, 0, None, "bf16", "bf16"),
     (2, 3, 64, 1, [0, 300, 511], 512, 0, None, "f16", "f32"),
     (1, 1, 128, 1, [2000, 4095], 4096, 0, None, "f32", "f32"),       # split over CTAs
+    (2, 4, 64, 1, [31, 700, 19999], 20000, 0, None, "bf16", "f32"),  # and joined through memory
+    (1, 6, 128, 1, [12345], 20000, 0, None, "f32", "f32"),
     (3, 5, 64, 1, [100, 1000, 5000], 128, 0, None, "f32", "f16"),     # rings that wrapped
     (2, 1, 128, 1, [100, 1000, 5000], 128, 33, None, "f32", "f32"),   # and a window in them
     (2, 1, 128, 1, [100, 1000, 5000], 128, 1, None, "f32", "f32"),    # a window of the position itself
