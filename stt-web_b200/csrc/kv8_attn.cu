@@ -640,8 +640,9 @@ Cut cut_items(int64_t items, int64_t blocks, int slots) {
             const double fill = std::min(1.0, (double)(items * runs) / slots);
             const double waves = (double)((items * runs + slots - 1) / slots);
             const double block_us = std::max(0.6, 1.5 * fill);
-            const double us = waves * (3.0 + block_us * (double)((blocks + runs * kWarps - 1) / (runs * kWarps))) +
-                              (cluster > 1 ? 1.0 : 0.0) + (parts > 1 ? 3.0 + 0.1 * parts : 0.0);
+            const double cta_us = 3.0 + block_us * (double)((blocks + runs * kWarps - 1) / (runs * kWarps));
+            // (a tenth of a CTA's time for contexts that differ in length)
+            const double us = (waves + 0.1) * cta_us + (cluster > 1 ? 1.0 : 0.0) + (parts > 1 ? 3.0 + 0.1 * parts : 0.0);
             if (us < least) least = us, best = Cut{parts, cluster};
         }
     return best;

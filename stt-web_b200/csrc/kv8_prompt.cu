@@ -6,9 +6,13 @@
 // What bounds it: per tile of 128 x 128 scores and 128 dimensions the two products take 1024 cycles of
 // the tensor cores, the 16384 exponentials 1024 cycles of the 16-per-cycle special function units; the
 // codes of K and V are turned into f16 once for both tiles.  Hence
-//  - roles per warp: 4 + 4 warps of softmax (a thread owns a row: no shuffles), 4 that turn codes into
-//    f16 operands, one that issues products, one that copies codes (bulk copies), with mbarriers
-//    between them: while one tile is in its softmax the other is on the tensor cores;
+//  - roles per warpgroup: one of softmax for each tile (a thread owns a row and holds its 128 scores in
+//    registers: no shuffles, one trip to TMEM), one that turns codes into f16 operands, one whose first
+//    warp issues products, with mbarriers between them: while one tile is in its softmax the other is
+//    on the tensor cores.  The registers go where they are needed (setmaxnreg);
+//  - the codes come straight into the registers of the threads that convert them, the next step's
+//    while this one's are written (staged through shared memory first, a step waited for its copies:
+//    3.4 us a step against 1.3);
 //  - K's and V's codes go to shared memory as whole numbers, exact in f16; the blocks' exponents enter
 //    in the softmax, where they are free: a score is the accumulator times (row step * 2^e_k), the
 //    argument of the exponential takes + e_v, and so the weight is 2^(s + e_v - M) with the running
@@ -35,8 +39,11 @@ namespace {
 constexpr int kTile = 128;                // rows of a query tile and keys of a step
 constexpr int kStepBlocks = kTile / kKv8Block;
 constexpr int kSoftmaxWarps = 8, kDequantWarps = 4;
-constexpr int kMmaWarp = kSoftmaxWarps + kDequantWarps, kCopyWarp = kMmaWarp + 1;
-constexpr int kThreads = 32 * (kCopyWarp + 1);
+constexpr int kMmaWarp = kSoftmaxWarps + kDequantWarps;
+constexpr int kThreads = 512;
+// registers of a thread: 128 at the launch, then by role (256 * 184 + 128 * 104 + 128 * 40 = 512 * 128)
+constexpr int kSoftmaxRegs = 184, kDequantRegs = 104, kMmaRegs = 40;
+static_assert(256 * kSoftmaxRegs + 128 * kDequantRegs + 128 * kMmaRegs == kThreads * 128, "the split is what the block has");
 constexpr uint32_t kTmemCols = 512;       // S of both tiles, O of both tiles
 constexpr uint32_t kOCol = 256;
 constexpr int kExpSlots = 4;              // steps whose exponents are kept
@@ -47,10 +54,9 @@ template <int D>
 struct PromptSmem {
     uint8_t q[2][kTile * D * 2];          // f16, core matrices of 8 rows x 16 bytes, D / 8 of them per 8 rows
     uint8_t k[2][kTile * D * 2], v[2][kTile * D * 2];
-    uint8_t k_raw[kTile * D], v_raw[kTile * D];
     float k_step[kExpSlots][kStepBlocks], v_exp[kExpSlots][kStepBlocks];
     uint64_t q_full[2], s_full[2], p_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], e_full[kExpSlots];
-    uint64_t kr_full, kr_empty, vr_full, vr_empty, done;
+    uint64_t done;
     uint32_t tmem;
     int abort;
 };
@@ -61,17 +67,21 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 128 rows of codes to f16 in core matrices; thread r (of 128) takes row r, its 16-code pieces in an
-// order of its own, so that the 8 threads of a quarter warp read and write different banks.
+// A row of 128 rows of codes, its 16-code pieces in an order of its own, so that the 8 threads of a
+// quarter warp write to different banks; and the pieces as f16 in core matrices.
 template <int D>
-__device__ __forceinline__ void dequant_rows(const uint8_t* raw, uint8_t* dst, int r) {
-    constexpr int CH = D / 16;
+__device__ __forceinline__ void load_row(const int8_t* src, bool there, int r, uint4 (&w)[D / 16]) {
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+        w[s] = there ? __ldg(reinterpret_cast<const uint4*>(src) + (s + r) % (D / 16)) : make_uint4(0, 0, 0, 0);
+}
+template <int D>
+__device__ __forceinline__ void store_row(const uint4 (&w)[D / 16], uint8_t* dst, int r) {
     uint8_t* out = dst + (r >> 3) * (D / 8) * 128 + (r & 7) * 16;
 #pragma unroll
-    for (int s = 0; s < CH; ++s) {
-        const int c = (s + r) % CH;
-        const uint4 w = *reinterpret_cast<const uint4*>(raw + r * D + c * 16);
-        const uint32_t x[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+    for (int s = 0; s < D / 16; ++s) {
+        const int c = (s + r) % (D / 16);
+        const uint32_t x[4] = {w[s].x ^ 0x80808080u, w[s].y ^ 0x80808080u, w[s].z ^ 0x80808080u, w[s].w ^ 0x80808080u};
 #pragma unroll
         for (int half = 0; half < 2; ++half)
             *reinterpret_cast<uint4*>(out + (2 * c + half) * 128) =
@@ -79,15 +89,18 @@ __device__ __forceinline__ void dequant_rows(const uint8_t* raw, uint8_t* dst, i
                            codes_to_f16<0x4140>(x[2 * half + 1]), codes_to_f16<0x4342>(x[2 * half + 1]));
     }
 }
-
-// 32 raw scores from TMEM, those outside [lo, hi] (column numbers) at -inf.
-__device__ __forceinline__ void load_scores(uint32_t taddr, bool masked, int lo, int hi, float (&x)[32]) {
-    tmem_ld32(taddr, x);
-    if (masked) {
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-            if (e < lo || e > hi) x[e] = -INFINITY;
-    }
+template <int N>
+__device__ __forceinline__ void registers_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 // CTA (row block from the last to the first, batch row, head).
@@ -128,10 +141,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
             mbar_init(&sm.v_empty[j], 1);
         }
         for (int j = 0; j < kExpSlots; ++j) mbar_init(&sm.e_full[j], 1);
-        mbar_init(&sm.kr_full, 1);
-        mbar_init(&sm.kr_empty, kDequantWarps);
-        mbar_init(&sm.vr_full, 1);
-        mbar_init(&sm.vr_empty, kDequantWarps);
         mbar_init(&sm.done, 1);
         sm.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -147,73 +156,52 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = sm.tmem;
 
-    if (warp == kCopyWarp) {
-        // codes of step j: at most two runs of blocks, where the ring wraps
-        int issued_k = 0, issued_v = 0;
-        const int8_t* kc = c.kc + head * c.cap * D;
-        const int8_t* vc = c.vc + head * c.cap * D;
-        for (int j = 0; j < steps; ++j) {
-            const int many = min(kStepBlocks, nb - j * kStepBlocks);
-            const int b0 = (kb0 + j * kStepBlocks) % cap_blocks;
-            const int run = min(many, cap_blocks - b0);
-            constexpr uint32_t BB = kKv8Block * D;
-            auto copy = [&](uint8_t* dst, const int8_t* src, uint64_t* full) {
-                if (elect_one()) {
-                    mbar_expect_tx(full, many * BB);
-                    bulk_g2s(dst, src + (int64_t)b0 * BB, run * BB, full);
-                    // (a ring shorter than a step: the rest starts over at its first block)
-                    if (run < many) bulk_g2s(dst + run * BB, src, (many - run) * BB, full);
-                }
-                __syncwarp();
-            };
-            if (j > 0 && !__all_sync(0xFFFFFFFFu, mbar_wait(&sm.kr_empty, (j - 1) & 1, abort, 64))) break;
-            copy(sm.k_raw, kc, &sm.kr_full);
-            issued_k = j + 1;
-            if (j > 0 && !__all_sync(0xFFFFFFFFu, mbar_wait(&sm.vr_empty, (j - 1) & 1, abort, 64))) break;
-            copy(sm.v_raw, vc, &sm.vr_full);
-            issued_v = j + 1;
-        }
-        // the last copies have landed before the CTA can exit
-        if (issued_k > 0) mbar_drain(&sm.kr_full, (issued_k - 1) & 1);
-        if (issued_v > 0) mbar_drain(&sm.vr_full, (issued_v - 1) & 1);
-    } else if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
+    if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
+        registers_down<kDequantRegs>();
         const int r = threadIdx.x - kSoftmaxWarps * 32;
         const int8_t* ke = c.ke + head * cap_blocks;
         const int8_t* ve = c.ve + head * cap_blocks;
+        // row r of step j is slot r % 16 of block kb0 + 8 j + r / 16
+        const int8_t* kc = c.kc + (head * c.cap + r % kKv8Block) * D;
+        const int8_t* vc = c.vc + (head * c.cap + r % kKv8Block) * D;
+        int at = (kb0 + r / kKv8Block) % cap_blocks;
+        const int stride = kStepBlocks % cap_blocks;
+        auto there = [&](int j) { return j * kStepBlocks + r / kKv8Block < nb; };
+        uint4 kq[D / 16], vq[D / 16];
+        load_row<D>(kc + (int64_t)at * (kKv8Block * D), there(0), r, kq);
+        load_row<D>(vc + (int64_t)at * (kKv8Block * D), there(0), r, vq);
         for (int j = 0; j < steps; ++j) {
             const int st = j & 1;
-            if (warp == kSoftmaxWarps) {
-                // the slot is free: K of step j - 1 was only taken after the softmax of step j - 3 or later
-                if (lane < kStepBlocks) {
-                    const int blk = j * kStepBlocks + lane;
-                    const int at = (kb0 + blk) % cap_blocks;
-                    sm.k_step[j % kExpSlots][lane] = blk < nb ? pow2i(ke[at]) : 1.0f;
-                    sm.v_exp[j % kExpSlots][lane] = blk < nb ? (float)ve[at] : 0.0f;
-                }
+            if (warp == kSoftmaxWarps && lane < kStepBlocks) {
+                // the slot is free: V of step j - 1 was written, so the products of step j - 3 are done,
+                // and with them the softmax of step j - 4
+                const int blk = j * kStepBlocks + lane;
+                const int where = (kb0 + blk) % cap_blocks;
+                sm.k_step[j % kExpSlots][lane] = blk < nb ? pow2i(ke[where]) : 1.0f;
+                sm.v_exp[j % kExpSlots][lane] = blk < nb ? (float)ve[where] : 0.0f;
             }
-            bool ok = mbar_wait(&sm.kr_full, j & 1, abort);
-            if (ok && j >= 2) ok = mbar_wait(&sm.k_empty[st], ((j >> 1) - 1) & 1, abort);
-            if (!__all_sync(0xFFFFFFFFu, ok)) break;
-            dequant_rows<D>(sm.k_raw, sm.k[st], r);
+            at += stride;
+            if (at >= cap_blocks) at -= cap_blocks;
+            if (!__all_sync(0xFFFFFFFFu, j < 2 || mbar_wait(&sm.k_empty[st], ((j >> 1) - 1) & 1, abort))) break;
+            store_row<D>(kq, sm.k[st], r);
+            load_row<D>(kc + (int64_t)at * (kKv8Block * D), j + 1 < steps && there(j + 1), r, kq);
             proxy_fence();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&sm.k_full[st]);
-                mbar_arrive(&sm.kr_empty);
                 if (warp == kSoftmaxWarps) mbar_arrive(&sm.e_full[j % kExpSlots]);
             }
-            ok = mbar_wait(&sm.vr_full, j & 1, abort);
-            if (ok && j >= 2) ok = mbar_wait(&sm.v_empty[st], ((j >> 1) - 1) & 1, abort);
-            if (!__all_sync(0xFFFFFFFFu, ok)) break;
-            dequant_rows<D>(sm.v_raw, sm.v[st], r);
+            if (!__all_sync(0xFFFFFFFFu, j < 2 || mbar_wait(&sm.v_empty[st], ((j >> 1) - 1) & 1, abort))) break;
+            store_row<D>(vq, sm.v[st], r);
+            load_row<D>(vc + (int64_t)at * (kKv8Block * D), j + 1 < steps && there(j + 1), r, vq);
             proxy_fence();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&sm.v_full[st]);
-                mbar_arrive(&sm.vr_empty);
-            }
+            if (lane == 0) mbar_arrive(&sm.v_full[st]);
         }
+    } else if (warp > kMmaWarp) {
+        registers_down<kMmaRegs>();
     } else if (warp == kMmaWarp) {
+        registers_down<kMmaRegs>();
         constexpr uint32_t GROUP = D * 16;  // bytes of 8 rows: D / 8 core matrices
         const uint32_t qk_desc = instr_desc_f16(kTile, kTile);
         const uint32_t pv_desc = instr_desc_f16(kTile, D) | (1u << 16);  // V is MN-major
@@ -269,7 +257,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         }
         if (elect_one()) mma_commit(&sm.done);  // also on abort: arrives once the products issued so far are done
         __syncwarp();
-    } else if (warp / 4 < tiles) {
+    } else {
+        registers_up<kSoftmaxRegs>();
+        if (warp / 4 < tiles) {
         const int q = warp / 4, quarter = warp & 3, r = q * kTile + quarter * 32 + lane;
         const bool live = r < rows;
         const int tok = live ? (r0 + r) / a.group : t0, qh = h * a.group + (r0 + r) % a.group;
@@ -331,19 +321,21 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
             const int p0 = (kb0 + j * kStepBlocks) * kKv8Block;
             const bool masked = p0 < all_lo || p0 + kTile - 1 > all_hi;
             const int lo = see_lo - p0, hi = see_hi - p0;  // (no overflow: see_lo <= 2^31 - 1, p0 >= 0)
+            float x[kTile];
+            tmem_ld128(s_col, x);
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < kTile; ++e)
+                    if (e < lo || e > hi) x[e] = -INFINITY;
+            }
             float mx = -INFINITY;
 #pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-                float x[32];
-                load_scores(s_col + 32 * ch, masked, lo - 32 * ch, hi - 32 * ch, x);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float bm = x[16 * u];
-#pragma unroll
-                    for (int e = 1; e < 16; ++e) bm = fmaxf(bm, x[16 * u + e]);
-                    const float step = fmaxf(q_step * k_step[2 * ch + u], 1e-37f);
-                    mx = fmaxf(mx, fmaf(bm, step, v_exp[2 * ch + u]));
-                }
+            for (int u = 0; u < kStepBlocks; ++u) {
+                const float* y = x + 16 * u;
+                const float m0 = max3(y[0], y[1], y[2]), m1 = max3(y[3], y[4], y[5]), m2 = max3(y[6], y[7], y[8]);
+                const float m3 = max3(y[9], y[10], y[11]), m4 = max3(y[12], y[13], y[14]);
+                const float bm = max3(max3(m0, m1, m2), max3(m3, m4, y[15]), -INFINITY);
+                mx = fmaxf(mx, fmaf(bm, fmaxf(q_step * k_step[u], 1e-37f), v_exp[u]));
             }
             const bool grow = mx > M + kLazy;
             if (__any_sync(0xFFFFFFFFu, grow)) {
@@ -351,40 +343,40 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                 if (grow) M = mx;
                 l *= f;
                 if (j > 0) {
+#pragma unroll 1
+                    for (int ch = 0; ch < D / 16; ++ch) {
+                        float o[16];
+                        tmem_ld16f(o_col + 16 * ch, o);
+                        uint32_t w[16];
 #pragma unroll
-                    for (int ch = 0; ch < D / 32; ++ch) {
-                        float o[32];
-                        tmem_ld32(o_col + 32 * ch, o);
-                        uint32_t w[2][16];
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) w[e >> 4][e & 15] = __float_as_uint(o[e] * f);
-                        tmem_st(o_col + 32 * ch, w[0]);
-                        tmem_st(o_col + 32 * ch + 16, w[1]);
+                        for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * f);
+                        tmem_st(o_col + 16 * ch, w);
                     }
                 }
             }
+            float part[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-                float x[32];
-                load_scores(s_col + 32 * ch, masked, lo - 32 * ch, hi - 32 * ch, x);
+            for (int u = 0; u < kStepBlocks; u += 2) {
                 uint32_t w[16];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float step = fmaxf(q_step * k_step[2 * ch + u], 1e-37f);
-                    const float ev = v_exp[2 * ch + u];
+                for (int v = 0; v < 2; ++v) {
+                    const float step = fmaxf(q_step * k_step[u + v], 1e-37f);
+                    const float ev = v_exp[u + v];
                     const float add = ev + (kWeightShift - M);
-                    const float to_sum = pow2i((int)(E - ev));
+                    float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float w0 = exp2_approx(fmaf(x[16 * u + e], step, add));
-                        const float w1 = exp2_approx(fmaf(x[16 * u + e + 1], step, add));
-                        l = fmaf(w0, to_sum, l);
-                        l = fmaf(w1, to_sum, l);
-                        w[8 * u + e / 2] = pack_f16(w0, w1);
+                        const float w0 = exp2_approx(fmaf(x[16 * (u + v) + e], step, add));
+                        const float w1 = exp2_approx(fmaf(x[16 * (u + v) + e + 1], step, add));
+                        s0 += w0;
+                        s1 += w1;
+                        w[8 * v + e / 2] = pack_f16(w0, w1);
                     }
+                    part[v] = fmaf(s0 + s1, pow2i((int)(E - ev)), part[v]);
                 }
-                tmem_st(s_col + 16 * ch, w);  // over scores that this thread has read
+                tmem_st(s_col + 8 * u, w);  // over scores, all of which this thread has read
             }
+            l += part[0] + part[1];
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -419,6 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                     }
                 }
             }
+        }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -129,6 +129,35 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// 16, and 128, consecutive columns, read.
+__device__ __forceinline__ void tmem_ld16f(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+            : "=f"(v[32 * c + 0]), "=f"(v[32 * c + 1]), "=f"(v[32 * c + 2]), "=f"(v[32 * c + 3]), "=f"(v[32 * c + 4]), "=f"(v[32 * c + 5]), "=f"(v[32 * c + 6]), "=f"(v[32 * c + 7]),
+              "=f"(v[32 * c + 8]), "=f"(v[32 * c + 9]), "=f"(v[32 * c + 10]), "=f"(v[32 * c + 11]), "=f"(v[32 * c + 12]), "=f"(v[32 * c + 13]), "=f"(v[32 * c + 14]), "=f"(v[32 * c + 15]),
+              "=f"(v[32 * c + 16]), "=f"(v[32 * c + 17]), "=f"(v[32 * c + 18]), "=f"(v[32 * c + 19]), "=f"(v[32 * c + 20]), "=f"(v[32 * c + 21]), "=f"(v[32 * c + 22]), "=f"(v[32 * c + 23]),
+              "=f"(v[32 * c + 24]), "=f"(v[32 * c + 25]), "=f"(v[32 * c + 26]), "=f"(v[32 * c + 27]), "=f"(v[32 * c + 28]), "=f"(v[32 * c + 29]), "=f"(v[32 * c + 30]), "=f"(v[32 * c + 31])
+            : "r"(taddr + 32 * c));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    // the loads' registers may not be read before the wait
+#pragma unroll
+    for (int i = 0; i < 128; ++i) asm volatile("" : "+f"(v[i]));
+}
+
 // 16 consecutive 32-bit columns of this thread's TMEM lane (warp-collective).
 __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
