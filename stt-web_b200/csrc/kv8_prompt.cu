@@ -54,7 +54,7 @@ template <int D>
 struct PromptSmem {
     uint8_t q[2][kTile * D * 2];          // f16, core matrices of 8 rows x 16 bytes, D / 8 of them per 8 rows
     uint8_t k[2][kTile * D * 2], v[2][kTile * D * 2];
-    float k_step[kExpSlots][kStepBlocks], v_exp[kExpSlots][kStepBlocks];
+    __align__(16) float k_step[kExpSlots][kStepBlocks], v_exp[kExpSlots][kStepBlocks];
     uint64_t q_full[2], s_full[2], p_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], e_full[kExpSlots];
     uint64_t done;
     uint32_t tmem;
@@ -170,15 +170,27 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         uint4 kq[D / 16], vq[D / 16];
         load_row<D>(kc + (int64_t)at * (kKv8Block * D), there(0), r, kq);
         load_row<D>(vc + (int64_t)at * (kKv8Block * D), there(0), r, vq);
+        // the next step's exponents, lane by lane
+        int ek = 0, ev = 0;
+        auto fetch_exps = [&](int j) {
+            const int blk = j * kStepBlocks + lane;
+            if (lane < kStepBlocks && blk < nb) {
+                const int where = (kb0 + blk) % cap_blocks;
+                ek = __ldg(ke + where);
+                ev = __ldg(ve + where);
+            }
+        };
+        if (warp == kSoftmaxWarps) fetch_exps(0);
         for (int j = 0; j < steps; ++j) {
             const int st = j & 1;
-            if (warp == kSoftmaxWarps && lane < kStepBlocks) {
+            if (warp == kSoftmaxWarps) {
                 // the slot is free: V of step j - 1 was written, so the products of step j - 3 are done,
                 // and with them the softmax of step j - 4
-                const int blk = j * kStepBlocks + lane;
-                const int where = (kb0 + blk) % cap_blocks;
-                sm.k_step[j % kExpSlots][lane] = blk < nb ? pow2i(ke[where]) : 1.0f;
-                sm.v_exp[j % kExpSlots][lane] = blk < nb ? (float)ve[where] : 0.0f;
+                if (lane < kStepBlocks) {
+                    sm.k_step[j % kExpSlots][lane] = pow2i(ek);
+                    sm.v_exp[j % kExpSlots][lane] = (float)ev;
+                }
+                fetch_exps(j + 1);
             }
             at += stride;
             if (at >= cap_blocks) at -= cap_blocks;
@@ -312,12 +324,20 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         float M = -FLT_MAX, l = 0.0f;
         bool ok = true;
         for (int j = 0; j < steps; ++j) {
-            ok = mbar_wait(&sm.s_full[q], j & 1, abort) && mbar_wait(&sm.e_full[j % kExpSlots], (j / kExpSlots) & 1, abort);
-            ok = __all_sync(0xFFFFFFFFu, ok);
+            // the scores (half of the lanes poll for them) and the exponents (the other half)
+            ok = __all_sync(0xFFFFFFFFu, lane < 16 ? mbar_wait(&sm.s_full[q], j & 1, abort)
+                                                   : mbar_wait(&sm.e_full[j % kExpSlots], (j / kExpSlots) & 1, abort));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float* k_step = sm.k_step[j % kExpSlots];
-            const float* v_exp = sm.v_exp[j % kExpSlots];
+            float k_step[kStepBlocks], v_exp[kStepBlocks];  // what turns block u's accumulators into scores, e_v
+#pragma unroll
+            for (int u = 0; u < kStepBlocks; u += 4) {
+                const float4 ks = *reinterpret_cast<const float4*>(&sm.k_step[j % kExpSlots][u]);
+                const float4 vs = *reinterpret_cast<const float4*>(&sm.v_exp[j % kExpSlots][u]);
+                const float s[4] = {ks.x, ks.y, ks.z, ks.w}, e[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+                for (int v = 0; v < 4; ++v) k_step[u + v] = fmaxf(q_step * s[v], 1e-37f), v_exp[u + v] = e[v];
+            }
             const int p0 = (kb0 + j * kStepBlocks) * kKv8Block;
             const bool masked = p0 < all_lo || p0 + kTile - 1 > all_hi;
             const int lo = see_lo - p0, hi = see_hi - p0;  // (no overflow: see_lo <= 2^31 - 1, p0 >= 0)
@@ -335,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                 const float m0 = max3(y[0], y[1], y[2]), m1 = max3(y[3], y[4], y[5]), m2 = max3(y[6], y[7], y[8]);
                 const float m3 = max3(y[9], y[10], y[11]), m4 = max3(y[12], y[13], y[14]);
                 const float bm = max3(max3(m0, m1, m2), max3(m3, m4, y[15]), -INFINITY);
-                mx = fmaxf(mx, fmaf(bm, fmaxf(q_step * k_step[u], 1e-37f), v_exp[u]));
+                mx = fmaxf(mx, fmaf(bm, k_step[u], v_exp[u]));
             }
             const bool grow = mx > M + kLazy;
             if (__any_sync(0xFFFFFFFFu, grow)) {
@@ -360,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                 uint32_t w[16];
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
-                    const float step = fmaxf(q_step * k_step[u + v], 1e-37f);
+                    const float step = k_step[u + v];
                     const float ev = v_exp[u + v];
                     const float add = ev + (kWeightShift - M);
                     float s0 = 0.0f, s1 = 0.0f;
