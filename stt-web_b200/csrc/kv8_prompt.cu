@@ -55,7 +55,7 @@ struct PromptSmem {
     uint8_t q[2][kTile * D * 2];          // f16, core matrices of 8 rows x 16 bytes, D / 8 of them per 8 rows
     uint8_t k[2][kTile * D * 2], v[2][kTile * D * 2];
     __align__(16) float k_step[kExpSlots][kStepBlocks], v_exp[kExpSlots][kStepBlocks];
-    uint64_t q_full[2], s_full[2], p_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], e_full[kExpSlots];
+    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], e_full[kExpSlots];
     uint64_t done;
     uint32_t tmem;
     int abort;
@@ -134,6 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         for (int j = 0; j < 2; ++j) {
             mbar_init(&sm.q_full[j], 4);
             mbar_init(&sm.s_full[j], 1);
+            mbar_init(&sm.p_half[j], 4);
             mbar_init(&sm.p_full[j], 4);
             mbar_init(&sm.k_full[j], kDequantWarps);
             mbar_init(&sm.k_empty[j], 1);
@@ -225,10 +226,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                            k > 0);
             mma_commit(&sm.s_full[q]);
         };
-        auto pv = [&](int q, int st, bool add) {
+        auto pv = [&](int q, int st, int half, bool add) {
             const uint32_t va = smem_u32(sm.v[st]);
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
+            for (int k = half * (kTile / 32); k < (half + 1) * (kTile / 32); ++k)
                 mma_f16_ts(tmem + kOCol + q * kTile, tmem + q * kTile + k * 8, smem_desc(va + k * 2 * GROUP, GROUP, 128), pv_desc,
                            add || k > 0);
         };
@@ -250,11 +251,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
             ok = mbar_wait(&sm.v_full[st], (j >> 1) & 1, abort);
             if (ok && more) ok = mbar_wait(&sm.k_full[nx], ((j + 1) >> 1) & 1, abort);
             for (int q = 0; ok && q < tiles; ++q) {
+                // the weights of the first 64 keys, then the others'
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.p_half[q], j & 1, abort));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (elect_one()) pv(q, st, 0, j > 0);
+                __syncwarp();
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.p_full[q], j & 1, abort));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_one()) {
-                    pv(q, st, j > 0);
+                    pv(q, st, 1, true);
                     if (more) qk(q, nx);
                 }
                 __syncwarp();
@@ -395,6 +402,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                     part[v] = fmaf(s0 + s1, pow2i((int)(E - ev)), part[v]);
                 }
                 tmem_st(s_col + 8 * u, w);  // over scores, all of which this thread has read
+                if (u == kStepBlocks / 2 - 2) {
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.p_half[q]);
+                }
             }
             l += part[0] + part[1];
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
