@@ -633,6 +633,7 @@ struct stt_streams {
     int8_t* d_exps = nullptr;
     float* d_kv8_part = nullptr; // workspace of the 8-bit rings' attention
     uint32_t* d_kv8_tickets = nullptr;
+    Kv8Machine kv8_machine{};
     int32_t* d_pos = nullptr;    // each batch row's position in this step
     size_t kv_stream_bytes = 0;
     StreamState* d_state = nullptr;
@@ -745,8 +746,7 @@ int enqueue_kv8_attention(stt_streams* s, const Ctx& c, int layer, __half* x16, 
     a.scale = m->attn_scale;
     a.part = s->d_kv8_part;
     a.tickets = s->d_kv8_tickets;
-    a.num_sms = m->num_sms;
-    CUDA_TRY(launch_kv8_attention(kv, batch, a, st));
+    CUDA_TRY(launch_kv8_attention(kv, batch, a, s->kv8_machine, st));
     if (x16) CUDA_TRY(launch_tc_prep(s->d_attn, nullptr, m->D, c.n, x16, st));
     return STT_OK;
 }
@@ -1086,7 +1086,7 @@ extern "C" int stt_streams_create(stt_model* m, int n_streams, int kv_dtype, stt
     s->d_kv8_part = reinterpret_cast<float*>(b + o_kv8_part);
     if (s->kv8_cap) {
         s->d_exps = static_cast<int8_t*>(s->d_kv) + kv_codes;
-        CUDA_TRY(kv8_configure());
+        CUDA_TRY(kv8_configure(m->num_sms, &s->kv8_machine));
     }
     CUDA_TRY(cudaMemset(s->d_scratch, 0, off));
     CUDA_TRY(cudaMemset(s->d_kv, 0, s->kv_stream_bytes * S));

@@ -53,20 +53,30 @@ struct Kv8Attention {
     // workspace: partial results [kKv8MaxPartials][kKv8Rows][dim + 4] and one ticket per merged item
     float* part;
     uint32_t* tickets;
-    int32_t num_sms;
 };
 
 size_t kv8_partial_bytes(int dim);
 
-cudaError_t kv8_configure();
+// What the choice between kernels needs to know of a device.
+struct Kv8Machine {
+    int num_sms;
+    int prompt_ctas[4];  // CTAs of the prompt kernel that run at a time, in clusters of 1, 2, 4 and 8
+};
+cudaError_t kv8_configure(int num_sms, Kv8Machine* m);
 cudaError_t launch_kv8_append(const Kv8Dev& c, const Kv8Batch& b, const void* k, const void* v, int dtype,
                               const Kv8Strides& ks, const Kv8Strides& vs, cudaStream_t st);
 cudaError_t launch_kv8_read(const Kv8Dev& c, const Kv8Batch& b, void* k, void* v, int dtype, const Kv8Strides& ks,
                             const Kv8Strides& vs, cudaStream_t st);
 // The two kernels of the attention: 8 query rows against a split of the keys (any type), and 256 query
 // rows on the 5th-generation tensor cores (16-bit queries and output).
-cudaError_t launch_kv8_prompt(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st);
-cudaError_t kv8_configure_prompt();
-cudaError_t launch_kv8_attention(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st);
+struct PromptPlan {
+    int cluster;  // CTAs that share a row block's keys
+    double us;    // the time that a model gives it
+};
+PromptPlan kv8_prompt_plan(int64_t rows, int64_t items, int64_t blocks, const Kv8Machine& m);
+cudaError_t launch_kv8_prompt(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, int cluster, cudaStream_t st);
+cudaError_t kv8_configure_prompt(Kv8Machine* m);
+cudaError_t launch_kv8_attention(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, const Kv8Machine& m,
+                                 cudaStream_t st);
 
 }  // namespace stt

@@ -25,6 +25,7 @@
 //  - every warp streams its own blocks of 16 keys through a private ring in shared memory
 //    (cp.async, 16 bytes per lane), without block-wide barriers, and the 4 warps are merged at the end.
 #include <cfloat>
+#include <climits>
 #include <algorithm>
 
 #include "kv8_attn.cuh"
@@ -58,29 +59,6 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// Cluster barrier, and loads from the same place of CTA `rank`'s shared memory.
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_at(uint32_t addr, int rank) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float2 cluster_load2(uint32_t addr, int rank) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_at(addr, rank)) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 cluster_load4(uint32_t addr, int rank) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(cluster_at(addr, rank))
-                 : "memory");
-    return v;
 }
 
 // Transposes the 8 x 8 matrix of 16-bit elements that the warp holds two to a lane, row g columns 2t, 2t + 1.
@@ -161,11 +139,11 @@ __device__ __forceinline__ float4 row_output(const RowState& r, float4 o) {
     return make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
 }
 
-// CTA (((batch row * row_groups + row group) * heads + head) * max_parts + part) * cluster + rank.  An
+// CTA (((batch row * groups + row group) * heads + head) * max_parts + part) * cluster + rank.  An
 // item's keys are cut into parts x cluster equal runs of blocks; a cluster joins its runs through shared
 // memory, the last cluster of an item its parts through global memory.
 template <int D, bool NARROW>
-__global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kernel(Kv8Dev c, Kv8Batch b, Kv8Attention a, int row_groups,
+__global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kernel(Kv8Dev c, Kv8Batch b, Kv8Attention a, int groups,
                                                                 int max_parts, int cluster) {
     constexpr int KS = D / 16;          // k steps of the first product
     constexpr int NT = NARROW ? D / 16 : D / 8;  // tiles of 16 (8) dimensions of the second
@@ -180,7 +158,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kern
     __shared__ uint32_t last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rank = blockIdx.x % cluster, part_of = blockIdx.x / cluster % max_parts, item = blockIdx.x / cluster / max_parts;
-    const int h = item % c.heads, rg = item / c.heads % row_groups, i = item / c.heads / row_groups;
+    const int h = item % c.heads, rg = item / c.heads % groups, i = item / c.heads / groups;
     Kv8Row row;
     if (!kv8_row(c, b, i, &row)) return;
     // the group's rows: row r is token r / group, query head h * group + r % group
@@ -627,14 +605,14 @@ constexpr size_t attend_smem() {
 // one, joining a cluster takes 1 us and joining parts through memory 3 us and a little for each.
 struct Cut {
     int parts, cluster;
+    double us;
 };
 Cut cut_items(int64_t items, int64_t blocks, int slots) {
-    Cut best{1, 1};
-    double least = 1e30;
+    Cut best{1, 1, 1e30};
     for (int cluster = 1; cluster <= kMaxCluster; cluster *= 2)
         for (int parts = 1; parts <= kMaxParts; parts = parts < 8 ? parts + 1 : parts + parts / 4) {
             const int64_t runs = (int64_t)parts * cluster;
-            if ((runs > 1 && runs * kWarps > blocks + kWarps) || (parts > 1 && (cluster < kMaxCluster / 2 || items * parts > kKv8MaxPartials ||
+            if ((runs > 1 && (runs * kWarps > blocks + kWarps || items * runs > INT_MAX)) || (parts > 1 && (cluster < kMaxCluster / 2 || items * parts > kKv8MaxPartials ||
                                                                          runs * kWarps * kMinBlocks > blocks)))
                 break;
             const double fill = std::min(1.0, (double)(items * runs) / slots);
@@ -643,18 +621,20 @@ Cut cut_items(int64_t items, int64_t blocks, int slots) {
             const double cta_us = 3.0 + block_us * (double)((blocks + runs * kWarps - 1) / (runs * kWarps));
             // (a tenth of a CTA's time for contexts that differ in length)
             const double us = (waves + 0.1) * cta_us + (cluster > 1 ? 1.0 : 0.0) + (parts > 1 ? 3.0 + 0.1 * parts : 0.0);
-            if (us < least) least = us, best = Cut{parts, cluster};
+            if (us < best.us) best = Cut{parts, cluster, us};
         }
     return best;
 }
 
+template <bool NARROW>
+int64_t row_groups(int64_t rows) {
+    return (rows + Shape<NARROW>::kRows - 1) / Shape<NARROW>::kRows;
+}
+
 template <int D, bool NARROW>
-cudaError_t attend_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st) {
-    using S = Shape<NARROW>;
-    const int row_groups = (b.tokens * a.group + S::kRows - 1) / S::kRows;
-    const int64_t items = (int64_t)b.n * c.heads * row_groups;
-    const int64_t blocks = (a.window > 0 ? std::min<int64_t>((int64_t)a.window + b.tokens, c.cap) : c.cap) / kKv8Block + 1;
-    const Cut cut = cut_items(items, blocks, S::kCtas * a.num_sms);
+cudaError_t attend_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, const Cut& cut, cudaStream_t st) {
+    const int groups = (int)row_groups<NARROW>((int64_t)b.tokens * a.group);
+    const int64_t items = (int64_t)b.n * c.heads * groups;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(items * cut.parts * cut.cluster));
     cfg.blockDim = dim3(kWarps * 32);
@@ -666,7 +646,7 @@ cudaError_t attend_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, 
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cut.cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, attend_kernel<D, NARROW>, c, b, a, row_groups, cut.parts, cut.cluster);
+    return cudaLaunchKernelEx(&cfg, attend_kernel<D, NARROW>, c, b, a, groups, cut.parts, cut.cluster);
 }
 
 template <int D>
@@ -682,17 +662,26 @@ cudaError_t configure_t() {
 
 size_t kv8_partial_bytes(int dim) { return (size_t)kKv8MaxPartials * kKv8Rows * (dim + 4) * sizeof(float); }
 
-cudaError_t kv8_configure() {
-    for (const cudaError_t e : {configure_t<128>(), configure_t<64>(), kv8_configure_prompt()})
+cudaError_t kv8_configure(int num_sms, Kv8Machine* m) {
+    m->num_sms = num_sms;
+    for (const cudaError_t e : {configure_t<128>(), configure_t<64>(), kv8_configure_prompt(m)})
         if (e != cudaSuccess) return e;
     return cudaSuccess;
 }
 
-cudaError_t launch_kv8_attention(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st) {
-    const int64_t rows = (int64_t)b.tokens * a.group;  // of a K/V head
-    if (a.q_dtype != DT_F32 && a.out_dtype != DT_F32 && rows >= 64) return launch_kv8_prompt(c, b, a, st);
-    if (rows <= Shape<true>::kRows) return c.dim == 128 ? attend_t<128, true>(c, b, a, st) : attend_t<64, true>(c, b, a, st);
-    return c.dim == 128 ? attend_t<128, false>(c, b, a, st) : attend_t<64, false>(c, b, a, st);
+cudaError_t launch_kv8_attention(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, const Kv8Machine& m,
+                                 cudaStream_t st) {
+    const int64_t rows = (int64_t)b.tokens * a.group, items = (int64_t)b.n * c.heads;  // rows of a K/V head
+    const int64_t blocks = (a.window > 0 ? std::min<int64_t>((int64_t)a.window + b.tokens, c.cap) : c.cap) / kKv8Block + 1;
+    const bool narrow = rows <= Shape<true>::kRows;
+    const Cut cut = narrow ? cut_items(items, blocks, Shape<true>::kCtas * m.num_sms)
+                           : cut_items(items * row_groups<false>(rows), blocks, Shape<false>::kCtas * m.num_sms);
+    if (rows > kKv8Rows && a.q_dtype != DT_F32 && a.out_dtype != DT_F32) {
+        const PromptPlan plan = kv8_prompt_plan(rows, items, blocks, m);
+        if (plan.us < cut.us) return launch_kv8_prompt(c, b, a, plan.cluster, st);
+    }
+    if (narrow) return c.dim == 128 ? attend_t<128, true>(c, b, a, cut, st) : attend_t<64, true>(c, b, a, cut, st);
+    return c.dim == 128 ? attend_t<128, false>(c, b, a, cut, st) : attend_t<64, false>(c, b, a, cut, st);
 }
 
 }  // namespace stt

@@ -12,6 +12,29 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// Cluster barrier, and loads from the same place of CTA `rank`'s shared memory.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_at(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr, int rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_at(addr, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_at(addr, rank))
+                 : "memory");
+    return v;
+}
+
 // Bytes `sel` of biased codes (code + 128) as a pair of f16 codes.
 template <int SEL>
 __device__ __forceinline__ uint32_t codes_to_f16(uint32_t biased) {

@@ -24,6 +24,8 @@
 //    lives in TMEM, is rescaled a few times per row instead of at every tile.
 // Both operands of a product lie in core matrices of 8 rows x 16 bytes: a key's 8 dimensions are one
 // row of K's K-major matrix and of V's MN-major one, so both are written alike.
+// Where there are fewer row blocks than SMs, a cluster of CTAs takes the steps of a row block in equal
+// runs; at the end each leaves its O, M and l in shared memory and joins a share of the rows from all.
 // Every wait is bounded: one that gives up sets the CTA's abort word, all roles leave, the copies and
 // products in flight are waited for, and the cache's error word records it.
 #include <cfloat>
@@ -48,6 +50,7 @@ constexpr uint32_t kTmemCols = 512;       // S of both tiles, O of both tiles
 constexpr uint32_t kOCol = 256;
 constexpr int kExpSlots = 4;              // steps whose exponents are kept
 constexpr float kWeightShift = 6.0f;
+constexpr int kMaxPromptCluster = 8;
 constexpr float kLazy = 8.0f;             // how far a score may exceed M
 
 template <int D>
@@ -57,6 +60,7 @@ struct PromptSmem {
     __align__(16) float k_step[kExpSlots][kStepBlocks], v_exp[kExpSlots][kStepBlocks];
     uint64_t q_full[2], s_full[2], p_half[2], p_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], e_full[kExpSlots];
     uint64_t done;
+    float2 state[2 * kTile];              // M and l of the rows, for a cluster
     uint32_t tmem;
     int abort;
 };
@@ -103,14 +107,25 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// CTA (row block from the last to the first, batch row, head).
+// 8 outputs: sums times the row's factor, in the output's type.
+__device__ __forceinline__ uint4 pack8(const float* o, float f, int dtype) {
+    uint32_t w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        w[u] = dtype == DT_BF16 ? pack2(o[2 * u] * f, o[2 * u + 1] * f, Elem<DT_BF16>())
+                                : pack2(o[2 * u] * f, o[2 * u + 1] * f, Elem<DT_F16>());
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// CTA (row block from the last to the first, batch row, head, rank in the cluster).
 template <int D, int DT>
-__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch b, Kv8Attention a, int row_blocks) {
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch b, Kv8Attention a, int row_blocks, int cluster) {
     extern __shared__ __align__(128) uint8_t prompt_smem[];
     PromptSmem<D>& sm = *reinterpret_cast<PromptSmem<D>*>(prompt_smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = blockIdx.x % c.heads, i = blockIdx.x / c.heads % b.n;
-    const int rb = row_blocks - 1 - blockIdx.x / c.heads / b.n;  // the later rows see more keys: they start first
+    const int rank = blockIdx.x % cluster, item = blockIdx.x / cluster;
+    const int h = item % c.heads, i = item / c.heads % b.n;
+    const int rb = row_blocks - 1 - item / c.heads / b.n;  // the later rows see more keys: they start first
     Kv8Row row;
     if (!kv8_row(c, b, i, &row)) return;
     const int r0 = rb * 2 * kTile;
@@ -123,9 +138,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
     sight.window = a.window;
     sight.ring = (row.pos + row.count + kKv8Block - 1) / kKv8Block * kKv8Block - c.cap;
     const int first = sight.lo(row.pos + t0), end = row.pos + t1;
-    const int kb0 = first / kKv8Block;
-    const int nb = first <= end ? end / kKv8Block - kb0 + 1 : 0;
-    const int steps = (nb + kStepBlocks - 1) / kStepBlocks;
+    const int kb_all = first / kKv8Block;
+    const int nb_all = first <= end ? end / kKv8Block - kb_all + 1 : 0;
+    // this CTA's run of steps, and its blocks
+    const int steps_all = (nb_all + kStepBlocks - 1) / kStepBlocks;
+    const int step0 = steps_all * rank / cluster, steps = steps_all * (rank + 1) / cluster - step0;
+    const int kb0 = kb_all + step0 * kStepBlocks, nb = min(nb_all - step0 * kStepBlocks, steps * kStepBlocks);
     const int64_t head = (int64_t)row.seq * c.heads + h;
     const int cap_blocks = c.cap / kKv8Block;
     volatile int* abort = &sm.abort;
@@ -157,6 +175,18 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = sm.tmem;
 
+    auto out_row = [&](int r) {
+        const int tok = (r0 + r) / a.group, qh = h * a.group + (r0 + r) % a.group;
+        return static_cast<uint16_t*>(a.out) + i * a.os.seq + (int64_t)tok * a.os.token + qh * a.os.head;
+    };
+    // the cluster's two barriers, which every thread passes
+    auto meet = [&] {
+        __syncwarp();
+        if (cluster > 1) {
+            cluster_sync();
+            cluster_sync();
+        }
+    };
     if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
         registers_down<kDequantRegs>();
         const int r = threadIdx.x - kSoftmaxWarps * 32;
@@ -211,8 +241,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.v_full[st]);
         }
+        meet();
     } else if (warp > kMmaWarp) {
         registers_down<kMmaRegs>();
+        meet();
     } else if (warp == kMmaWarp) {
         registers_down<kMmaRegs>();
         constexpr uint32_t GROUP = D * 16;  // bytes of 8 rows: D / 8 core matrices
@@ -276,22 +308,42 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         }
         if (elect_one()) mma_commit(&sm.done);  // also on abort: arrives once the products issued so far are done
         __syncwarp();
+        meet();
     } else {
         registers_up<kSoftmaxRegs>();
         if (warp / 4 < tiles) {
         const int q = warp / 4, quarter = warp & 3, r = q * kTile + quarter * 32 + lane;
         const bool live = r < rows;
-        const int tok = live ? (r0 + r) / a.group : t0, qh = h * a.group + (r0 + r) % a.group;
+        const int tok = live ? (r0 + r) / a.group : t0;
         const int P = row.pos + tok;
         const int see_lo = live ? sight.lo(P) : 0x7FFFFFFF, see_hi = live ? P : -1;
+        // the warp's 32 rows of the operand, and the thread's own row; global memory is read and written
+        // 8 rows x 64 bytes at a time through them (a row per thread took 2 us a tile on each way)
+        uint8_t* mine = sm.q[q] + quarter * 4 * (D / 8) * 128;
+        uint8_t* own = mine + (lane >> 3) * (D / 8) * 128 + (lane & 7) * 16;
         float q_step;
         {
             // the row of q: scaled to a maximum in [2^13, 2^14), which is exact, and with scale's sign
-            const typename Elem<DT>::T* src =
-                static_cast<const typename Elem<DT>::T*>(a.q) + i * a.qs.seq + (int64_t)tok * a.qs.token + qh * a.qs.head;
             uint4 raw[D / 8];
 #pragma unroll
-            for (int e = 0; e < D / 8; ++e) raw[e] = live ? __ldg(reinterpret_cast<const uint4*>(src) + e) : make_uint4(0, 0, 0, 0);
+            for (int v = 0; v < 4; ++v) {
+                const int row_v = r - lane + 8 * v + lane % 8;
+                const int64_t at = i * a.qs.seq + (int64_t)((r0 + row_v) / a.group) * a.qs.token +
+                                   (h * a.group + (r0 + row_v) % a.group) * a.qs.head;
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const typename Elem<DT>::T*>(a.q) + at);
+#pragma unroll
+                for (int e = 0; e < D / 32; ++e)
+                    raw[v * (D / 32) + e] = row_v < rows ? __ldg(src + 4 * e + lane / 8) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                for (int e = 0; e < D / 32; ++e)
+                    *reinterpret_cast<uint4*>(mine + v * (D / 8) * 128 + (4 * e + lane / 8) * 128 + lane % 8 * 16) =
+                        raw[v * (D / 32) + e];
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < D / 8; ++e) raw[e] = *reinterpret_cast<const uint4*>(own + e * 128);
             float amax = 0.0f;
 #pragma unroll
             for (int e = 0; e < D / 8; ++e) {
@@ -305,7 +357,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
             const int ex = amax > 0.0f ? (__float_as_int(amax) >> 23) - 127 - 13 : 0;
             const float up = a.scale == 0.0f ? 0.0f : copysignf(pow2i(-ex), a.scale);
             q_step = pow2i(ex) * (a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e);
-            uint8_t* dst = sm.q[q] + ((quarter * 32 + lane) >> 3) * (D / 8) * 128 + (lane & 7) * 16;
 #pragma unroll
             for (int e = 0; e < D / 8; ++e) {
                 const uint32_t w[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
@@ -315,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                     const float2 f = unpack2(w[u], Elem<DT>());
                     o[u] = pack_f16(f.x * up, f.y * up);
                 }
-                *reinterpret_cast<uint4*>(dst + e * 128) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4*>(own + e * 128) = make_uint4(o[0], o[1], o[2], o[3]);
             }
             proxy_fence();
             __syncwarp();
@@ -327,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         const int tt0 = (r0 + q * kTile) / a.group, tt1 = (r0 + min(rows, (q + 1) * kTile) - 1) / a.group;
         const int all_lo = sight.lo(row.pos + tt1), all_hi = row.pos + tt0;
         // the softmax's sum is held over 2^E; any E near the exponents of V serves
-        const float E = steps > 0 ? fminf(fmaxf((float)c.ve[head * cap_blocks + kb0 % cap_blocks], -60.0f), 60.0f) : 0.0f;
+        const float E = nb_all > 0 ? fminf(fmaxf((float)c.ve[head * cap_blocks + kb_all % cap_blocks], -60.0f), 60.0f) : 0.0f;
         float M = -FLT_MAX, l = 0.0f;
         bool ok = true;
         for (int j = 0; j < steps; ++j) {
@@ -418,33 +469,90 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         mbar_drain(&sm.done, 0);
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (__all_sync(0xFFFFFFFFu, ok && *abort == 0)) {
-            const float f = l == 0.0f ? 0.0f : pow2i((int)E) / l;
-            uint16_t* dst = static_cast<uint16_t*>(a.out) + i * a.os.seq + (int64_t)tok * a.os.token + qh * a.os.head;
-            const bool bf = a.out_dtype == DT_BF16;
+        const bool whole = __all_sync(0xFFFFFFFFu, ok && *abort == 0);
+        if (cluster > 1) sm.state[r] = make_float2(M, l);
+        // (rows of another tile's warps, and runs without a step, have nothing in TMEM)
+        float4* sums = reinterpret_cast<float4*>(&sm);  // over the operands: [256 rows][D / 4], pieces permuted by row
 #pragma unroll
-            for (int ch = 0; ch < D / 32; ++ch) {
-                float o[32];
-                if (steps > 0) {
-                    tmem_ld32(o_col + 32 * ch, o);
-                } else {
+        for (int ch = 0; ch < D / 32; ++ch) {
+            float o[32];
+            if (whole && steps > 0) {
+                tmem_ld32(o_col + 32 * ch, o);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+            }
+            if (cluster > 1) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    sums[r * (D / 4) + ((8 * ch + e) ^ (r & (D / 4 - 1)))] =
+                        make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            } else if (live && whole) {
+                const float f = l == 0.0f ? 0.0f : pow2i((int)E) / l;
+                if (l == 0.0f) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = 0.0f;
                 }
-                if (live) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const float x = l == 0.0f ? 0.0f : o[e + 2 * u] * f, y = l == 0.0f ? 0.0f : o[e + 2 * u + 1] * f;
-                            w[u] = bf ? pack2(x, y, Elem<DT_BF16>()) : pack2(x, y, Elem<DT_F16>());
-                        }
-                        *reinterpret_cast<uint4*>(dst + 32 * ch + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                }
+                for (int e = 0; e < 32; e += 8)
+                    *reinterpret_cast<uint4*>(own + (4 * ch + e / 8) * 128) = pack8(o + e, f, a.out_dtype);
             }
         }
+        if (cluster == 1) {
+            __syncwarp();
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const int row_v = r - lane + 8 * v + lane % 8;
+                if (row_v >= rows || !whole) continue;
+                uint4* dst = reinterpret_cast<uint4*>(out_row(row_v));
+#pragma unroll
+                for (int e = 0; e < D / 32; ++e)
+                    dst[4 * e + lane / 8] =
+                        *reinterpret_cast<const uint4*>(mine + v * (D / 8) * 128 + (4 * e + lane / 8) * 128 + lane % 8 * 16);
+            }
+        }
+        }
+        if (cluster > 1) {
+            cluster_sync();
+            // each CTA joins a share of the rows; a thread 8 dimensions of one at a time
+            if (*abort == 0) {
+                const int share = (rows + cluster - 1) / cluster;
+                const int end_row = min(rows, (rank + 1) * share);
+                const float E = nb_all > 0 ? fminf(fmaxf((float)c.ve[head * cap_blocks + kb_all % cap_blocks], -60.0f), 60.0f) : 0.0f;
+                for (int p = threadIdx.x; p < share * (D / 8); p += kSoftmaxWarps * 32) {
+                    const int r = rank * share + p / (D / 8), d8 = p % (D / 8);
+                    if (r >= end_row) break;
+                    float2 st[kMaxPromptCluster];
+                    float4 x[kMaxPromptCluster], y[kMaxPromptCluster];
+                    const uint32_t at = smem_u32(&sm) + r * D * 4;
+    #pragma unroll
+                    for (int k = 0; k < kMaxPromptCluster; ++k) {
+                        st[k] = make_float2(0.0f, 0.0f);
+                        x[k] = y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (k >= cluster) continue;
+                        st[k] = cluster_load2(smem_u32(&sm.state[r]), k);
+                        x[k] = cluster_load4(at + 16 * ((2 * d8) ^ (r & (D / 4 - 1))), k);
+                        y[k] = cluster_load4(at + 16 * ((2 * d8 + 1) ^ (r & (D / 4 - 1))), k);
+                    }
+                    float M = -FLT_MAX, l = 0.0f, o[8] = {};
+    #pragma unroll
+                    for (int k = 0; k < kMaxPromptCluster; ++k)
+                        if (st[k].y != 0.0f) M = fmaxf(M, st[k].x);
+    #pragma unroll
+                    for (int k = 0; k < kMaxPromptCluster; ++k) {
+                        if (st[k].y == 0.0f) continue;
+                        const float f = exp2f(st[k].x - M);
+                        l = fmaf(st[k].y, f, l);
+                        const float v[8] = {x[k].x, x[k].y, x[k].z, x[k].w, y[k].x, y[k].y, y[k].z, y[k].w};
+    #pragma unroll
+                        for (int e = 0; e < 8; ++e) o[e] = fmaf(v[e], f, o[e]);
+                    }
+                    const float f = l == 0.0f ? 0.0f : pow2i((int)E) / l;
+                    *reinterpret_cast<uint4*>(out_row(r) + 8 * d8) = pack8(o, f, a.out_dtype);
+                }
+            }
+            __syncwarp();
+            cluster_sync();  // no CTA leaves while another reads its shared memory
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -461,12 +569,27 @@ constexpr size_t prompt_smem_bytes() {
 }
 static_assert(prompt_smem_bytes<128>() <= 227 * 1024, "the stages fit one SM's shared memory");
 
+cudaLaunchConfig_t prompt_config(int64_t ctas, int cluster, size_t smem, cudaStream_t st, cudaLaunchAttribute* attr) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = cluster;
+    attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    return cfg;
+}
+
 template <int D, int DT>
-cudaError_t prompt_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st) {
-    const int row_blocks = (b.tokens * a.group + 2 * kTile - 1) / (2 * kTile);
-    prompt_kernel<D, DT><<<(unsigned)((int64_t)b.n * c.heads * row_blocks), kThreads, prompt_smem_bytes<D>(), st>>>(c, b, a,
-                                                                                                                 row_blocks);
-    return cudaGetLastError();
+cudaError_t prompt_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, int cluster, cudaStream_t st) {
+    const int row_blocks = (int)(((int64_t)b.tokens * a.group + 2 * kTile - 1) / (2 * kTile));
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg =
+        prompt_config((int64_t)b.n * c.heads * row_blocks * cluster, cluster, prompt_smem_bytes<D>(), st, attr);
+    return cudaLaunchKernelEx(&cfg, prompt_kernel<D, DT>, c, b, a, row_blocks, cluster);
 }
 
 template <int D>
@@ -480,14 +603,41 @@ cudaError_t configure_t() {
 
 }  // namespace
 
-cudaError_t kv8_configure_prompt() {
-    const cudaError_t e = configure_t<128>();
-    return e != cudaSuccess ? e : configure_t<64>();
+cudaError_t kv8_configure_prompt(Kv8Machine* m) {
+    for (const cudaError_t e : {configure_t<128>(), configure_t<64>()})
+        if (e != cudaSuccess) return e;
+    m->prompt_ctas[0] = m->num_sms;
+    for (int j = 1; j < 4; ++j) {
+        cudaLaunchAttribute attr[1];
+        const cudaLaunchConfig_t cfg = prompt_config(m->num_sms << j, 1 << j, prompt_smem_bytes<128>(), 0, attr);
+        int clusters = 0;
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, prompt_kernel<128, DT_BF16>, &cfg);
+        if (e != cudaSuccess) return e;
+        m->prompt_ctas[j] = std::min(clusters << j, m->num_sms);
+    }
+    return cudaSuccess;
 }
 
-cudaError_t launch_kv8_prompt(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, cudaStream_t st) {
-    if (c.dim == 128) return a.q_dtype == DT_BF16 ? prompt_t<128, DT_BF16>(c, b, a, st) : prompt_t<128, DT_F16>(c, b, a, st);
-    return a.q_dtype == DT_BF16 ? prompt_t<64, DT_BF16>(c, b, a, st) : prompt_t<64, DT_F16>(c, b, a, st);
+PromptPlan kv8_prompt_plan(int64_t rows, int64_t items, int64_t blocks, const Kv8Machine& m) {
+    // fitted to 16 .. 1024 tokens over 256 .. 30,000 positions: a CTA takes 6 us besides its steps, a step
+    // 2.3 us with two tiles and 2.0 us with one, joining a cluster 2 us and what the rows add
+    const int64_t ctas = items * ((rows + 2 * kTile - 1) / (2 * kTile)), steps = (blocks + kStepBlocks - 1) / kStepBlocks;
+    PromptPlan best{1, 1e30};
+    for (int j = 0; j < 4 && (1 << j) <= steps; ++j) {
+        const int cluster = 1 << j;
+        if (m.prompt_ctas[j] < cluster) break;
+        const double waves = (double)((ctas * cluster + m.prompt_ctas[j] - 1) / m.prompt_ctas[j]);
+        const double us = waves * (6.0 + (rows > kTile ? 2.3 : 2.0) * (double)((steps + cluster - 1) / cluster)) +
+                          (cluster > 1 ? 2.0 : 0.0);
+        if (us < best.us) best = PromptPlan{cluster, us};
+    }
+    return best;
+}
+
+cudaError_t launch_kv8_prompt(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, int cluster, cudaStream_t st) {
+    if (c.dim == 128)
+        return a.q_dtype == DT_BF16 ? prompt_t<128, DT_BF16>(c, b, a, cluster, st) : prompt_t<128, DT_F16>(c, b, a, cluster, st);
+    return a.q_dtype == DT_BF16 ? prompt_t<64, DT_BF16>(c, b, a, cluster, st) : prompt_t<64, DT_F16>(c, b, a, cluster, st);
 }
 
 }  // namespace stt

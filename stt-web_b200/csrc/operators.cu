@@ -12,7 +12,8 @@
 using namespace stt;
 
 struct stt_kv8_cache {
-    int device = 0, num_sms = 0;
+    int device = 0;
+    Kv8Machine machine{};
     Kv8Dev c{};
     void* memory = nullptr;   // codes and exponents; the library's own unless the caller gave it
     bool owned = false;
@@ -121,8 +122,9 @@ extern "C" int stt_kv8_cache_create(int device, int n_seqs, int n_kv_heads, int 
             if (h) stt_kv8_cache_destroy(h);
         }
     } release{h};
-    CUDA_TRY(cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, device));
-    CUDA_TRY(kv8_configure());
+    int num_sms = 0;
+    CUDA_TRY(cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, device));
+    CUDA_TRY(kv8_configure(num_sms, &h->machine));
     if (d_memory) {
         h->memory = d_memory;
     } else {
@@ -239,13 +241,12 @@ extern "C" int stt_kv8_attention_device(stt_kv8_cache* h, const stt_kv8_batch* b
     a.scale = scale;
     a.part = h->part;
     a.tickets = h->tickets;
-    a.num_sms = h->num_sms;
     const int64_t rows = (int64_t)b->n_tokens * a.group;
     if (rows > INT_MAX - 256 || (int64_t)b->n * h->c.heads > INT_MAX / (rows / 8 + 1))
         return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", b->n, b->n_tokens);
     DeviceScope ds(h->device);
     if (!ds.ok) return set_error(STT_E_CUDA, "cudaSetDevice(%d) failed", h->device);
-    CUDA_TRY(launch_kv8_attention(h->c, device_batch(*b), a, static_cast<cudaStream_t>(cuda_stream)));
+    CUDA_TRY(launch_kv8_attention(h->c, device_batch(*b), a, h->machine, static_cast<cudaStream_t>(cuda_stream)));
     return STT_OK;
 }
 
