@@ -12,7 +12,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// Cluster barrier, and loads from the same place of CTA `rank`'s shared memory.
+// Cluster barrier; loads from and stores to the same place of CTA `rank`'s shared memory.
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -33,6 +33,14 @@ __device__ __forceinline__ float4 cluster_load4(uint32_t addr, int rank) {
                  : "r"(cluster_at(addr, rank))
                  : "memory");
     return v;
+}
+__device__ __forceinline__ void cluster_store2(uint32_t addr, int rank, float x, float y) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_at(addr, rank)), "f"(x), "f"(y) : "memory");
+}
+__device__ __forceinline__ void cluster_store4(uint32_t addr, int rank, float x, float y, float z, float w) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_at(addr, rank)), "f"(x), "f"(y), "f"(z),
+                 "f"(w)
+                 : "memory");
 }
 
 // Bytes `sel` of biased codes (code + 128) as a pair of f16 codes.

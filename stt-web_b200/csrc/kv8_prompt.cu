@@ -25,7 +25,8 @@
 // Both operands of a product lie in core matrices of 8 rows x 16 bytes: a key's 8 dimensions are one
 // row of K's K-major matrix and of V's MN-major one, so both are written alike.
 // Where there are fewer row blocks than SMs, a cluster of CTAs takes the steps of a row block in equal
-// runs; at the end each leaves its O, M and l in shared memory and joins a share of the rows from all.
+// runs; at the end each sends O, M and l of every row to the shared memory of the CTA that joins that row
+// in its share.
 // Every wait is bounded: one that gives up sets the CTA's abort word, all roles leave, the copies and
 // products in flight are waited for, and the cache's error word records it.
 #include <cfloat>
@@ -59,8 +60,9 @@ struct PromptSmem {
     uint8_t k[2][kTile * D * 2], v[2][kTile * D * 2];
     __align__(16) float k_step[kExpSlots][kStepBlocks], v_exp[kExpSlots][kStepBlocks];
     uint64_t q_full[2], s_full[2], p_half[2], p_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], e_full[kExpSlots];
+    uint64_t q_raw[kSoftmaxWarps];
     uint64_t done;
-    float2 state[2 * kTile];              // M and l of the rows, for a cluster
+    float2 state[2 * kTile];              // M and l of the CTA's share of the rows, by rank of the cluster
     uint32_t tmem;
     int abort;
 };
@@ -161,6 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         }
         for (int j = 0; j < kExpSlots; ++j) mbar_init(&sm.e_full[j], 1);
         mbar_init(&sm.done, 1);
+        for (int j = 0; j < kSoftmaxWarps; ++j) mbar_init(&sm.q_raw[j], 1);
         sm.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -265,8 +268,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                 mma_f16_ts(tmem + kOCol + q * kTile, tmem + q * kTile + k * 8, smem_desc(va + k * 2 * GROUP, GROUP, 128), pv_desc,
                            add || k > 0);
         };
-        bool ok = steps > 0;
+        bool ok = true;  // (without a step too, `done` says that nothing writes the operands any more)
         for (int q = 0; ok && q < tiles; ++q) ok = mbar_wait(&sm.q_full[q], 0, abort);
+        ok = ok && steps > 0;
         if (ok) ok = mbar_wait(&sm.k_full[0], 0, abort);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (ok) {
@@ -317,33 +321,26 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         const int tok = live ? (r0 + r) / a.group : t0;
         const int P = row.pos + tok;
         const int see_lo = live ? sight.lo(P) : 0x7FFFFFFF, see_hi = live ? P : -1;
-        // the warp's 32 rows of the operand, and the thread's own row; global memory is read and written
-        // 8 rows x 64 bytes at a time through them (a row per thread took 2 us a tile on each way)
+        // the warp's 32 rows of the operand, and the thread's own row
         uint8_t* mine = sm.q[q] + quarter * 4 * (D / 8) * 128;
         uint8_t* own = mine + (lane >> 3) * (D / 8) * 128 + (lane & 7) * 16;
         float q_step;
         {
             // the row of q: scaled to a maximum in [2^13, 2^14), which is exact, and with scale's sign
-            uint4 raw[D / 8];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int row_v = r - lane + 8 * v + lane % 8;
-                const int64_t at = i * a.qs.seq + (int64_t)((r0 + row_v) / a.group) * a.qs.token +
-                                   (h * a.group + (r0 + row_v) % a.group) * a.qs.head;
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const typename Elem<DT>::T*>(a.q) + at);
-#pragma unroll
-                for (int e = 0; e < D / 32; ++e)
-                    raw[v * (D / 32) + e] = row_v < rows ? __ldg(src + 4 * e + lane / 8) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-#pragma unroll
-                for (int e = 0; e < D / 32; ++e)
-                    *reinterpret_cast<uint4*>(mine + v * (D / 8) * 128 + (4 * e + lane / 8) * 128 + lane % 8 * 16) =
-                        raw[v * (D / 32) + e];
+            const uint32_t there = __ballot_sync(0xFFFFFFFFu, live);
+            if (lane == 0) mbar_expect_tx(&sm.q_raw[warp], __popc(there) * 2 * D);
             __syncwarp();
+            if (live)
+                bulk_g2s(mine + lane * 2 * D, static_cast<const uint16_t*>(a.q) + i * a.qs.seq + (int64_t)tok * a.qs.token +
+                                                  (h * a.group + (r0 + r) % a.group) * a.qs.head,
+                         2 * D, &sm.q_raw[warp]);
+            __all_sync(0xFFFFFFFFu, mbar_wait(&sm.q_raw[warp], 0, abort));  // (one that gave up is seen below)
+            uint4 raw[D / 8];  // pieces in an order of the lane's own, as in load_row
 #pragma unroll
-            for (int e = 0; e < D / 8; ++e) raw[e] = *reinterpret_cast<const uint4*>(own + e * 128);
+            for (int e = 0; e < D / 8; ++e)
+                raw[e] = live ? *reinterpret_cast<const uint4*>(mine + lane * 2 * D + (e + lane) % (D / 8) * 16)
+                              : make_uint4(0, 0, 0, 0);
+            __syncwarp();
             float amax = 0.0f;
 #pragma unroll
             for (int e = 0; e < D / 8; ++e) {
@@ -366,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                     const float2 f = unpack2(w[u], Elem<DT>());
                     o[u] = pack_f16(f.x * up, f.y * up);
                 }
-                *reinterpret_cast<uint4*>(own + e * 128) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4*>(own + (e + lane) % (D / 8) * 128) = make_uint4(o[0], o[1], o[2], o[3]);
             }
             proxy_fence();
             __syncwarp();
@@ -470,24 +467,33 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const bool whole = __all_sync(0xFFFFFFFFu, ok && *abort == 0);
-        if (cluster > 1) sm.state[r] = make_float2(M, l);
-        // (rows of another tile's warps, and runs without a step, have nothing in TMEM)
-        float4* sums = reinterpret_cast<float4*>(&sm);  // over the operands: [256 rows][D / 4], pieces permuted by row
+        const int share = (rows + cluster - 1) / cluster;
+        if (cluster > 1) {
+            __syncwarp();
+            cluster_sync();  // every CTA's products are done: the sums may lie over the operands
+            if (live)
+                cluster_store2(smem_u32(&sm.state[r % share * cluster + rank]), r / share, M, l);
+        }
+        uint8_t* staged = reinterpret_cast<uint8_t*>(&sm) + r * (2 * D + 16);  // over the operands: no bank twice
+        float4* sums = reinterpret_cast<float4*>(&sm);  // [row of the share][rank][D / 4], pieces permuted by row
 #pragma unroll
         for (int ch = 0; ch < D / 32; ++ch) {
             float o[32];
-            if (whole && steps > 0) {
+            if (whole && steps > 0) {  // (a run without a step has nothing in TMEM)
                 tmem_ld32(o_col + 32 * ch, o);
             } else {
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = 0.0f;
             }
             if (cluster > 1) {
+                if (live) {
+                    const uint32_t at = smem_u32(sums + (r % share * cluster + rank) * (D / 4));
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    sums[r * (D / 4) + ((8 * ch + e) ^ (r & (D / 4 - 1)))] =
-                        make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            } else if (live && whole) {
+                    for (int e = 0; e < 8; ++e)
+                        cluster_store4(at + 16 * ((8 * ch + e) ^ (r % share & 7)), r / share, o[4 * e], o[4 * e + 1],
+                                       o[4 * e + 2], o[4 * e + 3]);
+                }
+            } else {
                 const float f = l == 0.0f ? 0.0f : pow2i((int)E) / l;
                 if (l == 0.0f) {
 #pragma unroll
@@ -495,64 +501,46 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e += 8)
-                    *reinterpret_cast<uint4*>(own + (4 * ch + e / 8) * 128) = pack8(o + e, f, a.out_dtype);
+                    *reinterpret_cast<uint4*>(staged + (32 * ch + e) * 2) = pack8(o + e, f, a.out_dtype);
             }
         }
         if (cluster == 1) {
+            proxy_fence();
+            if (live && whole) bulk_s2g(out_row(r), staged, 2 * D);
+            bulk_s2g_wait();
+        } else {
             __syncwarp();
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int row_v = r - lane + 8 * v + lane % 8;
-                if (row_v >= rows || !whole) continue;
-                uint4* dst = reinterpret_cast<uint4*>(out_row(row_v));
-#pragma unroll
-                for (int e = 0; e < D / 32; ++e)
-                    dst[4 * e + lane / 8] =
-                        *reinterpret_cast<const uint4*>(mine + v * (D / 8) * 128 + (4 * e + lane / 8) * 128 + lane % 8 * 16);
-            }
-        }
-        }
-        if (cluster > 1) {
             cluster_sync();
-            // each CTA joins a share of the rows; a thread 8 dimensions of one at a time
-            if (*abort == 0) {
-                const int share = (rows + cluster - 1) / cluster;
-                const int end_row = min(rows, (rank + 1) * share);
-                const float E = nb_all > 0 ? fminf(fmaxf((float)c.ve[head * cap_blocks + kb_all % cap_blocks], -60.0f), 60.0f) : 0.0f;
-                for (int p = threadIdx.x; p < share * (D / 8); p += kSoftmaxWarps * 32) {
-                    const int r = rank * share + p / (D / 8), d8 = p % (D / 8);
-                    if (r >= end_row) break;
-                    float2 st[kMaxPromptCluster];
-                    float4 x[kMaxPromptCluster], y[kMaxPromptCluster];
-                    const uint32_t at = smem_u32(&sm) + r * D * 4;
-    #pragma unroll
-                    for (int k = 0; k < kMaxPromptCluster; ++k) {
-                        st[k] = make_float2(0.0f, 0.0f);
-                        x[k] = y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (k >= cluster) continue;
-                        st[k] = cluster_load2(smem_u32(&sm.state[r]), k);
-                        x[k] = cluster_load4(at + 16 * ((2 * d8) ^ (r & (D / 4 - 1))), k);
-                        y[k] = cluster_load4(at + 16 * ((2 * d8 + 1) ^ (r & (D / 4 - 1))), k);
-                    }
-                    float M = -FLT_MAX, l = 0.0f, o[8] = {};
-    #pragma unroll
-                    for (int k = 0; k < kMaxPromptCluster; ++k)
-                        if (st[k].y != 0.0f) M = fmaxf(M, st[k].x);
-    #pragma unroll
-                    for (int k = 0; k < kMaxPromptCluster; ++k) {
-                        if (st[k].y == 0.0f) continue;
-                        const float f = exp2f(st[k].x - M);
-                        l = fmaf(st[k].y, f, l);
-                        const float v[8] = {x[k].x, x[k].y, x[k].z, x[k].w, y[k].x, y[k].y, y[k].z, y[k].w};
-    #pragma unroll
-                        for (int e = 0; e < 8; ++e) o[e] = fmaf(v[e], f, o[e]);
-                    }
-                    const float f = l == 0.0f ? 0.0f : pow2i((int)E) / l;
-                    *reinterpret_cast<uint4*>(out_row(r) + 8 * d8) = pack8(o, f, a.out_dtype);
+        }
+        } else {
+            meet();
+        }
+        if (cluster > 1 && *abort == 0) {
+            // each CTA joins its share of the rows; a thread 8 dimensions of one at a time
+            const int share = (rows + cluster - 1) / cluster;
+            const int mine = min(rows - rank * share, share);
+            const float E = nb_all > 0 ? fminf(fmaxf((float)c.ve[head * cap_blocks + kb_all % cap_blocks], -60.0f), 60.0f) : 0.0f;
+            for (int p = threadIdx.x; p < mine * (D / 8); p += kSoftmaxWarps * 32) {
+                const int at = p / (D / 8), d8 = p % (D / 8);
+                float M = -FLT_MAX, l = 0.0f, o[8] = {};
+                for (int k = 0; k < cluster; ++k) {
+                    const float2 st = sm.state[at * cluster + k];
+                    if (st.y != 0.0f) M = fmaxf(M, st.x);
                 }
+                for (int k = 0; k < cluster; ++k) {
+                    const float2 st = sm.state[at * cluster + k];
+                    if (st.y == 0.0f) continue;
+                    const float4* from = reinterpret_cast<const float4*>(&sm) + (at * cluster + k) * (D / 4);
+                    const float4 x = from[(2 * d8) ^ (at & 7)], y = from[(2 * d8 + 1) ^ (at & 7)];
+                    const float f = exp2f(st.x - M);
+                    l = fmaf(st.y, f, l);
+                    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] = fmaf(v[e], f, o[e]);
+                }
+                const float f = l == 0.0f ? 0.0f : pow2i((int)E) / l;
+                *reinterpret_cast<uint4*>(out_row(rank * share + at) + 8 * d8) = pack8(o, f, a.out_dtype);
             }
-            __syncwarp();
-            cluster_sync();  // no CTA leaves while another reads its shared memory
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -620,7 +608,9 @@ cudaError_t kv8_configure_prompt(Kv8Machine* m) {
 
 PromptPlan kv8_prompt_plan(int64_t rows, int64_t items, int64_t blocks, const Kv8Machine& m) {
     // fitted to 16 .. 1024 tokens over 256 .. 30,000 positions: a CTA takes 6 us besides its steps, a step
-    // 2.3 us with two tiles and 2.0 us with one, joining a cluster 2 us and what the rows add
+    // 2.3 us with two tiles and 2.0 us with one, a cluster 2 us more.  The other kernel's time comes from a
+    // model of the same calls: 64 tokens over 256 positions of 4 heads take 7.2 us there and 11 us here, 256
+    // over 4096 of 16 heads 117 us there and 36 us here
     const int64_t ctas = items * ((rows + 2 * kTile - 1) / (2 * kTile)), steps = (blocks + kStepBlocks - 1) / kStepBlocks;
     PromptPlan best{1, 1e30};
     for (int j = 0; j < 4 && (1 << j) <= steps; ++j) {
