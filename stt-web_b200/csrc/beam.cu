@@ -9,7 +9,7 @@
 // candidates compared in 64 bits; the exponentials themselves are f32, 16 of a thread added at a time
 // (their rounding errors, 2^-24 each, average out: 1e-8 of the sum at 8000 logits).
 //
-// The best of a tile of 8192 logits: the k-th largest of its 32 half warps' maxima bounds the k-th best
+// The best of a chunk: the k-th largest of the maxima of its 32 groups of 4 lanes bounds the k-th best
 // logit from below, and little more than the k best reach it; those few go to a list in shared memory,
 // with the list's and the tiles' bounds carried from tile to tile, and are ranked by counting.  A tile
 // costs a maximum, an exponential and a comparison per logit.  Where more reach the bound than the list
@@ -18,13 +18,15 @@
 
 #include "beam.h"
 #include "kv8.cuh"
+#include "tcgen05.cuh"
 
 namespace stt {
 
 namespace {
 
 constexpr int kWarps = kBeamThreads / 32;
-static_assert(kWarps == 16, "the tile's bound is taken from 32 half warps");
+constexpr int kGroup = kBeamThreads / 32;  // lanes of a group: 32 groups give a tile's bound
+static_assert(kGroup == 4, "a group lies in a warp");
 
 // Order-preserving 32 bits of an f32 (no NaN; -0 counts as +0).
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -53,21 +55,13 @@ __device__ __forceinline__ Key warp_sort(Key k, int lane, Greater greater, Shuff
     return k;
 }
 
-// How many of the n indexes the warp finds ahead: a comparison per lane, a ballot per 32.
-template <class Ahead>
-__device__ __forceinline__ int warp_rank(int n, int lane, Ahead ahead) {
-    int rank = 0;
-    for (int j0 = 0; j0 < n; j0 += 32) rank += __popc(__ballot_sync(0xFFFFFFFFu, j0 + lane < n && ahead(j0 + lane)));
-    return rank;
-}
-
 // A candidate of the whole utterance.
 struct Cand {
     double total;
     int32_t at;  // beam * vocab + token; 0x7FFFFFFF: none
 };
 __device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
-    return a.total > b.total || (a.total == b.total && a.at < b.at);
+    return (a.total > b.total) | ((a.total == b.total) & (a.at < b.at));  // (no branches)
 }
 
 template <int DT>
@@ -82,10 +76,31 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return r;
+}
 // Maximum that a NaN wins.
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -109,9 +124,8 @@ struct Best {
     }
 };
 
-constexpr int kList = 512;     // keys of the list: one per thread
-constexpr int kCounted = 96;   // up to this many are ranked by counting (4 instructions a pair); more by sorting
-static_assert(kList == kBeamThreads, "a thread loads one key of the list");
+constexpr int kList = 512;      // keys of the list
+constexpr int kCounted = 256;   // up to this many stay there, and are ranked by counting; more are sorted
 
 struct Lists {
     uint64_t list[kList], pending[kWarps][64], top[kWarps][32];
@@ -124,11 +138,11 @@ struct Sorted {
 // from index v0 on, one tile, that reach the bound.  Rarely needed and long: kept out of the tile loop's
 // code, whose instruction fetches it would stretch (it did: 900 cycles a tile).
 template <int DT>
-__device__ __noinline__ Sorted sort_list(Lists& s, uint32_t* many, int from, const typename Elem<DT>::T* row, int v0, int vocab,
+__device__ __noinline__ Sorted sort_list(Lists& s, int from, const typename Elem<DT>::T* row, int v0, int vocab,
                                          float bound, int k) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     Best best;
-    best.merge(tid < from ? s.list[tid] : 0, lane);
+    for (int j = 0; j < from; j += kBeamThreads) best.merge(j + tid < from ? s.list[j + tid] : 0, lane);
     if (row) {
         uint64_t* pending = s.pending[warp];
         uint64_t kth = 0;  // the warp's k-th best
@@ -168,60 +182,70 @@ __device__ __noinline__ Sorted sort_list(Lists& s, uint32_t* many, int from, con
     for (int j = 0; j < k; ++j) r.listed += s.top[0][j] != 0;
     if (tid < k) s.list[tid] = s.top[0][tid];
     if (r.listed == k) r.bound = fmaxf(bound, from_ordered((uint32_t)(s.top[0][k - 1] >> 32)));
-    if (tid == 0) *many = r.listed;
     __syncthreads();
     return r;
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
+__global__ void __launch_bounds__(kBeamThreads, kBeamCtas) select_kernel(BeamArgs a) {
     using T = typename Elem<DT>::T;
     constexpr int VEC = 16 / (int)sizeof(T);            // elements of a 16-byte load
     constexpr int LOADS = kBeamPerThread / VEC;
     constexpr int kRoom = 1024;                         // candidates of an utterance that are ranked at once
-    __shared__ union {
-        Lists s;
+    constexpr int kSlots = kRoom * sizeof(Cand) / (kBeamChunk * sizeof(T));
+    static_assert(kSlots >= 2, "a tile is fetched while another is worked on");
+    __shared__ __align__(128) union {
+        T tiles[kSlots][kBeamChunk];                    // as they come from memory
         Cand cands[kRoom];
     } sm;
-    __shared__ float wref[kWarps], half_max[2][2 * kWarps];
+    __shared__ Lists lists_of;
+    __shared__ uint64_t full[kSlots];
+    __shared__ int late;
+    __shared__ float wref[kWarps], group_max[2][32];
     __shared__ double wsum[kWarps];
-    __shared__ uint32_t many, last;
+    __shared__ uint32_t many, last, found, pushed[3];  // pushed: by the tiles, in turn
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int chunk = blockIdx.x % a.chunks, r = blockIdx.x / a.chunks;
     const int g = r / a.beams, k = a.beams;
     const int64_t part = (int64_t)r * a.chunks + chunk;
-    if (tid == 0) many = 0;
+    if (tid == 0) {
+        many = found = late = 0;
+        pushed[0] = pushed[1] = pushed[2] = 0;
+        for (int j = 0; j < kSlots; ++j) mbar_init(&full[j], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
     if (!(a.done && a.done[r])) {
         // Tiles are cut at 16-byte boundaries of memory, whatever the row's own alignment: vector j of
-        // thread t of a tile covers elements -lead + (tile * CTA + j * 512 + t) * VEC on.
+        // thread t of a tile covers elements -lead + tile * kBeamChunk + (j * kBeamThreads + t) * VEC on.
         const T* row = static_cast<const T*>(a.logits) + r * a.row_stride;
         const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-        const int inside = lead ? VEC - lead : 0;
-        const bool any_whole = inside + VEC <= a.vocab;
         float ref = -INFINITY;    // the sum's reference: within 60 of the largest so far
         double sum = 0.0;
         float bound = -INFINITY;  // the chunk has at least k logits that reach it
         int listed = 0;           // keys of the list
-        uint64_t* const list = sm.s.list;
+        uint64_t* const list = lists_of.list;
         const int tile0 = chunk * a.tiles_per_chunk;
         const int tile1 = min(tile0 + a.tiles_per_chunk, (a.vocab + lead + kBeamChunk - 1) / kBeamChunk);
-        // Vectors that lie inside the row are loaded whole and without a branch (the others read vector
-        // `inside` instead); the row's ragged ends are put in element by element.
-        auto first = [&](int tile) { return tile * kBeamChunk + tid * VEC - lead; };  // vector j is j * 512 * VEC on
+        // Vectors that lie inside the row come by a bulk copy of the tile; the row's ragged ends are put in
+        // element by element.
+        auto first = [&](int tile) { return tile * kBeamChunk + tid * VEC - lead; };
         auto whole = [&](int v0) { return v0 >= 0 && v0 + VEC <= a.vocab; };
-        auto issue = [&](int tile, uint4 (&raw)[LOADS]) {
-#pragma unroll
-            for (int j = 0; j < LOADS; ++j) {
-                const int v0 = first(tile) + j * kBeamThreads * VEC;
-                if (any_whole) raw[j] = __ldg(reinterpret_cast<const uint4*>(row + (whole(v0) ? v0 : inside)));
-            }
+        auto issue = [&](int tile) {  // by one thread
+            const int v0 = tile * kBeamChunk - lead, from = v0 < 0 ? VEC : 0;
+            const int to = min(kBeamChunk, (a.vocab - v0) / VEC * VEC);
+            const uint32_t bytes = to > from ? (uint32_t)(to - from) * sizeof(T) : 0;
+            mbar_expect_tx(&full[(tile - tile0) % kSlots], bytes);
+            if (bytes) bulk_g2s(&sm.tiles[(tile - tile0) % kSlots][from], row + v0 + from, bytes, &full[(tile - tile0) % kSlots]);
         };
-        auto unpack = [&](int tile, const uint4 (&raw)[LOADS], float (&x)[kBeamPerThread]) {
+        auto unpack = [&](int tile, float (&x)[kBeamPerThread]) {
+            const bool inner = tile * kBeamChunk >= lead && (tile + 1) * kBeamChunk - lead <= a.vocab;
+            const uint4* raw = reinterpret_cast<const uint4*>(sm.tiles[(tile - tile0) % kSlots]);
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) {
                 const int v0 = first(tile) + j * kBeamThreads * VEC;
-                const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-                const bool all = whole(v0);
+                const uint4 r4 = raw[j * kBeamThreads + tid];
+                const uint32_t w[4] = {r4.x, r4.y, r4.z, r4.w};
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     float y;
@@ -233,29 +257,47 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
                     }
                     x[j * VEC + e] = y;
                 }
-                if (!all) {
+                if (!inner && !whole(v0)) {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e)
                         x[j * VEC + e] = v0 + e >= 0 && v0 + e < a.vocab ? to_f32<DT>(row[v0 + e]) : -INFINITY;
                 }
             }
         };
-        uint4 raw[LOADS] = {};
-        if (tile0 < tile1) issue(tile0, raw);
+        if (tid == 0)
+            for (int tile = tile0; tile < min(tile0 + kSlots, tile1); ++tile) issue(tile);
+        // What a tile pushed is looked at after the next one's barrier (the tile's counter is its own until
+        // every thread has seen it), so that a tile takes one barrier.
+        uint32_t *counter = pushed, *counter1 = pushed + 1, *counter2 = pushed + 2;  // this tile's, the next's, the last's
+        auto settle = [&](int tile) {
+            const int now = listed + (int)*counter2;
+            if (now <= kCounted) {
+                listed = now;
+            } else {
+                const Sorted s = sort_list<DT>(lists_of, now <= kList ? now : listed, now <= kList ? nullptr : row,
+                                               tile * kBeamChunk - lead, a.vocab, bound, k);
+                listed = s.listed;
+                bound = s.bound;
+            }
+        };
+        float group = -INFINITY;  // the greatest of the lane's group so far
         for (int tile = tile0; tile < tile1; ++tile) {
             float x[kBeamPerThread];
             const int base = first(tile);
             auto index = [&](int e) { return base + e / VEC * (kBeamThreads * VEC) + e % VEC; };
-            unpack(tile, raw, x);
-            if (tile + 1 < tile1) issue(tile + 1, raw);  // on their way while this tile is worked on
-            float lane_max = x[0];
+            mbar_wait(&full[(tile - tile0) % kSlots], (tile - tile0) / kSlots & 1, &late);
+            unpack(tile, x);
+            float m0 = max_nan(x[0], x[1]), m1 = max_nan(x[2], x[3]);  // (two chains)
 #pragma unroll
-            for (int e = 1; e < kBeamPerThread; ++e) lane_max = max_nan(lane_max, x[e]);
+            for (int e = 4; e < kBeamPerThread; e += 4) m0 = max3_nan(m0, x[e], x[e + 1]), m1 = max3_nan(m1, x[e + 2], x[e + 3]);
+            const float lane_max = max_nan(m0, m1);
             float mx = lane_max;
 #pragma unroll
-            for (int o = 1; o < 16; o <<= 1) mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-            if ((lane & 15) == 0) half_max[tile & 1][2 * warp + (lane >> 4)] = mx;
-            mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+            for (int o = 1; o < kGroup; o <<= 1) mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+            group = max_nan(group, mx);
+            if (lane % kGroup == 0) group_max[tile & 1][tid / kGroup] = group;
+#pragma unroll
+            for (int o = kGroup; o < 32; o <<= 1) mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
             // the warp's sum; NaN and +inf carry into it and mark the row
             if (!(mx < INFINITY)) {
                 ref = INFINITY;
@@ -266,10 +308,14 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
                 }
                 // e^(x - ref) as 2^((x - ref) log2 e): the argument is off by 2^-23 of its size, the power
                 // by 2^-22; the difference first, since ref may be the type's lowest value
-                float s = 0.0f;
+                const float2 less = make_float2(-ref, -ref), log2e = make_float2(kLog2e, kLog2e);
+                float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int e = 0; e < kBeamPerThread; ++e) s += exp2_approx((x[e] - ref) * kLog2e);
-                sum += s;
+                for (int e = 0; e < kBeamPerThread; e += 2) {
+                    const float2 y = mul2(add2(make_float2(x[e], x[e + 1]), less), log2e);
+                    s = add2(s, make_float2(exp2_approx(y.x), exp2_approx(y.y)));
+                }
+                sum += s.x + s.y;
             }
             if (tile + 1 == tile1) {
                 double total = sum;
@@ -278,21 +324,27 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
                 if (lane == 0) wref[warp] = ref, wsum[warp] = total;
             }
             __syncthreads();
-            // k groups or more of neighbouring half warps: the least of their maxima
-            uint32_t hm = ordered(half_max[tile & 1][lane]);
-            for (int o = 1, groups = 16; groups >= k && groups > 0; o <<= 1, groups >>= 1)
-                hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, o));
-            float least = from_ordered(__reduce_min_sync(0xFFFFFFFFu, hm));
-            if (k > 8 || least == -INFINITY) {
-                // more groups than half of the half warps, or groups that a short or masked row leaves
-                // empty: the k-th largest of the half warps is worth the sort (at 16 beams 23 logits reach
-                // it, 54 the least of 16)
-                const uint32_t sorted = warp_sort(
-                    ordered(half_max[tile & 1][lane]), lane, [](uint32_t p, uint32_t q) { return p > q; },
-                    [](uint32_t p, int d) { return __shfl_xor_sync(0xFFFFFFFFu, p, d); });
-                least = from_ordered(__shfl_sync(0xFFFFFFFFu, sorted, k - 1));
+            if (tid == 0 && tile + kSlots < tile1) issue(tile + kSlots);  // every thread has read the slot
+            if (tile > tile0) settle(tile - 1);
+            if (tid == 0) *counter1 = 0;
+            const float gm = group_max[tile & 1][lane];
+            if (bound == -INFINITY || __popc(__ballot_sync(0xFFFFFFFFu, gm > bound)) >= k) {  // (else it stays)
+                // k or more sets of neighbouring groups: the least of their maxima
+                uint32_t hm = ordered(gm);
+                for (int o = 1, sets = 16; sets >= k && sets > 0; o <<= 1, sets >>= 1)
+                    hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, o));
+                float least = from_ordered(__reduce_min_sync(0xFFFFFFFFu, hm));
+                if (k > 8 || least == -INFINITY) {
+                    // more sets than half of the groups, or sets that a short or masked row leaves empty: the
+                    // k-th largest of the groups is worth the sort (at 16 beams 23 logits reach it, 54 the
+                    // least of 16)
+                    const uint32_t sorted = warp_sort(
+                        ordered(gm), lane, [](uint32_t p, uint32_t q) { return p > q; },
+                        [](uint32_t p, int d) { return __shfl_xor_sync(0xFFFFFFFFu, p, d); });
+                    least = from_ordered(__shfl_sync(0xFFFFFFFFu, sorted, k - 1));
+                }
+                bound = fmaxf(bound, least);
             }
-            bound = fmaxf(bound, least);
             if (lane_max >= bound) {
                 uint32_t reach = 0;
 #pragma unroll
@@ -303,7 +355,7 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
                         if (index(e) < 0 || index(e) >= a.vocab) reach &= ~(1u << e);
                 }
                 const uint32_t mine = __popc(reach);
-                uint32_t at = mine ? atomicAdd(&many, mine) : 0;
+                uint32_t at = listed + atomicAdd(counter, mine);
                 if (mine == 1) {  // as a rule
                     if (at < kList) list[at] = make_key(lane_max, (uint32_t)index(__ffs(reach) - 1));
                 } else {
@@ -315,29 +367,15 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
                         }
                 }
             }
-            __syncthreads();
-            const int now = (int)many;
-            if (now <= (tile + 1 == tile1 ? kCounted : kList / 2)) {
-                listed = now;
-            } else {
-                const Sorted s = sort_list<DT>(sm.s, &many, now <= kList ? now : listed, now <= kList ? nullptr : row,
-                                               tile * kBeamChunk - lead, a.vocab, bound, k);
-                listed = s.listed;
-                bound = s.bound;
-            }
+            uint32_t* const t = counter2;
+            counter2 = counter, counter = counter1, counter1 = t;
         }
+        __syncthreads();
+        if (tile1 > tile0) settle(tile1 - 1);
         if (tile1 <= tile0) {  // the row ends before this chunk
             if (lane == 0) wref[warp] = -INFINITY, wsum[warp] = 0.0;
             __syncthreads();
         }
-        // the k best of the list: a key's rank is the number of larger ones
-        uint64_t* out = a.part_keys + part * a.key_stride;
-        for (int q = warp; q < listed; q += kWarps) {
-            const uint64_t key = list[q];
-            const int rank = warp_rank(listed, lane, [&](int j) { return list[j] > key; });
-            if (lane == 0 && rank < k) out[rank] = key;
-        }
-        if (tid >= listed && tid < k) out[tid] = 0;  // a chunk of fewer elements
         if (warp == kWarps - 1) {
             const float m = lane < kWarps ? wref[lane] : -INFINITY;
             float top = m;
@@ -348,8 +386,25 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
             for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
             if (lane == 0) a.part_max[part] = top, a.part_sum[part] = s;
         }
+        // the k best of the list, among those that reach the last bound: a key's rank is the number of larger ones
+        uint64_t* out = a.part_keys + part * a.key_stride;
+        uint64_t* const left = lists_of.pending[0];
+        static_assert(kWarps * 64 >= kCounted, "the list's keys have room");
+        for (int q = tid; q < listed; q += kBeamThreads)
+            if ((uint32_t)(list[q] >> 32) >= ordered(bound)) left[atomicAdd(&found, 1u)] = list[q];
+        __syncthreads();
+        listed = (int)found;
+        for (int q = tid; q < listed; q += kBeamThreads) {
+            const uint64_t key = left[q];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < listed; ++j) rank += left[j] > key;
+            if (rank < k) out[rank] = key;
+        }
+        if (tid >= listed && tid < k) out[tid] = 0;  // a chunk of fewer elements
     }
     __syncthreads();
+    if (tid == 0 && late) atomicCAS(a.err, 0, -5);  // STT_E_DEVICE_FLAG: a copy that never came
     if (tid == 0) last = ticket(a.tickets + g) == (uint32_t)(a.beams * a.chunks - 1);
     __syncthreads();
     if (!last) return;
@@ -360,21 +415,23 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
     __shared__ uint8_t state[kMaxBeams], over[kMaxBeams];  // state 0 live, 1 ended, 2 all candidates at -inf
     const int64_t row0 = (int64_t)g * k;
     static_assert(kBeamMaxChunks <= 32, "a lane joins one chunk");
-    for (int b = warp; b < k; b += kWarps) {
-        const int64_t p = (row0 + b) * a.chunks + lane;
-        const bool end_b = a.done && a.done[row0 + b], here = !end_b && lane < a.chunks;
-        const float s = a.scores[row0 + b];
+    int per_beam = 1;  // lanes of a beam
+    while (per_beam < a.chunks) per_beam <<= 1;
+    for (int b0 = warp * (32 / per_beam); b0 < k; b0 += kBeamThreads / per_beam) {
+        const int b = b0 + lane / per_beam, at = lane % per_beam;
+        const bool real = b < k;
+        const bool end_b = real && a.done && a.done[row0 + b], here = real && !end_b && at < a.chunks;
+        const int64_t p = (row0 + b) * a.chunks + at;
+        const float s = real ? a.scores[row0 + b] : 0.0f;
         const float mc = here ? __ldcg(a.part_max + p) : -INFINITY;
         double sum = here ? __ldcg(a.part_sum + p) : 0.0;
         float m = mc;
         if (a.chunks > 1) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            for (int o = per_beam / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
             sum = mc > -INFINITY && m < INFINITY ? sum * exp((double)mc - (double)m) : 0.0;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            for (int o = per_beam / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
         }
-        if (lane == 0) {
+        if (real && at == 0) {
             const bool bad = !(s < INFINITY) || (!end_b && m == INFINITY);
             if (bad) atomicCAS(a.err, 0, -5);  // STT_E_DEVICE_FLAG
             const int st = bad || s == -INFINITY || (!end_b && m == -INFINITY) ? 2 : end_b ? 1 : 0;
@@ -385,7 +442,6 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
             if (st == 0) lse[b] = log(sum);
         }
     }
-    if (tid == 0) many = 0;
     __syncthreads();
     // List l = beam * chunks + chunk holds k candidates, best first.
     const int lists = k * a.chunks;
@@ -420,64 +476,47 @@ __global__ void __launch_bounds__(kBeamThreads, 2) select_kernel(BeamArgs a) {
         a.tokens[o] = token;
         if (a.next_done) a.next_done[o] = over[b] || token == a.eos;
     };
-    // Where there are many, only candidates that reach the k-th best of the lists' first ones count.
+    // The lists that can hold one of the k best: where there are more than k, those with the k best first
+    // candidates (fewer than k may have one), best first; then candidate j of the list at place p counts if
+    // p + j < k and it reaches the k-th best of the first ones.
     Cand L = kNone;
     Cand* cands = sm.cands;
-    __shared__ Cand limit[kWarps];
-    if (lists >= k && lists * k > kCounted) {
+    __shared__ Cand limit;
+    __shared__ int alive[kMaxBeams];
+    int places = lists;
+    if (lists > k) {
+        if (tid == 0) limit = kNone, found = 0;
         for (int l = tid; l < lists; l += kBeamThreads) cands[l] = candidate(l, 0);
-        // (fewer than k of them may be candidates: then everything counts)
-        if (tid == 0) limit[0] = kNone;
         __syncthreads();
-        for (int l = warp; l < lists; l += kWarps) {
+        for (int l = tid; l < lists; l += kBeamThreads) {
             const Cand c = cands[l];
-            if (c.at != 0x7FFFFFFF && warp_rank(lists, lane, [&](int j) { return better(cands[j], c); }) == k - 1 && lane == 0) limit[0] = c;
+            if (c.at == 0x7FFFFFFF) continue;
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < lists; ++j) rank += better(cands[j], c);
+            if (rank < k) alive[rank] = l, atomicAdd(&found, 1u);
+            if (rank == k - 1) limit = c;
         }
         __syncthreads();
-        L = limit[0];
-        __syncthreads();
+        L = limit;
+        places = (int)found;
     }
-    for (int q = tid; q < lists * k; q += kBeamThreads) {
-        const Cand c = candidate(q / k, q % k);
+    for (int q = tid; q < places * k; q += kBeamThreads) {
+        const int p = q / k, j = q % k;
+        if (lists > k && p + j >= k) continue;
+        const Cand c = candidate(lists > k ? alive[p] : p, j);
         if (c.at == 0x7FFFFFFF || better(L, c)) continue;
-        const uint32_t at = atomicAdd(&many, 1u);
-        if (at < kRoom) cands[at] = c;
+        cands[atomicAdd(&many, 1u)] = c;
     }
+    static_assert(kMaxBeams * kMaxBeams <= kRoom && 256 <= kRoom, "all that count, and the lists' first ones, have room");
     __syncthreads();
     const int n = (int)many;
-    if (n <= kRoom) {
-        for (int q = warp; q < n; q += kWarps) {
-            const Cand c = cands[q];
-            const int rank = warp_rank(n, lane, [&](int j) { return better(cands[j], c); });
-            if (lane == 0 && rank < k) write(rank, c);
-        }
-    } else {
-        // more than the list holds (a bound that a few poor lists pulled down): merged best by best
-        Cand prev{INFINITY, -1};
-        for (int rank = 0; rank < k; ++rank) {
-            Cand best = kNone;
-            for (int l = tid; l < lists; l += kBeamThreads)
-                for (int j = 0; j < k; ++j) {
-                    const Cand c = candidate(l, j);
-                    if (!better(c, best)) break;
-                    if (better(prev, c)) {
-                        best = c;
-                        break;
-                    }
-                }
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) {
-                const Cand o{__shfl_xor_sync(0xFFFFFFFFu, best.total, d), __shfl_xor_sync(0xFFFFFFFFu, best.at, d)};
-                if (better(o, best)) best = o;
-            }
-            __syncthreads();
-            if (lane == 0) limit[warp] = best;
-            __syncthreads();
-            for (int w = 0; w < kWarps; ++w)
-                if (better(limit[w], best)) best = limit[w];
-            if (tid == 0) write(rank, best);
-            prev = best;
-        }
+    for (int q = tid; q < n; q += kBeamThreads) {
+        const Cand c = cands[q];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) rank += better(cands[j], c);
+        if (rank < k) write(rank, c);
     }
     if (tid == 0) a.tickets[g] = 0u;
 }

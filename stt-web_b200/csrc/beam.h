@@ -11,10 +11,11 @@
 namespace stt {
 
 constexpr int kMaxBeams = 32;
-constexpr int kBeamThreads = 512;
+constexpr int kBeamThreads = 128;
+constexpr int kBeamCtas = 8;                                  // of an SM
 constexpr int kBeamPerThread = 16;                            // logits of a thread
 constexpr int kBeamChunk = kBeamThreads * kBeamPerThread;     // logits of a CTA's tile
-constexpr int kBeamMaxChunks = 16;                            // CTAs of a row
+constexpr int kBeamMaxChunks = 32;                            // CTAs of a row
 
 struct BeamArgs {
     const void* logits;   // [batch * beams][vocab], rows row_stride elements apart

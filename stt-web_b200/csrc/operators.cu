@@ -289,7 +289,7 @@ extern "C" int stt_beam_create(int device, int max_batch, int max_beams, int max
     if (max_batch <= 0 || max_beams <= 0 || max_beams > kMaxBeams || max_vocab <= 0)
         return set_error(STT_E_INVALID_ARG, "no selection of %d utterances, %d beams (1..%d), %d tokens", max_batch, max_beams,
                          kMaxBeams, max_vocab);
-    if ((int64_t)max_beams * max_vocab > INT_MAX - kBeamChunk || (int64_t)max_batch * max_beams * beam_max_chunks(max_vocab) > INT_MAX)
+    if ((int64_t)max_beams * max_vocab > INT_MAX - 2 * kBeamChunk || (int64_t)max_batch * max_beams * beam_max_chunks(max_vocab) > INT_MAX)
         return set_error(STT_E_INVALID_ARG, "%d utterances of %d beams over %d tokens are too many", max_batch, max_beams, max_vocab);
     DeviceScope ds(device);
     if (!ds.ok) {
@@ -309,7 +309,9 @@ extern "C" int stt_beam_create(int device, int max_batch, int max_beams, int max
     h->max_batch = max_batch;
     h->max_beams = max_beams;
     h->max_vocab = max_vocab;
-    const size_t parts = (size_t)max_batch * max_beams * beam_max_chunks(max_vocab);
+    // a call has a CTA for each row, or as many as are resident
+    const int64_t rows = (int64_t)max_batch * max_beams;
+    const size_t parts = (size_t)std::max(rows, std::min<int64_t>(rows * beam_max_chunks(max_vocab), kBeamCtas * h->num_sms));
     size_t off = 256;
     auto take = [&](size_t bytes) {
         const size_t o = off;
@@ -378,9 +380,9 @@ extern "C" int stt_beam_select_device(stt_beam* h, const stt_beam_step* s, void*
     a.batch = s->batch;
     a.beams = s->beams;
     a.vocab = s->vocab;
-    // about four CTAs per SM, twice what is resident (rows that ended leave gaps); a CTA takes whole tiles
+    // as many CTAs as are resident; a CTA takes whole tiles, and the last one joins 256 lists at most
     const int tiles = beam_tiles(s->vocab), rows = s->batch * s->beams;
-    const int want = std::min(beam_max_chunks(s->vocab), (4 * h->num_sms + rows - 1) / rows);
+    const int want = std::max(1, std::min({beam_max_chunks(s->vocab), kBeamCtas * h->num_sms / rows, 256 / s->beams}));
     a.tiles_per_chunk = (tiles + want - 1) / want;
     a.chunks = (tiles + a.tiles_per_chunk - 1) / a.tiles_per_chunk;
     a.scores = s->d_scores;
