@@ -46,25 +46,74 @@ __device__ __forceinline__ void check_repeated(const Kv8Dev& c, const Kv8Batch& 
     if (__any_sync(0xFFFFFFFFu, twice) && lane == 0) atomicCAS(c.err, 0, -1);
 }
 
+// N elements of a row as they lie in memory, in words.
+template <int DT, int N>
+struct Raw {
+    static constexpr bool kShort = DT != DT_F32;
+    static constexpr int kWords = kShort ? N / 2 : N;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const typename Elem<DT>::T* p) {
+        if constexpr (kWords == 4) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+            w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        } else if constexpr (kWords == 2) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+            w[0] = u.x, w[1] = u.y;
+        } else {
+            w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        }
+    }
+    __device__ __forceinline__ void values(float (&x)[N]) const {
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) {
+            if constexpr (kShort) {
+                const float2 f = unpack2(w[j], Elem<DT>());
+                x[2 * j] = f.x, x[2 * j + 1] = f.y;
+            } else {
+                x[j] = __uint_as_float(w[j]);
+            }
+        }
+    }
+    // Greatest magnitude so far, as bits; 16-bit types two at a time (they order like the values too).
+    __device__ __forceinline__ uint32_t take_max(uint32_t m) const {
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) {
+            if constexpr (kShort) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
+            else m = max(m, w[j] & 0x7FFFFFFFu);
+        }
+        return m;
+    }
+    // The f32 bits of such a maximum; 0x7F800000 and more are not finite.
+    static __device__ __forceinline__ uint32_t bits(uint32_t m) {
+        if constexpr (kShort) {
+            const float2 f = unpack2(max(m >> 16, m & 0xFFFFu), Elem<DT>());
+            return __float_as_uint(f.x);
+        } else {
+            return m;
+        }
+    }
+};
+
 // One warp per (block, K or V, head) of a batch row: every new token of the block is loaded once
 // (32 lanes x dim / 32 elements, all rows in flight together), the maximum goes through shuffles,
 // and a token's codes leave as one row of `dim` bytes.  A CTA's warps take neighbouring heads, so that
 // they read neighbouring pieces of a token.  MAX is the most new tokens of a block: 1 for calls of one
-// token, whose warps then need a third of the registers.
+// token, whose warps need a third of the registers and take K and V of a head together.
 //
 // The maximum is taken over the bit patterns of |x| (they order like the values; anything from
-// 0x7F800000 on is not finite and sends the warp through the checked conversion below), and a code is
+// 0x7F800000 on is not finite, and sends the warp through the checks below), and a code is
 // the low byte of x * 2^-e + 1.5 * 2^23, whose unit is 1: the addition rounds to nearest, ties to even.
 template <int D, int DT, int MAX>
-__global__ void __launch_bounds__(kThreads, MAX == 1 ? 6 : 2) append_kernel(Kv8Dev c, Kv8Batch b, const typename Elem<DT>::T* __restrict__ k,
+__global__ void __launch_bounds__(kThreads, MAX == 1 ? 6 : DT == DT_F32 ? 2 : 4) append_kernel(Kv8Dev c, Kv8Batch b, const typename Elem<DT>::T* __restrict__ k,
                                                           const typename Elem<DT>::T* __restrict__ v, Kv8Strides ks, Kv8Strides vs,
                                                           int nb, int ctas_per_block) {
     constexpr int N = D / 32;
+    constexpr int KV = MAX == 1 ? 2 : 1;  // of K and V, how many a warp takes
     const int lane = threadIdx.x & 31;
     const int rest = blockIdx.x / ctas_per_block;
     const int task = (blockIdx.x - rest * ctas_per_block) * (kThreads / 32) + (threadIdx.x >> 5);
-    if (task >= 2 * c.heads) return;
-    const int kv = task >= c.heads, h = task - kv * c.heads;
+    if (task >= 2 / KV * c.heads) return;
+    const int kv0 = task >= c.heads, h = task - kv0 * c.heads;
     const int i = rest / nb, blk = rest - i * nb;
     Kv8Row r;
     if (!kv8_row(c, b, i, &r)) return;
@@ -78,62 +127,69 @@ __global__ void __launch_bounds__(kThreads, MAX == 1 ? 6 : 2) append_kernel(Kv8D
     if (lo >= hi) return;
     const int slot = p0 % c.cap;
     const int64_t head = (int64_t)r.seq * c.heads + h;
-    int8_t* codes = (kv ? c.vc : c.kc) + (head * c.cap + slot) * D + lane * N;
-    int8_t* exps = (kv ? c.ve : c.ke) + head * (c.cap / kKv8Block) + slot / kKv8Block;
-    const Kv8Strides s = kv ? vs : ks;
-    const typename Elem<DT>::T* src = (kv ? v : k) + i * s.seq + (int64_t)(lo - r.pos) * s.token + h * s.head + lane * N;
+    const int64_t code_at = (head * c.cap + slot) * D + lane * N, exp_at = head * (c.cap / kKv8Block) + slot / kKv8Block;
     const int old = lo - p0, many = hi - lo;
-    float x[MAX][N];
+    Raw<DT, N> x[KV][MAX];
+    int was[KV];
     // (a block with fewer tokens loads its last one again: no branch keeps the loads apart)
 #pragma unroll
-    for (int t = 0; t < MAX; ++t) load_elems<DT, N>(src + min(t, many - 1) * s.token, x[t]);
-    const int was = old ? *exps : kKv8MinExp;
-    uint32_t amax = 0;
+    for (int u = 0; u < KV; ++u) {
+        const Kv8Strides& s = kv0 + u ? vs : ks;
+        const typename Elem<DT>::T* src = (kv0 + u ? v : k) + i * s.seq + (int64_t)(lo - r.pos) * s.token + h * s.head + lane * N;
 #pragma unroll
-    for (int t = 0; t < MAX; ++t)
+        for (int t = 0; t < MAX; ++t) x[u][t].load(src + min(t, many - 1) * s.token);
+        was[u] = (kv0 + u ? c.ve : c.ke)[exp_at];
+    }
 #pragma unroll
-        for (int j = 0; j < N; ++j) amax = max(amax, __float_as_uint(x[t][j]) & 0x7FFFFFFFu);
-    amax = __reduce_max_sync(0xFFFFFFFFu, amax);
-    int e;
-    float f;
-    if (amax >= 0x7F800000u) {
-        // infinities or NaN: the exponent of the finite values; infinities become +-127 steps, NaN 0
-        if (lane == 0) atomicCAS(c.err, 0, -5);  // STT_E_DEVICE_FLAG
-        amax = 0;
+    for (int u = 0; u < KV; ++u) {
+        int8_t* codes = (kv0 + u ? c.vc : c.kc) + code_at;
+        if (old == 0) was[u] = kKv8MinExp;
+        uint32_t amax = 0;
 #pragma unroll
-        for (int t = 0; t < MAX; ++t)
+        for (int t = 0; t < MAX; ++t) amax = x[u][t].take_max(amax);
+        amax = __reduce_max_sync(0xFFFFFFFFu, Raw<DT, N>::bits(amax));
+        const bool finite = amax < 0x7F800000u;
+        if (!finite) {
+            // infinities or NaN: the exponent of the finite values; infinities become +-127 steps, NaN 0
+            if (lane == 0) atomicCAS(c.err, 0, -5);  // STT_E_DEVICE_FLAG
+            amax = 0;
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const uint32_t u = __float_as_uint(x[t][j]) & 0x7FFFFFFFu;
-                if (u < 0x7F800000u) amax = max(amax, u);
+            for (int t = 0; t < MAX; ++t) {
+                float y[N];
+                x[u][t].values(y);
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const uint32_t w = __float_as_uint(y[j]) & 0x7FFFFFFFu;
+                    if (w < 0x7F800000u) amax = max(amax, w);
+                }
             }
-        amax = __reduce_max_sync(0xFFFFFFFFu, amax);
-        e = max(was, kv8_exponent(__uint_as_float(amax)));
-        const float inv = pow2i(-e);
+            amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+        }
+        const int e = max(was[u], kv8_exponent(__uint_as_float(amax)));
+        const float f = pow2i(-e);
+        if (old && e > was[u]) {
+            const float shift = pow2i(was[u] - e);
+#pragma unroll 4
+            for (int t = 0; t < old; ++t) {
+                const uint32_t q = load_codes<N>(codes + t * D);
+                float y[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) y[j] = (float)(int8_t)(q >> (8 * j));
+                store_codes<N>(codes + t * D, pack_codes<N>(y, shift));
+            }
+        }
 #pragma unroll
         for (int t = 0; t < MAX; ++t)
+            if (t < many) {
+                float y[N];
+                x[u][t].values(y);
+                if (!finite)
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[t][j] = x[t][j] != x[t][j] ? 0.0f : fminf(fmaxf(x[t][j] * inv, -127.0f), 127.0f);
-        f = 1.0f;
-    } else {
-        e = max(was, kv8_exponent(__uint_as_float(amax)));
-        f = pow2i(-e);
+                    for (int j = 0; j < N; ++j) y[j] = y[j] != y[j] ? 0.0f : fminf(fmaxf(y[j], -127.0f / f), 127.0f / f);
+                store_codes<N>(codes + (old + t) * D, pack_codes<N>(y, f));
+            }
+        if (lane == 0 && (e != was[u] || !old)) (kv0 + u ? c.ve : c.ke)[exp_at] = (int8_t)e;
     }
-    if (old && e > was) {
-        const float shift = pow2i(was - e);
-#pragma unroll 4
-        for (int t = 0; t < old; ++t) {
-            const uint32_t q = load_codes<N>(codes + t * D);
-            float y[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) y[j] = (float)(int8_t)(q >> (8 * j));
-            store_codes<N>(codes + t * D, pack_codes<N>(y, shift));
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < MAX; ++t)
-        if (t < many) store_codes<N>(codes + (old + t) * D, pack_codes<N>(x[t], f));
-    if (lane == 0 && (e != was || !old)) *exps = (int8_t)e;
 }
 
 constexpr int kReadTokens = 16;  // of a CTA
@@ -195,7 +251,7 @@ cudaError_t append_t(const Kv8Dev& c, const Kv8Batch& b, const void* k, const vo
     using T = typename Elem<DT>::T;
     const T *kt = static_cast<const T*>(k), *vt = static_cast<const T*>(v);
     const int nb = (b.tokens + 2 * kKv8Block - 2) / kKv8Block;  // blocks that `tokens` tokens can touch
-    const int per_block = (2 * c.heads + kThreads / 32 - 1) / (kThreads / 32);
+    const int per_block = ((b.tokens == 1 ? 1 : 2) * c.heads + kThreads / 32 - 1) / (kThreads / 32);
     const unsigned grid = (unsigned)((int64_t)b.n * nb * per_block);
     if (b.tokens == 1) append_kernel<D, DT, 1><<<grid, kThreads, 0, st>>>(c, b, kt, vt, ks, vs, nb, per_block);
     else append_kernel<D, DT, kKv8Block><<<grid, kThreads, 0, st>>>(c, b, kt, vt, ks, vs, nb, per_block);
