@@ -192,7 +192,9 @@ __global__ void __launch_bounds__(kThreads, MAX == 1 ? 6 : DT == DT_F32 ? 2 : 4)
     }
 }
 
-constexpr int kReadTokens = 16;  // of a CTA
+// Tokens of a CTA.  16 leave a last wave nearly empty where rows hold about 16 (8.5 tokens of 512 sequences,
+// f32: 20.7 us, 8 take 18.1 us for 106 MB); 4 do no better, and 2 take 22 us.
+constexpr int kReadTokens = 8;
 
 // Values of a range of tokens.  A thread keeps its place in a token (as many codes as fill 16 bytes of
 // values, in K and in V) and walks over the tokens, several in flight.  A code becomes a value in two
