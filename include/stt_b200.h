@@ -330,7 +330,7 @@ int stt_kv8_cache_get_info(const stt_kv8_cache* cache, stt_kv8_cache_info* out);
 /* Waits for the device, then reports and clears what the calls since the last check raised:
  * STT_E_INVALID_ARG for a row out of range (skipped) or a sequence twice in one append (its blocks are
  * undefined), STT_E_DEVICE_FLAG for an infinity (stored as the largest code) or a NaN (stored as 0)
- * that was appended. */
+ * that was appended, or for a wait inside an attention kernel that ran out (its outputs are missing). */
 int stt_kv8_cache_status(stt_kv8_cache* cache);
 
 /* Writes positions d_pos[i] .. d_pos[i] + d_count[i] - 1 of K and V (one dtype).  The new tokens of a
@@ -371,7 +371,8 @@ int stt_kv8_reorder_device(stt_kv8_cache* cache, const int32_t* d_parents, int g
 int stt_beam_create(int device, int max_batch, int max_beams, int max_vocab, stt_beam** out);
 int stt_beam_destroy(stt_beam* beam);
 /* Waits for the device, then reports (STT_E_DEVICE_FLAG) and clears a NaN or +inf among the logits or
- * scores of the calls since the last check; such a beam's candidates counted as -inf. */
+ * scores of the calls since the last check (such a beam's candidates counted as -inf), or a wait for a
+ * copy of logits that ran out. */
 int stt_beam_status(stt_beam* beam);
 /* The `beams` best continuations of each utterance, best first.  Row g * beams + b of the logits (dtype
  * 0 f32, 1 bf16, 2 f16, rows row_stride elements apart) and of the other device arrays is beam b of

@@ -14,6 +14,13 @@
 // with the list's and the tiles' bounds carried from tile to tile, and are ranked by counting.  A tile
 // costs a maximum, an exponential and a comparison per logit.  Where more reach the bound than the list
 // takes (ties, masked rows), the warps sort them 32 at a time by a bitonic network instead.
+//
+// What bounds it: instructions (about 15 a logit and lane with a tile's fixed work) and the latency of a
+// CTA's chain (copy, two passes over a tile, ranking, a ticket) rather than memory; so CTAs are small, 8 of
+// them share an SM, and tiles come by bulk copies, which hold no registers.  CTAs of 512 threads, two to an
+// SM, with tiles of 8192 through registers took 21.8 us where this takes 18.7 us (128 x 8 rows of 8000 f32
+// logits, 32.8 MB), and 34 us where this takes 31 us (16 x 16 rows of 65,537 bf16 logits, some ended).  One
+// utterance of 4 beams and 8000 tokens takes 7 us, half of it the last CTA's join.
 #include <algorithm>
 
 #include "beam.h"
@@ -527,6 +534,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) select_kernel(BeamArg
 // that another beam takes, then stores it to the beams that change.  All of a position is read
 // before any of it is written, and no other thread touches it, so the rows are permuted in place,
 // with each source read once (a beam that two others take is read twice, the second time from L1).
+// HBM bounds it: 32 x 8 rows of 64 pieces of up to 751 x 256 bytes take 565 us for 3.4 GB, 5.9 TB/s.
 template <int B, class V, int U>
 __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a, int64_t per_segment) {
     __shared__ int parent[B];

@@ -178,7 +178,8 @@ extern "C" int stt_kv8_cache_status(stt_kv8_cache* h) {
     if (code == STT_E_INVALID_ARG)
         return set_error(code, "a call on this cache had a sequence, position or count out of range, or a sequence "
                                "twice in one append: that row was skipped, or its blocks are undefined");
-    return set_error(STT_E_DEVICE_FLAG, "an infinity or NaN was appended to this cache and stored as a finite value");
+    return set_error(STT_E_DEVICE_FLAG, "an infinity or NaN was appended to this cache and stored as a finite value, or a wait in "
+                                        "an attention kernel ran out");
 }
 
 extern "C" int stt_kv8_append_device(stt_kv8_cache* h, const stt_kv8_batch* b, const stt_kv8_tensor* k,
@@ -355,7 +356,8 @@ extern "C" int stt_beam_status(stt_beam* h) {
     CUDA_TRY(cudaMemcpy(&code, h->err, sizeof code, cudaMemcpyDeviceToHost));
     if (code == 0) return STT_OK;
     CUDA_TRY(cudaMemset(h->err, 0, sizeof code));
-    return set_error(STT_E_DEVICE_FLAG, "a beam had a NaN or +inf logit or score: its candidates were taken as -inf");
+    return set_error(STT_E_DEVICE_FLAG, "a beam had a NaN or +inf logit or score (its candidates were taken as -inf), or a wait for "
+                                        "logits ran out");
 }
 
 extern "C" int stt_beam_select_device(stt_beam* h, const stt_beam_step* s, void* cuda_stream) {
