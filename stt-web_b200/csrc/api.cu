@@ -1469,7 +1469,7 @@ int queue_reorder(stt_streams* s, int groups, int beams, const BeamBufs& d, bool
 
 // The host keeps the offsets itself: they move with the streams.
 void move_offsets(stt_streams* s, const int32_t* ids, int groups, int beams, const int32_t* parents) {
-    std::vector<int32_t> off(beams);
+    int32_t off[kMaxBeams];
     for (int g = 0; g < groups; ++g) {
         for (int b = 0; b < beams; ++b) off[b] = s->h_state[ids[g * beams + parents[g * beams + b]]].offset;
         for (int b = 0; b < beams; ++b) s->h_state[ids[g * beams + b]].offset = off[b];

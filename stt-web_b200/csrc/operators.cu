@@ -207,7 +207,7 @@ extern "C" int stt_kv8_read_device(const stt_kv8_cache* h, const stt_kv8_batch* 
     TRY(check_batch(h, b, &some));
     if (!some) return STT_OK;
     TRY(check_kv(k, v));
-    if ((int64_t)b->n * (b->n_tokens / 16 + 1) > INT_MAX / (h->c.heads / 8 + 1))
+    if ((int64_t)b->n * (b->n_tokens / 8 + 1) > INT_MAX / (h->c.heads / 8 + 1))
         return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", b->n, b->n_tokens);
     DeviceScope ds(h->device);
     if (!ds.ok) return set_error(STT_E_CUDA, "cudaSetDevice(%d) failed", h->device);

@@ -8,9 +8,10 @@ two f16 parts (2^-22) a weight is off by 19 * 2^-23 * S + 4 * 2^-23, numerator a
 by twice that, plus the accumulation of the keys (at most 2^-23 per 16 keys of a warp's share, 64 such
 steps at the lengths used here) and of the merges (under 64 * 2^-24): in all
 (2 * (19 * S + 4) + 128) * 2^-23 of the largest |v|.  The output's rounding adds eps / 2 of its value.
-Where queries and output have 16 bits and a K/V head has 64 query rows or more, the weights of the
+Where queries and output have 16 bits and a K/V head has more than 8 query rows, the weights of the
 numerator may be f16: 2^-12 of each (and 2^-31 of the largest below f16's normal range, at most 2^12
-keys), so at most 2^-12 + 2^-19 of the largest |v|."""
+keys), so at most 2^-12 + 2^-19 of the largest |v|.  (The longest of these cases take up to 160 steps of 16
+keys, 2^-16 more; a weight's rounding is 2^-13 on average, so that the bound of 2^-12 has room for it.)"""
 import numpy as np
 import pytest
 
@@ -374,6 +375,100 @@ def test_operators_in_a_captured_graph_follow_the_positions():
 
 
 # ------------------------------------------------------------------------------------ beam search
+
+
+def test_chunks_that_share_keys_in_a_captured_graph():
+    """The tensor-core kernel in clusters, replayed for positions whose runs of keys are of other lengths (some empty)."""
+    import torch
+    p = Pair(1, 4, 128, 4096)
+    q, out = rand((1, 300, 4, 128), "bf16", 30), rand((1, 300, 4, 128), "bf16", 31)
+    pos = i32([0])
+    p.cache.attention(q, out, pos)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        p.cache.attention(q, out, pos, stream=torch.cuda.current_stream().cuda_stream)
+    for at in (0, 130, 3700, 1):
+        pos.fill_(at)
+        g.replay()
+        torch.cuda.synchronize()
+        check_attention(p, q, out, out, [at], [300], [0], 1 / 128 ** 0.5)
+    p.cache.status()
+
+
+@pytest.mark.parametrize("tokens,dtype", [(1, "f32"), (9, "bf16"), (300, "bf16"), (300, "f32")])
+def test_starts_at_both_ends_of_the_integers(tokens, dtype):
+    import torch
+    p = Pair(3, 2, 64, 4096)
+    q, out = rand((3, tokens, 2, 64), dtype, 35), rand((3, tokens, 2, 64), dtype, 36)
+    pos, start = [3000, 100, 2500], [2 ** 31 - 1, -2 ** 31, 2600]
+    before = out.clone()
+    p.cache.attention(q, out, i32(pos), start=i32(start), window=2 ** 31 - 1)
+    p.cache.status()
+    assert not out[0].any()
+    check_attention(p, q, out, before, pos, [tokens] * 3, [0, 1, 2], 0.125, 2 ** 31 - 1, start)
+
+
+def test_two_caches_and_selectors_at_once_on_streams_of_their_own():
+    import torch
+    caches = [Pair(2, 2, 128, 20000, seed=s) for s in (1, 2)]
+    beams = [BeamSelector(4, 8, 9000) for _ in range(2)]
+    q = rand((2, 1, 8, 128), "f32", 32)
+    chunk = rand((2, 40, 8, 128), "f16", 33)
+    logits = rand((32, 9000), "f32", 34, 3.0)
+    pos, chunk_pos = i32([19000, 12345]), i32([19000, 300])
+    scores = torch.zeros(4, 8, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+
+    def outputs():
+        return (torch.empty_like(q), torch.empty_like(chunk), torch.empty_like(scores),
+                torch.empty(4, 8, dtype=torch.int32, device="cuda"), torch.empty(4, 8, dtype=torch.int32, device="cuda"))
+
+    def call(k, o, stream):
+        caches[k].cache.attention(q, o[0], pos, stream=stream)
+        caches[k].cache.attention(chunk, o[1], chunk_pos, stream=stream)
+        beams[k].select(logits, scores, o[2], o[3], o[4], stream=stream)
+
+    alone = [outputs() for _ in range(2)]
+    for k in range(2):
+        call(k, alone[k], 0)
+        torch.cuda.synchronize()
+    together = [[outputs() for _ in range(8)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(8):
+        for k in range(2):
+            call(k, together[k][i], streams[k].cuda_stream)
+    torch.cuda.synchronize()
+    for k in range(2):
+        for o in together[k]:
+            assert all(torch.equal(x, y) for x, y in zip(o, alone[k]))
+
+
+def test_allocation_failures_of_the_handles_release_everything():
+    import torch
+    from stt_b200._lib import STT_E_OOM, lib
+    torch.cuda.synchronize()
+    free0 = torch.cuda.mem_get_info()[0]
+    for make, least in ((lambda: Kv8Cache(64, 8, 128, 16384), 2), (lambda: BeamSelector(64, 32, 65537), 1)):
+        failures = 0
+        for k in range(10):
+            assert lib().stt_debug_fail_allocation(k) == 0
+            h = None
+            try:
+                h = make()
+            except SttError as e:
+                assert e.code == STT_E_OOM, e
+                failures += 1
+            finally:
+                lib().stt_debug_fail_allocation(-1)
+            done = h is not None
+            if done:
+                h.close()
+            torch.cuda.synchronize()
+            assert abs(torch.cuda.mem_get_info()[0] - free0) < (64 << 20), k
+            if done:
+                break
+        assert failures == least and done
 
 
 def run_select(logits, scores, done=None, eos=-1, selector=None):
