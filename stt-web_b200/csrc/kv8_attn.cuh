@@ -7,11 +7,6 @@ namespace stt {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float exp2_approx(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 // Cluster barrier; loads from and stores to the same place of CTA `rank`'s shared memory.
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");

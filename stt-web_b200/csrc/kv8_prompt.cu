@@ -27,9 +27,11 @@
 // Where there are fewer row blocks than SMs, a cluster of CTAs takes the steps of a row block in equal
 // runs; at the end each sends O, M and l of every row to the shared memory of the CTA that joins that row
 // in its share.
-// Measured: the last 1024 of 4096 positions, 4 sequences x 16 heads of 128, 151 us, 0.79 PFLOP/s; a step of
-// two tiles takes 2.3 us (its products 1.1 us, its exponentials as long on the other units), a CTA 6 to 11 us
-// besides (its rows in and out, the first step's latency).
+// Measured: the last 1024 of 4096 positions, 4 sequences x 16 heads of 128, 145 us, 0.83 PFLOP/s; a step of
+// two tiles takes 2.1 us (its products 1.1 us, its exponentials as long on the other units; a tile's softmax
+// waits 0.7 us a step for its products), a CTA 6 to 11 us besides (its rows in and out, the first step's
+// latency).  Halves of 64 keys with scores and weights in alternating buffers hide that wait, but products of
+// 64 columns are less than half as fast: 165 us.
 // Every wait is bounded: one that gives up sets the CTA's abort word, all roles leave, the copies and
 // products in flight are waited for, and the cache's error word records it.
 #include <cfloat>
@@ -61,7 +63,7 @@ template <int D>
 struct PromptSmem {
     uint8_t q[2][kTile * D * 2];          // f16, core matrices of 8 rows x 16 bytes, D / 8 of them per 8 rows
     uint8_t k[2][kTile * D * 2], v[2][kTile * D * 2];
-    __align__(16) float k_step[kExpSlots][kStepBlocks], v_exp[kExpSlots][kStepBlocks];
+    __align__(16) float k_step[kExpSlots][kStepBlocks], v_exp[kExpSlots][kStepBlocks], to_sum[kExpSlots][kStepBlocks];
     uint64_t q_full[2], s_full[2], p_half[2], p_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], e_full[kExpSlots];
     uint64_t q_raw[kSoftmaxWarps];
     uint64_t done;
@@ -152,6 +154,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
     const int64_t head = (int64_t)row.seq * c.heads + h;
     const int cap_blocks = c.cap / kKv8Block;
     volatile int* abort = &sm.abort;
+    // the softmax's sum is held over 2^E; any E near the exponents of V serves
+    auto base_exp = [&] {
+        return nb_all > 0 ? fminf(fmaxf((float)c.ve[head * cap_blocks + kb_all % cap_blocks], -60.0f), 60.0f) : 0.0f;
+    };
 
     if (threadIdx.x == 0) {
         for (int j = 0; j < 2; ++j) {
@@ -218,6 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
             }
         };
         if (warp == kSoftmaxWarps) fetch_exps(0);
+        const int E = (int)base_exp();
         for (int j = 0; j < steps; ++j) {
             const int st = j & 1;
             if (warp == kSoftmaxWarps) {
@@ -226,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                 if (lane < kStepBlocks) {
                     sm.k_step[j % kExpSlots][lane] = pow2i(ek);
                     sm.v_exp[j % kExpSlots][lane] = (float)ev;
+                    sm.to_sum[j % kExpSlots][lane] = pow2i(E - ev);
                 }
                 fetch_exps(j + 1);
             }
@@ -377,8 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         // the tile's rows see all of [all_lo, all_hi]
         const int tt0 = (r0 + q * kTile) / a.group, tt1 = (r0 + min(rows, (q + 1) * kTile) - 1) / a.group;
         const int all_lo = sight.lo(row.pos + tt1), all_hi = row.pos + tt0;
-        // the softmax's sum is held over 2^E; any E near the exponents of V serves
-        const float E = nb_all > 0 ? fminf(fmaxf((float)c.ve[head * cap_blocks + kb_all % cap_blocks], -60.0f), 60.0f) : 0.0f;
+        const float E = base_exp();
         float M = -FLT_MAX, l = 0.0f;
         bool ok = true;
         for (int j = 0; j < steps; ++j) {
@@ -441,16 +448,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                     const float step = k_step[u + v];
                     const float ev = v_exp[u + v];
                     const float add = ev + (kWeightShift - M);
-                    float s0 = 0.0f, s1 = 0.0f;
+                    float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float w0 = exp2_approx(fmaf(x[16 * (u + v) + e], step, add));
-                        const float w1 = exp2_approx(fmaf(x[16 * (u + v) + e + 1], step, add));
-                        s0 += w0;
-                        s1 += w1;
-                        w[8 * v + e / 2] = pack_f16(w0, w1);
+                        const float2 y = fma2(make_float2(x[16 * (u + v) + e], x[16 * (u + v) + e + 1]), make_float2(step, step),
+                                              make_float2(add, add));
+                        const float2 z = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                        s = add2(s, z);
+                        w[8 * v + e / 2] = pack_f16(z.x, z.y);
                     }
-                    part[v] = fmaf(s0 + s1, pow2i((int)(E - ev)), part[v]);
+                    part[v] = fmaf(s.x + s.y, sm.to_sum[j % kExpSlots][u + v], part[v]);
                 }
                 tmem_st(s_col + 8 * u, w);  // over scores, all of which this thread has read
                 if (u == kStepBlocks / 2 - 2) {
@@ -522,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
             // each CTA joins its share of the rows; a thread 8 dimensions of one at a time
             const int share = (rows + cluster - 1) / cluster;
             const int mine = min(rows - rank * share, share);
-            const float E = nb_all > 0 ? fminf(fmaxf((float)c.ve[head * cap_blocks + kb_all % cap_blocks], -60.0f), 60.0f) : 0.0f;
+            const float E = base_exp();
             for (int p = threadIdx.x; p < mine * (D / 8); p += kSoftmaxWarps * 32) {
                 const int at = p / (D / 8), d8 = p % (D / 8);
                 float M = -FLT_MAX, l = 0.0f, o[8] = {};
@@ -611,16 +618,16 @@ cudaError_t kv8_configure_prompt(Kv8Machine* m) {
 
 PromptPlan kv8_prompt_plan(int64_t rows, int64_t items, int64_t blocks, const Kv8Machine& m) {
     // fitted to 16 .. 1024 tokens over 256 .. 30,000 positions: a CTA takes 6 us besides its steps, a step
-    // 2.3 us with two tiles and 2.0 us with one, a cluster 2 us more.  The other kernel's time comes from a
+    // 2.1 us with two tiles and 1.9 us with one, a cluster 2 us more.  The other kernel's time comes from a
     // model of the same calls: 64 tokens over 256 positions of 4 heads take 7.2 us there and 11 us here, 256
-    // over 4096 of 16 heads 117 us there and 36 us here
+    // over 4096 of 16 heads 117 us there and 34 us here
     const int64_t ctas = items * ((rows + 2 * kTile - 1) / (2 * kTile)), steps = (blocks + kStepBlocks - 1) / kStepBlocks;
     PromptPlan best{1, 1e30};
     for (int j = 0; j < 4 && (1 << j) <= steps; ++j) {
         const int cluster = 1 << j;
         if (m.prompt_ctas[j] < cluster) break;
         const double waves = (double)((ctas * cluster + m.prompt_ctas[j] - 1) / m.prompt_ctas[j]);
-        const double us = waves * (6.0 + (rows > kTile ? 2.3 : 2.0) * (double)((steps + cluster - 1) / cluster)) +
+        const double us = waves * (6.0 + (rows > kTile ? 2.1 : 1.9) * (double)((steps + cluster - 1) / cluster)) +
                           (cluster > 1 ? 2.0 : 0.0);
         if (us < best.us) best = PromptPlan{cluster, us};
     }
