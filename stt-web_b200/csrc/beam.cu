@@ -6,8 +6,8 @@
 // reference value, its sum of exponentials over it, and its `beams` best logits (no more of one row can
 // be among the best of all); the last CTA of an utterance joins the rows' sums and picks among the
 // chunks' bests.  The order of two beams' candidates can hang on the last digits, so sums are joined and
-// candidates compared in 64 bits; the exponentials themselves are f32, 16 of a thread added at a time
-// (their rounding errors, 2^-24 each, average out: 1e-8 of the sum at 8000 logits).
+// candidates compared in 64 bits; the exponentials themselves are f32, 16 or 32 of a thread added at a
+// time (their rounding errors, 2^-24 each, average out: 1e-8 of the sum at 8000 logits).
 //
 // The best of a chunk: the k-th largest of the maxima of its 32 groups of 4 lanes bounds the k-th best
 // logit from below, and little more than the k best reach it; those few go to a list in shared memory,
@@ -127,6 +127,7 @@ struct Sorted {
 template <int DT>
 __device__ __noinline__ Sorted sort_list(Lists& s, int from, const typename Elem<DT>::T* row, int v0, int vocab,
                                          float bound, int k) {
+    constexpr int kPerThread = beam_per_thread(DT);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     Best best;
     for (int j = 0; j < from; j += kBeamThreads) best.merge(j + tid < from ? s.list[j + tid] : 0, lane);
@@ -134,9 +135,9 @@ __device__ __noinline__ Sorted sort_list(Lists& s, int from, const typename Elem
         uint64_t* pending = s.pending[warp];
         uint64_t kth = 0;  // the warp's k-th best
         int pend = 0;
-        for (int i = 0; i < kBeamPerThread || pend > 0; ++i) {
-            if (i < kBeamPerThread) {
-                const int v = v0 + (warp * kBeamPerThread + i) * 32 + lane;
+        for (int i = 0; i < kPerThread || pend > 0; ++i) {
+            if (i < kPerThread) {
+                const int v = v0 + (warp * kPerThread + i) * 32 + lane;
                 uint64_t key = 0;
                 if (v >= 0 && v < vocab) {
                     const float x = to_f32<DT>(row[v]);
@@ -174,15 +175,16 @@ __device__ __noinline__ Sorted sort_list(Lists& s, int from, const typename Elem
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kBeamThreads, kBeamCtas) select_kernel(BeamArgs a) {
+__global__ void __launch_bounds__(kBeamThreads, beam_ctas(DT)) select_kernel(BeamArgs a) {
     using T = typename Elem<DT>::T;
     constexpr int VEC = 16 / (int)sizeof(T);            // elements of a 16-byte load
-    constexpr int LOADS = kBeamPerThread / VEC;
+    constexpr int kPerThread = beam_per_thread(DT), kTile = beam_tile(DT);
+    constexpr int LOADS = kPerThread / VEC;
     constexpr int kRoom = 1024;                         // candidates of an utterance that are ranked at once
-    constexpr int kSlots = kRoom * sizeof(Cand) / (kBeamChunk * sizeof(T));
+    constexpr int kSlots = kRoom * sizeof(Cand) / (kTile * sizeof(T));
     static_assert(kSlots >= 2, "a tile is fetched while another is worked on");
     __shared__ __align__(128) union {
-        T tiles[kSlots][kBeamChunk];                    // as they come from memory
+        T tiles[kSlots][kTile];                    // as they come from memory
         Cand cands[kRoom];
     } sm;
     __shared__ Lists lists_of;
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) select_kernel(BeamArg
     __syncthreads();
     if (!(a.done && a.done[r])) {
         // Tiles are cut at 16-byte boundaries of memory, whatever the row's own alignment: vector j of
-        // thread t of a tile covers elements -lead + tile * kBeamChunk + (j * kBeamThreads + t) * VEC on.
+        // thread t of a tile covers elements -lead + tile * kTile + (j * kBeamThreads + t) * VEC on.
         const T* row = static_cast<const T*>(a.logits) + r * a.row_stride;
         const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
         float ref = -INFINITY;    // the sum's reference: within 60 of the largest so far
@@ -213,20 +215,20 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) select_kernel(BeamArg
         int listed = 0;           // keys of the list
         uint64_t* const list = lists_of.list;
         const int tile0 = chunk * a.tiles_per_chunk;
-        const int tile1 = min(tile0 + a.tiles_per_chunk, (a.vocab + lead + kBeamChunk - 1) / kBeamChunk);
+        const int tile1 = min(tile0 + a.tiles_per_chunk, (a.vocab + lead + kTile - 1) / kTile);
         // Vectors that lie inside the row come by a bulk copy of the tile; the row's ragged ends are put in
         // element by element.
-        auto first = [&](int tile) { return tile * kBeamChunk + tid * VEC - lead; };
+        auto first = [&](int tile) { return tile * kTile + tid * VEC - lead; };
         auto whole = [&](int v0) { return v0 >= 0 && v0 + VEC <= a.vocab; };
         auto issue = [&](int tile) {  // by one thread
-            const int v0 = tile * kBeamChunk - lead, from = v0 < 0 ? VEC : 0;
-            const int to = min(kBeamChunk, (a.vocab - v0) / VEC * VEC);
+            const int v0 = tile * kTile - lead, from = v0 < 0 ? VEC : 0;
+            const int to = min(kTile, (a.vocab - v0) / VEC * VEC);
             const uint32_t bytes = to > from ? (uint32_t)(to - from) * sizeof(T) : 0;
             mbar_expect_tx(&full[(tile - tile0) % kSlots], bytes);
             if (bytes) bulk_g2s(&sm.tiles[(tile - tile0) % kSlots][from], row + v0 + from, bytes, &full[(tile - tile0) % kSlots]);
         };
-        auto unpack = [&](int tile, float (&x)[kBeamPerThread]) {
-            const bool inner = tile * kBeamChunk >= lead && (tile + 1) * kBeamChunk - lead <= a.vocab;
+        auto unpack = [&](int tile, float (&x)[kPerThread]) {
+            const bool inner = tile * kTile >= lead && (tile + 1) * kTile - lead <= a.vocab;
             const uint4* raw = reinterpret_cast<const uint4*>(sm.tiles[(tile - tile0) % kSlots]);
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) {
@@ -262,21 +264,21 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) select_kernel(BeamArg
                 listed = now;
             } else {
                 const Sorted s = sort_list<DT>(lists_of, now <= kList ? now : listed, now <= kList ? nullptr : row,
-                                               tile * kBeamChunk - lead, a.vocab, bound, k);
+                                               tile * kTile - lead, a.vocab, bound, k);
                 listed = s.listed;
                 bound = s.bound;
             }
         };
         float group = -INFINITY;  // the greatest of the lane's group so far
         for (int tile = tile0; tile < tile1; ++tile) {
-            float x[kBeamPerThread];
+            float x[kPerThread];
             const int base = first(tile);
             auto index = [&](int e) { return base + e / VEC * (kBeamThreads * VEC) + e % VEC; };
             mbar_wait(&full[(tile - tile0) % kSlots], (tile - tile0) / kSlots & 1, &late);
             unpack(tile, x);
             float m0 = max_nan(x[0], x[1]), m1 = max_nan(x[2], x[3]);  // (two chains)
 #pragma unroll
-            for (int e = 4; e < kBeamPerThread; e += 4) m0 = max3_nan(m0, x[e], x[e + 1]), m1 = max3_nan(m1, x[e + 2], x[e + 3]);
+            for (int e = 4; e < kPerThread; e += 4) m0 = max3_nan(m0, x[e], x[e + 1]), m1 = max3_nan(m1, x[e + 2], x[e + 3]);
             const float lane_max = max_nan(m0, m1);
             float mx = lane_max;
 #pragma unroll
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) select_kernel(BeamArg
                 const float2 less = make_float2(-ref, -ref), log2e = make_float2(kLog2e, kLog2e);
                 float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int e = 0; e < kBeamPerThread; e += 2) {
+                for (int e = 0; e < kPerThread; e += 2) {
                     const float2 y = mul2(add2(make_float2(x[e], x[e + 1]), less), log2e);
                     s = add2(s, make_float2(exp2_approx(y.x), exp2_approx(y.y)));
                 }
@@ -335,10 +337,10 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) select_kernel(BeamArg
             if (lane_max >= bound) {
                 uint32_t reach = 0;
 #pragma unroll
-                for (int e = 0; e < kBeamPerThread; ++e) reach |= (uint32_t)(x[e] >= bound) << e;
+                for (int e = 0; e < kPerThread; ++e) reach |= (uint32_t)(x[e] >= bound) << e;
                 if (bound == -INFINITY) {  // the places outside the row count as -inf: not candidates
 #pragma unroll
-                    for (int e = 0; e < kBeamPerThread; ++e)
+                    for (int e = 0; e < kPerThread; ++e)
                         if (index(e) < 0 || index(e) >= a.vocab) reach &= ~(1u << e);
                 }
                 const uint32_t mine = __popc(reach);
@@ -346,12 +348,10 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) select_kernel(BeamArg
                 if (mine == 1) {  // as a rule
                     if (at < kList) list[at] = make_key(lane_max, (uint32_t)index(__ffs(reach) - 1));
                 } else {
-#pragma unroll
-                    for (int e = 0; e < kBeamPerThread; ++e)
-                        if (reach >> e & 1u) {
-                            if (at < kList) list[at] = make_key(x[e], (uint32_t)index(e));
-                            ++at;
-                        }
+                    for (; reach; reach &= reach - 1, ++at) {
+                        const int v = index(__ffs(reach) - 1);
+                        if (at < kList) list[at] = make_key(to_f32<DT>(row[v]), (uint32_t)v);
+                    }
                 }
             }
             uint32_t* const t = counter2;

@@ -12,9 +12,11 @@ namespace stt {
 
 constexpr int kMaxBeams = 32;
 constexpr int kBeamThreads = 128;
-constexpr int kBeamCtas = 8;                                  // of an SM
-constexpr int kBeamPerThread = 16;                            // logits of a thread
-constexpr int kBeamChunk = kBeamThreads * kBeamPerThread;     // logits of a CTA's tile
+// Logits of a thread in a tile of 8 or 16 KB, which needs twice the registers for 16-bit logits; CTAs of an
+// SM; logits of a tile.
+constexpr int beam_per_thread(int dtype) { return dtype == DT_F32 ? 16 : 32; }
+constexpr int beam_ctas(int dtype) { return dtype == DT_F32 ? 8 : 7; }
+constexpr int beam_tile(int dtype) { return kBeamThreads * beam_per_thread(dtype); }
 constexpr int kBeamMaxChunks = 32;                            // CTAs of a row
 
 struct BeamArgs {

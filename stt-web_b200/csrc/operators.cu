@@ -35,8 +35,8 @@ namespace {
 int elem_bytes(int dtype) { return dtype == DT_F32 ? 4 : 2; }
 
 // Tiles of a row, which may start 7 elements into its first vector, and the most CTAs that share them.
-int beam_tiles(int vocab) { return (vocab + 7 + kBeamChunk - 1) / kBeamChunk; }
-int beam_max_chunks(int vocab) { return std::min(kBeamMaxChunks, beam_tiles(vocab)); }
+int beam_tiles(int vocab, int dtype) { return (vocab + 7 + beam_tile(dtype) - 1) / beam_tile(dtype); }
+int beam_max_chunks(int vocab, int dtype) { return std::min(kBeamMaxChunks, beam_tiles(vocab, dtype)); }
 
 // n_seqs * heads * capacity * dim and the sizes derived from it; false if the arguments do not make a cache.
 bool kv8_sizes(int n_seqs, int heads, int dim, int cap, size_t* codes, size_t* exps) {
@@ -290,7 +290,8 @@ extern "C" int stt_beam_create(int device, int max_batch, int max_beams, int max
     if (max_batch <= 0 || max_beams <= 0 || max_beams > kMaxBeams || max_vocab <= 0)
         return set_error(STT_E_INVALID_ARG, "no selection of %d utterances, %d beams (1..%d), %d tokens", max_batch, max_beams,
                          kMaxBeams, max_vocab);
-    if ((int64_t)max_beams * max_vocab > INT_MAX - 2 * kBeamChunk || (int64_t)max_batch * max_beams * beam_max_chunks(max_vocab) > INT_MAX)
+    if ((int64_t)max_beams * max_vocab > INT_MAX - 4 * beam_tile(DT_BF16) ||
+        (int64_t)max_batch * max_beams * beam_max_chunks(max_vocab, DT_F32) > INT_MAX)
         return set_error(STT_E_INVALID_ARG, "%d utterances of %d beams over %d tokens are too many", max_batch, max_beams, max_vocab);
     DeviceScope ds(device);
     if (!ds.ok) {
@@ -312,7 +313,7 @@ extern "C" int stt_beam_create(int device, int max_batch, int max_beams, int max
     h->max_vocab = max_vocab;
     // a call has a CTA for each row, or as many as are resident
     const int64_t rows = (int64_t)max_batch * max_beams;
-    const size_t parts = (size_t)std::max(rows, std::min<int64_t>(rows * beam_max_chunks(max_vocab), kBeamCtas * h->num_sms));
+    const size_t parts = (size_t)std::max(rows, std::min<int64_t>(rows * beam_max_chunks(max_vocab, DT_F32), beam_ctas(DT_F32) * h->num_sms));
     size_t off = 256;
     auto take = [&](size_t bytes) {
         const size_t o = off;
@@ -383,8 +384,8 @@ extern "C" int stt_beam_select_device(stt_beam* h, const stt_beam_step* s, void*
     a.beams = s->beams;
     a.vocab = s->vocab;
     // as many CTAs as are resident; a CTA takes whole tiles, and the last one joins 256 lists at most
-    const int tiles = beam_tiles(s->vocab), rows = s->batch * s->beams;
-    const int want = std::max(1, std::min({beam_max_chunks(s->vocab), kBeamCtas * h->num_sms / rows, 256 / s->beams}));
+    const int tiles = beam_tiles(s->vocab, s->dtype), rows = s->batch * s->beams;
+    const int want = std::max(1, std::min({beam_max_chunks(s->vocab, s->dtype), beam_ctas(s->dtype) * h->num_sms / rows, 256 / s->beams}));
     a.tiles_per_chunk = (tiles + want - 1) / want;
     a.chunks = (tiles + a.tiles_per_chunk - 1) / a.tiles_per_chunk;
     a.scores = s->d_scores;
