@@ -15,12 +15,12 @@
 // costs a maximum, an exponential and a comparison per logit.  Where more reach the bound than the list
 // takes (ties, masked rows), the warps sort them 32 at a time by a bitonic network instead.
 //
-// What bounds it: instructions (about 15 a logit and lane with a tile's fixed work) and the latency of a
-// CTA's chain (copy, two passes over a tile, ranking, a ticket) rather than memory; so CTAs are small, 8 of
-// them share an SM, and tiles come by bulk copies, which hold no registers.  CTAs of 512 threads, two to an
-// SM, with tiles of 8192 through registers took 21.8 us where this takes 18.7 us (128 x 8 rows of 8000 f32
-// logits, 32.8 MB), and 34 us where this takes 31 us (16 x 16 rows of 65,537 bf16 logits, some ended).  One
-// utterance of 4 beams and 8000 tokens takes 7 us, half of it the last CTA's join.
+// What bounds it: instructions (about 15 a logit and lane with a tile's fixed work, 11 where a thread takes 32
+// logits of a tile) and the latency of a CTA's chain (copy, two passes over a tile, ranking, a ticket) rather
+// than memory; so CTAs are small, 7 or 8 of them share an SM, and tiles come by bulk copies, which hold no
+// registers.  128 x 8 rows of 8000 f32 logits (32.8 MB) take 14.9 us, 16 x 16 rows of 65,537 bf16 logits 24 us
+// (28 us with 16 logits to a thread, 34 us with CTAs of 512 threads, two to an SM, and tiles through
+// registers).  One utterance of 4 beams and 8000 tokens takes 7.2 us, half of it the last CTA's join.
 #include <algorithm>
 
 #include "beam.h"
@@ -62,13 +62,34 @@ __device__ __forceinline__ Key warp_sort(Key k, int lane, Greater greater, Shuff
     return k;
 }
 
-// A candidate of the whole utterance.
+// A candidate of the whole utterance: its total as 64 bits that order like the f64, and beam * vocab + token.
 struct Cand {
-    double total;
-    int32_t at;  // beam * vocab + token; 0x7FFFFFFF: none
+    int64_t order;
+    int32_t at;  // 0x7FFFFFFF: none
 };
 __device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
-    return (a.total > b.total) | ((a.total == b.total) & (a.at < b.at));  // (no branches)
+    return (a.order > b.order) | ((a.order == b.order) & (a.at < b.at));  // (no branches)
+}
+// (no NaN; -0 counts as +0.  The map is its own inverse.)
+__device__ __forceinline__ int64_t order_of(double x) {
+    const int64_t u = __double_as_longlong(x + 0.0);
+    return u ^ (u >> 63 & 0x7FFFFFFFFFFFFFFFll);
+}
+__device__ __forceinline__ double total_of(int64_t order) {
+    return __longlong_as_double(order ^ (order >> 63 & 0x7FFFFFFFFFFFFFFFll));
+}
+// How many of the n candidates are better than c.
+__device__ __forceinline__ int rank_of(const Cand& c, const Cand* cands, int n) {
+    int rank = 0, j = 0;
+    for (; j + 8 <= n; j += 8) {
+        Cand o[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) o[u] = cands[j + u];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) rank += better(o[u], c);
+    }
+    for (; j < n; ++j) rank += better(cands[j], c);
+    return rank;
 }
 
 template <int DT>
@@ -432,7 +453,8 @@ __global__ void __launch_bounds__(kBeamThreads, beam_ctas(DT)) select_kernel(Bea
     __syncthreads();
     // List l = beam * chunks + chunk holds k candidates, best first.
     const int lists = k * a.chunks;
-    constexpr Cand kNone{-INFINITY, 0x7FFFFFFF};
+    const int64_t lowest = order_of(-INFINITY);
+    const Cand kNone{lowest, 0x7FFFFFFF};
     auto candidate = [&](int l, int j) {
         const int b = l / a.chunks;
         Cand c = kNone;
@@ -440,7 +462,7 @@ __global__ void __launch_bounds__(kBeamThreads, beam_ctas(DT)) select_kernel(Bea
             const uint64_t key = __ldcg(a.part_keys + (row0 * a.chunks + l) * a.key_stride + j);
             if (key == 0) return c;
             const double x = from_ordered((uint32_t)(key >> 32));
-            c.total = ((x - (double)rmax[b]) - lse[b]) + score[b];
+            c.order = order_of(((x - (double)rmax[b]) - lse[b]) + score[b]);
             c.at = b * a.vocab + (int)~(uint32_t)key;
             return c;
         }
@@ -449,7 +471,7 @@ __global__ void __launch_bounds__(kBeamThreads, beam_ctas(DT)) select_kernel(Bea
         if (l % a.chunks != 0) return c;
         int token = j;
         if (state[b] == 1 && a.eos >= 0 && a.eos < a.vocab) {
-            if (j == 0) c.total = score[b];
+            if (j == 0) c.order = order_of(score[b]);
             token = j == 0 ? a.eos : j - 1 < a.eos ? j - 1 : j;
         }
         if (token < a.vocab) c.at = b * a.vocab + token;
@@ -458,7 +480,7 @@ __global__ void __launch_bounds__(kBeamThreads, beam_ctas(DT)) select_kernel(Bea
     auto write = [&](int rank, const Cand& c) {
         const int b = c.at / a.vocab, token = c.at % a.vocab;
         const int64_t o = row0 + rank;
-        a.next_scores[o] = (float)c.total;
+        a.next_scores[o] = (float)total_of(c.order);
         a.parents[o] = b;
         a.tokens[o] = token;
         if (a.next_done) a.next_done[o] = over[b] || token == a.eos;
@@ -478,9 +500,7 @@ __global__ void __launch_bounds__(kBeamThreads, beam_ctas(DT)) select_kernel(Bea
         for (int l = tid; l < lists; l += kBeamThreads) {
             const Cand c = cands[l];
             if (c.at == 0x7FFFFFFF) continue;
-            int rank = 0;
-#pragma unroll 4
-            for (int j = 0; j < lists; ++j) rank += better(cands[j], c);
+            const int rank = rank_of(c, cands, lists);
             if (rank < k) alive[rank] = l, atomicAdd(&found, 1u);
             if (rank == k - 1) limit = c;
         }
@@ -495,14 +515,12 @@ __global__ void __launch_bounds__(kBeamThreads, beam_ctas(DT)) select_kernel(Bea
         if (c.at == 0x7FFFFFFF || better(L, c)) continue;
         cands[atomicAdd(&many, 1u)] = c;
     }
-    static_assert(kMaxBeams * kMaxBeams <= kRoom && 256 <= kRoom, "all that count, and the lists' first ones, have room");
+    static_assert(kMaxBeams * kMaxBeams <= kRoom && kBeamThreads <= kRoom, "all that count, and the lists' first ones, have room");
     __syncthreads();
     const int n = (int)many;
     for (int q = tid; q < n; q += kBeamThreads) {
         const Cand c = cands[q];
-        int rank = 0;
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) rank += better(cands[j], c);
+        const int rank = rank_of(c, cands, n);
         if (rank < k) write(rank, c);
     }
     if (tid == 0) a.tickets[g] = 0u;
