@@ -44,6 +44,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kMaxParts = 64;
 constexpr int kMaxCluster = 8;
+constexpr int kMaxRun = 32;     // blocks of a warp where the output is f32, as far as clusters go
 constexpr int kMinBlocks = 4;   // of a warp in a part that is joined through memory
 // Query rows of a CTA, stages of a warp's ring, CTAs per SM.
 template <bool NARROW>
@@ -610,11 +611,14 @@ constexpr size_t attend_smem() {
 // 3 us besides its blocks, a block of 16 keys takes a warp 0.6 us on an idle SM and 1.5 us on a full
 // one, joining a cluster takes 1 us and joining parts through memory 3 us and a little for each.  (Parts
 // alone, without clusters: 751 positions of 16 heads 11.0 us, with them 7.2 us.)
+// A product's f32 accumulator is truncated, not rounded, at every block: a warp's sums drift by about 1.3e-8
+// of themselves a block (10,000 positions in runs of 156 blocks 2.0e-6, of 20 blocks 3.7e-7), so for f32
+// outputs a warp takes max_run blocks at most where a cluster can be larger.
 struct Cut {
     int parts, cluster;
     double us;
 };
-Cut cut_items(int64_t items, int64_t blocks, int slots) {
+Cut cut_items(int64_t items, int64_t blocks, int slots, int max_run) {
     Cut best{1, 1, 1e30};
     for (int cluster = 1; cluster <= kMaxCluster; cluster *= 2)
         for (int parts = 1; parts <= kMaxParts; parts = parts < 8 ? parts + 1 : parts + parts / 4) {
@@ -622,6 +626,7 @@ Cut cut_items(int64_t items, int64_t blocks, int slots) {
             if ((runs > 1 && (runs * kWarps > blocks + kWarps || items * runs > INT_MAX)) || (parts > 1 && (cluster < kMaxCluster / 2 || items * parts > kKv8MaxPartials ||
                                                                          runs * kWarps * kMinBlocks > blocks)))
                 break;
+            if (cluster < kMaxCluster && blocks > runs * kWarps * max_run) continue;
             const double fill = std::min(1.0, (double)(items * runs) / slots);
             const double waves = (double)((items * runs + slots - 1) / slots);
             const double block_us = std::max(0.6, 1.5 * fill);
@@ -684,8 +689,9 @@ cudaError_t launch_kv8_attention(const Kv8Dev& c, const Kv8Batch& b, const Kv8At
     // query heads each 107 us (117); calls of a few microseconds are within 0.3 us, or up to 1 us slower with
     // head_dim 64.
     const bool narrow = rows <= Shape<true>::kRows;
-    const Cut cut = narrow ? cut_items(items, blocks, Shape<true>::kCtas * m.num_sms)
-                           : cut_items(items * row_groups<false>(rows), blocks, Shape<false>::kCtas * m.num_sms);
+    const int max_run = a.out_dtype == DT_F32 ? kMaxRun : INT_MAX / kWarps;
+    const Cut cut = narrow ? cut_items(items, blocks, Shape<true>::kCtas * m.num_sms, max_run)
+                           : cut_items(items * row_groups<false>(rows), blocks, Shape<false>::kCtas * m.num_sms, max_run);
     if (rows > kKv8Rows && a.q_dtype != DT_F32 && a.out_dtype != DT_F32) {
         const PromptPlan plan = kv8_prompt_plan(rows, items, blocks, m);
         if (plan.us < cut.us) return launch_kv8_prompt(c, b, a, plan.cluster, st);

@@ -291,6 +291,23 @@ def test_attention_matches_the_formula(heads, group, dim, tokens, pos, cap, wind
     assert torch.equal(out, again)  # the order of the sums does not depend on the run
 
 
+def test_long_sums_do_not_drift():
+    """More items than CTAs fit, 60,000 positions each.  A product's accumulator is truncated at every block of 16 keys, by half a
+    unit on average, at most 2^-24 of the running sum: runs of 128 blocks stay within 128 * 2^-24 of the output's norm (runs of
+    all 938 blocks of a warp do not), and the softmax's 22 bits and exponents add under 2^-20."""
+    import torch
+    n, heads, dim, cap = 80, 8, 128, 60000
+    p = Pair(1, heads, dim, cap, seed=3)
+    q, out = rand((n, 1, heads, dim), "f32", 37), torch.zeros(n, 1, heads, dim, device="cuda")
+    p.cache.attention(q, out, i32([cap - 1] * n), seqs=i32([0] * n), scale=0.01)
+    p.cache.status()
+    k, v = (torch.from_numpy(x.values(0, range(cap))).cuda() for x in (p.k, p.v))
+    w = torch.softmax(torch.einsum("nhd,phd->nhp", q[:, 0].double(), k) * 0.01, -1)
+    exact = torch.einsum("nhp,phd->nhd", w, v)
+    error = ((out[:, 0].double() - exact).norm() / exact.norm()).item()
+    assert error < 128 * 2.0 ** -24 + 2.0 ** -20, error
+
+
 def test_attention_of_codes_in_masked_slots_and_uneven_exponents():
     """Exponents far apart between blocks, all-zero V blocks, and slots behind the last position that hold the largest codes."""
     import torch
