@@ -533,12 +533,14 @@ __global__ void __launch_bounds__(kBeamThreads, beam_ctas(DT)) select_kernel(Bea
 // before any of it is written, and no other thread touches it, so the rows are permuted in place,
 // with each source read once (a beam that two others take is read twice, the second time from L1).
 // HBM bounds it: 32 x 8 rows of 64 pieces of up to 751 x 256 bytes take 565 us for 3.4 GB, 5.9 TB/s.
-template <int B, class V, int U>
+// FLAT: segments that do not fill a CTA are taken one after another, so that its threads all have work
+// (64 x 16 rows of 200 segments of 3 units of 144 bytes: 22 us, with a CTA to each segment 102 us).
+template <int B, class V, int U, bool FLAT>
 __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a, int64_t per_segment) {
     __shared__ int parent[B];
     __shared__ int64_t place[B];
     __shared__ int64_t limit[B];
-    const int g = blockIdx.z, s = a.first_segment + blockIdx.y;
+    const int g = blockIdx.z;
     const int64_t row0 = (int64_t)g * a.beams;
     const int64_t per_unit = a.unit_bytes / (int64_t)sizeof(V);
     for (int b = threadIdx.x; b < B; b += 256) {
@@ -554,29 +556,37 @@ __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a, int64_t per
         limit[b] = p == b ? 0 : m * per_unit;
     }
     __syncthreads();
-    uint8_t* base = a.states + (s / a.inner) * a.outer_stride + (s % a.inner) * a.segment_stride;
-    const int64_t first = (int64_t)blockIdx.x * 256 * U + threadIdx.x;
+    uint8_t* base[U];  // of the thread's U segments, and its positions in them
+    int64_t q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        q[u] = (int64_t)blockIdx.x * 256 * U + u * 256 + threadIdx.x;
+        int s = blockIdx.y;
+        if constexpr (FLAT) {  // (fewer than 2^31: 65535 segments of fewer than 1024 positions)
+            const uint32_t at = (uint32_t)q[u], per = (uint32_t)per_segment;
+            s = (int)(at / per);
+            q[u] = s < a.segments ? (int64_t)(at % per) : INT64_MAX;
+        }
+        s += a.first_segment;
+        base[u] = a.states + (s / a.inner) * a.outer_stride + (s % a.inner) * a.segment_stride;
+    }
     V v[U][B];
 #pragma unroll
     for (int b = 0; b < B; ++b)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t q = first + u * 256;
-            if (q < limit[b]) v[u][b] = *reinterpret_cast<const V*>(base + place[parent[b]] + q * sizeof(V));
-        }
+        for (int u = 0; u < U; ++u)
+            if (q[u] < limit[b]) v[u][b] = *reinterpret_cast<const V*>(base[u] + place[parent[b]] + q[u] * sizeof(V));
 #pragma unroll
     for (int b = 0; b < B; ++b)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t q = first + u * 256;
-            if (q < limit[b]) *reinterpret_cast<V*>(base + place[b] + q * sizeof(V)) = v[u][b];
-        }
+        for (int u = 0; u < U; ++u)
+            if (q[u] < limit[b]) *reinterpret_cast<V*>(base[u] + place[b] + q[u] * sizeof(V)) = v[u][b];
 }
 
 template <int B, class V, int U>
 cudaError_t reorder_t(const ReorderArgs& a, cudaStream_t st) {
     const int64_t per_segment = a.units * a.unit_bytes / (int64_t)sizeof(V);
-    const int64_t x = (per_segment + 256 * U - 1) / (256 * U);
+    const bool flat = per_segment < 256 * U;
     // grid y and z end at 65535: more segments or groups than that go in several launches
     for (int g0 = 0; g0 < a.groups; g0 += 65535)
         for (int s0 = 0; s0 < a.segments; s0 += 65535) {
@@ -588,7 +598,9 @@ cudaError_t reorder_t(const ReorderArgs& a, cudaStream_t st) {
             b.first_segment = s0;
             b.parents += (int64_t)g0 * a.beams;
             if (b.held) b.held += (int64_t)g0 * a.beams;
-            reorder_kernel<B, V, U><<<dim3((unsigned)x, b.segments, b.groups), 256, 0, st>>>(b, per_segment);
+            const int64_t x = ((flat ? b.segments * per_segment : per_segment) + 256 * U - 1) / (256 * U);
+            if (flat) reorder_kernel<B, V, U, true><<<dim3((unsigned)x, 1, b.groups), 256, 0, st>>>(b, per_segment);
+            else reorder_kernel<B, V, U, false><<<dim3((unsigned)x, b.segments, b.groups), 256, 0, st>>>(b, per_segment);
             const cudaError_t e = cudaGetLastError();
             if (e != cudaSuccess) return e;
         }
