@@ -342,7 +342,9 @@ int stt_kv8_cache_status(stt_kv8_cache* cache);
 int stt_kv8_append_device(stt_kv8_cache* cache, const stt_kv8_batch* batch, const stt_kv8_tensor* k,
                           const stt_kv8_tensor* v, void* cuda_stream);
 /* The way back: the values of positions d_pos[i] .. d_pos[i] + d_count[i] - 1 (which the ring must
- * still hold) into k and v (one dtype), exact in every dtype unless an exponent leaves f16's range. */
+ * still hold) into k and v (one dtype), exact in every dtype unless a value leaves its range (in f16, and
+ * where a number next to f32's largest was rounded up to 2^128; it is read as infinity, or as the nearest
+ * subnormal). */
 int stt_kv8_read_device(const stt_kv8_cache* cache, const stt_kv8_batch* batch, const stt_kv8_tensor* k,
                         const stt_kv8_tensor* v, void* cuda_stream);
 /* Causal attention of the positions that an append with the same batch has just written: the query of

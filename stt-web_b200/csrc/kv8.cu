@@ -202,9 +202,10 @@ __global__ void __launch_bounds__(kThreads, MAX == 1 ? 6 : DT == DT_F32 ? 2 : 4)
 constexpr int kReadTokens = 8;
 
 // Values of a range of tokens.  A thread keeps its place in a token (as many codes as fill 16 bytes of
-// values, in K and in V) and walks over the tokens, several in flight.  A code becomes a value in two
-// instructions: the byte code + 128 under 0x4B0000 is the f32 value 2^23 + 128 + code, and
-// (2^23 + 128 + code) * step - (2^23 + 128) * step is exact in one fused multiply-add.
+// values, in K and in V) and walks over the tokens, several in flight.  A code becomes a value in three
+// instructions: the byte code + 128 under 0x4B0000 is the f32 value 2^23 + 128 + code; the difference to
+// 2^23 + 128 is exact, and so is its product with a power of two.  (The difference after the product, in one
+// fused multiply-add, leaves f32's range from the exponent 105 on.)
 template <int D, int DT>
 __global__ void __launch_bounds__(kThreads) read_kernel(Kv8Dev c, Kv8Batch b, void* __restrict__ k, void* __restrict__ v,
                                                         Kv8Strides ks, Kv8Strides vs, int token_ctas, int head_ctas) {
@@ -233,11 +234,10 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Kv8Dev c, Kv8Batch b, vo
         if (++slot == c.cap) slot = 0;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const float bias = -8388736.0f * step[half];
             float y[N];
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                y[j] = fmaf(__uint_as_float(__byte_perm(q[half][j / 4] ^ 0x80808080u, 0x4B000000u, 0x7650 | (j % 4))), step[half], bias);
+                y[j] = (__uint_as_float(__byte_perm(q[half][j / 4] ^ 0x80808080u, 0x4B000000u, 0x7650 | (j % 4))) - 8388736.0f) * step[half];
             void* out = half ? v : k;
             const Kv8Strides& s = half ? vs : ks;
             const int64_t at = i * s.seq + t * s.token + h * s.head + piece * N;

@@ -1,0 +1,54 @@
+"""The decode operators at the ends of their ranges, on the GPU, against the plain 64-bit implementations
+of tests/operators_ref.py: exponents and positions near their limits, peaked and masked rows of logits,
+padded batches.  Tolerances are those of tests/test_gpu_operators.py unless a test derives its own."""
+import numpy as np
+import pytest
+
+import operators_ref as R
+from stt_b200 import BeamSelector, SttError
+from stt_b200._lib import STT_E_DEVICE_FLAG, STT_E_INVALID_ARG
+from test_gpu_operators import Pair, check_attention, check_select, dt, i32, rand, run_select
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_read_is_exact_for_every_exponent(dim, dtype):
+    """A value is a whole number of at most 7 bits times a power of two: exact in f32 and bf16 (the largest here
+    is 127 * 2^121 < 2^128), and in f16 the nearest f16 (infinity beyond 65,504)."""
+    import torch
+    exps = [-100, -60, -27, 0, 9, 60, 103, 104, 105, 106, 113, 120, 121, 121, -99, 105]
+    p = Pair(1, 2, dim, 16 * len(exps), seed=1)
+    raw = p.mem.cpu().numpy()
+    raw[2 * p.a:] = np.tile(np.array(exps, np.int8), 4)
+    raw[0:p.a:dim] = 0  # a zero in every row
+    p.mem.copy_(torch.from_numpy(raw))
+    p.k, p.v = p.halves(raw)
+    out = torch.zeros(2, 1, p.shape[2], 2, dim, dtype=dt(dtype), device="cuda")
+    p.cache.read(out[0], out[1], i32([0]))
+    p.cache.status()
+    for got, half in ((out[0, 0], p.k), (out[1, 0], p.v)):
+        exp = half.values(0, range(p.shape[2]))
+        if dtype == "f16":
+            with np.errstate(over="ignore"):
+                exp = exp.astype(np.float16).astype(np.float64)
+        assert np.array_equal(got.double().cpu().numpy(), exp)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("value", [2.5e33, 2.7e33, -1e36, 3e38])
+def test_the_largest_values_are_read_back_as_they_were_appended(dtype, value):
+    import torch
+    p = Pair(1, 2, 64, 32, fill=False)
+    x = rand((1, 5, 2, 64), dtype, 2, 1e33)
+    x[0, 1, 0, 5] = value
+    x[0, 3, 1, 9] = 0.0
+    out = torch.zeros(2, 1, 5, 2, 64, dtype=dt(dtype), device="cuda")
+    p.cache.append(x, -x, i32([7]))
+    p.append(x, -x, [7], [5], [0])
+    p.same()
+    p.cache.read(out[0], out[1], i32([7]))
+    p.cache.status()
+    assert np.array_equal(out[0, 0].double().cpu().numpy(), p.k.values(0, range(7, 12)))
+    assert np.array_equal(out[1, 0].double().cpu().numpy(), p.v.values(0, range(7, 12)))
