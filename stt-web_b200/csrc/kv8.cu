@@ -188,10 +188,10 @@ __global__ void __launch_bounds__(kThreads, MAX == 1 ? 6 : DT == DT_F32 ? 2 : 4)
             if (t < many) {
                 float y[N];
                 x[u][t].values(y);
-                if (!finite)
+                if (!finite)  // clamped as steps: 127 * 2^122 is more than an f32 holds
 #pragma unroll
-                    for (int j = 0; j < N; ++j) y[j] = y[j] != y[j] ? 0.0f : fminf(fmaxf(y[j], -127.0f / f), 127.0f / f);
-                store_codes<N>(codes + (old + t) * D, pack_codes<N>(y, f));
+                    for (int j = 0; j < N; ++j) y[j] = y[j] != y[j] ? 0.0f : fminf(fmaxf(y[j] * f, -127.0f), 127.0f);
+                store_codes<N>(codes + (old + t) * D, pack_codes<N>(y, finite ? f : 1.0f));
             }
         if (lane == 0 && (e != was[u] || !old)) (kv0 + u ? c.ve : c.ke)[exp_at] = (int8_t)e;
     }

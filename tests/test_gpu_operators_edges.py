@@ -52,3 +52,20 @@ def test_the_largest_values_are_read_back_as_they_were_appended(dtype, value):
     p.cache.status()
     assert np.array_equal(out[0, 0].double().cpu().numpy(), p.k.values(0, range(7, 12)))
     assert np.array_equal(out[1, 0].double().cpu().numpy(), p.v.values(0, range(7, 12)))
+
+
+@pytest.mark.parametrize("dtype,largest", [("f32", 3.4e38), ("bf16", 3.3895313892515355e38), ("f16", 65504.0), ("f32", 1e-38)])
+def test_an_infinity_next_to_the_largest_values_is_the_largest_code(dtype, largest):
+    """The block's exponent is then 122 in f32 and bf16, where 127 steps are more than an f32 holds."""
+    import torch
+    for infinite in (float("inf"), -float("inf")):
+        p = Pair(1, 1, 64, 16, fill=False)
+        x = torch.ones(1, 3, 1, 64, dtype=dt(dtype), device="cuda")
+        x[0, 0, 0, 0], x[0, 1, 0, 1], x[0, 2, 0, 2] = largest, infinite, float("nan")
+        p.cache.append(x, -x, i32([3]))
+        p.append(x, -x, [3], [3], [0])
+        p.same()
+        assert p.k.codes[0, 0, 4, 1] == (127 if infinite > 0 else -127)
+        with pytest.raises(SttError) as e:
+            p.cache.status()
+        assert e.value.code == STT_E_DEVICE_FLAG
