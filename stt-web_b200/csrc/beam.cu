@@ -6,8 +6,9 @@
 // reference value, its sum of exponentials over it, and its `beams` best logits (no more of one row can
 // be among the best of all); the last CTA of an utterance joins the rows' sums and picks among the
 // chunks' bests.  The order of two beams' candidates can hang on the last digits, so sums are joined and
-// candidates compared in 64 bits; the exponentials themselves are f32, 16 or 32 of a thread added at a
-// time (their rounding errors, 2^-24 each, average out: 1e-8 of the sum at 8000 logits).
+// candidates compared in 64 bits; the exponentials themselves are f32 over the largest logit so far, 16 or
+// 32 of a thread added at a time in two chains: a sum is off by 16 * 2^-24 of itself at most, and where
+// many terms are alike their roundings average out (1e-8 of the sum at 8000 normally distributed logits).
 //
 // The best of a chunk: the k-th largest of the maxima of its 32 groups of 4 lanes bounds the k-th best
 // logit from below, and little more than the k best reach it; those few go to a list in shared memory,
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(kBeamThreads, beam_ctas(DT)) select_kernel(Bea
         // thread t of a tile covers elements -lead + tile * kTile + (j * kBeamThreads + t) * VEC on.
         const T* row = static_cast<const T*>(a.logits) + r * a.row_stride;
         const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-        float ref = -INFINITY;    // the sum's reference: within 60 of the largest so far
+        float ref = -INFINITY;    // the sum's reference: the warp's largest so far
         double sum = 0.0;
         float bound = -INFINITY;  // the chunk has at least k logits that reach it
         int listed = 0;           // keys of the list
@@ -312,7 +313,10 @@ __global__ void __launch_bounds__(kBeamThreads, beam_ctas(DT)) select_kernel(Bea
             if (!(mx < INFINITY)) {
                 ref = INFINITY;
             } else if (mx > -INFINITY && ref < INFINITY) {
-                if (mx > ref + 60.0f || ref == -INFINITY) {
+                // every larger maximum becomes the reference: a term e^d above an older one would carry the
+                // rounding of its argument, 3 d 2^-24 of it (rows with a peak of 30 .. 59 in a later tile: the
+                // log sum 2.7e-6 .. 5.3e-6 off; a peak that is the reference itself is exact)
+                if (mx > ref) {
                     if (sum != 0.0) sum *= exp((double)ref - (double)mx);
                     ref = mx;
                 }

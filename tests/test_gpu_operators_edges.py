@@ -69,3 +69,30 @@ def test_an_infinity_next_to_the_largest_values_is_the_largest_code(dtype, large
         with pytest.raises(SttError) as e:
             p.cache.status()
         assert e.value.code == STT_E_DEVICE_FLAG
+
+
+def select_error(logits, scores, tolerance):
+    """Checks a selection, its scores to `tolerance` and their rounding to f32."""
+    sel, out = run_select(logits, scores)
+    check_select(logits, scores, None, -1, out)
+    sel.status()
+    exp = R.select(logits.double().cpu().numpy().reshape(*scores.shape, -1), scores.cpu().numpy())[0]
+    got = out[0].double().cpu().numpy()
+    fin = np.isfinite(exp)
+    off = np.abs(got[fin] - exp[fin]) - 2.0 ** -24 * np.abs(exp[fin])
+    assert off.max() <= tolerance, off.max()
+
+
+@pytest.mark.parametrize("dtype,vocab,tile", [("f32", 8000, 2048), ("bf16", 16000, 4096), ("f16", 16000, 4096)])
+def test_log_sums_of_rows_with_one_large_logit(dtype, vocab, tile):
+    """A trained model's rows: one logit far above the others, in a later tile of a CTA that takes several.  The
+    large logit is the sum's reference, its term 1: a thread's at most 32 terms, added in two chains, are off by
+    16 * 2^-24 of the sum, the powers by 2^-22 of themselves, and the arguments of the others (d below the
+    reference, d * 3 * 2^-24 off) weigh e^-d: 2^-20 + 2^-22 + 2^-23 in all."""
+    rng = np.random.default_rng(vocab)
+    logits = rand((64 * 8, vocab), dtype, 3, 1.0)
+    scores = rand((64, 8), "f32", 4, 2.0)
+    for row in range(64 * 8):
+        at = int(rng.integers(tile, 2 * tile) if row % 2 else rng.integers(3 * tile, vocab))
+        logits[row, at] = float(rng.uniform(25.0, 62.0))
+    select_error(logits, scores, 2.0 ** -20 + 2.0 ** -22 + 2.0 ** -23)
