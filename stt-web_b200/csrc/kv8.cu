@@ -43,11 +43,12 @@ __device__ __forceinline__ uint32_t pack_codes(const float (&x)[N], float f) {
 }
 
 // Raises the error word where a sequence comes twice in one append: its two rows would write the
-// same blocks.  One warp per batch row looks at the rows before it.
+// same blocks.  One warp per batch row looks at the rows before it; rows without tokens, a padded batch's,
+// write nothing and do not count.
 __device__ __forceinline__ void check_repeated(const Kv8Dev& c, const Kv8Batch& b, int i, int seq, int lane) {
     if (!b.seqs) return;
     bool twice = false;
-    for (int j = lane; j < i; j += 32) twice |= __ldg(b.seqs + j) == seq;
+    for (int j = lane; j < i; j += 32) twice |= __ldg(b.seqs + j) == seq && (!b.count || __ldg(b.count + j) > 0);
     if (__any_sync(0xFFFFFFFFu, twice) && lane == 0) atomicCAS(c.err, 0, -1);
 }
 
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, MAX == 1 ? 6 : DT == DT_F32 ? 2 : 4)
     const int i = rest / nb, blk = rest - i * nb;
     Kv8Row r;
     if (!kv8_row(c, b, i, &r)) return;
-    if (task == 0 && blk == 0) check_repeated(c, b, i, r.seq, lane);
+    if (task == 0 && blk == 0 && r.count > 0) check_repeated(c, b, i, r.seq, lane);
     if (r.count > 0 && (r.pos + r.count - 1) / kKv8Block - r.pos / kKv8Block >= c.cap / kKv8Block) {
         if (lane == 0) atomicCAS(c.err, 0, -1);  // the call's tokens would overwrite one another in the ring
         return;

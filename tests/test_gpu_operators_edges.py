@@ -96,3 +96,19 @@ def test_log_sums_of_rows_with_one_large_logit(dtype, vocab, tile):
         at = int(rng.integers(tile, 2 * tile) if row % 2 else rng.integers(3 * tile, vocab))
         logits[row, at] = float(rng.uniform(25.0, 62.0))
     select_error(logits, scores, 2.0 ** -20 + 2.0 ** -22 + 2.0 ** -23)
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 20])
+def test_padding_rows_do_not_count_as_repeated_sequences(tokens):
+    p = Pair(4, 2, 64, 64)
+    x = rand((5, tokens, 2, 64), "f32", 5)
+    seqs, pos, count = [2, 0, 0, 2, 0], [5, 0, 9, 17, 0], [tokens, 0, tokens, 0, 0]
+    p.cache.append(x, x, i32(pos), count=i32(count), seqs=i32(seqs))
+    p.append(x, x, pos, count, seqs)
+    p.same()
+    p.cache.status()
+    count[3] = 1  # now sequence 2 does come twice
+    p.cache.append(x, x, i32(pos), count=i32(count), seqs=i32(seqs))
+    with pytest.raises(SttError) as e:
+        p.cache.status()
+    assert e.value.code == STT_E_INVALID_ARG
