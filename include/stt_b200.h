@@ -291,7 +291,8 @@ int stt_q4_tensor_dequant(const stt_q4_tensor* w, float* out_host);
  * on: device arrays, so that a captured graph can be replayed for other positions.  Tensors
  * (stt_kv8_tensor) are [n][n_tokens][heads][head_dim] on the device, dtype 0 f32, 1 bf16, 2 f16, with
  * strides in elements, head_dim contiguous; they start at, and their strides are, multiples of 16
- * bytes.  What lies behind a row's count is neither read nor written.
+ * bytes.  What lies behind a row's count is neither read nor written.  No two rows of a tensor that is
+ * written may share memory (strides that could do so are refused); rows that are read may.
  *
  * Calls are queued on cuda_stream (NULL = legacy default stream) without synchronisation and
  * allocate nothing.  Calls on one cache share its workspace: they must not overlap in time, nor may

@@ -60,6 +60,24 @@ int check_tensor(const char* what, const stt_kv8_tensor& t) {
     return STT_OK;
 }
 
+// A tensor that is written: no two of its rows [n][tokens][heads] of `dim` elements may share memory.  Each
+// dimension, from the least stride up, has to step over what the ones before it span.
+int check_written(const char* what, const stt_kv8_tensor& t, const stt_kv8_batch& b, int heads, int dim) {
+    struct Step {
+        __int128 stride;
+        int size;
+    } d[3] = {{t.seq_stride, b.n}, {t.token_stride, b.n_tokens}, {t.head_stride, heads}};
+    for (Step& x : d) x.stride = x.size == 1 ? 0 : x.stride < 0 ? -x.stride : x.stride;
+    std::sort(d, d + 3, [](const Step& x, const Step& y) { return x.stride < y.stride; });
+    __int128 span = dim;
+    for (const Step& x : d) {
+        if (x.size == 1) continue;
+        if (x.stride < span) return set_error(STT_E_INVALID_ARG, "rows of %s lie on one another", what);
+        span += x.stride * (x.size - 1);
+    }
+    return STT_OK;
+}
+
 // A batch's host-side checks; *some is false for one without rows or tokens, which is nothing to do.
 int check_batch(const stt_kv8_cache* h, const stt_kv8_batch* b, bool* some) {
     if (!h || !b || b->n < 0 || b->n_tokens < 0) return set_error(STT_E_INVALID_ARG, "bad arguments");
@@ -207,6 +225,9 @@ extern "C" int stt_kv8_read_device(const stt_kv8_cache* h, const stt_kv8_batch* 
     TRY(check_batch(h, b, &some));
     if (!some) return STT_OK;
     TRY(check_kv(k, v));
+    TRY(check_written("K", *k, *b, h->c.heads, h->c.dim));
+    TRY(check_written("V", *v, *b, h->c.heads, h->c.dim));
+    if (k->d_data == v->d_data) return set_error(STT_E_INVALID_ARG, "K and V are one memory");
     if ((int64_t)b->n * (b->n_tokens / 8 + 1) > INT_MAX / (h->c.heads / 8 + 1))
         return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", b->n, b->n_tokens);
     DeviceScope ds(h->device);
@@ -229,6 +250,7 @@ extern "C" int stt_kv8_attention_device(stt_kv8_cache* h, const stt_kv8_batch* b
     if (!q || !out) return set_error(STT_E_INVALID_ARG, "NULL argument");
     TRY(check_tensor("the queries", *q));
     TRY(check_tensor("the output", *out));
+    TRY(check_written("the output", *out, *b, n_heads, h->c.dim));
     Kv8Attention a{};
     a.q = q->d_data;
     a.out = out->d_data;

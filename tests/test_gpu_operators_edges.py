@@ -112,3 +112,36 @@ def test_padding_rows_do_not_count_as_repeated_sequences(tokens):
     with pytest.raises(SttError) as e:
         p.cache.status()
     assert e.value.code == STT_E_INVALID_ARG
+
+
+def test_outputs_whose_rows_lie_on_one_another_are_refused():
+    import torch
+    p = Pair(2, 2, 64, 32)
+    q = rand((2, 3, 4, 64), "f32", 6)
+    wide = torch.zeros(2, 3, 4, 128, device="cuda")
+    flat = torch.zeros(64 * 64, device="cuda")
+
+    def refused(call, text):
+        with pytest.raises(SttError) as e:
+            call()
+        assert e.value.code == STT_E_INVALID_ARG and text in str(e.value)
+
+    bad = [torch.zeros(1, 3, 4, 64, device="cuda").expand(2, 3, 4, 64), torch.zeros(2, 1, 4, 64, device="cuda").expand(2, 3, 4, 64),
+           torch.zeros(2, 3, 1, 64, device="cuda").expand(2, 3, 4, 64), flat.as_strided((2, 3, 4, 64), (768, 256, 60, 1)),
+           flat.as_strided((2, 3, 4, 64), (768, 128, 64, 1)), flat.as_strided((2, 3, 4, 64), (512, 256, 64, 1))]
+    for out in bad:
+        refused(lambda: p.cache.attention(q, out, i32([5, 6])), "on one another")
+    k = torch.zeros(2, 3, 2, 64, device="cuda")
+    for out in (torch.zeros(1, 3, 2, 64, device="cuda").expand(2, 3, 2, 64), flat.as_strided((2, 3, 2, 64), (384, 64, 64, 1))):
+        refused(lambda: p.cache.read(out, k, i32([5, 6])), "on one another")
+        refused(lambda: p.cache.read(k, out, i32([5, 6])), "on one another")
+    refused(lambda: p.cache.read(k, k, i32([5, 6])), "one memory")
+    # gaps, another order of the dimensions, and strides of dimensions of one entry are as good as any
+    p.cache.attention(q, wide[..., :64], i32([5, 6]))
+    p.cache.attention(q, torch.zeros(4, 3, 2, 64, device="cuda").permute(2, 1, 0, 3), i32([5, 6]))
+    one = flat.as_strided((1, 1, 4, 64), (0, 0, 64, 1))
+    p.cache.attention(q[:1, :1], one, i32([5]))
+    # inputs may repeat: one query, key and value for all rows
+    p.cache.attention(q[:1].expand(2, 3, 4, 64), torch.zeros(2, 3, 4, 64, device="cuda"), i32([5, 6]))
+    p.cache.append(k[:1].expand(2, 3, 2, 64), k[:1].expand(2, 3, 2, 64), i32([5, 6]))
+    p.cache.status()
