@@ -100,6 +100,7 @@ __device__ __forceinline__ void store_row(const uint4 (&w)[D / 16], uint8_t* dst
                            codes_to_f16<0x4140>(x[2 * half + 1]), codes_to_f16<0x4342>(x[2 * half + 1]));
     }
 }
+// (All warps of a warpgroup execute the same one of these, once.)
 template <int N>
 __device__ __forceinline__ void registers_up() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -256,73 +257,72 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
             if (lane == 0) mbar_arrive(&sm.v_full[st]);
         }
         meet();
-    } else if (warp > kMmaWarp) {
-        registers_down<kMmaRegs>();
-        meet();
-    } else if (warp == kMmaWarp) {
-        registers_down<kMmaRegs>();
-        constexpr uint32_t GROUP = D * 16;  // bytes of 8 rows: D / 8 core matrices
-        const uint32_t qk_desc = instr_desc_f16(kTile, kTile);
-        const uint32_t pv_desc = instr_desc_f16(kTile, D) | (1u << 16);  // V is MN-major
-        auto qk = [&](int q, int st) {
-            const uint32_t qa = smem_u32(sm.q[q]), ka = smem_u32(sm.k[st]);
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-                mma_f16_ss(tmem + q * kTile, smem_desc(qa + k * 256, 128, GROUP), smem_desc(ka + k * 256, 128, GROUP), qk_desc,
-                           k > 0);
-            mma_commit(&sm.s_full[q]);
-        };
-        auto pv = [&](int q, int st, int half, bool add) {
-            const uint32_t va = smem_u32(sm.v[st]);
-#pragma unroll
-            for (int k = half * (kTile / 32); k < (half + 1) * (kTile / 32); ++k)
-                mma_f16_ts(tmem + kOCol + q * kTile, tmem + q * kTile + k * 8, smem_desc(va + k * 2 * GROUP, GROUP, 128), pv_desc,
-                           add || k > 0);
-        };
-        bool ok = true;  // (without a step too, `done` says that nothing writes the operands any more)
-        for (int q = 0; ok && q < tiles; ++q) ok = mbar_wait(&sm.q_full[q], 0, abort);
-        ok = ok && steps > 0;
-        if (ok) ok = mbar_wait(&sm.k_full[0], 0, abort);
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        if (ok) {
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (elect_one()) {
-                for (int q = 0; q < tiles; ++q) qk(q, 0);
-                mma_commit(&sm.k_empty[0]);
-            }
-            __syncwarp();
-        }
-        for (int j = 0; ok && j < steps; ++j) {
-            const int st = j & 1, nx = (j + 1) & 1;
-            const bool more = j + 1 < steps;
-            ok = mbar_wait(&sm.v_full[st], (j >> 1) & 1, abort);
-            if (ok && more) ok = mbar_wait(&sm.k_full[nx], ((j + 1) >> 1) & 1, abort);
-            for (int q = 0; ok && q < tiles; ++q) {
-                // the weights of the first 64 keys, then the others'
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.p_half[q], j & 1, abort));
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (elect_one()) pv(q, st, 0, j > 0);
-                __syncwarp();
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.p_full[q], j & 1, abort));
-                if (!ok) break;
+    } else if (warp >= kMmaWarp) {
+        registers_down<kMmaRegs>();  // (one instruction for the four warps, as the ISA asks of a warpgroup)
+        if (warp == kMmaWarp) {
+            constexpr uint32_t GROUP = D * 16;  // bytes of 8 rows: D / 8 core matrices
+            const uint32_t qk_desc = instr_desc_f16(kTile, kTile);
+            const uint32_t pv_desc = instr_desc_f16(kTile, D) | (1u << 16);  // V is MN-major
+            auto qk = [&](int q, int st) {
+                const uint32_t qa = smem_u32(sm.q[q]), ka = smem_u32(sm.k[st]);
+    #pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    mma_f16_ss(tmem + q * kTile, smem_desc(qa + k * 256, 128, GROUP), smem_desc(ka + k * 256, 128, GROUP), qk_desc,
+                               k > 0);
+                mma_commit(&sm.s_full[q]);
+            };
+            auto pv = [&](int q, int st, int half, bool add) {
+                const uint32_t va = smem_u32(sm.v[st]);
+    #pragma unroll
+                for (int k = half * (kTile / 32); k < (half + 1) * (kTile / 32); ++k)
+                    mma_f16_ts(tmem + kOCol + q * kTile, tmem + q * kTile + k * 8, smem_desc(va + k * 2 * GROUP, GROUP, 128), pv_desc,
+                               add || k > 0);
+            };
+            bool ok = true;  // (without a step too, `done` says that nothing writes the operands any more)
+            for (int q = 0; ok && q < tiles; ++q) ok = mbar_wait(&sm.q_full[q], 0, abort);
+            ok = ok && steps > 0;
+            if (ok) ok = mbar_wait(&sm.k_full[0], 0, abort);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (ok) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_one()) {
-                    pv(q, st, 1, true);
-                    if (more) qk(q, nx);
+                    for (int q = 0; q < tiles; ++q) qk(q, 0);
+                    mma_commit(&sm.k_empty[0]);
                 }
                 __syncwarp();
             }
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok) break;
-            if (elect_one()) {
-                mma_commit(&sm.v_empty[st]);
-                if (more) mma_commit(&sm.k_empty[nx]);
+            for (int j = 0; ok && j < steps; ++j) {
+                const int st = j & 1, nx = (j + 1) & 1;
+                const bool more = j + 1 < steps;
+                ok = mbar_wait(&sm.v_full[st], (j >> 1) & 1, abort);
+                if (ok && more) ok = mbar_wait(&sm.k_full[nx], ((j + 1) >> 1) & 1, abort);
+                for (int q = 0; ok && q < tiles; ++q) {
+                    // the weights of the first 64 keys, then the others'
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.p_half[q], j & 1, abort));
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elect_one()) pv(q, st, 0, j > 0);
+                    __syncwarp();
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.p_full[q], j & 1, abort));
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elect_one()) {
+                        pv(q, st, 1, true);
+                        if (more) qk(q, nx);
+                    }
+                    __syncwarp();
+                }
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                if (elect_one()) {
+                    mma_commit(&sm.v_empty[st]);
+                    if (more) mma_commit(&sm.k_empty[nx]);
+                }
+                __syncwarp();
             }
+            if (elect_one()) mma_commit(&sm.done);  // also on abort: arrives once the products issued so far are done
             __syncwarp();
         }
-        if (elect_one()) mma_commit(&sm.done);  // also on abort: arrives once the products issued so far are done
-        __syncwarp();
         meet();
     } else {
         registers_up<kSoftmaxRegs>();
