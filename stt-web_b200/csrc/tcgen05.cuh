@@ -121,6 +121,21 @@ __device__ __forceinline__ void mma_commit(uint64_t* m) {
                  : "memory");
 }
 
+// Waits for the thread's loads from tensor memory, and ties the registers they fill to the wait: a memory
+// clobber alone does not keep arithmetic on them behind it.
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld(float (&r)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(r[i]));
+}
+
 // 32 consecutive 32-bit columns of this thread's TMEM lane, read (warp-collective).
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
     uint32_t r[32];
@@ -132,7 +147,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    tmem_wait_ld(r);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -145,7 +160,7 @@ __device__ __forceinline__ void tmem_ld16f(uint32_t taddr, float (&v)[16]) {
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    tmem_wait_ld(r);
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -160,10 +175,7 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
               "=f"(v[32 * c + 16]), "=f"(v[32 * c + 17]), "=f"(v[32 * c + 18]), "=f"(v[32 * c + 19]), "=f"(v[32 * c + 20]), "=f"(v[32 * c + 21]), "=f"(v[32 * c + 22]), "=f"(v[32 * c + 23]),
               "=f"(v[32 * c + 24]), "=f"(v[32 * c + 25]), "=f"(v[32 * c + 26]), "=f"(v[32 * c + 27]), "=f"(v[32 * c + 28]), "=f"(v[32 * c + 29]), "=f"(v[32 * c + 30]), "=f"(v[32 * c + 31])
             : "r"(taddr + 32 * c));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-    // the loads' registers may not be read before the wait
-#pragma unroll
-    for (int i = 0; i < 128; ++i) asm volatile("" : "+f"(v[i]));
+    tmem_wait_ld(v);
 }
 
 // 16 consecutive 32-bit columns of this thread's TMEM lane (warp-collective).

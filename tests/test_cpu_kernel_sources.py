@@ -22,3 +22,23 @@ def test_a_warpgroup_executes_one_setmaxnreg():
     roles = re.findall(r"if \(([^{}]*)\) \{\s*registers_\w+<(\w+)>", text) + re.findall(r"(else) \{\s*registers_\w+<(\w+)>", text)
     assert sorted(roles) == [("else", "kSoftmaxRegs"), ("warp >= kMmaWarp", "kMmaRegs"),
                              ("warp >= kSoftmaxWarps && warp < kMmaWarp", "kDequantRegs")]
+
+
+def test_registers_loaded_from_tensor_memory_are_tied_to_the_wait():
+    """tcgen05.ld fills its registers until tcgen05.wait::ld: the compiler may move what reads them in front of a wait that
+    does not name them, so every load is followed by tmem_wait_ld, the one place that waits."""
+    waits = loads = 0
+    for name in sorted(os.listdir(CSRC)):
+        if not name.endswith((".cu", ".cuh")):
+            continue
+        text = source(name)
+        waits += text.count("tcgen05.wait::ld")
+        for function in re.split(r"\n}\n", text):
+            if "tcgen05.ld." in function:
+                loads += 1
+                assert "tmem_wait_ld(" in function[function.rindex("tcgen05.ld."):], name
+    helper = source("tcgen05.cuh")
+    bodies = re.findall(r"void tmem_wait_ld\((?:uint32_t|float) \(&r\)\[N\]\) \{(.*?)\n\}", helper, flags=re.S)
+    assert len(bodies) == waits == 2 and loads >= 4
+    for body in bodies:
+        assert re.search(r'wait::ld.*for \(int i = 0; i < N; \+\+i\) asm volatile\("" : "\+[rf]"\(r\[i\]\)\);', body, flags=re.S)
