@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                 for (int v = 0; v < 4; ++v) k_step[u + v] = fmaxf(q_step * s[v], 1e-37f), v_exp[u + v] = e[v];
             }
             const int p0 = (kb0 + j * kStepBlocks) * kKv8Block;
-            const bool masked = p0 < all_lo || p0 + kTile - 1 > all_hi;
+            const bool masked = p0 < all_lo || p0 > all_hi - (kTile - 1);  // (p0 + kTile can pass 2^31)
             const int lo = see_lo - p0, hi = see_hi - p0;  // (no overflow: see_lo <= 2^31 - 1, p0 >= 0)
             float x[kTile];
             tmem_ld128(s_col, x);

@@ -145,3 +145,17 @@ def test_outputs_whose_rows_lie_on_one_another_are_refused():
     p.cache.attention(q[:1].expand(2, 3, 4, 64), torch.zeros(2, 3, 4, 64, device="cuda"), i32([5, 6]))
     p.cache.append(k[:1].expand(2, 3, 2, 64), k[:1].expand(2, 3, 2, 64), i32([5, 6]))
     p.cache.status()
+
+
+@pytest.mark.parametrize("tokens,group,dtype", [(20, 16, "bf16"), (20, 16, "f16"), (20, 16, "f32"), (1, 1, "f32"), (5, 1, "bf16")])
+def test_attention_at_the_last_positions(tokens, group, dtype):
+    """Positions up to the largest that a batch may have, the last step of 128 keys reaching past 2^31."""
+    heads, cap = 2, 4096
+    pos = 2 ** 31 - 1 - 32 - tokens
+    end = -(-(pos + tokens) // 16) * 16
+    p = Pair(1, heads, 128, cap, seed=7)
+    q, out = (rand((1, tokens, heads * group, 128), dtype, seed) for seed in (8, 9))
+    for start in (0, end - cap + 64):
+        p.cache.attention(q, out, i32([pos]), start=i32([start]), scale=0.05)
+        p.cache.status()
+        check_attention(p, q, out, out, [pos], [tokens], [0], 0.05, 0, [start])
