@@ -258,8 +258,9 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kern
         }
         amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
-        // the row scaled to a maximum in [2^13, 2^14): the parts of its small elements stay normal in f16
-        const int ex = amax > 0.0f ? (__float_as_int(amax) >> 23) - 127 - 13 : 0;
+        // the row scaled to a maximum in [2^13, 2^14): the parts of its small elements stay normal in f16 (a row
+        // below 2^-113 by 2^126, whose inverse is the least normal number)
+        const int ex = amax > 0.0f ? max((__float_as_int(amax) >> 23) - 127 - 13, -126) : 0;
         const float up = pow2i(-ex);
         q_step = pow2i(ex);
 #pragma unroll

@@ -14,7 +14,7 @@
 //    while this one's are written (staged through shared memory first, a step waited for its copies:
 //    3.4 us a step against 1.3);
 //  - K's and V's codes go to shared memory as whole numbers, exact in f16; the blocks' exponents enter
-//    in the softmax, where they are free: a score is the accumulator times (row step * 2^e_k), the
+//    in the softmax, where they are free: a score is the accumulator times (row step * 2^e_k * scale), the
 //    argument of the exponential takes + e_v, and so the weight is 2^(s + e_v - M) with the running
 //    maximum M of s + e_v: any spread of exponents is held.  The sum of the softmax takes the
 //    weight times 2^(E - e_v), one fused multiply-add in the place of the addition;
@@ -335,9 +335,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
         // the warp's 32 rows of the operand, and the thread's own row
         uint8_t* mine = sm.q[q] + quarter * 4 * (D / 8) * 128;
         uint8_t* own = mine + (lane >> 3) * (D / 8) * 128 + (lane & 7) * 16;
-        float q_step;
+        float q_step, q_scale;  // scores = accumulator * (q_step * 2^e_k) * q_scale
         {
-            // the row of q: scaled to a maximum in [2^13, 2^14), which is exact, and with scale's sign
+            // the row of q: scaled to a maximum in [2^13, 2^14), which is exact, and with scale's sign (a row below
+            // 2^-113 by 2^126, whose inverse is the least normal number)
             const uint32_t there = __ballot_sync(0xFFFFFFFFu, live);
             if (lane == 0) mbar_expect_tx(&sm.q_raw[warp], __popc(there) * 2 * D);
             __syncwarp();
@@ -362,9 +363,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                     amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
                 }
             }
-            const int ex = amax > 0.0f ? (__float_as_int(amax) >> 23) - 127 - 13 : 0;
+            const int ex = amax > 0.0f ? max((__float_as_int(amax) >> 23) - 127 - 13, -126) : 0;
             const float up = a.scale == 0.0f ? 0.0f : copysignf(pow2i(-ex), a.scale);
-            q_step = pow2i(ex) * (a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e);
+            q_step = pow2i(ex);
+            q_scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
 #pragma unroll
             for (int e = 0; e < D / 8; ++e) {
                 const uint32_t w[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                 const float4 vs = *reinterpret_cast<const float4*>(&sm.v_exp[j % kExpSlots][u]);
                 const float s[4] = {ks.x, ks.y, ks.z, ks.w}, e[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
-                for (int v = 0; v < 4; ++v) k_step[u + v] = fmaxf(q_step * s[v], 1e-37f), v_exp[u + v] = e[v];
+                for (int v = 0; v < 4; ++v) k_step[u + v] = fmaxf(q_step * s[v] * q_scale, 1e-37f), v_exp[u + v] = e[v];
             }
             const int p0 = (kb0 + j * kStepBlocks) * kKv8Block;
             const bool masked = p0 < all_lo || p0 > all_hi - (kTile - 1);  // (p0 + kTile can pass 2^31)

@@ -159,3 +159,18 @@ def test_attention_at_the_last_positions(tokens, group, dtype):
         p.cache.attention(q, out, i32([pos]), start=i32([start]), scale=0.05)
         p.cache.status()
         check_attention(p, q, out, out, [pos], [tokens], [0], 0.05, 0, [start])
+
+
+@pytest.mark.parametrize("tokens,group,dtype", [(1, 1, "f32"), (3, 2, "f32"), (20, 16, "bf16")])
+def test_attention_of_queries_near_the_least_normal_values(tokens, group, dtype):
+    """Keys near the largest values: the scores are ordinary numbers."""
+    import torch
+    p = Pair(1, 2, 128, 4096, seed=10)
+    raw = p.mem.cpu().numpy()
+    raw[2 * p.a:2 * p.a + p.b] = 114
+    p.mem.copy_(torch.from_numpy(raw))
+    p.k, p.v = p.halves(raw)
+    q, out = rand((1, tokens, 2 * group, 128), dtype, 11, 1e-36), rand((1, tokens, 2 * group, 128), dtype, 12)
+    p.cache.attention(q, out, i32([3700]), scale=0.25)
+    p.cache.status()
+    check_attention(p, q, out, out, [3700], [tokens], [0], 0.25)
