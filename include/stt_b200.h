@@ -354,7 +354,7 @@ int stt_kv8_read_device(const stt_kv8_cache* cache, const stt_kv8_batch* batch, 
  *   once d_pos[i] + d_count[i] - 1 is written;
  * out = softmax(scale * q . k) v over them, 0 where there is none.  n_heads (of q and out) is a multiple
  * of n_kv_heads; query head j reads K/V head j / (n_heads / n_kv_heads).  Sums and the softmax are f32,
- * the output is rounded once (where q and out both have 16 bits, the weights may be rounded to f16
+ * the output is rounded once (where q has 16 bits and out is bf16, the weights may be rounded to f16
  * first).  q and out are of any dtype each.  A sequence may come in several rows. */
 int stt_kv8_attention_device(stt_kv8_cache* cache, const stt_kv8_batch* batch, const stt_kv8_tensor* q, int n_heads,
                              const int32_t* d_start, int window, float scale, const stt_kv8_tensor* out,

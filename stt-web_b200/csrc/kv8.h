@@ -73,7 +73,7 @@ struct PromptPlan {
     int cluster;  // CTAs that share a row block's keys
     double us;    // the time that a model gives it
 };
-PromptPlan kv8_prompt_plan(int64_t rows, int64_t items, int64_t blocks, const Kv8Machine& m);
+PromptPlan kv8_prompt_plan(int64_t rows, int64_t items, int64_t blocks, int out_dtype, const Kv8Machine& m);
 cudaError_t launch_kv8_prompt(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, int cluster, cudaStream_t st);
 cudaError_t kv8_configure_prompt(Kv8Machine* m);
 cudaError_t launch_kv8_attention(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, const Kv8Machine& m,

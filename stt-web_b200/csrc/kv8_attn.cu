@@ -694,7 +694,7 @@ cudaError_t launch_kv8_attention(const Kv8Dev& c, const Kv8Batch& b, const Kv8At
     const Cut cut = narrow ? cut_items(items, blocks, Shape<true>::kCtas * m.num_sms, max_run)
                            : cut_items(items * row_groups<false>(rows), blocks, Shape<false>::kCtas * m.num_sms, max_run);
     if (rows > kKv8Rows && a.q_dtype != DT_F32 && a.out_dtype != DT_F32) {
-        const PromptPlan plan = kv8_prompt_plan(rows, items, blocks, m);
+        const PromptPlan plan = kv8_prompt_plan(rows, items, blocks, a.out_dtype, m);
         if (plan.us < cut.us) return launch_kv8_prompt(c, b, a, plan.cluster, st);
     }
     if (narrow) return c.dim == 128 ? attend_t<128, true>(c, b, a, cut, st) : attend_t<64, true>(c, b, a, cut, st);

@@ -18,8 +18,11 @@
 //    argument of the exponential takes + e_v, and so the weight is 2^(s + e_v - M) with the running
 //    maximum M of s + e_v: any spread of exponents is held.  The sum of the softmax takes the
 //    weight times 2^(E - e_v), one fused multiply-add in the place of the addition;
-//  - q is exact in f16 once its row is scaled by a power of two; weights are rounded to f16, scaled by
-//    2^6 (2^-12 of each, the outputs being 16-bit themselves);
+//  - q is exact in f16 once its row is scaled by a power of two.  Weights, scaled by 2^6, are rounded to f16
+//    for bf16 outputs: 2^-12 of each against the output's own 2^-9 (its error grows by 1%).  For f16 outputs
+//    that would be half of their own 2^-11 (errors up to 25% above those of the rounding alone), so there P
+//    has two f16 parts, the rest behind the first in what the scores leave free of their 128 columns, and
+//    O += P V two products: 22 bits, for 20% more time;
 //  - M moves only when a score exceeds it by 8 (weights then reach 2^14, inside f16), so that O, which
 //    lives in TMEM, is rescaled a few times per row instead of at every tile.
 // Both operands of a product lie in core matrices of 8 rows x 16 bytes: a key's 8 dimensions are one
@@ -27,7 +30,8 @@
 // Where there are fewer row blocks than SMs, a cluster of CTAs takes the steps of a row block in equal
 // runs; at the end each sends O, M and l of every row to the shared memory of the CTA that joins that row
 // in its share.
-// Measured: the last 1024 of 4096 positions, 4 sequences x 16 heads of 128, 145 us, 0.83 PFLOP/s; a step of
+// Measured: the last 1024 of 4096 positions, 4 sequences x 16 heads of 128, 149 us with bf16 outputs, 0.81
+// PFLOP/s, and 179 us with f16 ones; a step of
 // two tiles takes 2.1 us (its products 1.1 us, its exponentials as long on the other units; a tile's softmax
 // waits 0.7 us a step for its products), a CTA 6 to 11 us besides (its rows in and out, the first step's
 // latency).  Halves of 64 keys with scores and weights in alternating buffers hide that wait, but products of
@@ -125,8 +129,8 @@ __device__ __forceinline__ uint4 pack8(const float* o, float f, int dtype) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// CTA (row block from the last to the first, batch row, head, rank in the cluster).
-template <int D, int DT>
+// CTA (row block from the last to the first, batch row, head, rank in the cluster).  FINE: weights in two f16 parts.
+template <int D, int DT, bool FINE>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch b, Kv8Attention a, int row_blocks, int cluster) {
     extern __shared__ __align__(128) uint8_t prompt_smem[];
     PromptSmem<D>& sm = *reinterpret_cast<PromptSmem<D>*>(prompt_smem);
@@ -273,10 +277,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
             };
             auto pv = [&](int q, int st, int half, bool add) {
                 const uint32_t va = smem_u32(sm.v[st]);
-    #pragma unroll
-                for (int k = half * (kTile / 32); k < (half + 1) * (kTile / 32); ++k)
-                    mma_f16_ts(tmem + kOCol + q * kTile, tmem + q * kTile + k * 8, smem_desc(va + k * 2 * GROUP, GROUP, 128), pv_desc,
-                               add || k > 0);
+#pragma unroll
+                for (int part = 0; part < (FINE ? 2 : 1); ++part)
+#pragma unroll
+                    for (int k = half * (kTile / 32); k < (half + 1) * (kTile / 32); ++k)
+                        mma_f16_ts(tmem + kOCol + q * kTile, tmem + q * kTile + part * (kTile / 2) + k * 8,
+                                   smem_desc(va + k * 2 * GROUP, GROUP, 128), pv_desc, add || part > 0 || k > 0);
             };
             bool ok = true;  // (without a step too, `done` says that nothing writes the operands any more)
             for (int q = 0; ok && q < tiles; ++q) ok = mbar_wait(&sm.q_full[q], 0, abort);
@@ -444,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
             float part[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int u = 0; u < kStepBlocks; u += 2) {
-                uint32_t w[16];
+                uint32_t w[16], rest[16];
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
                     const float step = k_step[u + v];
@@ -458,10 +464,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv8Dev c, Kv8Batch 
                         const float2 z = make_float2(exp2_approx(y.x), exp2_approx(y.y));
                         s = add2(s, z);
                         w[8 * v + e / 2] = pack_f16(z.x, z.y);
+                        if constexpr (FINE) {
+                            const float2 first = unpack2(w[8 * v + e / 2], Elem<DT_F16>());
+                            rest[8 * v + e / 2] = pack_f16(z.x - first.x, z.y - first.y);
+                        }
                     }
                     part[v] = fmaf(s.x + s.y, sm.to_sum[j % kExpSlots][u + v], part[v]);
                 }
                 tmem_st(s_col + 8 * u, w);  // over scores, all of which this thread has read
+                if constexpr (FINE) tmem_st(s_col + kTile / 2 + 8 * u, rest);
                 if (u == kStepBlocks / 2 - 2) {
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -583,22 +594,23 @@ cudaLaunchConfig_t prompt_config(int64_t ctas, int cluster, size_t smem, cudaStr
     return cfg;
 }
 
-template <int D, int DT>
+template <int D, int DT, bool FINE>
 cudaError_t prompt_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, int cluster, cudaStream_t st) {
     const int row_blocks = (int)(((int64_t)b.tokens * a.group + 2 * kTile - 1) / (2 * kTile));
     cudaLaunchAttribute attr[1];
     const cudaLaunchConfig_t cfg =
         prompt_config((int64_t)b.n * c.heads * row_blocks * cluster, cluster, prompt_smem_bytes<D>(), st, attr);
-    return cudaLaunchKernelEx(&cfg, prompt_kernel<D, DT>, c, b, a, row_blocks, cluster);
+    return cudaLaunchKernelEx(&cfg, prompt_kernel<D, DT, FINE>, c, b, a, row_blocks, cluster);
 }
 
 template <int D>
 cudaError_t configure_t() {
-    cudaError_t e = cudaFuncSetAttribute(prompt_kernel<D, DT_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)prompt_smem_bytes<D>());
-    if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(prompt_kernel<D, DT_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)prompt_smem_bytes<D>());
+    for (const auto kernel : {prompt_kernel<D, DT_BF16, false>, prompt_kernel<D, DT_F16, false>, prompt_kernel<D, DT_BF16, true>,
+                              prompt_kernel<D, DT_F16, true>}) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem_bytes<D>());
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace
@@ -611,35 +623,41 @@ cudaError_t kv8_configure_prompt(Kv8Machine* m) {
         cudaLaunchAttribute attr[1];
         const cudaLaunchConfig_t cfg = prompt_config(m->num_sms << j, 1 << j, prompt_smem_bytes<128>(), 0, attr);
         int clusters = 0;
-        const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, prompt_kernel<128, DT_BF16>, &cfg);
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, prompt_kernel<128, DT_BF16, false>, &cfg);
         if (e != cudaSuccess) return e;
         m->prompt_ctas[j] = std::min(clusters << j, m->num_sms);
     }
     return cudaSuccess;
 }
 
-PromptPlan kv8_prompt_plan(int64_t rows, int64_t items, int64_t blocks, const Kv8Machine& m) {
+PromptPlan kv8_prompt_plan(int64_t rows, int64_t items, int64_t blocks, int out_dtype, const Kv8Machine& m) {
     // fitted to 16 .. 1024 tokens over 256 .. 30,000 positions: a CTA takes 6 us besides its steps, a step
-    // 2.1 us with two tiles and 1.9 us with one, a cluster 2 us more.  The other kernel's time comes from a
+    // 2.1 us with two tiles and 1.9 us with one (2.6 and 2.35 with weights in two parts), a cluster 2 us more.  The other kernel's time comes from a
     // model of the same calls: 64 tokens over 256 positions of 4 heads take 7.2 us there and 11 us here, 256
     // over 4096 of 16 heads 117 us there and 34 us here
     const int64_t ctas = items * ((rows + 2 * kTile - 1) / (2 * kTile)), steps = (blocks + kStepBlocks - 1) / kStepBlocks;
+    const double step = rows > kTile ? (out_dtype == DT_F16 ? 2.6 : 2.1) : (out_dtype == DT_F16 ? 2.35 : 1.9);
     PromptPlan best{1, 1e30};
     for (int j = 0; j < 4 && (1 << j) <= steps; ++j) {
         const int cluster = 1 << j;
         if (m.prompt_ctas[j] < cluster) break;
         const double waves = (double)((ctas * cluster + m.prompt_ctas[j] - 1) / m.prompt_ctas[j]);
-        const double us = waves * (6.0 + (rows > kTile ? 2.1 : 1.9) * (double)((steps + cluster - 1) / cluster)) +
+        const double us = waves * (6.0 + step * (double)((steps + cluster - 1) / cluster)) +
                           (cluster > 1 ? 2.0 : 0.0);
         if (us < best.us) best = PromptPlan{cluster, us};
     }
     return best;
 }
 
+template <int D, int DT>
+cudaError_t prompt_fine(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, int cluster, cudaStream_t st) {
+    return a.out_dtype == DT_F16 ? prompt_t<D, DT, true>(c, b, a, cluster, st) : prompt_t<D, DT, false>(c, b, a, cluster, st);
+}
+
 cudaError_t launch_kv8_prompt(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, int cluster, cudaStream_t st) {
     if (c.dim == 128)
-        return a.q_dtype == DT_BF16 ? prompt_t<128, DT_BF16>(c, b, a, cluster, st) : prompt_t<128, DT_F16>(c, b, a, cluster, st);
-    return a.q_dtype == DT_BF16 ? prompt_t<64, DT_BF16>(c, b, a, cluster, st) : prompt_t<64, DT_F16>(c, b, a, cluster, st);
+        return a.q_dtype == DT_BF16 ? prompt_fine<128, DT_BF16>(c, b, a, cluster, st) : prompt_fine<128, DT_F16>(c, b, a, cluster, st);
+    return a.q_dtype == DT_BF16 ? prompt_fine<64, DT_BF16>(c, b, a, cluster, st) : prompt_fine<64, DT_F16>(c, b, a, cluster, st);
 }
 
 }  // namespace stt

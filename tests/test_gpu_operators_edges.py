@@ -174,3 +174,25 @@ def test_attention_of_queries_near_the_least_normal_values(tokens, group, dtype)
     p.cache.attention(q, out, i32([3700]), scale=0.25)
     p.cache.status()
     check_attention(p, q, out, out, [3700], [tokens], [0], 0.25)
+
+
+@pytest.mark.parametrize("dim,tokens,window,spread", [(128, 20, 0, 1.0), (128, 20, 0, 12.0), (64, 24, 0, 4.0), (128, 30, 3000, 4.0), (128, 3, 0, 4.0)])
+@pytest.mark.parametrize("qt", ["f16", "bf16"])
+def test_f16_chunks_are_as_near_as_their_rounding_allows(dim, tokens, window, spread, qt):
+    """An f16 output holds 11 bits and is rounded once: the result may be no further from the 64-bit values than those
+    rounded to f16 are, but for sums in f32 and weights in two f16 parts.  These are off by e <= 2^-17 of a value here
+    (18 S 2^-23 of it and less, S under 100), independent of the rounding of up to 2^-11, in the mean over an output
+    2^-11 / sqrt(3) * about 0.7: together sqrt(1 + (2^-17 / 2^-12.3)^2) < 1.001 times the rounding alone."""
+    import torch
+    heads, group, pos = 2, 16, 3700
+    p = Pair(1, heads, dim, 4096, seed=13)
+    q = rand((1, tokens, heads * group, dim), qt, 14, spread)
+    out = torch.zeros(1, tokens, heads * group, dim, dtype=torch.float16, device="cuda")
+    scale = dim ** -0.5
+    p.cache.attention(q, out, i32([pos]), window=window, scale=scale)
+    p.cache.status()
+    exact, _ = R.attention(p.k, p.v, 0, pos, q[0].double().cpu().numpy(), scale, window)
+    least = np.linalg.norm(exact.astype(np.float16).astype(np.float64) - exact)
+    off = np.linalg.norm(out[0].double().cpu().numpy() - exact)
+    print("error", off, "rounding alone", least)
+    assert off <= 1.001 * least
