@@ -214,9 +214,13 @@ int stt_streams_set_product_precision(stt_streams* streams, int precision);
  * score + log_softmax(logits), and the streams are reordered so that stream ids[g * beams + b] carries the
  * b-th best, with the chosen token as its last text token and its frame count advanced.  scores
  * (groups * beams floats, in and out), parents_out and tokens_out are host arrays, best first.  Begin an
- * utterance with reset streams and scores 0, -inf, -inf, ...: its beams start alike.  Tokens of frames
+ * utterance with reset streams and scores 0, -inf, -inf, ... (not NaN or +inf): its beams start alike.  Tokens of frames
  * inside the text delay (frame_count of stt_stream_get_state below text_delay) count for the scores but
- * are not part of the transcript. */
+ * are not part of the transcript.
+ * STT_E_DEVICE_FLAG comes in two forms.  A NaN or +inf among a beam's logits: the frame is done all the same,
+ * that beam's candidates counted as -inf, and the outputs are written.  An error of the frame's own step
+ * (stt_last_error names it): nothing is chosen, the outputs and scores are left as they were, and every stream
+ * keeps its place, with the frame in its ring as after an stt_forward that failed; reset the streams. */
 int stt_streams_reorder(stt_streams* streams, const int32_t* ids, int groups, int beams, const int32_t* parents);
 typedef struct stt_beam stt_beam;
 int stt_streams_beam_frame(stt_streams* streams, stt_beam* beam, const int32_t* ids, int groups, int beams,

@@ -1413,26 +1413,29 @@ int check_beams(stt_streams* s, const int32_t* ids, int groups, int beams) {
     return check_ids(s, ids, groups * beams);
 }
 
-// Device and pinned arrays of a beam call for n streams.
+// Device and pinned arrays of a beam call for n streams, in this order: ids and the error word go up in one
+// copy, the error word, parents and tokens come back in one.
 struct BeamBufs {
-    int32_t *ids, *parents, *tokens, *held;
+    int32_t *ids, *err, *parents, *tokens, *held;
     float* scores;
 };
 int beam_bufs(stt_streams* s, int n, BeamBufs* d, BeamBufs* h) {
-    TRY(s->beam_dev.ensure((size_t)5 * n * 4));
-    TRY(s->h_beam.ensure((size_t)5 * n * 4));
+    const size_t bytes = ((size_t)5 * n + 1) * 4;
+    TRY(s->beam_dev.ensure(bytes));
+    TRY(s->h_beam.ensure(bytes));
     for (int i = 0; i < 2; ++i) {
         int32_t* p = static_cast<int32_t*>(i ? s->h_beam.p : s->beam_dev.p);
-        *(i ? h : d) = BeamBufs{p, p + n, p + 2 * n, p + 3 * n, reinterpret_cast<float*>(p + 4 * n)};
+        *(i ? h : d) = BeamBufs{p, p + n, p + n + 1, p + 2 * n + 1, p + 3 * n + 1, reinterpret_cast<float*>(p + 4 * n + 1)};
     }
+    *h->err = 0;
     return STT_OK;
 }
 
 // Queues the reordering of the streams' states and rings by d.parents; with tokens, as a beam step's end.
 int queue_reorder(stt_streams* s, int groups, int beams, const BeamBufs& d, bool step) {
     const stt_model* m = s->m;
-    CUDA_TRY(launch_beam_states(s->d_state, d.ids, groups, beams, d.parents, step ? d.tokens : nullptr, s->kv8_cap != 0, d.held,
-                                s->stream));
+    CUDA_TRY(launch_beam_states(s->d_state, d.ids, groups, beams, d.parents, step ? d.tokens : nullptr, step ? s->d_desc : nullptr,
+                                s->kv8_cap != 0, d.held, s->stream));
     ReorderArgs a{};
     a.groups = groups;
     a.beams = beams;
@@ -1493,7 +1496,7 @@ extern "C" int stt_streams_reorder(stt_streams* s, const int32_t* ids, int group
     TRY(beam_bufs(s, n, &d, &h));
     std::memcpy(h.ids, ids, sizeof(int32_t) * n);
     std::memcpy(h.parents, parents, sizeof(int32_t) * n);
-    CUDA_TRY(cudaMemcpyAsync(d.ids, h.ids, sizeof(int32_t) * 2 * n, cudaMemcpyHostToDevice, s->stream));
+    CUDA_TRY(cudaMemcpyAsync(d.ids, h.ids, sizeof(int32_t) * (2 * n + 1), cudaMemcpyHostToDevice, s->stream));
     TRY(queue_reorder(s, groups, beams, d, false));
     CUDA_TRY(cudaStreamSynchronize(s->stream));
     move_offsets(s, ids, groups, beams, parents);
@@ -1515,6 +1518,8 @@ extern "C" int stt_streams_beam_frame(stt_streams* s, stt_beam* beam, const int3
     if (m->V > m->TV)
         return set_error(STT_E_STATE, "a chosen token can be outside the %d text embeddings (%d outputs)", m->TV, m->V);
     const int n = groups * beams, nc = m->NC;
+    for (int i = 0; i < n; ++i)
+        if (!(scores[i] < INFINITY)) return set_error(STT_E_INVALID_ARG, "score %g (index %d) is NaN or +inf", scores[i], i);
     DeviceScope ds(m->device);
     TRY(check_tokens(m, audio, (size_t)groups * nc, nullptr, 0));
     TRY(check_positions(s, ids, n, 1));
@@ -1530,27 +1535,30 @@ extern "C" int stt_streams_beam_frame(stt_streams* s, stt_beam* beam, const int3
     std::memcpy(h.ids, ids, sizeof(int32_t) * n);
     std::memcpy(h.scores, scores, sizeof(float) * n);
     CUDA_TRY(cudaMemcpyAsync(s->in_audio.p, rep, (size_t)n * nc * 4, cudaMemcpyHostToDevice, s->stream));
-    CUDA_TRY(cudaMemcpyAsync(d.ids, h.ids, sizeof(int32_t) * n, cudaMemcpyHostToDevice, s->stream));
+    CUDA_TRY(cudaMemcpyAsync(d.ids, h.ids, sizeof(int32_t) * (n + 1), cudaMemcpyHostToDevice, s->stream));
     CUDA_TRY(cudaMemcpyAsync(d.scores, h.scores, sizeof(float) * n, cudaMemcpyHostToDevice, s->stream));
     float* logits = static_cast<float*>(s->out_logits.p);
     TRY(run_steps(s, ids, n, 1, static_cast<uint32_t*>(s->in_audio.p), nullptr, static_cast<int32_t*>(s->out_tokens.p), logits, 0,
                   s->stream));
     const stt_beam_step step{logits, m->V, DT_F32, groups, beams, m->V, d.scores, nullptr, d.scores, d.parents, d.tokens, nullptr, -1, 0};
-    TRY(stt_beam_select_device(beam, &step, s->stream));
+    TRY(beam_select(beam, &step, d.err, s->stream));
     TRY(queue_reorder(s, groups, beams, d, true));
-    CUDA_TRY(cudaMemcpyAsync(h.parents, d.parents, sizeof(int32_t) * 2 * n, cudaMemcpyDeviceToHost, s->stream));
+    CUDA_TRY(cudaMemcpyAsync(h.err, d.err, sizeof(int32_t) * (2 * n + 1), cudaMemcpyDeviceToHost, s->stream));
     CUDA_TRY(cudaMemcpyAsync(h.scores, d.scores, sizeof(float) * n, cudaMemcpyDeviceToHost, s->stream));
     TRY(s->h_stage.ensure(sizeof(StepDesc)));
     StepDesc* desc = static_cast<StepDesc*>(s->h_stage.p);
     CUDA_TRY(cudaMemcpyAsync(desc, s->d_desc, sizeof(StepDesc), cudaMemcpyDeviceToHost, s->stream));
     CUDA_TRY(cudaStreamSynchronize(s->stream));
     move_offsets(s, ids, groups, beams, h.parents);
-    if (desc->error != 0)
+    if (desc->error != 0)  // (nothing was moved: the parents that came back are every beam's own)
         return set_error(desc->error == STT_E_INVALID_ARG ? STT_E_INVALID_ARG : STT_E_DEVICE_FLAG,
-                         "a kernel raised error %d", desc->error);
+                         "a kernel of the frame's step raised error %d: the streams keep their order", desc->error);
     std::memcpy(parents_out, h.parents, sizeof(int32_t) * n);
     std::memcpy(tokens_out, h.tokens, sizeof(int32_t) * n);
     std::memcpy(scores, h.scores, sizeof(float) * n);
+    if (*h.err != 0)
+        return set_error(STT_E_DEVICE_FLAG, "the frame is done, but a beam had a NaN or +inf among its logits (its candidates were "
+                                            "taken as -inf), or a wait for logits ran out");
     return STT_OK;
 }
 

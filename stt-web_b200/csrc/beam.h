@@ -56,6 +56,8 @@ struct ReorderArgs {
 // The selector's device, and whether it was made for such a call.
 int beam_device(const stt_beam* beam);
 bool beam_fits(const stt_beam* beam, int batch, int beams, int vocab);
+// stt_beam_select_device that raises `err` (a device word; NULL: the selector's own).
+int beam_select(stt_beam* beam, const stt_beam_step* step, int32_t* err, cudaStream_t st);
 cudaError_t launch_beam_select(const BeamArgs& a, int dtype, cudaStream_t st);
 cudaError_t launch_reorder(const ReorderArgs& a, cudaStream_t st);
 

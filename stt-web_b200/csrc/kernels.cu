@@ -1200,9 +1200,13 @@ cudaError_t launch_positions(const Ctx& c, int32_t* pos, cudaStream_t st) {
 }
 
 // One CTA per group: all of its beams' states are read before any is written.
-static __global__ void beam_states_kernel(StreamState* state, const int32_t* ids, int beams, const int32_t* parents,
-                                          const int32_t* tokens, int whole, int32_t* held) {
+static __global__ void beam_states_kernel(StreamState* state, const int32_t* ids, int beams, int32_t* parents,
+                                          const int32_t* tokens, const StepDesc* step, int whole, int32_t* held) {
     const int r0 = blockIdx.x * beams, b = threadIdx.x;
+    if (step && step->error != 0) {  // the step's logits mean nothing: every stream stays what it is
+        if (b < beams) parents[r0 + b] = b, held[r0 + b] = 0;
+        return;
+    }
     StreamState st{};
     if (b < beams) st = state[ids[r0 + parents[r0 + b]]];
     __syncthreads();
@@ -1215,9 +1219,9 @@ static __global__ void beam_states_kernel(StreamState* state, const int32_t* ids
     state[ids[r0 + b]] = st;
 }
 
-cudaError_t launch_beam_states(StreamState* state, const int32_t* ids, int groups, int beams, const int32_t* parents,
-                               const int32_t* tokens, int whole, int32_t* held, cudaStream_t st) {
-    beam_states_kernel<<<groups, 32, 0, st>>>(state, ids, beams, parents, tokens, whole, held);
+cudaError_t launch_beam_states(StreamState* state, const int32_t* ids, int groups, int beams, int32_t* parents,
+                               const int32_t* tokens, const StepDesc* step, int whole, int32_t* held, cudaStream_t st) {
+    beam_states_kernel<<<groups, 32, 0, st>>>(state, ids, beams, parents, tokens, step, whole, held);
     return cudaGetLastError();
 }
 

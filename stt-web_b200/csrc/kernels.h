@@ -70,9 +70,10 @@ cudaError_t launch_finish(const Ctx& c, cudaStream_t st);
 cudaError_t launch_positions(const Ctx& c, int32_t* pos, cudaStream_t st);
 // Stream states of a beam step: stream ids[g * beams + b] takes the state of stream
 // ids[g * beams + parents[g * beams + b]]; with tokens, its last text token becomes tokens[..] and its frame
-// count advances.  held[..] receives what its new K/V ring holds: `whole` ? positions : valid slots.
-cudaError_t launch_beam_states(StreamState* state, const int32_t* ids, int groups, int beams, const int32_t* parents,
-                               const int32_t* tokens, int whole, int32_t* held, cudaStream_t st);
+// count advances.  held[..] receives what its new K/V ring holds: `whole` ? positions : valid slots.  With a
+// step whose error word is set nothing moves, and parents become every beam's own number.
+cudaError_t launch_beam_states(StreamState* state, const int32_t* ids, int groups, int beams, int32_t* parents,
+                               const int32_t* tokens, const StepDesc* step, int whole, int32_t* held, cudaStream_t st);
 // Adds the K-slice partial sums part[slices][rows][a.W.n] of a tensor-core product in slice order
 // and applies the epilogue `epi` as launch_gemv does.
 cudaError_t launch_tc_epilogue(const Ctx& c, const GemvArgs& a, int epi, int rows, const float* part, int slices,

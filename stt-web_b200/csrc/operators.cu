@@ -385,6 +385,10 @@ extern "C" int stt_beam_status(stt_beam* h) {
 
 extern "C" int stt_beam_select_device(stt_beam* h, const stt_beam_step* s, void* cuda_stream) {
     clear_error();
+    return beam_select(h, s, nullptr, static_cast<cudaStream_t>(cuda_stream));
+}
+
+int stt::beam_select(stt_beam* h, const stt_beam_step* s, int32_t* err, cudaStream_t st) {
     if (!h || !s || s->batch < 0) return set_error(STT_E_INVALID_ARG, "bad arguments");
     if (s->batch > 0 && (!s->d_logits || !s->d_scores || !s->d_next_scores || !s->d_parents || !s->d_tokens))
         return set_error(STT_E_INVALID_ARG, "NULL array");
@@ -419,9 +423,10 @@ extern "C" int stt_beam_select_device(stt_beam* h, const stt_beam_step* s, void*
     a.parents = s->d_parents;
     a.tokens = s->d_tokens;
     a.next_done = s->d_next_done;
+    if (err) a.err = err;
     DeviceScope ds(h->device);
     if (!ds.ok) return set_error(STT_E_CUDA, "cudaSetDevice(%d) failed", h->device);
-    CUDA_TRY(launch_beam_select(a, s->dtype, static_cast<cudaStream_t>(cuda_stream)));
+    CUDA_TRY(launch_beam_select(a, s->dtype, st));
     return STT_OK;
 }
 

@@ -182,17 +182,22 @@ class LayerCaches:
     def beam_frame(self, beam: "BeamSelector", stream_ids, audio, scores):
         """One frame of beam search: stream_ids [groups, beams], audio [groups, num_codebooks], scores
         [groups, beams].  Returns (scores, parents, tokens), each [groups, beams], best first; the
-        streams then carry the beams in that order."""
+        streams then carry the beams in that order.  An SttError of the device carries the same triple as
+        ``frame``: a frame done in spite of NaN logits, or (tokens -1) streams left in their order."""
         ids = np.ascontiguousarray(np.asarray(stream_ids, dtype=np.int32))
         sc = np.array(scores, dtype=np.float32, order="C")
         a = _u32(audio)
         if ids.ndim != 2 or sc.shape != ids.shape or a.size != ids.shape[0] * self.model.info.num_codebooks:
             raise SttError(-1, "stt_streams_beam_frame",
                            "stream_ids and scores must be [groups, beams], audio [groups, num_codebooks]")
-        par, tok = np.empty_like(ids), np.empty_like(ids)
-        check(lib().stt_streams_beam_frame(self._h, beam._h, _ptr(ids, C.c_int32), ids.shape[0], ids.shape[1],
-                                           _ptr(a, C.c_uint32), _ptr(sc, C.c_float), _ptr(par, C.c_int32),
-                                           _ptr(tok, C.c_int32)), "stt_streams_beam_frame")
+        par, tok = np.empty_like(ids), np.full_like(ids, -1)
+        par[:] = np.arange(ids.shape[1])
+        code = lib().stt_streams_beam_frame(self._h, beam._h, _ptr(ids, C.c_int32), ids.shape[0], ids.shape[1],
+                                            _ptr(a, C.c_uint32), _ptr(sc, C.c_float), _ptr(par, C.c_int32), _ptr(tok, C.c_int32))
+        if code:
+            e = SttError(code, "stt_streams_beam_frame")
+            e.frame = (sc, par, tok)
+            raise e
         return sc, par, tok
 
     def state(self, stream_id: int) -> dict:
