@@ -343,7 +343,8 @@ int stt_kv8_cache_status(stt_kv8_cache* cache);
  * block's own where that is larger and the block holds earlier positions; those move along when the
  * exponent grows.  Codes are rounded to nearest, ties to even.  Token by token or many at once, a value
  * ends up within one step 2^e of what was appended (half a step where its block's exponent did not grow
- * afterwards).  Sequences of one call are distinct, but for rows of count 0 (the padding of a batch). */
+ * afterwards).  Sequences of one call are distinct, but for rows of count 0 (the padding of a batch).  A row's
+ * positions lie in at most capacity / 16 blocks, or it is out of range. */
 int stt_kv8_append_device(stt_kv8_cache* cache, const stt_kv8_batch* batch, const stt_kv8_tensor* k,
                           const stt_kv8_tensor* v, void* cuda_stream);
 /* The way back: the values of positions d_pos[i] .. d_pos[i] + d_count[i] - 1 (which the ring must

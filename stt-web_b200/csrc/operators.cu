@@ -207,7 +207,7 @@ extern "C" int stt_kv8_append_device(stt_kv8_cache* h, const stt_kv8_batch* b, c
     TRY(check_batch(h, b, &some));
     if (!some) return STT_OK;
     TRY(check_kv(k, v));
-    if (b->n_tokens > h->c.cap)
+    if (!b->d_count && b->n_tokens > h->c.cap)  // (counts are the device's to check)
         return set_error(STT_E_INVALID_ARG, "%d tokens in one call exceed the capacity %d", b->n_tokens, h->c.cap);
     if ((int64_t)b->n * (b->n_tokens / kKv8Block + 2) > INT_MAX / (h->c.heads + 8))
         return set_error(STT_E_INVALID_ARG, "%d rows of %d tokens are too many for one call", b->n, b->n_tokens);

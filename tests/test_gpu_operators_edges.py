@@ -196,3 +196,21 @@ def test_f16_chunks_are_as_near_as_their_rounding_allows(dim, tokens, window, sp
     off = np.linalg.norm(out[0].double().cpu().numpy() - exact)
     print("error", off, "rounding alone", least)
     assert off <= 1.001 * least
+
+
+def test_append_takes_a_batch_padded_beyond_the_capacity():
+    p = Pair(3, 2, 64, 32)
+    x = rand((3, 50, 2, 64), "bf16", 50)
+    p.cache.append(x, x, i32([5, 16, 0]), count=i32([20, 32, 0]))
+    p.append(x, x, [5, 16, 0], [20, 32, 0], [0, 1, 2])
+    p.same()
+    p.cache.status()
+    with pytest.raises(SttError) as e:
+        p.cache.append(x, x, i32([0, 0, 0]))
+    assert e.value.code == STT_E_INVALID_ARG and "capacity" in str(e.value)
+    p.cache.append(x, x, i32([0, 3, 0]), count=i32([33, 32, 1]))  # two rows that the ring does not hold
+    p.append(x, x, [0, 0, 0], [0, 0, 1], [0, 1, 2])
+    p.same()
+    with pytest.raises(SttError) as e:
+        p.cache.status()
+    assert e.value.code == STT_E_INVALID_ARG
