@@ -360,7 +360,11 @@ int stt_kv8_read_device(const stt_kv8_cache* cache, const stt_kv8_batch* batch, 
  * out = softmax(scale * q . k) v over them, 0 where there is none.  n_heads (of q and out) is a multiple
  * of n_kv_heads; query head j reads K/V head j / (n_heads / n_kv_heads).  Sums and the softmax are f32,
  * the output is rounded once (where q has 16 bits and out is bf16, the weights may be rounded to f16
- * first).  q and out are of any dtype each.  A sequence may come in several rows. */
+ * first).  q and out are of any dtype each.  A sequence may come in several rows.
+ * Ranges: scale * q . k within f32's, V's exponents (those of blocks of zeros, -100, among them) within 110
+ * of one another, beyond which a key can be lost from the softmax's sum.  What a key adds to an output is
+ * exact to about 2^-30 of the row's largest |weight| * 127 * 2^exponent, also in dimensions where all v are
+ * small. */
 int stt_kv8_attention_device(stt_kv8_cache* cache, const stt_kv8_batch* batch, const stt_kv8_tensor* q, int n_heads,
                              const int32_t* d_start, int window, float scale, const stt_kv8_tensor* out,
                              void* cuda_stream);

@@ -7,6 +7,9 @@
 //   w_p = 2^(s_p + e_v(p) - M),   O = sum w_p * code_p,   l = sum w_p * 2^-e_v(p),   out = O / l,
 // with M the running maximum of s_p + e_v(p).  One pass over the codes keeps (M, l, O) per row.  M moves
 // only when it falls more than 8 behind, so that O is rescaled a few times per row.
+// What this holds: w is two f16 parts, scaled by 2^7, so a key's share of O is lost where s_p + e_v(p) is 2^32
+// below the row's largest; l is f32, and a key's share of it is lost where s_p + e_v(p) is 2^133 below: as
+// long as V's exponents lie within 110 of one another, only keys with less than 2^-23 of the largest share are.
 //
 // What bounds it: a decode step reads 2 * dim bytes per position and head and does 4 * dim flops per
 // query row with them, so HBM bounds it as long as turning codes into operands costs little.  Hence

@@ -16,8 +16,12 @@
 //  - K's and V's codes go to shared memory as whole numbers, exact in f16; the blocks' exponents enter
 //    in the softmax, where they are free: a score is the accumulator times (row step * 2^e_k * scale), the
 //    argument of the exponential takes + e_v, and so the weight is 2^(s + e_v - M) with the running
-//    maximum M of s + e_v: any spread of exponents is held.  The sum of the softmax takes the
-//    weight times 2^(E - e_v), one fused multiply-add in the place of the addition;
+//    maximum M of s + e_v.  The sum of the softmax takes the weight times 2^(E - e_v), one fused
+//    multiply-add in the place of the addition.  What that holds: in f16 a weight keeps its bits down to
+//    2^-20 of the row's largest and is lost below 2^-31, so a key whose s + e_v is that far below the
+//    others adds nothing to the output, in whichever dimension; and the f32 sum keeps every key whose
+//    share is above 2^-22 of the largest while V's exponents lie within 110 of one another (a weight is
+//    flushed to zero below 2^-126, 2^132 below the row's largest);
 //  - q is exact in f16 once its row is scaled by a power of two.  Weights, scaled by 2^6, are rounded to f16
 //    for bf16 outputs: 2^-12 of each against the output's own 2^-9 (its error grows by 1%).  For f16 outputs
 //    that would be half of their own 2^-11 (errors up to 25% above those of the rounding alone), so there P
@@ -60,7 +64,6 @@ constexpr uint32_t kTmemCols = 512;       // S of both tiles, O of both tiles
 constexpr uint32_t kOCol = 256;
 constexpr int kExpSlots = 4;              // steps whose exponents are kept
 constexpr float kWeightShift = 6.0f;
-constexpr int kMaxPromptCluster = 8;
 constexpr float kLazy = 8.0f;             // how far a score may exceed M
 
 template <int D>

@@ -214,3 +214,27 @@ def test_append_takes_a_batch_padded_beyond_the_capacity():
     with pytest.raises(SttError) as e:
         p.cache.status()
     assert e.value.code == STT_E_INVALID_ARG
+
+
+@pytest.mark.parametrize("tokens,group,dtype", [(1, 1, "f32"), (5, 1, "f32"), (20, 16, "bf16")])
+def test_attention_over_blocks_of_v_110_binades_apart(tokens, group, dtype):
+    """The widest spread that the softmax's sum is promised to hold: blocks of nothing but zeros (exponent -100) beside
+    blocks of values up to 127 * 2^10, the zeros' scores below the others' and above them."""
+    import torch
+    heads = 2
+    for high in (0, 1):
+        p = Pair(1, heads, 128, 4096, seed=15)
+        raw = p.mem.cpu().numpy()
+        codes = raw[p.a:2 * p.a].reshape(heads, 256, 16 * 128)
+        codes[:, ::2] = 0
+        raw[2 * p.a + p.b:] = np.tile(np.array([-100, 10], np.int8), heads * 128)
+        keys = raw[:p.a].reshape(heads, 256, 16, 128)
+        keys[..., 0] = 100
+        keys[:, high::2, :, 0] = 127  # these blocks' scores are the higher ones
+        p.mem.copy_(torch.from_numpy(raw))
+        p.k, p.v = p.halves(raw)
+        q, out = rand((1, tokens, heads * group, 128), dtype, 16, 0.1), rand((1, tokens, heads * group, 128), dtype, 17)
+        q[..., 0] = 10.0
+        p.cache.attention(q, out, i32([3700]), scale=1.0)
+        p.cache.status()
+        check_attention(p, q, out, out, [3700], [tokens], [0], 1.0)
