@@ -238,3 +238,50 @@ def test_attention_over_blocks_of_v_110_binades_apart(tokens, group, dtype):
         p.cache.attention(q, out, i32([3700]), scale=1.0)
         p.cache.status()
         check_attention(p, q, out, out, [3700], [tokens], [0], 1.0)
+
+
+@pytest.mark.parametrize("beams", [1, 2, 4, 8])
+@pytest.mark.parametrize("vocab,dtype", [(65537, "f32"), (65537, "bf16"), (130000, "bf16")])
+def test_select_joins_many_chunks_of_a_row(beams, vocab, dtype):
+    """One utterance's rows in 9 to 32 chunks each: whole chunks masked, chunks with fewer finite logits than beams,
+    beams that ended, and ties across chunks."""
+    import torch
+    inf = float("inf")
+    eos = vocab - 3
+    for case in range(5):
+        logits = rand((beams, vocab), dtype, 20 + case, 3.0)
+        scores = rand((1, beams), "f32", 30 + case, 2.0)
+        done = None
+        if case == 1:    # all but the row's ends
+            logits[:, 1000:vocab - 1000] = -inf
+        elif case == 2:  # a chunk or more with a single finite logit, the others' ones poor
+            logits[:, vocab // 4:vocab // 2] = -inf
+            logits[:, vocab // 3] = 20.0
+            logits[0, vocab // 2:] = -inf
+        elif case == 3:  # fewer finite logits in the whole row than beams
+            logits[:] = -inf
+            logits[0, vocab - 1] = 1.0
+            logits[beams - 1, 5] = 1.0
+        elif case == 4:
+            logits[:] = 0.0
+            logits[:, vocab // 2] = 1.0
+            done = torch.zeros(1, beams, dtype=torch.uint8, device="cuda")
+            done[0, beams // 2] = 1
+        sel, out = run_select(logits, scores, done, eos if case == 4 else -1)
+        check_select(logits, scores, done, eos if case == 4 else -1, out)
+        sel.status()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_select_when_a_chunk_is_masked_behind_a_poor_one(dtype):
+    """32 beams: four chunks a row, one of them masked whole, one with fewer finite logits than beams: their bounds stay at
+    -inf, which more logits reach than a list takes."""
+    inf = float("inf")
+    logits = rand((32, 131064), dtype, 40, 0.001)
+    logits[:, 32768:65536] = -inf
+    logits[:, 65536 + 20:98304] = -inf
+    logits[5] = 0.25   # ties all over a row
+    logits[6, 40000:] = -inf
+    scores = rand((1, 32), "f32", 41, 0.001)
+    _, out = run_select(logits, scores)
+    check_select(logits, scores, None, -1, out)
