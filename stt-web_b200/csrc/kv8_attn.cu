@@ -47,7 +47,6 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kMaxParts = 64;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxRun = 32;     // blocks of a warp where the output is f32, as far as clusters go
 constexpr int kMinBlocks = 4;   // of a warp in a part that is joined through memory
 // Query rows of a CTA, stages of a warp's ring, CTAs per SM.
 template <bool NARROW>
@@ -152,7 +151,8 @@ __device__ __forceinline__ float4 row_output(const RowState& r, float4 o) {
 // CTA (((batch row * groups + row group) * heads + head) * max_parts + part) * cluster + rank.  An
 // item's keys are cut into parts x cluster equal runs of blocks; a cluster joins its runs through shared
 // memory, the last cluster of an item its parts through global memory.
-template <int D, bool NARROW>
+// SUMS: a block's products are added to O by f32 additions, not by the products' own accumulators (attend_sums).
+template <int D, bool NARROW, bool SUMS>
 __global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kernel(Kv8Dev c, Kv8Batch b, Kv8Attention a, int groups,
                                                                 int max_parts, int cluster) {
     constexpr int KS = D / 16;          // k steps of the first product
@@ -412,6 +412,17 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kern
         // V: keys 2t, 2t + 1, 2t + 8, 2t + 9 of dimensions VB * g + 0 .. VB - 1: n tile n takes dimension n
         // of each lane, or (narrow) the 16 rows of tile n dimensions 2n and 2n + 1 of each
         {
+            auto add_product = [](float (&sum)[4], const uint32_t (&A)[4], uint32_t b0, uint32_t b1) {
+                if constexpr (SUMS) {
+                    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma16816(x, A, b0, b1);
+                    const float2 u = add2(make_float2(sum[0], sum[1]), make_float2(x[0], x[1]));
+                    const float2 v = add2(make_float2(sum[2], sum[3]), make_float2(x[2], x[3]));
+                    sum[0] = u.x, sum[1] = u.y, sum[2] = v.x, sum[3] = v.y;
+                } else {
+                    mma16816(sum, A, b0, b1);
+                }
+            };
             uint32_t r[4][VW];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -432,13 +443,13 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<NARROW>::kCtas) attend_kern
                                y2 = codes_to_f16<0x4140>(ce1), y3 = codes_to_f16<0x4342>(ce1);
                 if constexpr (NARROW) {
                     const uint32_t A0[4] = {x0, x1, y0, y1}, A1[4] = {x2, x3, y2, y3};
-                    mma16816(o[2 * w], A0, pa[0], pa[1]);
-                    mma16816(o[2 * w + 1], A1, pa[0], pa[1]);
+                    add_product(o[2 * w], A0, pa[0], pa[1]);
+                    add_product(o[2 * w + 1], A1, pa[0], pa[1]);
                 } else {
-                    mma16816(o[4 * w], pa, x0, y0);
-                    mma16816(o[4 * w + 1], pa, x1, y1);
-                    mma16816(o[4 * w + 2], pa, x2, y2);
-                    mma16816(o[4 * w + 3], pa, x3, y3);
+                    add_product(o[4 * w], pa, x0, y0);
+                    add_product(o[4 * w + 1], pa, x1, y1);
+                    add_product(o[4 * w + 2], pa, x2, y2);
+                    add_product(o[4 * w + 3], pa, x3, y3);
                 }
             }
         }
@@ -615,14 +626,11 @@ constexpr size_t attend_smem() {
 // 3 us besides its blocks, a block of 16 keys takes a warp 0.6 us on an idle SM and 1.5 us on a full
 // one, joining a cluster takes 1 us and joining parts through memory 3 us and a little for each.  (Parts
 // alone, without clusters: 751 positions of 16 heads 11.0 us, with them 7.2 us.)
-// A product's f32 accumulator is truncated, not rounded, at every block: a warp's sums drift by about 1.3e-8
-// of themselves a block (10,000 positions in runs of 156 blocks 2.0e-6, of 20 blocks 3.7e-7), so for f32
-// outputs a warp takes max_run blocks at most where a cluster can be larger.
 struct Cut {
     int parts, cluster;
     double us;
 };
-Cut cut_items(int64_t items, int64_t blocks, int slots, int max_run) {
+Cut cut_items(int64_t items, int64_t blocks, int slots) {
     Cut best{1, 1, 1e30};
     for (int cluster = 1; cluster <= kMaxCluster; cluster *= 2)
         for (int parts = 1; parts <= kMaxParts; parts = parts < 8 ? parts + 1 : parts + parts / 4) {
@@ -630,7 +638,6 @@ Cut cut_items(int64_t items, int64_t blocks, int slots, int max_run) {
             if ((runs > 1 && (runs * kWarps > blocks + kWarps || items * runs > INT_MAX)) || (parts > 1 && (cluster < kMaxCluster / 2 || items * parts > kKv8MaxPartials ||
                                                                          runs * kWarps * kMinBlocks > blocks)))
                 break;
-            if (cluster < kMaxCluster && blocks > runs * kWarps * max_run) continue;
             const double fill = std::min(1.0, (double)(items * runs) / slots);
             const double waves = (double)((items * runs + slots - 1) / slots);
             const double block_us = std::max(0.6, 1.5 * fill);
@@ -647,7 +654,7 @@ int64_t row_groups(int64_t rows) {
     return (rows + Shape<NARROW>::kRows - 1) / Shape<NARROW>::kRows;
 }
 
-template <int D, bool NARROW>
+template <int D, bool NARROW, bool SUMS>
 cudaError_t attend_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, const Cut& cut, cudaStream_t st) {
     const int groups = (int)row_groups<NARROW>((int64_t)b.tokens * a.group);
     const int64_t items = (int64_t)b.n * c.heads * groups;
@@ -662,16 +669,28 @@ cudaError_t attend_t(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, 
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cut.cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, attend_kernel<D, NARROW>, c, b, a, groups, cut.parts, cut.cluster);
+    return cudaLaunchKernelEx(&cfg, attend_kernel<D, NARROW, SUMS>, c, b, a, groups, cut.parts, cut.cluster);
 }
 
-template <int D>
+// A product's f32 accumulator is truncated, not rounded, at every block: a warp's sums drift by about 1.3e-8
+// of themselves a block.  f32 outputs of runs that are longer than 32 blocks for a warp therefore get their own
+// additions (80 x 8 heads over 60,000 positions 3.2e-7 off, without them 2e-6 and more, whose growth has no end),
+// at 3% of the time where HBM does not hide them; shorter runs (512 x 16 heads over 751 positions: 267 us, with
+// the additions 275 us) and 16-bit outputs do without.
+constexpr int kMaxRun = 32;
+template <int D, bool NARROW>
+cudaError_t attend_sums(const Kv8Dev& c, const Kv8Batch& b, const Kv8Attention& a, const Cut& cut, int64_t blocks, cudaStream_t st) {
+    const bool sums = a.out_dtype == DT_F32 && blocks > (int64_t)cut.parts * cut.cluster * kWarps * kMaxRun;
+    return sums ? attend_t<D, NARROW, true>(c, b, a, cut, st) : attend_t<D, NARROW, false>(c, b, a, cut, st);
+}
+
+template <int D, bool NARROW>
 cudaError_t configure_t() {
-    const cudaError_t e = cudaFuncSetAttribute(attend_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)attend_smem<D, true>());
-    if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(attend_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)attend_smem<D, false>());
+    for (const auto kernel : {attend_kernel<D, NARROW, true>, attend_kernel<D, NARROW, false>}) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attend_smem<D, NARROW>());
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace
@@ -680,7 +699,8 @@ size_t kv8_partial_bytes(int dim) { return (size_t)kKv8MaxPartials * kKv8Rows * 
 
 cudaError_t kv8_configure(int num_sms, Kv8Machine* m) {
     m->num_sms = num_sms;
-    for (const cudaError_t e : {configure_t<128>(), configure_t<64>(), kv8_configure_prompt(m)})
+    for (const cudaError_t e : {configure_t<128, true>(), configure_t<128, false>(), configure_t<64, true>(), configure_t<64, false>(),
+                                kv8_configure_prompt(m)})
         if (e != cudaSuccess) return e;
     return cudaSuccess;
 }
@@ -693,15 +713,14 @@ cudaError_t launch_kv8_attention(const Kv8Dev& c, const Kv8Batch& b, const Kv8At
     // query heads each 107 us (117); calls of a few microseconds are within 0.3 us, or up to 1 us slower with
     // head_dim 64.
     const bool narrow = rows <= Shape<true>::kRows;
-    const int max_run = a.out_dtype == DT_F32 ? kMaxRun : INT_MAX / kWarps;
-    const Cut cut = narrow ? cut_items(items, blocks, Shape<true>::kCtas * m.num_sms, max_run)
-                           : cut_items(items * row_groups<false>(rows), blocks, Shape<false>::kCtas * m.num_sms, max_run);
+    const Cut cut = narrow ? cut_items(items, blocks, Shape<true>::kCtas * m.num_sms)
+                           : cut_items(items * row_groups<false>(rows), blocks, Shape<false>::kCtas * m.num_sms);
     if (rows > kKv8Rows && a.q_dtype != DT_F32 && a.out_dtype != DT_F32) {
         const PromptPlan plan = kv8_prompt_plan(rows, items, blocks, a.out_dtype, m);
         if (plan.us < cut.us) return launch_kv8_prompt(c, b, a, plan.cluster, st);
     }
-    if (narrow) return c.dim == 128 ? attend_t<128, true>(c, b, a, cut, st) : attend_t<64, true>(c, b, a, cut, st);
-    return c.dim == 128 ? attend_t<128, false>(c, b, a, cut, st) : attend_t<64, false>(c, b, a, cut, st);
+    if (narrow) return c.dim == 128 ? attend_sums<128, true>(c, b, a, cut, blocks, st) : attend_sums<64, true>(c, b, a, cut, blocks, st);
+    return c.dim == 128 ? attend_sums<128, false>(c, b, a, cut, blocks, st) : attend_sums<64, false>(c, b, a, cut, blocks, st);
 }
 
 }  // namespace stt

@@ -285,3 +285,26 @@ def test_select_when_a_chunk_is_masked_behind_a_poor_one(dtype):
     scores = rand((1, 32), "f32", 41, 0.001)
     _, out = run_select(logits, scores)
     check_select(logits, scores, None, -1, out)
+
+
+@pytest.mark.parametrize("n,group,tokens,cap", [(80, 1, 1, 60000), (80, 1, 1, 16000), (16, 8, 1, 60000), (6, 1, 24, 60000), (80, 1, 1, 2048)])
+def test_the_error_of_f32_outputs_does_not_grow_with_the_context(n, group, tokens, cap):
+    """Relative to the outputs' norm: weights in two f16 parts and their exponentials 2^-22, a block's product 2^-24, and a
+    warp's additions, at most 938 here and each rounded to nearest (0.29 of 2^-24 in the mean) over a sum that grows like
+    the root of their number, 0.29 * sqrt(938 / 2) * 2^-24; runs of up to 32 blocks may truncate instead, 32 * 2^-26."""
+    import torch
+    heads, dim = 8, 128
+    p = Pair(1, heads, dim, cap, seed=3)
+    q, out = rand((n, tokens, heads * group, dim), "f32", 37), torch.zeros(n, tokens, heads * group, dim, device="cuda")
+    p.cache.attention(q, out, i32([cap - tokens] * n), seqs=i32([0] * n), scale=0.01)
+    p.cache.status()
+    k, v = (torch.from_numpy(x.values(0, range(cap))).cuda().permute(1, 0, 2) for x in (p.k, p.v))
+    hidden = torch.arange(cap, device="cuda") > cap - tokens + torch.arange(tokens, device="cuda")[:, None]
+    error = []
+    for i in range(0, n, max(1, n // 12)):
+        s = torch.einsum("thgd,hpd->htgp", q[i].double().view(tokens, heads, group, dim), k) * 0.01
+        w = torch.softmax(s.masked_fill(hidden[None, :, None], -float("inf")), -1)
+        exact = torch.einsum("htgp,hpd->thgd", w, v)
+        error.append(((out[i].double().view_as(exact) - exact).norm() / exact.norm()).item())
+    print("errors", error)
+    assert np.mean(error) < 2.0 ** -22 + 2.0 ** -24 + max(0.29 * (938 / 2) ** 0.5 * 2.0 ** -24, 32 * 2.0 ** -26), error
