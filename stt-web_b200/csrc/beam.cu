@@ -16,12 +16,14 @@
 // costs a maximum, an exponential and a comparison per logit.  Where more reach the bound than the list
 // takes (ties, masked rows), the warps sort them 32 at a time by a bitonic network instead.
 //
-// What bounds it: instructions (about 15 a logit and lane with a tile's fixed work, 11 where a thread takes 32
-// logits of a tile) and the latency of a CTA's chain (copy, two passes over a tile, ranking, a ticket) rather
-// than memory; so CTAs are small, 7 or 8 of them share an SM, and tiles come by bulk copies, which hold no
-// registers.  128 x 8 rows of 8000 f32 logits (32.8 MB) take 14.9 us, 16 x 16 rows of 65,537 bf16 logits 24 us
-// (28 us with 16 logits to a thread, 34 us with CTAs of 512 threads, two to an SM, and tiles through
-// registers).  One utterance of 4 beams and 8000 tokens takes 7.2 us, half of it the last CTA's join.
+// What bounds it: the latency of a CTA's chain (copy, two passes over a tile, ranking, a ticket, the last CTA's
+// join) rather than memory or issue: the two batches below keep the issue slots 48% and 43% busy with 28
+// instructions a logit and lane in f32 (16 logits of a thread in a tile) and 21 in bf16 (32), joins included,
+// and 36% and 29% of the warps resident.  So CTAs are small, 7 or 8 of them share an SM, and tiles come by bulk
+// copies, which hold no registers.  128 x 8 rows of 8000 f32 logits (32.8 MB) take 16 us with the logits in L2 and
+// 19.4 us from memory, 16 x 16 rows of 65,537 bf16 logits, some ended, 26 and 29.5 us (16 logits to a thread
+// cost 4 us more, CTAs of 512 threads, two to an SM, and tiles through registers 10 us more).  One utterance of 4
+// beams and 8000 tokens takes 8.4 us, half of it the last CTA's join.
 #include <algorithm>
 
 #include "beam.h"

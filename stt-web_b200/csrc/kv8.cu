@@ -8,10 +8,11 @@
 // machine.  A block can grow while it fills, each move rounding once more: a code ends up within
 // 1/2 + 1/4 + 1/8 + ... < 1 step of its value.
 //
-// Both are bound by memory, so what counts is loads in flight.  Measured: append of 2048 tokens of 8 sequences
-// x 16 heads of 128 (bf16) 33 us for 201 MB, 6.1 TB/s (with the rows held as f32, half the warps on an SM,
-// 52 us); of one token of 512 sequences (f32) 8.4 us for 10.5 MB, a launch and three dependent loads (a warp
-// for K and another for V took 10.5 us); read of 2055 tokens of the 8 sequences (bf16) 32 us for 202 MB, 6.3 TB/s.
+// Both are bound by memory, so what counts is loads in flight.  Measured from cold caches: append of 2048 tokens of
+// 8 sequences x 16 heads of 128 in bf16 34 us for 201 MB, 5.9 TB/s (with the rows held as f32, half the warps on an
+// SM, 52 us), in f32, whose rows take twice the registers, 60 us for 336 MB, 5.6 TB/s; of one token of 512
+// sequences (f32) 10 us for 10.5 MB, a launch and three dependent loads (8.4 us in L2; a warp for K and another
+// for V took 10.5 us there); read of 2055 tokens of the 8 sequences (bf16) 35 us for 202 MB, 5.9 TB/s.
 #include "kv8.cuh"
 
 namespace stt {

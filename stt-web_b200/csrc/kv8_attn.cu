@@ -30,9 +30,12 @@
 //  - where there are fewer (row, head) items than CTAs fit, an item's blocks are cut into runs for the CTAs
 //    of a cluster, joined through distributed shared memory, and beyond that into parts joined through
 //    global memory, the last part to finish doing it (cut_items chooses).
-// Measured (time of a launch): 512 sequences x 16 heads x 751 positions 278 us for 1.61 GB, 5.8 TB/s;
-// 4 sequences x 8 heads of up to 65,521 positions, 4 query heads each, 103 us for 0.51 GB, 5.0 TB/s;
-// 1 sequence x 16 heads: 130 positions 6.2 us, 751 positions 7.5 us; 64 sequences x 751 positions 41 us.
+// Measured (time of a launch): 512 sequences x 16 heads x 751 positions 267 us for 1.61 GB, 6.0 TB/s (281 us from
+// cold caches); with a ring of 4,096 the same at 130 positions 119 us, at 4,000 1.22 ms; 4 sequences x 8 heads of up to
+// 65,521 positions, 4 query heads each, 105 us for 0.51 GB, 4.9 TB/s; 1 sequence x 16 heads: 130 positions 6.6 us,
+// 751 positions 7.5 us; 64 sequences x 751 positions 41 us.  Chunks with f32 on either side come here too, 8 rows
+// at a time: the last 1024 of 4096 positions of 4 x 16 heads take 1.65 ms, where 16-bit ones take 149 us on the
+// other kernel.
 #include <cfloat>
 #include <climits>
 #include <algorithm>
