@@ -81,6 +81,7 @@ int check_written(const char* what, const stt_kv8_tensor& t, const stt_kv8_batch
 // A batch's host-side checks; *some is false for one without rows or tokens, which is nothing to do.
 int check_batch(const stt_kv8_cache* h, const stt_kv8_batch* b, bool* some) {
     if (!h || !b || b->n < 0 || b->n_tokens < 0) return set_error(STT_E_INVALID_ARG, "bad arguments");
+    if (b->n_tokens > INT_MAX - 1024) return set_error(STT_E_INVALID_ARG, "%d tokens are too many for one call", b->n_tokens);
     *some = b->n > 0 && b->n_tokens > 0;
     if (*some && !b->d_pos) return set_error(STT_E_INVALID_ARG, "NULL positions");
     if (!b->d_seqs && b->n > h->c.n_seqs)

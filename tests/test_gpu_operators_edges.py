@@ -308,3 +308,19 @@ def test_the_error_of_f32_outputs_does_not_grow_with_the_context(n, group, token
         error.append(((out[i].double().view_as(exact) - exact).norm() / exact.norm()).item())
     print("errors", error)
     assert np.mean(error) < 2.0 ** -22 + 2.0 ** -24 + max(0.29 * (938 / 2) ** 0.5 * 2.0 ** -24, 32 * 2.0 ** -26), error
+
+
+def test_more_tokens_than_positions_are_refused():
+    """The counts of such a batch could be small, but its grid has no size."""
+    from stt_b200._lib import KV8_BATCH, KV8_TENSOR, lib
+    p = Pair(1, 1, 64, 32)
+    x, one = rand((1, 1, 1, 64), "f32", 60), i32([0])
+    tensor = KV8_TENSOR.pack(x.data_ptr(), 256, 64, 64, 0, 0)
+    out = KV8_TENSOR.pack(rand((1, 1, 1, 64), "f32", 61).data_ptr(), 2 ** 40, 64, 64, 0, 0)
+    for tokens in (2 ** 31 - 1, 2 ** 31 - 31, 2 ** 31 - 1000):
+        batch = KV8_BATCH.pack(0, one.data_ptr(), one.data_ptr(), 1, tokens)
+        assert lib().stt_kv8_append_device(p.cache._h, batch, tensor, tensor, None) == STT_E_INVALID_ARG
+        assert lib().stt_kv8_read_device(p.cache._h, batch, out, tensor, None) == STT_E_INVALID_ARG
+        assert lib().stt_kv8_attention_device(p.cache._h, batch, tensor, 1, None, 0, 1.0, out, None) == STT_E_INVALID_ARG
+    p.cache.status()
+    p.same()
