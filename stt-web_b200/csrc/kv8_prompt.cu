@@ -23,8 +23,8 @@
 //    share is above 2^-22 of the largest while V's exponents lie within 110 of one another (a weight is
 //    flushed to zero below 2^-126, 2^132 below the row's largest);
 //  - q is exact in f16 once its row is scaled by a power of two.  Weights, scaled by 2^6, are rounded to f16
-//    for bf16 outputs: 2^-12 of each against the output's own 2^-9 (its error grows by 1%).  For f16 outputs
-//    that would be half of their own 2^-11 (errors up to 25% above those of the rounding alone), so there P
+//    for bf16 outputs: at most 2^-11 of each against the output's own 2^-8 (its error grows by 1%).  For f16
+//    outputs that would be as much as their own rounding (errors up to 25% above its alone), so there P
 //    has two f16 parts, the rest behind the first in what the scores leave free of their 128 columns, and
 //    O += P V two products: 22 bits, for 20% more time;
 //  - M moves only when a score exceeds it by 8 (weights then reach 2^14, inside f16), so that O, which
@@ -35,10 +35,9 @@
 // runs; at the end each sends O, M and l of every row to the shared memory of the CTA that joins that row
 // in its share.
 // Measured: the last 1024 of 4096 positions, 4 sequences x 16 heads of 128, 149 us with bf16 outputs, 0.81
-// PFLOP/s, and 179 us with f16 ones; a step of
-// two tiles takes 2.1 us (its products 1.1 us, its exponentials as long on the other units; a tile's softmax
-// waits 0.7 us a step for its products), a CTA 6 to 11 us besides (its rows in and out, the first step's
-// latency).  Halves of 64 keys with scores and weights in alternating buffers hide that wait, but products of
+// PFLOP/s, and 179 us with f16 ones; a step of two tiles takes 2.1 us (its products 1.1 us, its exponentials as
+// long on the other units; a tile's softmax waits 0.7 us a step for its products), with weights in two parts
+// 2.6 us, a CTA 6 to 11 us besides (its rows in and out, the first step's latency).  Halves of 64 keys with scores and weights in alternating buffers hide that wait, but products of
 // 64 columns are less than half as fast: 165 us.
 // Every wait is bounded: one that gives up sets the CTA's abort word, all roles leave, the copies and
 // products in flight are waited for, and the cache's error word records it.
